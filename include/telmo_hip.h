@@ -16,6 +16,8 @@
  *   Kernels::layer_norm          src/kernels/mod.rs:458       -> tg_layer_norm_device
  *   Kernels::dwconv1d_frame + silu  src/kernels/mod.rs:464-475  -> tg_dwconv1d_device
  *   BView::row_major + matmul    src/kernels/mod.rs:320-339, 657-688 -> tg_matmul_rowmajor_device
+ *   Parakeet::attention          src/parakeet.rs:1176-1282    -> tg_attention_device
+ *   Granite::attention           src/granite.rs:962-1036      -> tg_attention_device
  *   Parakeet::predict_rows       src/parakeet.rs:1524-1577    -> tg_tdt_predict_device
  *   Parakeet::decode_inner       src/parakeet.rs:1412-1513    -> tg_tdt_decode_device
  *   Pack::open / from_bytes      src/pack.rs:79-96            -> tg_pack_open, tg_pack_from_bytes
@@ -318,6 +320,102 @@ int tg_dwconv1d_quant_device(tg_ctx *ctx, const float *x, size_t x_len, size_t l
                              size_t channels, const float *w, size_t w_len, size_t kernel, const float *bias,
                              size_t bias_len, uint32_t act, float *out, size_t out_len, size_t ldo, void *qa,
                              size_t qa_len, int32_t *exps, size_t exps_len);
+
+/* ---- attention ------------------------------------------------------------------------------
+ * The attention core that Parakeet::layer and Granite::block_span leave between the qkv product and
+ * the output product (src/parakeet.rs:1176-1282, src/granite.rs:962-1036), over rows of any number of
+ * sequences, and the forms of it that text encoders and decoders use. For head h of query row i, with the
+ * keys and values of head h / (heads / kv_heads):
+ *
+ *   s_ij = softcap tanh(scale ((q_i + u) k_j + (q_i + w) rel_c) / softcap) - slope |j - i| + table[c']
+ *   out_i = sum_j softmax_j(s_ij) v_j    over the keys j that i is shown
+ *
+ * Each part but scale q k is optional. i and j are positions in the sequence: a sequence of n query rows
+ * and m keys has its rows at positions m - n, ..., m - 1 (its last n). c and c' are j - i clamped to
+ * [-span, span], counted from the first of 2 span + 1 rows or values.
+ * Shown are the keys j of the query's sequence with i - left <= j <= i + right (a negative left or right:
+ * no limit on that side; right 0: causal) or j < prefix, and, with documents, of the query's document
+ * (docs equal and not negative). A query that is shown no key, or only keys whose score is -infinity,
+ * gets zeros. Keys that no query is shown may hold anything.
+ * Scores, softmax statistics and sums are f32; with 16-bit types the weights round to that type (half a
+ * step) before they multiply the values, and the outputs once. f32 rows are computed to f32's accuracy.
+ * Rows of q and out behind the last sequence are neither read nor written. */
+typedef struct {
+    const void *p; /* device, 16-byte aligned */
+    size_t len;    /* elements reachable from p */
+    size_t ld, hs; /* elements between rows and between heads: whole multiples of 16 bytes */
+} tg_rows;
+typedef struct {
+    uint32_t type;                /* TG_F32, TG_F16 or TG_BF16: of q, k, v and out */
+    size_t heads, kv_heads, d;    /* kv_heads divides heads; d a multiple of 8 up to 256 */
+    float scale, softcap;         /* scale > 0; softcap 0: none */
+    int64_t left, right;
+    const float *slopes;          /* device, heads values, or null */
+    size_t slopes_len;
+    const float *table;           /* device, heads x (2 table_span + 1), or null */
+    size_t table_len, table_span;
+    const float *rel;             /* device, 16-byte aligned, 2 rel_span + 1 rows of f32 (type TG_F32 only), or null */
+    size_t rel_len, ldrel, hsrel; /* rows ldrel apart, heads hsrel apart (0: one set for all heads) */
+    size_t rel_span;
+    const float *rel_u, *rel_v;   /* device, heads x d each (u and w above), or null: zeros */
+    size_t rel_u_len, rel_v_len;
+    size_t batch;                 /* sequences, at most 65535 */
+    size_t q_rows, k_rows;        /* rows of q and out, rows of k and v (k_rows unused when paged) */
+    size_t longest;               /* most query rows of a sequence; rows past it stay as they were. 0: any */
+    const int32_t *q_starts;      /* device, batch + 1 first rows (the last one: the end), or null: sequences */
+    const int32_t *k_starts;      /*   of equal length, stacked along the rows. k_starts null: as q_starts */
+    size_t q_starts_len, k_starts_len;
+    const int32_t *prefix;        /* device, batch values, or null */
+    size_t prefix_len;
+    const int32_t *q_docs;        /* device, q_rows values, or null */
+    const int32_t *k_docs;        /* device, k_rows values; null with q_docs: q_docs */
+    size_t q_docs_len, k_docs_len;
+    tg_rows q, k, v, out;         /* out must not overlap q, k and v */
+    /* tg_attention_paged_device and tg_cache_append_device: key position j of sequence b is row j % page of
+     * page tables[b * ldt + j / page]; sequence b holds lengths[b] keys, its new ones included. */
+    const int32_t *tables;        /* device, batch rows of width entries, ldt apart */
+    size_t tables_len, ldt, width;
+    const int32_t *lengths;       /* device, batch values */
+    size_t lengths_len;
+    size_t pages, page;           /* pages of the cache, rows per page */
+    size_t k_page, v_page;        /* elements between pages of k and of v */
+    void *workspace;              /* device, 16-byte aligned, or null: see tg_attention_workspace_bytes */
+    size_t workspace_len;         /* bytes */
+} tg_attention_desc;
+/* Device pointers, queued on the context's stream; nothing is allocated, so the calls can be captured
+ * into a graph. Row numbers, lengths and page numbers in device memory are read by the kernels only: ones
+ * that leave the buffers are cut to them, and keys in a page that the cache does not have are not shown. */
+int tg_attention_device(tg_ctx *ctx, const tg_attention_desc *desc);
+/* A chunk of new rows of each sequence, or a single one, over a paged cache that holds its keys and values
+ * (those of the new rows too, tg_cache_append_device). No documents. */
+int tg_attention_paged_device(tg_ctx *ctx, const tg_attention_desc *desc);
+/* A workspace of this many bytes lets a call of `rows` query rows in `batch` sequences of up to `keys` keys
+ * split long sequences over the GPU and join the parts; 0 where it would not. With a smaller one, or none,
+ * the call does without. Calls that may overlap on the GPU (other streams, captured graphs replayed at
+ * once) need workspaces of their own. */
+size_t tg_attention_workspace_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys);
+
+/* Rotary positions: the first dim values of each head are rotated in dim / 2 pairs, pair i of a row at
+ * position p by the angle 2 pi p turns[i]: (x, y) becomes amplitude (x cos - y sin, y cos + x sin). */
+typedef struct {
+    const double *turns;  /* device, dim / 2 values: turns per position */
+    size_t turns_len;
+    size_t dim;           /* even, at most 256; 0: no rotation */
+    int32_t interleaved;  /* pairs (2 i, 2 i + 1); else (i, i + dim / 2) */
+    float amplitude;
+} tg_rotary;
+/* out[r] = x[r] rotated, in another type if wanted (rounded once); values past dim are copied. Row r stands
+ * at positions[r] (device), or at start + r where positions is null. out may be x itself (the same address,
+ * strides and type) and must not overlap it otherwise. d a multiple of 8 up to 256. */
+int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, tg_rows out, size_t rows, size_t heads,
+                     size_t d, const int32_t *positions, size_t positions_len, int64_t start, const tg_rotary *rotary);
+/* New rows' keys and values into their pages, in the cache's type: row r of the n new rows of sequence b (rows
+ * q_starts[b] .. of k_new and v_new, or equal lengths) is written at key position lengths[b] - n + r, its key
+ * rotated for that position first where rotary is given. desc names the cache as tg_attention_paged_device
+ * reads it (type, kv_heads, d, k, v, k_page, v_page, page, pages, tables, lengths, batch, q_rows, q_starts,
+ * longest). Rows whose position has no page are not written; two rows in one place leave either of them. */
+int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
+                           const tg_rotary *rotary);
 
 /* ---- the TDT decoder (src/parakeet.rs:1412-1577) --------------------------------------------
  * Parakeet's prediction network (embedding, LSTM layers, projection) and joint, decoded greedily

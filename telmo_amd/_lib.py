@@ -31,6 +31,32 @@ class TdtStream(ctypes.Structure):
                 ("count", _sz)]
 
 
+class Rows(ctypes.Structure):
+    """tg_rows."""
+    _fields_ = [("p", _p), ("len", _sz), ("ld", _sz), ("hs", _sz)]
+
+
+class AttentionDesc(ctypes.Structure):
+    """tg_attention_desc."""
+    _fields_ = [("type", _u32), ("heads", _sz), ("kv_heads", _sz), ("d", _sz), ("scale", ctypes.c_float),
+                ("softcap", ctypes.c_float), ("left", ctypes.c_int64), ("right", ctypes.c_int64), ("slopes", _p),
+                ("slopes_len", _sz), ("table", _p), ("table_len", _sz), ("table_span", _sz), ("rel", _p),
+                ("rel_len", _sz), ("ldrel", _sz), ("hsrel", _sz), ("rel_span", _sz), ("rel_u", _p), ("rel_v", _p),
+                ("rel_u_len", _sz), ("rel_v_len", _sz), ("batch", _sz), ("q_rows", _sz), ("k_rows", _sz),
+                ("longest", _sz), ("q_starts", _p), ("k_starts", _p), ("q_starts_len", _sz), ("k_starts_len", _sz),
+                ("prefix", _p), ("prefix_len", _sz), ("q_docs", _p), ("k_docs", _p), ("q_docs_len", _sz),
+                ("k_docs_len", _sz), ("q", Rows), ("k", Rows), ("v", Rows), ("out", Rows), ("tables", _p),
+                ("tables_len", _sz), ("ldt", _sz), ("width", _sz), ("lengths", _p), ("lengths_len", _sz),
+                ("pages", _sz), ("page", _sz), ("k_page", _sz), ("v_page", _sz), ("workspace", _p),
+                ("workspace_len", _sz)]
+
+
+class RotaryDesc(ctypes.Structure):
+    """tg_rotary."""
+    _fields_ = [("turns", _p), ("turns_len", _sz), ("dim", _sz), ("interleaved", ctypes.c_int32),
+                ("amplitude", ctypes.c_float)]
+
+
 _szp = ctypes.POINTER(_sz)
 
 # name: (restype, argtypes), in the order of include/telmo_hip.h
@@ -75,6 +101,13 @@ SIGNATURES = {
                                            _u32, _p, _sz, _sz]),
     "tg_dwconv1d_quant_device": (ctypes.c_int, [_p, _p, _sz, _sz, _sz, _sz, _sz, _p, _sz, _sz, _p, _sz, _u32, _p,
                                                  _sz, _sz, _p, _sz, _p, _sz]),
+    "tg_attention_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc)]),
+    "tg_attention_paged_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc)]),
+    "tg_attention_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
+    "tg_rotary_device": (ctypes.c_int, [_p, _u32, Rows, _u32, Rows, _sz, _sz, _sz, _p, _sz, ctypes.c_int64,
+                                        ctypes.POINTER(RotaryDesc)]),
+    "tg_cache_append_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc), _u32, Rows, Rows,
+                                              ctypes.POINTER(RotaryDesc)]),
     "tg_tdt_create": (ctypes.c_int, [_p, _p, ctypes.POINTER(_p)]),
     "tg_tdt_destroy": (None, [_p]),
     "tg_tdt_max_rows": (_sz, [_p]),

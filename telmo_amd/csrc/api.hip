@@ -10,8 +10,9 @@
 // (gemv_fits) take the MFMA GEMV, or for int8 the dot4 GEMV, in one launch; otherwise the row
 // quantiser then the MFMA GEMM, whose kernel launch_gemm_i8 picks by shape. The exact mode, other
 // precisions and longer inputs run the exact kernel.
-#include <cstring>
 #include <algorithm>
+#include <cmath>
+#include <cstring>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -1531,6 +1532,268 @@ int tg_tdt_set_resident_limits(tg_ctx *ctx, tg_tdt *tdt, uint32_t steps_per_laun
     tdt->launch_steps = steps_per_launch ? (int)steps_per_launch : TDT_RESIDENT_STEPS;
     const uint64_t ticks = wait_us ? wait_us * tdt->clock_khz / 1000 : tdt->clock_khz * 1000;
     tdt->wait_ticks = ticks ? ticks : 1;
+    return TG_OK;
+}
+
+// -------------------------------------------------------------------------- attention
+
+namespace {
+
+constexpr size_t MAX_ATTN_ROWS = (size_t)1 << 30;  // rows, keys and strides that the kernels count in 32 bits
+constexpr size_t MAX_ATTN_GRID = 65535;            // sequences and heads, each a grid dimension
+
+bool attn_type(uint32_t t) { return t == TG_F32 || t == TG_F16 || t == TG_BF16; }
+size_t type_bytes(uint32_t t) { return t == TG_F32 ? 4 : 2; }
+
+// a + b and a * b, SIZE_MAX where they do not fit.
+size_t sat_add(size_t a, size_t b) { return a > SIZE_MAX - b ? SIZE_MAX : a + b; }
+size_t sat_mul(size_t a, size_t b) { return b && a > SIZE_MAX / b ? SIZE_MAX : a * b; }
+
+// Elements that heads of d values in rows (in `outer` groups of them, og apart) reach from the first.
+size_t rows_span(const tg_rows &r, size_t rows, size_t heads, size_t d, size_t outer = 1, size_t og = 0) {
+    if (!rows || !heads || !outer) return 0;
+    return sat_add(sat_add(sat_mul(rows - 1, r.ld), sat_mul(heads - 1, r.hs)), sat_add(sat_mul(outer - 1, og), d));
+}
+
+int check_rows(tg_ctx *ctx, const char *name, const tg_rows &r, uint32_t type, size_t span) {
+    const std::string n(name);
+    if (span == 0) return TG_OK;
+    if (!r.p) return fail(ctx, TG_ERR_NULL, n + " is null");
+    if (r.len < span) return fail(ctx, TG_ERR_SHAPE, n + " is too short");
+    if (span > SIZE_MAX / 16) return fail(ctx, TG_ERR_SHAPE, n + " does not fit in memory");
+    const size_t bytes = type_bytes(type);
+    if (reinterpret_cast<uintptr_t>(r.p) % 16 || r.ld * bytes % 16 || r.hs * bytes % 16)
+        return fail(ctx, TG_ERR_ALIGN, n + ": address and strides must be multiples of 16 bytes");
+    return TG_OK;
+}
+
+// Rows that are written: no two heads of any row in one place.
+bool rows_distinct(const tg_rows &r, size_t rows, size_t heads, size_t d) {
+    if (rows <= 1 && heads <= 1) return true;
+    if (heads <= 1) return r.ld >= d;
+    if (rows <= 1) return r.hs >= d;
+    return (r.hs >= d && r.ld >= sat_add(sat_mul(heads - 1, r.hs), d)) ||
+           (r.ld >= d && r.hs >= sat_add(sat_mul(rows - 1, r.ld), d));
+}
+
+bool ranges_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
+// The heads, sequences and (paged) the cache that attention and append both name, and their lengths.
+int check_seqs(tg_ctx *ctx, const tg_attention_desc &a, bool paged, tg::AttnSeqs &s) {
+    if (!attn_type(a.type)) return fail(ctx, TG_ERR_ARG, "type must be f32, f16 or bf16");
+    if (a.d < 8 || a.d > 256 || a.d % 8) return fail(ctx, TG_ERR_UNSUPPORTED, "d must be a multiple of 8 up to 256");
+    if (a.kv_heads < 1 || a.kv_heads > MAX_ATTN_GRID || a.batch > MAX_ATTN_GRID)
+        return fail(ctx, TG_ERR_UNSUPPORTED, "1 to 65535 heads and at most 65535 sequences");
+    if (a.q_rows > MAX_ATTN_ROWS) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^30 rows");
+    if (a.batch && !a.q_starts && a.q_rows % a.batch)
+        return fail(ctx, TG_ERR_SHAPE, "the rows do not split into equal sequences");
+    if (a.q_starts && a.q_starts_len < a.batch + 1) return fail(ctx, TG_ERR_SHAPE, "q_starts is too short");
+    s = tg::AttnSeqs{};
+    s.batch = (int)a.batch;
+    s.q_rows = (int)a.q_rows;
+    const size_t most = a.q_starts || !a.batch ? a.q_rows : a.q_rows / a.batch;
+    s.longest = (int)(a.longest && a.longest < most ? a.longest : most);
+    s.q_starts = a.q_starts;
+    if (!paged) return TG_OK;
+    if (!a.tables || !a.lengths) return fail(ctx, TG_ERR_NULL, "tables or lengths are null");
+    if (!a.page || a.page > MAX_ATTN_ROWS || a.pages > MAX_ATTN_ROWS || a.width > MAX_ATTN_ROWS)
+        return fail(ctx, TG_ERR_UNSUPPORTED, "1 to 2^30 rows per page, at most 2^30 pages and table entries");
+    if (a.batch && (a.ldt > SIZE_MAX / 16 || a.tables_len < span(a.batch, a.ldt, a.width)))
+        return fail(ctx, TG_ERR_SHAPE, "tables is too short");
+    if (a.lengths_len < a.batch) return fail(ctx, TG_ERR_SHAPE, "lengths is too short");
+    s.tables = a.tables;
+    s.lengths = a.lengths;
+    s.ldt = (int64_t)a.ldt;
+    s.width = (int)a.width;
+    s.page = (int)a.page;
+    s.pages = (int)a.pages;
+    int rc = check_rows(ctx, "k", a.k, a.type, rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page));
+    if (rc) return rc;
+    if ((rc = check_rows(ctx, "v", a.v, a.type, rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page)))) return rc;
+    if (a.k_page * type_bytes(a.type) % 16 || a.v_page * type_bytes(a.type) % 16)
+        return fail(ctx, TG_ERR_ALIGN, "page strides must be multiples of 16 bytes");
+    return TG_OK;
+}
+
+int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
+    // The arguments need no context: they are judged first, a null context after them.
+    if (!desc) return fail(ctx, TG_ERR_NULL, "null description");
+    const tg_attention_desc &a = *desc;
+    tg::AttnArgs k{};
+    int rc = check_seqs(ctx, a, paged, k.seqs);
+    if (rc) return rc;
+    if (a.heads < 1 || a.heads > MAX_ATTN_GRID || a.heads % a.kv_heads)
+        return fail(ctx, TG_ERR_SHAPE, "kv_heads must divide heads, at most 65535");
+    if (!(a.scale > 0.0f) || !std::isfinite(a.scale)) return fail(ctx, TG_ERR_ARG, "scale must be positive and finite");
+    if (!(a.softcap >= 0.0f) || !std::isfinite(a.softcap))
+        return fail(ctx, TG_ERR_ARG, "softcap must be finite and not negative");
+    if (a.slopes && a.slopes_len < a.heads) return fail(ctx, TG_ERR_SHAPE, "slopes is too short");
+    if (a.table && (a.table_span > MAX_ATTN_ROWS || a.table_len < a.heads * (2 * a.table_span + 1)))
+        return fail(ctx, TG_ERR_SHAPE, "table is too short");
+    if (a.rel) {
+        if (a.type != TG_F32) return fail(ctx, TG_ERR_UNSUPPORTED, "position rows are f32 and go with f32 rows");
+        if (a.rel_span > MAX_ATTN_ROWS) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^31 position rows");
+        const tg_rows rel{a.rel, a.rel_len, a.ldrel, a.hsrel};
+        if ((rc = check_rows(ctx, "rel", rel, TG_F32, rows_span(rel, 2 * a.rel_span + 1, a.heads, a.d)))) return rc;
+        if ((a.rel_u && a.rel_u_len < a.heads * a.d) || (a.rel_v && a.rel_v_len < a.heads * a.d))
+            return fail(ctx, TG_ERR_SHAPE, "rel_u or rel_v is too short");
+    } else if (a.rel_u || a.rel_v) {
+        return fail(ctx, TG_ERR_ARG, "rel_u and rel_v go with position rows");
+    }
+    if (a.prefix && a.prefix_len < a.batch) return fail(ctx, TG_ERR_SHAPE, "prefix is too short");
+    if (paged) {
+        if (a.q_docs || a.k_docs || a.k_starts)
+            return fail(ctx, TG_ERR_ARG, "a paged cache takes no documents and no k_starts");
+    } else {
+        if (a.tables || a.lengths) return fail(ctx, TG_ERR_ARG, "tables and lengths go with a paged cache");
+        if (a.k_rows > MAX_ATTN_ROWS) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^30 keys");
+        k.seqs.k_rows = (int)a.k_rows;
+        if (a.k_starts) {
+            if (a.k_starts_len < a.batch + 1) return fail(ctx, TG_ERR_SHAPE, "k_starts is too short");
+            k.seqs.k_starts = a.k_starts;
+        } else if (a.q_starts) {
+            if (a.k_rows != a.q_rows) return fail(ctx, TG_ERR_SHAPE, "without k_starts k has as many rows as q");
+            k.seqs.k_starts = a.q_starts;
+        } else if (a.batch && a.k_rows % a.batch) {
+            return fail(ctx, TG_ERR_SHAPE, "the keys do not split into equal sequences");
+        }
+        if ((rc = check_rows(ctx, "k", a.k, a.type, rows_span(a.k, a.k_rows, a.kv_heads, a.d)))) return rc;
+        if ((rc = check_rows(ctx, "v", a.v, a.type, rows_span(a.v, a.k_rows, a.kv_heads, a.d)))) return rc;
+        if (a.k_docs && !a.q_docs) return fail(ctx, TG_ERR_ARG, "k_docs goes with q_docs");
+        if (a.q_docs) {
+            if (a.q_docs_len < a.q_rows) return fail(ctx, TG_ERR_SHAPE, "q_docs is too short");
+            if (!a.k_docs && a.k_rows != a.q_rows)
+                return fail(ctx, TG_ERR_SHAPE, "without k_docs k has as many rows as q");
+            if (a.k_docs && a.k_docs_len < a.k_rows) return fail(ctx, TG_ERR_SHAPE, "k_docs is too short");
+            k.q_docs = a.q_docs;
+            k.k_docs = a.k_docs ? a.k_docs : a.q_docs;
+        }
+    }
+    const size_t q_span = rows_span(a.q, a.q_rows, a.heads, a.d), o_span = rows_span(a.out, a.q_rows, a.heads, a.d);
+    if ((rc = check_rows(ctx, "q", a.q, a.type, q_span))) return rc;
+    if ((rc = check_rows(ctx, "out", a.out, a.type, o_span))) return rc;
+    if (!rows_distinct(a.out, a.q_rows, a.heads, a.d))
+        return fail(ctx, TG_ERR_SHAPE, "out's strides put two heads in one place");
+    const size_t size = type_bytes(a.type);
+    const size_t k_span = paged ? rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page)
+                                : rows_span(a.k, a.k_rows, a.kv_heads, a.d);
+    const size_t v_span = paged ? rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page)
+                                : rows_span(a.v, a.k_rows, a.kv_heads, a.d);
+    if (ranges_overlap(a.out.p, o_span * size, a.q.p, q_span * size) ||
+        ranges_overlap(a.out.p, o_span * size, a.k.p, k_span * size) ||
+        ranges_overlap(a.out.p, o_span * size, a.v.p, v_span * size))
+        return fail(ctx, TG_ERR_ARG, "out must not overlap q, k or v");
+    if (a.workspace && reinterpret_cast<uintptr_t>(a.workspace) % 16)
+        return fail(ctx, TG_ERR_ALIGN, "workspace must be 16-byte aligned");
+    if (!ctx) return TG_ERR_NULL;
+    if (k.seqs.batch == 0 || k.seqs.longest == 0) return TG_OK;
+    const auto clip = [](int64_t w) { return w < 0 ? -1 : w > INT32_MAX ? -1 : (int32_t)w; };
+    k.q = a.q.p, k.k = a.k.p, k.v = a.v.p, k.out = const_cast<void *>(a.out.p);
+    k.ldq = (int64_t)a.q.ld, k.hsq = (int64_t)a.q.hs, k.ldk = (int64_t)a.k.ld, k.hsk = (int64_t)a.k.hs;
+    k.ldv = (int64_t)a.v.ld, k.hsv = (int64_t)a.v.hs, k.ldo = (int64_t)a.out.ld, k.hso = (int64_t)a.out.hs;
+    k.psk = (int64_t)a.k_page, k.psv = (int64_t)a.v_page;
+    k.type = a.type;
+    k.heads = (int)a.heads, k.kv_heads = (int)a.kv_heads, k.d = (int)a.d;
+    k.scale = a.scale, k.cap = a.softcap;
+    k.left = clip(a.left), k.right = clip(a.right);
+    k.slopes = a.slopes, k.table = a.table, k.table_span = (int)a.table_span;
+    k.rel = a.rel, k.rel_u = a.rel_u, k.rel_v = a.rel_v;
+    k.ldrel = (int64_t)a.ldrel, k.hsrel = (int64_t)a.hsrel, k.rel_span = (int)a.rel_span;
+    k.prefix = a.prefix;
+    k.work = a.workspace, k.work_bytes = a.workspace ? a.workspace_len : 0;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    TG_HIP(ctx, tg::launch_attention(k, ctx->stream));
+    return TG_OK;
+}
+
+int check_rotary(tg_ctx *ctx, const tg_rotary *r, size_t d, tg::RotaryArgs &out) {
+    out = tg::RotaryArgs{nullptr, 0, 0, 1.0f};
+    if (!r || r->dim == 0) return TG_OK;
+    if (r->dim % 2 || r->dim > d) return fail(ctx, TG_ERR_SHAPE, "dim must be even and at most d");
+    if (!r->turns) return fail(ctx, TG_ERR_NULL, "turns is null");
+    if (r->turns_len < r->dim / 2) return fail(ctx, TG_ERR_SHAPE, "turns is too short");
+    if (!std::isfinite(r->amplitude)) return fail(ctx, TG_ERR_ARG, "amplitude must be finite");
+    out = tg::RotaryArgs{r->turns, (int)r->dim, r->interleaved != 0, r->amplitude};
+    return TG_OK;
+}
+
+}  // namespace
+
+int tg_attention_device(tg_ctx *ctx, const tg_attention_desc *desc) { return run_attention(ctx, desc, false); }
+
+int tg_attention_paged_device(tg_ctx *ctx, const tg_attention_desc *desc) { return run_attention(ctx, desc, true); }
+
+size_t tg_attention_workspace_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys) {
+    if (!rows || !heads || !kv_heads || heads % kv_heads || heads > MAX_ATTN_GRID || !d || d > 256 || !batch ||
+        batch > MAX_ATTN_GRID || rows > MAX_ATTN_ROWS)
+        return 0;
+    return tg::attention_work_bytes(rows, heads, kv_heads, d, batch, keys < MAX_ATTN_ROWS ? keys : MAX_ATTN_ROWS);
+}
+
+int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, tg_rows out, size_t rows, size_t heads,
+                     size_t d, const int32_t *positions, size_t positions_len, int64_t start,
+                     const tg_rotary *rotary) {
+    if (!attn_type(type) || !attn_type(out_type)) return fail(ctx, TG_ERR_ARG, "types must be f32, f16 or bf16");
+    if (d < 8 || d > 256 || d % 8) return fail(ctx, TG_ERR_UNSUPPORTED, "d must be a multiple of 8 up to 256");
+    if (heads > MAX_ATTN_GRID || rows > MAX_ATTN_ROWS)
+        return fail(ctx, TG_ERR_UNSUPPORTED, "at most 65535 heads and 2^30 rows");
+    tg::RotaryArgs r;
+    int rc = check_rotary(ctx, rotary, d, r);
+    if (rc) return rc;
+    const size_t x_span = rows_span(x, rows, heads, d), o_span = rows_span(out, rows, heads, d);
+    if ((rc = check_rows(ctx, "x", x, type, x_span))) return rc;
+    if ((rc = check_rows(ctx, "out", out, out_type, o_span))) return rc;
+    if (!rows_distinct(out, rows, heads, d)) return fail(ctx, TG_ERR_SHAPE, "out's strides put two heads in one place");
+    if (positions && positions_len < rows) return fail(ctx, TG_ERR_SHAPE, "positions is too short");
+    const bool same = x.p == out.p && x.ld == out.ld && x.hs == out.hs && type == out_type;
+    if (!same && ranges_overlap(x.p, x_span * type_bytes(type), out.p, o_span * type_bytes(out_type)))
+        return fail(ctx, TG_ERR_ARG, "out must be x itself or not overlap it");
+    if (!ctx) return TG_ERR_NULL;
+    if (rows == 0 || heads == 0) return TG_OK;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    TG_HIP(ctx, tg::launch_rotary(x.p, type, (int64_t)x.ld, (int64_t)x.hs, const_cast<void *>(out.p), out_type,
+                                  (int64_t)out.ld, (int64_t)out.hs, rows, (int)heads, (int)d, positions, start, r,
+                                  ctx->stream));
+    return TG_OK;
+}
+
+int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
+                           const tg_rotary *rotary) {
+    if (!desc) return fail(ctx, TG_ERR_NULL, "null description");
+    const tg_attention_desc &a = *desc;
+    tg::AttnSeqs s;
+    int rc = check_seqs(ctx, a, true, s);
+    if (rc) return rc;
+    if (!attn_type(type)) return fail(ctx, TG_ERR_ARG, "type must be f32, f16 or bf16");
+    tg::RotaryArgs r;
+    if ((rc = check_rotary(ctx, rotary, a.d, r))) return rc;
+    const size_t nk = rows_span(k_new, a.q_rows, a.kv_heads, a.d), nv = rows_span(v_new, a.q_rows, a.kv_heads, a.d);
+    if ((rc = check_rows(ctx, "k_new", k_new, type, nk))) return rc;
+    if ((rc = check_rows(ctx, "v_new", v_new, type, nv))) return rc;
+    const size_t ks = rows_span(a.k, a.page, a.kv_heads, a.d), vs = rows_span(a.v, a.page, a.kv_heads, a.d);
+    if (!rows_distinct(a.k, a.page, a.kv_heads, a.d) || !rows_distinct(a.v, a.page, a.kv_heads, a.d) ||
+        (a.pages > 1 && (a.k_page < ks || a.v_page < vs)))
+        return fail(ctx, TG_ERR_SHAPE, "the cache's strides put two rows in one place");
+    const size_t size = type_bytes(a.type), from = type_bytes(type);
+    const size_t kc = rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page) * size;
+    const size_t vc = rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page) * size;
+    if (ranges_overlap(a.k.p, kc, k_new.p, nk * from) || ranges_overlap(a.k.p, kc, v_new.p, nv * from) ||
+        ranges_overlap(a.v.p, vc, k_new.p, nk * from) || ranges_overlap(a.v.p, vc, v_new.p, nv * from))
+        return fail(ctx, TG_ERR_ARG, "the new rows must not overlap the cache");
+    if (!ctx) return TG_ERR_NULL;
+    if (s.batch == 0 || s.longest == 0 || s.pages == 0 || s.width == 0) return TG_OK;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    TG_HIP(ctx, tg::launch_append(k_new.p, (int64_t)k_new.ld, (int64_t)k_new.hs, v_new.p, (int64_t)v_new.ld,
+                                  (int64_t)v_new.hs, type, const_cast<void *>(a.k.p), (int64_t)a.k.ld,
+                                  (int64_t)a.k.hs, (int64_t)a.k_page, const_cast<void *>(a.v.p), (int64_t)a.v.ld,
+                                  (int64_t)a.v.hs, (int64_t)a.v_page, a.type, (int)a.kv_heads, (int)a.d, s, r,
+                                  ctx->stream));
     return TG_OK;
 }
 

@@ -317,6 +317,59 @@ hipError_t launch_exact_rows(const float *a, size_t lda, size_t m, const DeviceW
 hipError_t launch_rowmajor(const float *a, size_t lda, size_t m, size_t k, const float *b, size_t ldb, size_t n,
                            float *c, size_t ldc, const EpiArgs &epi, hipStream_t s);
 
+// Attention and its neighbours (kernels_attn.hip, kernels_rotary.hip). Strides are in elements; the
+// values of a row's head are contiguous. Lengths and tables live in device memory, so kernels clamp
+// what they read of them to the sizes below, which the host has checked against the buffers.
+struct AttnSeqs {
+    int batch;            // sequences
+    int q_rows, longest;  // query rows in all; the most rows of one sequence that a call works on
+    int k_rows;           // key rows in all (contiguous keys)
+    const int32_t *q_starts, *k_starts;  // batch + 1 row numbers each, or null: equal lengths
+    // Paged keys: key j of sequence b is row j % page of page tables[b ldt + j / page].
+    const int32_t *tables, *lengths;
+    int64_t ldt;
+    int width, page, pages;  // table entries per sequence, rows per page, pages of the cache
+};
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    void *out;
+    int64_t ldq, hsq, ldk, hsk, ldv, hsv, ldo, hso;
+    int64_t psk, psv;  // page strides of k and v
+    uint32_t type;     // Precision: F32, F16 or BF16
+    int heads, kv_heads, d;
+    float scale, cap;            // cap 0: none
+    int32_t left, right;         // the window's keys before and after a query; negative: no limit
+    const float *slopes, *table; // per head; heads x (2 table_span + 1); null: none
+    int table_span;
+    const float *rel, *rel_u, *rel_v;  // position rows (2 rel_span + 1), ldrel apart, heads hsrel apart
+    int64_t ldrel, hsrel;              // hsrel 0: one set of rows for all heads
+    int rel_span;
+    const int32_t *prefix, *q_docs, *k_docs;
+    AttnSeqs seqs;
+    void *work;        // split partials, or null
+    size_t work_bytes;
+};
+hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
+// Bytes with which launch_attention splits the keys of sequences of up to max_keys keys.
+size_t attention_work_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t max_keys);
+
+// Rotary positions: turns holds, per pair, 1 / (2 pi) of its angle per position, in 64 bits.
+struct RotaryArgs {
+    const double *turns;  // null: no rotation
+    int dim;              // values rotated at the front of each head, even
+    int interleaved;      // pairs (2 i, 2 i + 1), or else (i, i + dim / 2)
+    float amplitude;      // factor of the rotated values
+};
+hipError_t launch_rotary(const void *x, uint32_t type, int64_t ldx, int64_t hsx, void *out, uint32_t out_type,
+                         int64_t ldo, int64_t hso, size_t rows, int heads, int d, const int32_t *positions,
+                         int64_t start, const RotaryArgs &r, hipStream_t s);
+// The last rows of each sequence (positions lengths[b] - its rows and on) into their pages.
+hipError_t launch_append(const void *k, int64_t ldk, int64_t hsk, const void *v, int64_t ldv, int64_t hsv,
+                         uint32_t type, void *ck, int64_t ldck, int64_t hsck, int64_t psk, void *cv, int64_t ldcv,
+                         int64_t hscv, int64_t psv, uint32_t cache_type, int heads, int d, const AttnSeqs &q,
+                         const RotaryArgs &r, hipStream_t s);
+
 // The greedy TDT decode (kernels_tdt.hip). The control block lives in device memory; the host
 // writes it before a decode and reads it between batches of steps.
 constexpr int TDT_ROWS = 16;            // most frames the joint scores per step; rows of a prediction

@@ -249,6 +249,7 @@ class Kernels:
         if rc != 0:
             raise TelmoError(rc, f"no gfx950 context on device {device}")
         self._ctx = ctx
+        self.device = device
         self.set_mode(mode)
 
     def set_mode(self, mode: int) -> None:
