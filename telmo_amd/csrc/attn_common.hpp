@@ -65,7 +65,7 @@ __host__ __device__ inline AttnSpan span_of(const AttnSeqs &s, int b) {
     if (s.tables) {
         const int64_t held = (int64_t)s.width * s.page;
         r.k0 = 0;
-        r.nk = clamp_to(s.lengths[b], 0, held < INT32_MAX ? (int)held : INT32_MAX);
+        r.nk = s.pages ? clamp_to(s.lengths[b], 0, held < INT32_MAX ? (int)held : INT32_MAX) : 0;
     } else if (s.k_starts) {
         r.k0 = clamp_to(s.k_starts[b], 0, s.k_rows);
         r.nk = clamp_to(s.k_starts[b + 1], r.k0, s.k_rows) - r.k0;
@@ -94,6 +94,126 @@ __host__ __device__ inline AttnWindow window_of(int i, int nk, int32_t left, int
     w.hi = hi < 0 ? 0 : hi > nk ? nk : (int)hi;
     w.prefix = clamp_to(prefix, 0, nk);
     return w;
+}
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+// tanh to f32's accuracy: an odd polynomial below 0.3 (Taylor's, off by less than 2^-24 of x there), past it
+// 1 - 2 / (e^2x + 1), whose absolute error of 2^-23 is relative to at least 0.29.
+__device__ __forceinline__ float tanh_f32(float x) {
+    const float a = fabsf(x), q = x * x;
+    const float big = __builtin_copysignf(1.0f - 2.0f / (exp2f(2.0f * LOG2E * a) + 1.0f), x);
+    float p = -1382.0f / 155925.0f;
+    p = __builtin_fmaf(p, q, 62.0f / 2835.0f);
+    p = __builtin_fmaf(p, q, -17.0f / 315.0f);
+    p = __builtin_fmaf(p, q, 2.0f / 15.0f);
+    p = __builtin_fmaf(p, q, -1.0f / 3.0f);
+    return a < 0.3f ? __builtin_fmaf(x * q, p, x) : big;
+}
+// tanh to 2^-22 absolutely, with the hardware's reciprocal: for 16-bit rows, whose weights keep less.
+__device__ __forceinline__ float tanh_fast(float x) {
+    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * x) + 1.0f);
+}
+
+// A product's score of head h at the distance key - query, with what the call does to scores.
+template <bool FAST>
+__device__ __forceinline__ float score_of(const AttnArgs &a, float dot, int h, float slope, int distance) {
+    float s = dot * a.scale;
+    if (a.cap > 0.0f) s = a.cap * (FAST ? tanh_fast(s / a.cap) : tanh_f32(s / a.cap));
+    if (a.slopes) s -= slope * fabsf((float)distance);
+    if (a.table)
+        s += a.table[(int64_t)h * (2 * a.table_span + 1) + clamp_to(distance, -a.table_span, a.table_span) +
+                     a.table_span];
+    return s;
+}
+
+// Row r of sequence b, head h, by one wavefront from the definition: a lane scores one key of 64 at a time,
+// then the wavefront adds the weighted value rows of the keys that are shown, and of no others. The tile
+// kernels multiply hidden keys' values by weights of zero, which makes a NaN of a NaN or an infinity: rows that
+// come out of them not finite are computed again by this, slowly.
+template <typename T>
+__device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
+    const AttnSpan sp = span_of(a.seqs, b);
+    const int64_t row = sp.q0 + r;
+    const int kvh = h / (a.heads / a.kv_heads), i = sp.shift() + r;
+    const T *q = static_cast<const T *>(a.q) + row * a.ldq + h * a.hsq;
+    const AttnWindow win = window_of(i, sp.nk, a.left, a.right, a.prefix ? a.prefix[b] : 0);
+    const int doc = a.q_docs ? a.q_docs[row] : 0;
+    const float slope = a.slopes ? a.slopes[h] : 0.0f;
+    float m = -INFINITY, l = 0.0f, acc[4] = {};
+    for (int j0 = 0; j0 < sp.nk; j0 += 64) {
+        const int j = j0 + lane;
+        bool shown = j < sp.nk && win.has(j);
+        int64_t kat = 0, vat = 0;
+        if (shown) {
+            if (a.seqs.tables) {
+                const int p = page_of(a.seqs, b, j);
+                shown = p >= 0;
+                kat = p * a.psk + (j % a.seqs.page) * a.ldk;
+                vat = p * a.psv + (j % a.seqs.page) * a.ldv;
+            } else {
+                kat = (int64_t)(sp.k0 + j) * a.ldk;
+                vat = (int64_t)(sp.k0 + j) * a.ldv;
+                if (a.q_docs) shown = doc >= 0 && a.k_docs[sp.k0 + j] == doc;
+            }
+        }
+        float s = -INFINITY;
+        if (shown) {
+            const T *k = static_cast<const T *>(a.k) + kat + kvh * a.hsk;
+            float dot = 0.0f;
+            for (int c = 0; c < a.d; c++)
+                dot = __builtin_fmaf(to_f32(q[c]) + (a.rel_u ? a.rel_u[h * a.d + c] : 0.0f), to_f32(k[c]), dot);
+            if (a.rel) {
+                const float *rr = a.rel + (clamp_to(j - i, -a.rel_span, a.rel_span) + a.rel_span) * a.ldrel + h * a.hsrel;
+                float term = 0.0f;
+                for (int c = 0; c < a.d; c++)
+                    term = __builtin_fmaf(to_f32(q[c]) + (a.rel_v ? a.rel_v[h * a.d + c] : 0.0f), rr[c], term);
+                dot += term;
+            }
+            s = score_of<false>(a, dot, h, slope, j - i);
+            shown = s != -INFINITY;
+        }
+        unsigned long long live = __ballot(shown);
+        if (!live) continue;
+        float top = s;
+        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
+        const float p = shown ? expf(s - base) : 0.0f;
+        const float fade = expf(m - base);
+        l = l * fade + p;
+        for (int e = 0; e < 4; e++) acc[e] *= fade;
+        while (live) {
+            const int t = __builtin_ctzll(live);
+            live &= live - 1;
+            const float w = __shfl(p, t);
+            const T *v = static_cast<const T *>(a.v) + __shfl(vat, t) + kvh * a.hsv;
+            for (int e = 0; e < 4; e++)
+                if (e * 64 + lane < a.d) acc[e] = __builtin_fmaf(w, to_f32(v[e * 64 + lane]), acc[e]);
+        }
+        m = mn;
+    }
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    T *out = static_cast<T *>(a.out) + row * a.ldo + h * a.hso;
+    for (int e = 0; e < 4; e++)
+        if (e * 64 + lane < a.d) out[e * 64 + lane] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+}
+
+// The parts of a call that splits its keys: per part, query row and head the score maximum, the sum of
+// weights and the unnormalised output, in f32.
+struct AttnParts {
+    float *top, *sum, *out;  // [parts][rows x heads], [..], [parts][rows x heads][d]
+    int parts;
+    size_t pairs;  // rows x heads
+};
+inline size_t part_bytes(size_t pairs, size_t d) { return pairs * (d + 2) * sizeof(float); }
+inline AttnParts parts_of(const AttnArgs &a, int parts) {
+    AttnParts p;
+    p.parts = parts;
+    p.pairs = (size_t)a.seqs.q_rows * a.heads;
+    p.out = static_cast<float *>(a.work);
+    p.top = p.out + (size_t)parts * p.pairs * a.d;
+    p.sum = p.top + (size_t)parts * p.pairs;
+    return p;
 }
 
 }  // namespace tg

@@ -1,0 +1,14 @@
+// The attention launchers behind launch_attention.
+#pragma once
+
+#include "tg_internal.hpp"
+
+namespace tg {
+
+// Workgroups of 256 threads that a grid holds.
+constexpr size_t MAX_ATTN_BLOCKS = ((size_t)1 << 32) / 256 - 1;
+
+// 16-bit rows; the keys in `splits` parts (a.work holds them) where that is more than one.
+hipError_t launch_attention16(const AttnArgs &a, int splits, hipStream_t s);
+
+}  // namespace tg

@@ -7,8 +7,10 @@
 // window or prefix, in its document. A query that is shown nothing gets zeros.
 //
 // Statistics and sums are held in f32: one pass over the keys carries the running maximum m, the sum of
-// exp(s - m) and the unnormalised output, both rescaled where m grows.
+// exp(s - m) and the unnormalised output, both rescaled where m grows. Long keys of few rows are split over
+// workgroups and the parts joined by a second kernel, in their order.
 #include "attn_common.hpp"
+#include "attn_launch.hpp"
 
 namespace tg {
 
@@ -16,113 +18,93 @@ namespace {
 
 constexpr int ROW_WAVES = 4;
 
-// One wavefront per query row and head: a lane scores one key of 64 at a time, then the wavefront adds
-// the 64 weighted value rows, a lane holding every 64th value of the output.
-template <typename T, int DMAX>
+template <typename T>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_rows_kernel(const AttnArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int b = blockIdx.z, h = blockIdx.y, r = blockIdx.x * ROW_WAVES + wave;
+    const int b = blockIdx.z, r = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
+    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<T>(a, b, blockIdx.y, r, threadIdx.x & 63);
+}
+
+// The parts of a row and head, joined by one wavefront: with M the largest maximum, the sums and outputs of
+// part p count e^(m_p - M) times.
+template <typename T>
+__global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArgs a, const AttnParts parts) {
+    const int lane = threadIdx.x & 63, b = blockIdx.z, h = blockIdx.y, r = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
     const AttnSpan sp = span_of(a.seqs, b);
-    __shared__ float qs[ROW_WAVES][2][DMAX];
-    if (r >= sp.nq) return;
-    const int64_t row = sp.q0 + r;
-    const int kvh = h / (a.heads / a.kv_heads), i = sp.shift() + r;
-    const T *q = static_cast<const T *>(a.q) + row * a.ldq + h * a.hsq;
-    float *qu = qs[wave][0], *qw = qs[wave][1];
-    for (int c = lane; c < a.d; c += 64) {
-        const float x = to_f32(q[c]);
-        qu[c] = a.rel_u ? x + a.rel_u[h * a.d + c] : x;
-        qw[c] = a.rel_v ? x + a.rel_v[h * a.d + c] : x;
+    if (r >= sp.nq || r >= a.seqs.longest) return;
+    const size_t at = (size_t)(sp.q0 + r) * a.heads + h;
+    float m = -INFINITY;
+    for (int p = 0; p < parts.parts; p++) m = fmaxf(m, parts.top[p * parts.pairs + at]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f, acc[4] = {};
+    for (int p = 0; p < parts.parts; p++) {
+        const size_t from = p * parts.pairs + at;
+        const float w = exp2f((parts.top[from] - base) * LOG2E), sum = parts.sum[from];
+        if (sum == 0.0f) continue;  // no key of this part was shown
+        l = __builtin_fmaf(w, sum, l);
+        for (int e = 0; e < 4; e++)
+            if (e * 64 + lane < a.d) acc[e] = __builtin_fmaf(w, parts.out[from * a.d + e * 64 + lane], acc[e]);
     }
-    const AttnWindow win = window_of(i, sp.nk, a.left, a.right, a.prefix ? a.prefix[b] : 0);
-    const int doc = a.q_docs ? a.q_docs[row] : 0;
-    float m = -INFINITY, l = 0.0f, acc[DMAX / 64] = {};
-    for (int j0 = 0; j0 < sp.nk; j0 += 64) {
-        const int j = j0 + lane;
-        bool shown = j < sp.nk && win.has(j);
-        int64_t kat = 0, vat = 0;
-        if (shown) {
-            if (a.seqs.tables) {
-                const int p = page_of(a.seqs, b, j);
-                shown = p >= 0;
-                kat = p * a.psk + (j % a.seqs.page) * a.ldk;
-                vat = p * a.psv + (j % a.seqs.page) * a.ldv;
-            } else {
-                kat = (int64_t)(sp.k0 + j) * a.ldk;
-                vat = (int64_t)(sp.k0 + j) * a.ldv;
-                if (a.q_docs) shown = doc >= 0 && a.k_docs[sp.k0 + j] == doc;
-            }
+    T *out = static_cast<T *>(a.out) + (int64_t)(sp.q0 + r) * a.ldo + h * a.hso;
+    bool sound = true;
+    for (int e = 0; e < 4; e++)
+        if (e * 64 + lane < a.d) {
+            const float v = l == 0.0f ? 0.0f : acc[e] / l;
+            sound = sound && v - v == 0.0f;
+            out[e * 64 + lane] = (T)v;
         }
-        float s = -INFINITY;
-        if (shown) {
-            const T *k = static_cast<const T *>(a.k) + kat + kvh * a.hsk;
-            float dot = 0.0f;
-            for (int c = 0; c < a.d; c += 8) {
-                float x[8];
-                load8(k + c, x);
-                for (int e = 0; e < 8; e++) dot = __builtin_fmaf(qu[c + e], x[e], dot);
-            }
-            if (a.rel) {
-                const int at = clamp_to(j - i, -a.rel_span, a.rel_span) + a.rel_span;
-                const float *rr = a.rel + at * a.ldrel + h * a.hsrel;
-                float term = 0.0f;
-                for (int c = 0; c < a.d; c++) term = __builtin_fmaf(qw[c], rr[c], term);
-                dot += term;
-            }
-            s = dot * a.scale;
-            if (a.cap > 0.0f) s = a.cap * tanhf(s / a.cap);
-            if (a.slopes) s -= a.slopes[h] * fabsf((float)(j - i));
-            if (a.table)
-                s += a.table[(int64_t)h * (2 * a.table_span + 1) + clamp_to(j - i, -a.table_span, a.table_span) +
-                             a.table_span];
-        }
-        unsigned long long live = __ballot(shown);
-        if (!live) continue;
-        float top = s;
-        for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-        const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.0f : mn;
-        const float p = shown ? expf(s - base) : 0.0f;
-        const float fade = expf(m - base);
-        l = l * fade + p;
-        for (int e = 0; e < DMAX / 64; e++) acc[e] *= fade;
-        while (live) {
-            const int t = __builtin_ctzll(live);
-            live &= live - 1;
-            const float w = __shfl(p, t);
-            const T *v = static_cast<const T *>(a.v) + __shfl(vat, t) + kvh * a.hsv;
-            for (int e = 0; e < DMAX / 64; e++)
-                if (e * 64 + lane < a.d) acc[e] = __builtin_fmaf(w, to_f32(v[e * 64 + lane]), acc[e]);
-        }
-        m = mn;
-    }
-    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
-    T *out = static_cast<T *>(a.out) + row * a.ldo + h * a.hso;
-    for (int e = 0; e < DMAX / 64; e++)
-        if (e * 64 + lane < a.d) out[e * 64 + lane] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+    if (!__all(sound) && l - l == 0.0f) attend_row<T>(a, b, h, r, lane);
 }
 
 template <typename T>
 hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)div_ceil((size_t)a.seqs.longest, ROW_WAVES), (unsigned)a.heads, (unsigned)a.seqs.batch);
-    if (a.d <= 64)
-        hipLaunchKernelGGL((attn_rows_kernel<T, 64>), grid, dim3(64 * ROW_WAVES), 0, s, a);
-    else if (a.d <= 128)
-        hipLaunchKernelGGL((attn_rows_kernel<T, 128>), grid, dim3(64 * ROW_WAVES), 0, s, a);
-    else
-        hipLaunchKernelGGL((attn_rows_kernel<T, 256>), grid, dim3(64 * ROW_WAVES), 0, s, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a);
     return hipGetLastError();
+}
+
+template <typename T>
+hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
+    const dim3 grid((unsigned)div_ceil((size_t)a.seqs.longest, ROW_WAVES), (unsigned)a.heads, (unsigned)a.seqs.batch);
+    hipLaunchKernelGGL((attn_join_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a, parts_of(a, splits));
+    return hipGetLastError();
+}
+
+constexpr size_t TARGET = 512;      // workgroups that fill the GPU: two on each of 256 CUs
+constexpr size_t LEAST_KEYS = 256;  // a part works on at least as many
+constexpr size_t MOST_PARTS = 64;
+
+// Parts for workgroups of `wgs` without splitting, over up to `keys` keys.
+size_t parts_for(size_t wgs, size_t keys) {
+    size_t n = TARGET / (wgs ? wgs : 1);
+    if (n > keys / LEAST_KEYS) n = keys / LEAST_KEYS;
+    return n < 1 ? 1 : n > MOST_PARTS ? MOST_PARTS : n;
 }
 
 }  // namespace
 
-size_t attention_work_bytes(size_t, size_t, size_t, size_t, size_t, size_t) { return 0; }
+size_t attention_work_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys) {
+    // The fewest workgroups that calls of these sizes have give the most parts.
+    const size_t tiles = div_ceil(rows * (heads / kv_heads), 128);
+    const size_t n = parts_for(kv_heads * (tiles > batch ? tiles : batch), keys);
+    return n > 1 ? n * part_bytes(rows * heads, d) : 0;
+}
 
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
-    switch (a.type) {
-        case F16: return launch_rows<_Float16>(a, s);
-        case BF16: return launch_rows<__bf16>(a, s);
-        default: return launch_rows<float>(a, s);
+    if (a.type == F32) return launch_rows<float>(a, s);
+    const size_t group = a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, 128);
+    size_t keys = a.seqs.tables ? (size_t)a.seqs.width * a.seqs.page
+                                : (size_t)(a.seqs.k_starts ? a.seqs.k_rows : a.seqs.k_rows / a.seqs.batch);
+    if (a.left >= 0 && a.right >= 0 && !a.prefix) {  // no row tile reaches further than its window
+        const size_t reach = (size_t)a.left + a.right + 1 + 128;
+        keys = keys < reach ? keys : reach;
     }
+    size_t n = parts_for(tiles * a.kv_heads * a.seqs.batch, keys);
+    const size_t bytes = part_bytes((size_t)a.seqs.q_rows * a.heads, a.d);
+    if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
+    if (n < 1) n = 1;
+    const hipError_t e = launch_attention16(a, (int)n, s);
+    if (e != hipSuccess || n == 1) return e;
+    return a.type == F16 ? launch_join<_Float16>(a, (int)n, s) : launch_join<__bf16>(a, (int)n, s);
 }
 
 }  // namespace tg

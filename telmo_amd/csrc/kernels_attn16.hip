@@ -1,0 +1,354 @@
+// Attention over 16-bit rows on the matrix cores, tiles of 128 query rows by 64 keys.
+//
+// The query heads that share a key head are rows of one matrix: row g r + x is head x of the group in query
+// row r. A workgroup takes 128 of them, a wavefront 32, and walks the keys 64 at a time through LDS. The
+// products are S' = K Q' and O' = V' P', 32 x 32 x 16 each: in S' a lane holds the scores of one query (its
+// column) with 32 of the 64 keys, so the softmax is arithmetic in the lane's registers and one exchange with
+// the lane of the other half, and the same registers, rounded to 16 bits, are the operand P' of the second
+// product, whose keys are taken in the order in which the lanes hold them. V' comes from LDS by transposing
+// reads. The weights are rounded once to the rows' type, f16's scaled by 2^8 (as is their sum) so that weights
+// down to 2^-22 of the largest are normal numbers.
+#include "attn_common.hpp"
+#include "attn_launch.hpp"
+
+namespace tg {
+
+namespace {
+
+constexpr int THREADS = 256, TILE_Q = 128, TILE_K = 64;
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+template <typename T>
+struct Half;
+template <>
+struct Half<_Float16> {
+    typedef f16x8 v8;
+    static constexpr float shift = 8.0f;
+    static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Half<__bf16> {
+    typedef bf16x8 v8;
+    static constexpr float shift = 0.0f;
+    static __device__ __forceinline__ f32x16 mfma(v8 a, v8 b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+// The greater (the sum) of a lane's value and that of the lane 32 away.
+__device__ __forceinline__ float max_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Where the 16-byte chunk c of a tile's row lies. K rows are read a chunk of 32 rows at a time and V rows four
+// rows of 64 bytes at a time: either way the chunks that one read touches fall on different banks.
+template <int CHUNKS>
+__device__ __forceinline__ int k_place(int row, int c) {
+    return row * CHUNKS + (c ^ (CHUNKS == 8 ? (row >> 1) & 7 : row & 15));
+}
+template <int CHUNKS>
+__device__ __forceinline__ int v_place(int row, int c) {
+    return row * CHUNKS + (c ^ (CHUNKS == 8 ? (row << 1) & 4 : (row & 3) << 2));
+}
+
+// The key tiles that a range of query positions needs: those of the prefix, then those of the window.
+struct Tiles {
+    int front, start, count;
+    __device__ __forceinline__ int at(int n) const { return (n < front ? n : start + n - front) * TILE_K; }
+};
+__device__ __forceinline__ Tiles tiles_of(const AttnWindow &first, const AttnWindow &last) {
+    Tiles t;
+    t.front = (first.prefix + TILE_K - 1) / TILE_K;
+    t.start = first.lo / TILE_K > t.front ? first.lo / TILE_K : t.front;
+    const int end = (last.hi + TILE_K - 1) / TILE_K;
+    t.count = t.front + (end > t.start ? end - t.start : 0);
+    return t;
+}
+
+// D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
+template <typename T, int D, bool PAGED, bool EXTRA>
+__global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnParts parts,
+                                                                              const int q_tiles, const int groups) {
+    typedef typename Half<T>::v8 v8;
+    constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
+    __shared__ __align__(16) T ks[TILE_K * D], vs[TILE_K * D];
+    __shared__ int marks[TILE_K];
+
+    // Workgroups go round the 8 XCDs in turn: those of one key head and part share an XCD and its L2, the
+    // rows with the most keys (the last ones of causal calls) first.
+    const int id = blockIdx.x, in_xcd = id / 8;
+    const int head_part = (in_xcd / q_tiles) * 8 + id % 8, tile = q_tiles - 1 - in_xcd % q_tiles;
+    if (head_part >= groups) return;
+    const int part = head_part % parts.parts, head_batch = head_part / parts.parts;
+    const int kvh = head_batch % a.kv_heads, b = head_batch / a.kv_heads;
+    const AttnSpan sp = span_of(a.seqs, b);
+    const int group = a.heads / a.kv_heads;
+    const int rows = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest);
+    const int64_t pairs = (int64_t)rows * group, pair0 = (int64_t)tile * TILE_Q;
+    if (pair0 >= pairs) return;
+
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    // The lane's query, and the first and last of the wavefront's and the workgroup's.
+    const int64_t pair = pair0 + wave * 32 + col;
+    const bool live = pair < pairs;
+    const int r = live ? (int)(pair / group) : 0, h = kvh * group + (live ? (int)(pair % group) : 0);
+    const int i = sp.shift() + r;
+    const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
+    const int64_t wave0 = pair0 + wave * 32, wave1 = wave0 + 31 < pairs - 1 ? wave0 + 31 : pairs - 1;
+    const int64_t pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
+    const auto window_at = [&](int64_t p) {
+        return window_of(sp.shift() + (int)(p / group), sp.nk, a.left, a.right, prefix);
+    };
+    const bool wave_live = wave0 < pairs;
+    const AttnWindow w_first = window_at(wave_live ? wave0 : 0), w_last = window_at(wave_live ? wave1 : 0);
+    const Tiles tiles = tiles_of(window_at(pair0), window_at(pair1));
+    const int n0 = (int)((int64_t)tiles.count * part / parts.parts);
+    const int n1 = (int)((int64_t)tiles.count * (part + 1) / parts.parts);
+
+    const int64_t row = (int64_t)sp.q0 + r;
+    const int doc = a.q_docs ? (live ? a.q_docs[row] : -1) : 0;
+    const float slope = EXTRA && a.slopes ? a.slopes[h] : 0.0f;
+
+    v8 qf[D / 16];
+    const T *q = static_cast<const T *>(a.q) + row * a.ldq + h * a.hsq;
+    for (int s = 0; s < D / 16; s++) {
+        const int c = s * 16 + half * 8;
+        qf[s] = live && c < a.d ? *reinterpret_cast<const v8 *>(q + c) : v8{};
+    }
+
+    // This thread's part of the tiles: rows row0 + u STEP, chunk c of each.
+    const int row0 = t / CHUNKS, c = t % CHUNKS;
+    const bool in_d = c * 8 < a.d;
+    const T *kp = static_cast<const T *>(a.k) + kvh * a.hsk + (in_d ? c * 8 : 0);
+    const T *vp = static_cast<const T *>(a.v) + kvh * a.hsv + (in_d ? c * 8 : 0);
+    u32x4 kr[PER], vr[PER];
+    int mark[PER];
+    const auto load = [&](int kb) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            int j = kb + row0 + u * STEP;
+            const bool in = j < sp.nk && in_d;
+            j = j < sp.nk ? j : sp.nk - 1;
+            int64_t kat, vat;
+            if (PAGED) {
+                const int p = page_of(a.seqs, b, j), s = j % a.seqs.page;
+                mark[u] = p < 0 ? -1 : 0;
+                kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
+                vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
+            } else {
+                kat = (int64_t)(sp.k0 + j) * a.ldk;
+                vat = (int64_t)(sp.k0 + j) * a.ldv;
+                if (EXTRA && a.q_docs) mark[u] = a.k_docs[sp.k0 + j];
+            }
+            kr[u] = *reinterpret_cast<const u32x4 *>(kp + kat);
+            vr[u] = *reinterpret_cast<const u32x4 *>(vp + vat);
+            if (!in) kr[u] = vr[u] = u32x4{};
+        }
+    };
+
+    f32x16 acc[D / 32] = {};
+    float m = -INFINITY, l = 0.0f;
+    const float mul = a.scale * LOG2E;
+    const bool marked = PAGED || (EXTRA && a.q_docs);
+
+    if (n0 < n1) load(tiles.at(n0));
+    for (int n = n0; n < n1; n++) {
+        const int kb = tiles.at(n);
+        __syncthreads();  // every wavefront has read the last tile
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int krow = row0 + u * STEP;
+            reinterpret_cast<u32x4 *>(ks)[k_place<CHUNKS>(krow, c)] = kr[u];
+            reinterpret_cast<u32x4 *>(vs)[v_place<CHUNKS>(krow, c)] = vr[u];
+            if (marked && c == 0) marks[krow] = mark[u];
+        }
+        __syncthreads();
+        if (n + 1 < n1) load(tiles.at(n + 1));
+
+        const bool none = !wave_live || ((kb + TILE_K <= w_first.lo || kb >= w_last.hi) && kb >= w_first.prefix);
+        if (none) continue;
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int e = 0; e < D / 16; e++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const v8 kf = reinterpret_cast<const v8 *>(ks)[k_place<CHUNKS>(x * 32 + col, e * 2 + half)];
+                s[x] = Half<T>::mfma(kf, qf[e], s[x]);
+            }
+
+        // Scores, and -infinity where the key is not shown.
+        const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
+        bool compare = false;  // marks decide key by key
+        if (marked) {
+            const int mk = marks[lane];
+            if (EXTRA && a.q_docs) {
+                const int first = __builtin_amdgcn_readfirstlane(mk);
+                compare = !__all(mk == first && doc == first) || first < 0;
+            } else {
+                compare = __any(mk < 0);
+            }
+        }
+        if (EXTRA) {
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int j = kb + x * 32 + 8 * (e / 4) + 4 * half + e % 4;
+                    s[x][e] = score_of<true>(a, s[x][e], h, slope, j - i);
+                }
+        }
+        if (!full) {
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int j = kb + x * 32 + 8 * (e / 4) + 4 * half + e % 4;
+                    if (!win.has(j)) s[x][e] = -INFINITY;
+                }
+        }
+        if (compare) {
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int mk = marks[x * 32 + 8 * (e / 4) + 4 * half + e % 4];
+                    if (mk < 0 || mk != doc) s[x][e] = -INFINITY;
+                }
+        }
+
+        float top = s[0][0];
+#pragma unroll
+        for (int e = 1; e < 32; e++) top = fmaxf(top, s[e / 16][e % 16]);
+        top = max_halves(top);
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float fade = m == -INFINITY ? 0.0f
+                                              : __builtin_amdgcn_exp2f(EXTRA ? (m - mn) * LOG2E : (m - mn) * mul);
+            l *= fade;
+#pragma unroll
+            for (int x = 0; x < D / 32; x++) acc[x] *= fade;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float off = Half<T>::shift - base * mul;
+        v8 pf[4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            f32x8 p;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = s[g / 2][(g % 2) * 8 + e];
+                // The difference first where a bias can be the type's lowest value: its multiple is infinite.
+                p[e] = __builtin_amdgcn_exp2f(EXTRA ? __builtin_fmaf(x - base, LOG2E, Half<T>::shift)
+                                                    : __builtin_fmaf(x, mul, off));
+                l += p[e];
+            }
+            pf[g] = __builtin_convertvector(p, v8);
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+#pragma unroll
+            for (int x = 0; x < D / 32; x++) {
+                // Columns 32 x + (lane % 32) of eight keys: two reads of four keys each, transposed by the read.
+                const int vrow = g * 16 + half * 4 + (lane & 15) / 4, vc = x * 32 + (lane >> 4 & 1) * 16 + lane % 4 * 4;
+                s16x4 lo, hi;
+                lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4 *)(vs + v_place<CHUNKS>(vrow, vc / 8) * 8 + vc % 8));
+                hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (__attribute__((address_space(3))) s16x4 *)(vs + v_place<CHUNKS>(vrow + 8, vc / 8) * 8 + vc % 8));
+                const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[x] = Half<T>::mfma(__builtin_bit_cast(v8, both), pf[g], acc[x]);
+            }
+    }
+
+    l = sum_halves(l);
+    if (parts.parts > 1) {
+        if (!live) return;
+        const size_t at = (size_t)part * parts.pairs + row * a.heads + h;
+        if (half == 0) {
+            parts.top[at] = EXTRA ? m : m * a.scale;
+            parts.sum[at] = l;
+        }
+        float *o = parts.out + at * a.d;
+#pragma unroll
+        for (int x = 0; x < D / 32; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int oc = x * 32 + 8 * e + 4 * half;
+                if (oc < a.d)
+                    *reinterpret_cast<f32x4 *>(o + oc) =
+                        f32x4{acc[x][4 * e], acc[x][4 * e + 1], acc[x][4 * e + 2], acc[x][4 * e + 3]};
+            }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *out = static_cast<T *>(a.out) + row * a.ldo + h * a.hso;
+    float worst = 0.0f;
+#pragma unroll
+    for (int x = 0; x < D / 32; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int oc = x * 32 + 8 * e + 4 * half;
+            T o[4];
+            for (int y = 0; y < 4; y++) {
+                const float v = acc[x][4 * e + y] * inv;
+                worst = fmaxf(worst, v - v == 0.0f ? 0.0f : 1.0f);
+                o[y] = (T)v;
+            }
+            if (live && oc < a.d) *reinterpret_cast<u32x2 *>(out + oc) = *reinterpret_cast<u32x2 *>(o);
+        }
+    // A NaN in the sum of weights comes from a shown score and is the result; one beside a sound sum may come
+    // from a hidden key's value.
+    unsigned long long again = __ballot(live && worst > 0.0f && l - l == 0.0f);
+    again = (again | again >> 32) & 0xffffffffull;
+    while (again) {
+        const int64_t p = wave0 + __builtin_ctzll(again);
+        again &= again - 1;
+        attend_row<T>(a, b, kvh * group + (int)(p % group), (int)(p / group), lane);
+    }
+}
+
+template <typename T, int D, bool PAGED, bool EXTRA>
+hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
+    const int group = a.heads / a.kv_heads;
+    const size_t q_tiles = div_ceil((size_t)a.seqs.longest * group, TILE_Q);
+    const size_t groups = (size_t)a.seqs.batch * a.kv_heads * splits, blocks = div_ceil(groups, 8) * 8 * q_tiles;
+    if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((attn_tile_kernel<T, D, PAGED, EXTRA>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a,
+                       parts_of(a, splits), (int)q_tiles, (int)groups);
+    return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_kind(const AttnArgs &a, int splits, hipStream_t s) {
+    const bool extra = a.cap > 0.0f || a.slopes || a.table || a.q_docs;
+    if (a.seqs.tables)
+        return extra ? launch_tile<T, D, true, true>(a, splits, s) : launch_tile<T, D, true, false>(a, splits, s);
+    return extra ? launch_tile<T, D, false, true>(a, splits, s) : launch_tile<T, D, false, false>(a, splits, s);
+}
+
+template <typename T>
+hipError_t launch_size(const AttnArgs &a, int splits, hipStream_t s) {
+    if (a.d <= 64) return launch_kind<T, 64>(a, splits, s);
+    if (a.d <= 128) return launch_kind<T, 128>(a, splits, s);
+    return launch_kind<T, 256>(a, splits, s);
+}
+
+}  // namespace
+
+hipError_t launch_attention16(const AttnArgs &a, int splits, hipStream_t s) {
+    return a.type == F16 ? launch_size<_Float16>(a, splits, s) : launch_size<__bf16>(a, splits, s);
+}
+
+}  // namespace tg
