@@ -11,4 +11,8 @@ constexpr size_t MAX_ATTN_BLOCKS = ((size_t)1 << 32) / 256 - 1;
 // 16-bit rows; the keys in `splits` parts (a.work holds them) where that is more than one.
 hipError_t launch_attention16(const AttnArgs &a, int splits, hipStream_t s);
 
+// f32 rows; with position rows only heads of up to 128 (attention32_fits).
+inline bool attention32_fits(const AttnArgs &a) { return !a.rel || a.d <= 128; }
+hipError_t launch_attention32(const AttnArgs &a, int splits, hipStream_t s);
+
 }  // namespace tg

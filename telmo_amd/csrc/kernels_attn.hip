@@ -18,10 +18,9 @@ namespace {
 
 constexpr int ROW_WAVES = 4;
 
-template <typename T>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_rows_kernel(const AttnArgs a) {
     const int b = blockIdx.z, r = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
-    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<T>(a, b, blockIdx.y, r, threadIdx.x & 63);
+    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<float>(a, b, blockIdx.y, r, threadIdx.x & 63);
 }
 
 // The parts of a row and head, joined by one wavefront: with M the largest maximum, the sums and outputs of
@@ -52,13 +51,13 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArg
             sound = sound && v - v == 0.0f;
             out[e * 64 + lane] = (T)v;
         }
-    if (!__all(sound) && l - l == 0.0f) attend_row<T>(a, b, h, r, lane);
+    // As the tile kernels do for rows that they finish themselves.
+    if (!__all(sound) && (sizeof(T) == 4 || l - l == 0.0f)) attend_row<T>(a, b, h, r, lane);
 }
 
-template <typename T>
 hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)div_ceil((size_t)a.seqs.longest, ROW_WAVES), (unsigned)a.heads, (unsigned)a.seqs.batch);
-    hipLaunchKernelGGL((attn_rows_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a);
+    hipLaunchKernelGGL(attn_rows_kernel, grid, dim3(64 * ROW_WAVES), 0, s, a);
     return hipGetLastError();
 }
 
@@ -90,21 +89,26 @@ size_t attention_work_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d
 }
 
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
-    if (a.type == F32) return launch_rows<float>(a, s);
-    const size_t group = a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, 128);
+    // LDS holds the blocks of position rows of heads of up to 128; longer ones take a wavefront per row.
+    if (a.type == F32 && !attention32_fits(a)) return launch_rows(a, s);
+    const size_t group = a.rel ? 1 : a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, 128);
     size_t keys = a.seqs.tables ? (size_t)a.seqs.width * a.seqs.page
                                 : (size_t)(a.seqs.k_starts ? a.seqs.k_rows : a.seqs.k_rows / a.seqs.batch);
     if (a.left >= 0 && a.right >= 0 && !a.prefix) {  // no row tile reaches further than its window
         const size_t reach = (size_t)a.left + a.right + 1 + 128;
         keys = keys < reach ? keys : reach;
     }
-    size_t n = parts_for(tiles * a.kv_heads * a.seqs.batch, keys);
+    size_t n = parts_for(tiles * (a.heads / group) * a.seqs.batch, keys);
     const size_t bytes = part_bytes((size_t)a.seqs.q_rows * a.heads, a.d);
     if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
     if (n < 1) n = 1;
-    const hipError_t e = launch_attention16(a, (int)n, s);
+    const hipError_t e = a.type == F32 ? launch_attention32(a, (int)n, s) : launch_attention16(a, (int)n, s);
     if (e != hipSuccess || n == 1) return e;
-    return a.type == F16 ? launch_join<_Float16>(a, (int)n, s) : launch_join<__bf16>(a, (int)n, s);
+    switch (a.type) {
+        case F16: return launch_join<_Float16>(a, (int)n, s);
+        case BF16: return launch_join<__bf16>(a, (int)n, s);
+        default: return launch_join<float>(a, (int)n, s);
+    }
 }
 
 }  // namespace tg

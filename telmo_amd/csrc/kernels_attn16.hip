@@ -8,18 +8,14 @@
 // product, whose keys are taken in the order in which the lanes hold them. V' comes from LDS by transposing
 // reads. The weights are rounded once to the rows' type, f16's scaled by 2^8 (as is their sum) so that weights
 // down to 2^-22 of the largest are normal numbers.
-#include "attn_common.hpp"
 #include "attn_launch.hpp"
+#include "attn_tile.hpp"
 
 namespace tg {
 
 namespace {
 
 constexpr int THREADS = 256, TILE_Q = 128, TILE_K = 64;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 template <typename T>
 struct Half;
@@ -40,41 +36,6 @@ struct Half<__bf16> {
     }
 };
 
-// The greater (the sum) of a lane's value and that of the lane 32 away.
-__device__ __forceinline__ float max_halves(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float sum_halves(float x) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
-// Where the 16-byte chunk c of a tile's row lies. K rows are read a chunk of 32 rows at a time and V rows four
-// rows of 64 bytes at a time: either way the chunks that one read touches fall on different banks.
-template <int CHUNKS>
-__device__ __forceinline__ int k_place(int row, int c) {
-    return row * CHUNKS + (c ^ (CHUNKS == 8 ? (row >> 1) & 7 : row & 15));
-}
-template <int CHUNKS>
-__device__ __forceinline__ int v_place(int row, int c) {
-    return row * CHUNKS + (c ^ (CHUNKS == 8 ? (row << 1) & 4 : (row & 3) << 2));
-}
-
-// The key tiles that a range of query positions needs: those of the prefix, then those of the window.
-struct Tiles {
-    int front, start, count;
-    __device__ __forceinline__ int at(int n) const { return (n < front ? n : start + n - front) * TILE_K; }
-};
-__device__ __forceinline__ Tiles tiles_of(const AttnWindow &first, const AttnWindow &last) {
-    Tiles t;
-    t.front = (first.prefix + TILE_K - 1) / TILE_K;
-    t.start = first.lo / TILE_K > t.front ? first.lo / TILE_K : t.front;
-    const int end = (last.hi + TILE_K - 1) / TILE_K;
-    t.count = t.front + (end > t.start ? end - t.start : 0);
-    return t;
-}
-
 // D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
 template <typename T, int D, bool PAGED, bool EXTRA>
 __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnParts parts,
@@ -84,18 +45,11 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     __shared__ __align__(16) T ks[TILE_K * D], vs[TILE_K * D];
     __shared__ int marks[TILE_K];
 
-    // Workgroups go round the 8 XCDs in turn: those of one key head and part share an XCD and its L2, the
-    // rows with the most keys (the last ones of causal calls) first.
-    const int id = blockIdx.x, in_xcd = id / 8;
-    const int head_part = (in_xcd / q_tiles) * 8 + id % 8, tile = q_tiles - 1 - in_xcd % q_tiles;
-    if (head_part >= groups) return;
-    const int part = head_part % parts.parts, head_batch = head_part / parts.parts;
-    const int kvh = head_batch % a.kv_heads, b = head_batch / a.kv_heads;
-    const AttnSpan sp = span_of(a.seqs, b);
-    const int group = a.heads / a.kv_heads;
-    const int rows = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest);
-    const int64_t pairs = (int64_t)rows * group, pair0 = (int64_t)tile * TILE_Q;
-    if (pair0 >= pairs) return;
+    Place at;
+    if (!at.find(a, parts.parts, q_tiles, groups, a.kv_heads, TILE_Q)) return;
+    const int part = at.part, kvh = at.head, b = at.b, group = at.group;
+    const AttnSpan sp = at.sp;
+    const int64_t pairs = at.pairs, pair0 = at.pair0;
 
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
     const int prefix = a.prefix ? a.prefix[b] : 0;
@@ -112,7 +66,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     };
     const bool wave_live = wave0 < pairs;
     const AttnWindow w_first = window_at(wave_live ? wave0 : 0), w_last = window_at(wave_live ? wave1 : 0);
-    const Tiles tiles = tiles_of(window_at(pair0), window_at(pair1));
+    const Tiles<TILE_K> tiles(window_at(pair0), window_at(pair1));
     const int n0 = (int)((int64_t)tiles.count * part / parts.parts);
     const int n1 = (int)((int64_t)tiles.count * (part + 1) / parts.parts);
 
@@ -259,28 +213,19 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
 #pragma unroll
         for (int g = 0; g < 4; g++)
 #pragma unroll
-            for (int x = 0; x < D / 32; x++) {
-                // Columns 32 x + (lane % 32) of eight keys: two reads of four keys each, transposed by the read.
-                const int vrow = g * 16 + half * 4 + (lane & 15) / 4, vc = x * 32 + (lane >> 4 & 1) * 16 + lane % 4 * 4;
-                s16x4 lo, hi;
-                lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *)(vs + v_place<CHUNKS>(vrow, vc / 8) * 8 + vc % 8));
-                hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) s16x4 *)(vs + v_place<CHUNKS>(vrow + 8, vc / 8) * 8 + vc % 8));
-                const s16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[x] = Half<T>::mfma(__builtin_bit_cast(v8, both), pf[g], acc[x]);
-            }
+            for (int x = 0; x < D / 32; x++)
+                acc[x] = Half<T>::mfma(__builtin_bit_cast(v8, v_fragment<CHUNKS>(vs, g * 16, x, lane)), pf[g], acc[x]);
     }
 
     l = sum_halves(l);
     if (parts.parts > 1) {
         if (!live) return;
-        const size_t at = (size_t)part * parts.pairs + row * a.heads + h;
+        const size_t to = (size_t)part * parts.pairs + row * a.heads + h;
         if (half == 0) {
-            parts.top[at] = EXTRA ? m : m * a.scale;
-            parts.sum[at] = l;
+            parts.top[to] = EXTRA ? m : m * a.scale;
+            parts.sum[to] = l;
         }
-        float *o = parts.out + at * a.d;
+        float *o = parts.out + to * a.d;
 #pragma unroll
         for (int x = 0; x < D / 32; x++)
 #pragma unroll

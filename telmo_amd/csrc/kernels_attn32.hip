@@ -1,0 +1,457 @@
+// Attention over f32 rows on the matrix cores, tiles of 128 query rows by 32 keys, to f32's accuracy.
+//
+// The f32 matrix instructions run at an eighth of the rate that the 16-bit ones have for the same shape and k,
+// so each f32 operand is held as a sum of 16-bit ones. For the scores a row x of q, k or the position rows is
+// scaled by a power of two to |x| < 2^15 and held as h + l in f16, 22 bits of it; three products h h', h l' and
+// l h' leave out less than 2^-22 of each term. The weights and the values, which may not share a scale (a
+// value is weighted by other rows' weights), are held as three bf16 each, 24 bits, and six products leave out
+// less than 2^-23. The 32 x 32 x 16 products then cost 3 and 6 instructions in the place of 8 f32 ones that
+// take 8 times as long in all; layout and softmax are those of the 16-bit kernel.
+//
+// Position rows: with T[c, i] = (q_i + w) r_c, the score of key j needs T[j - i, i]. In a tile of 32 queries by
+// 32 keys the distances j - i are those of two blocks of 32 position rows, and the second one is the first
+// of the next tile: each tile adds one product of 32 rows, kept in LDS as [query][64 distances], a ring of
+// two blocks, from which a lane reads its own diagonal. The blocks of the workgroup's wavefronts, whose queries
+// are 32 apart, are the same ones tiles apart: LDS holds the last four. (q + w) r = (q + u) r + (w - u) r, the
+// second part a number per position row, so one copy of the queries serves both products.
+#include "attn_launch.hpp"
+#include "attn_tile.hpp"
+
+namespace tg {
+
+namespace {
+
+constexpr int THREADS = 256, TILE_Q = 128, TILE_K = 32, RING = 4;
+
+// The power of two that brings a row whose largest magnitude is `top` below 2^15, and its inverse. Both stay
+// normal numbers: a row of subnormals is scaled less, which loses nothing that f32 sums would keep.
+struct Scale {
+    float by, back;
+};
+__device__ __forceinline__ Scale scale_for(float top) {
+    const int e = (int)(__float_as_uint(top) >> 23), s = 268 - e < 253 ? 268 - e : 253;
+    return Scale{__uint_as_float((uint32_t)s << 23), __uint_as_float((uint32_t)(254 - s) << 23)};
+}
+
+// Eight values as sums of two f16 (three bf16) ones.
+__device__ __forceinline__ void split2(const float *x, f16x8 &hi, f16x8 &lo) {
+    f32x8 v;
+    for (int e = 0; e < 8; e++) v[e] = x[e];
+    hi = __builtin_convertvector(v, f16x8);
+    lo = __builtin_convertvector(v - __builtin_convertvector(hi, f32x8), f16x8);
+}
+__device__ __forceinline__ void split3(const f32x8 v, bf16x8 &hi, bf16x8 &mid, bf16x8 &lo) {
+    hi = __builtin_convertvector(v, bf16x8);
+    const f32x8 r = v - __builtin_convertvector(hi, f32x8);
+    mid = __builtin_convertvector(r, bf16x8);
+    lo = __builtin_convertvector(r - __builtin_convertvector(mid, f32x8), bf16x8);
+}
+
+__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// Reductions over the CHUNKS neighbouring lanes that hold one row: quads, halves and whole rows of 16 lanes
+// by the lane permutations that arithmetic instructions carry.
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+template <int CHUNKS>
+__device__ __forceinline__ float row_max(float x) {
+    x = fmaxf(x, lane_move<0xb1>(x));   // lanes 1 0 3 2
+    x = fmaxf(x, lane_move<0x4e>(x));   // lanes 2 3 0 1
+    x = fmaxf(x, lane_move<0x141>(x));  // mirrored in 8 lanes
+    if (CHUNKS > 8) x = fmaxf(x, lane_move<0x140>(x));  // mirrored in 16
+    if (CHUNKS > 16) x = fmaxf(x, __shfl_xor(x, 16));
+    return x;
+}
+template <int CHUNKS>
+__device__ __forceinline__ float row_sum(float x) {
+    x += lane_move<0xb1>(x);
+    x += lane_move<0x4e>(x);
+    x += lane_move<0x141>(x);
+    if (CHUNKS > 8) x += lane_move<0x140>(x);
+    if (CHUNKS > 16) x += __shfl_xor(x, 16);
+    return x;
+}
+
+template <int D, bool REL>
+struct Shared {
+    f16x8 k[2][TILE_K * D / 8];
+    bf16x8 v[3][TILE_K * D / 8];
+    float k_back[TILE_K];
+    int marks[TILE_K];
+    f16x8 r[REL ? RING : 1][2][REL ? TILE_K * D / 8 : 1];
+    float r_back[REL ? RING : 1][TILE_K], r_add[REL ? RING : 1][TILE_K];
+    float terms[REL ? 4 : 1][REL ? 32 * 64 : 1];  // per wavefront [query][64 distances], turned by 4 per query
+};
+
+// D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
+template <int D, bool PAGED, bool EXTRA, bool REL>
+__global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_kernel(
+    const AttnArgs a, const AttnParts parts, const int q_tiles, const int groups) {
+    constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
+    __shared__ __align__(16) Shared<D, REL> sh;
+
+    Place at;
+    if (!at.find(a, parts.parts, q_tiles, groups, REL ? a.heads : a.kv_heads, TILE_Q)) return;
+    const int part = at.part, b = at.b, group = at.group;
+    const int kvh = REL ? at.head / (a.heads / a.kv_heads) : at.head;
+    const AttnSpan sp = at.sp;
+    const int64_t pairs = at.pairs, pair0 = at.pair0;
+
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    const int64_t pair = pair0 + wave * 32 + col;
+    const bool live = pair < pairs;
+    const int r = live ? (int)(pair / group) : 0, h = at.head * group + (live ? (int)(pair % group) : 0);
+    const int i = sp.shift() + r;
+    const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
+    const int64_t wave0 = pair0 + wave * 32, wave1 = wave0 + 31 < pairs - 1 ? wave0 + 31 : pairs - 1;
+    const int64_t pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
+    const auto window_at = [&](int64_t p) {
+        return window_of(sp.shift() + (int)(p / group), sp.nk, a.left, a.right, prefix);
+    };
+    const bool wave_live = wave0 < pairs;
+    const AttnWindow w_first = window_at(wave_live ? wave0 : 0), w_last = window_at(wave_live ? wave1 : 0);
+    const Tiles<TILE_K> tiles(window_at(pair0), window_at(pair1));
+    const int n0 = (int)((int64_t)tiles.count * part / parts.parts);
+    const int n1 = (int)((int64_t)tiles.count * (part + 1) / parts.parts);
+
+    const int64_t row = (int64_t)sp.q0 + r;
+    const int doc = a.q_docs ? (live ? a.q_docs[row] : -1) : 0;
+    const float slope = EXTRA && a.slopes ? a.slopes[h] : 0.0f;
+
+    // The lane's half of its query (plus u), split.
+    f16x8 qh[D / 16], ql[D / 16];
+    float q_back;
+    {
+        const float *q = static_cast<const float *>(a.q) + row * a.ldq + h * a.hsq;
+        float x[D / 16][8], top = 0.0f;
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) {
+            const int c = s * 16 + half * 8;
+            const bool in = live && c < a.d;
+            if (in) {
+                load8(q + c, x[s]);
+            } else {
+                for (int e = 0; e < 8; e++) x[s][e] = 0.0f;
+            }
+            if (REL && a.rel_u && in)
+                for (int e = 0; e < 8; e++) x[s][e] += a.rel_u[(int64_t)h * a.d + c + e];
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[s][e]));
+        }
+        const Scale sc = scale_for(max_halves(top));
+        q_back = sc.back;
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) {
+            for (int e = 0; e < 8; e++) x[s][e] *= sc.by;
+            split2(x[s], qh[s], ql[s]);
+        }
+    }
+
+    // This thread's part of the tiles: rows row0 + u STEP, chunk c of each.
+    const int row0 = t / CHUNKS, c = t % CHUNKS;
+    const bool in_d = c * 8 < a.d;
+    const float *kp = static_cast<const float *>(a.k) + kvh * a.hsk + (in_d ? c * 8 : 0);
+    const float *vp = static_cast<const float *>(a.v) + kvh * a.hsv + (in_d ? c * 8 : 0);
+    const float *rp = REL ? a.rel + h * a.hsrel + (in_d ? c * 8 : 0) : nullptr;
+    float kr[PER][8], vr[PER][8], rr[PER][8], wu[8];
+    int mark[PER];
+    const auto load = [&](int kb) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            int j = kb + row0 + u * STEP;
+            const bool in = j < sp.nk && in_d;
+            j = j < sp.nk ? j : sp.nk - 1;
+            int64_t kat, vat;
+            if (PAGED) {
+                const int p = page_of(a.seqs, b, j), s = j % a.seqs.page;
+                mark[u] = p < 0 ? -1 : 0;
+                kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
+                vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
+            } else {
+                kat = (int64_t)(sp.k0 + j) * a.ldk;
+                vat = (int64_t)(sp.k0 + j) * a.ldv;
+                if (EXTRA && a.q_docs) mark[u] = a.k_docs[sp.k0 + j];
+            }
+            load8(kp + kat, kr[u]);
+            load8(vp + vat, vr[u]);
+            for (int e = 0; e < 8; e++) kr[u][e] = in ? kr[u][e] : 0.0f, vr[u][e] = in ? vr[u][e] : 0.0f;
+        }
+    };
+    // Block n of position rows: distances 32 n - (the workgroup's first position) and on.
+    const int first_i = sp.shift() + (int)pair0;
+    const auto load_block = [&](int n) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int64_t distance = (int64_t)n * 32 - first_i + row0 + u * STEP;
+            const int64_t at = distance < -a.rel_span ? 0 : distance > a.rel_span ? 2 * (int64_t)a.rel_span : distance + a.rel_span;
+            load8(rp + at * a.ldrel, rr[u]);
+            for (int e = 0; e < 8; e++) rr[u][e] = in_d ? rr[u][e] : 0.0f;
+        }
+    };
+    const auto store_block = [&](int n) {
+        const int slot = n & (RING - 1);
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int brow = row0 + u * STEP;
+            float top = 0.0f, add = 0.0f;
+            for (int e = 0; e < 8; e++) {
+                top = fmaxf(top, fabsf(rr[u][e]));
+                add = __builtin_fmaf(wu[e], rr[u][e], add);
+            }
+            const Scale sc = scale_for(row_max<CHUNKS>(top));
+            add = row_sum<CHUNKS>(add);
+            float x[8];
+            for (int e = 0; e < 8; e++) x[e] = rr[u][e] * sc.by;
+            const int to = k_place<CHUNKS>(brow, c);
+            split2(x, sh.r[slot][0][to], sh.r[slot][1][to]);
+            if (c == 0) {
+                sh.r_back[slot][brow] = sc.back;
+                sh.r_add[slot][brow] = add;
+            }
+        }
+    };
+    // T of block n for the wavefront's queries, into its ring of two blocks.
+    const auto terms_of = [&](int n) {
+        const int slot = n & (RING - 1);
+        f32x16 acc = {};
+#pragma unroll
+        for (int s = 0; s < D / 16; s++) {
+            const int from = k_place<CHUNKS>(col, s * 2 + half);
+            const f16x8 rh = sh.r[slot][0][from], rl = sh.r[slot][1][from];
+            acc = mfma(rl, qh[s], acc);
+            acc = mfma(rh, ql[s], acc);
+            acc = mfma(rh, qh[s], acc);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int d0 = 8 * e + 4 * half;  // the lane's four distances of this register group
+            const f32x4 back = *reinterpret_cast<const f32x4 *>(&sh.r_back[slot][d0]);
+            const f32x4 add = *reinterpret_cast<const f32x4 *>(&sh.r_add[slot][d0]);
+            f32x4 x;
+            for (int y = 0; y < 4; y++) x[y] = __builtin_fmaf(acc[4 * e + y], back[y] * q_back, add[y]);
+            *reinterpret_cast<f32x4 *>(&sh.terms[wave][col * 64 + (((n & 1) * 32 + d0 + 4 * col) & 63)]) = x;
+        }
+    };
+
+    f32x16 acc[D / 32] = {};
+    float m = -INFINITY, l = 0.0f;
+    const float mul = a.scale * LOG2E;
+    const bool marked = PAGED || (EXTRA && a.q_docs);
+
+    if (REL) {
+        for (int e = 0; e < 8; e++) {
+            const int64_t x = (int64_t)h * a.d + c * 8 + e;
+            wu[e] = in_d ? (a.rel_v ? a.rel_v[x] : 0.0f) - (a.rel_u ? a.rel_u[x] : 0.0f) : 0.0f;
+        }
+    }
+    if (n0 < n1) {
+        load(tiles.at(n0));
+        if (REL) load_block(tiles.at(n0) / TILE_K);
+    }
+    for (int n = n0; n < n1; n++) {
+        const int kb = tiles.at(n), block = kb / TILE_K;
+        if (REL && (n == n0 || tiles.at(n - 1) != kb - TILE_K)) {
+            // The first tile of a run: the four blocks before its own, and T of each wavefront's first.
+            float keep[PER][8];
+            for (int u = 0; u < PER; u++)
+                for (int e = 0; e < 8; e++) keep[u][e] = rr[u][e];
+            __syncthreads();
+            for (int x = 1; x <= RING; x++) {
+                load_block(block - x);
+                store_block(block - x);
+            }
+            __syncthreads();
+            terms_of(block - 1 - wave);
+            for (int u = 0; u < PER; u++)
+                for (int e = 0; e < 8; e++) rr[u][e] = keep[u][e];
+        }
+        __syncthreads();  // every wavefront has read the last tile
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int krow = row0 + u * STEP, kto = k_place<CHUNKS>(krow, c), vto = v_place<CHUNKS>(krow, c);
+            float top = 0.0f, x[8];
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(kr[u][e]));
+            const Scale sc = scale_for(row_max<CHUNKS>(top));
+            for (int e = 0; e < 8; e++) x[e] = kr[u][e] * sc.by;
+            split2(x, sh.k[0][kto], sh.k[1][kto]);
+            f32x8 v;
+            for (int e = 0; e < 8; e++) v[e] = vr[u][e];
+            split3(v, sh.v[0][vto], sh.v[1][vto], sh.v[2][vto]);
+            if (c == 0) {
+                sh.k_back[krow] = sc.back;
+                if (marked) sh.marks[krow] = mark[u];
+            }
+        }
+        if (REL) store_block(block);
+        __syncthreads();
+        if (n + 1 < n1) {
+            load(tiles.at(n + 1));
+            if (REL) load_block(tiles.at(n + 1) / TILE_K);
+        }
+
+        if (REL) terms_of(block - wave);
+        const bool none = !wave_live || ((kb + TILE_K <= w_first.lo || kb >= w_last.hi) && kb >= w_first.prefix);
+        if (none) continue;
+        f32x16 s = {};
+#pragma unroll
+        for (int e = 0; e < D / 16; e++) {
+            const int from = k_place<CHUNKS>(col, e * 2 + half);
+            const f16x8 kh = sh.k[0][from], kl = sh.k[1][from];
+            s = mfma(kl, qh[e], s);
+            s = mfma(kh, ql[e], s);
+            s = mfma(kh, qh[e], s);
+        }
+
+        // Scores, and -infinity where the key is not shown.
+        const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
+        bool compare = false;  // marks decide key by key
+        if (marked) {
+            const int mk = sh.marks[col];
+            if (EXTRA && a.q_docs) {
+                const int first = __builtin_amdgcn_readfirstlane(mk);
+                compare = !__all(mk == first && doc == first) || first < 0;
+            } else {
+                compare = __any(mk < 0);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; g++) {
+            const f32x4 back = *reinterpret_cast<const f32x4 *>(&sh.k_back[8 * g + 4 * half]);
+#pragma unroll
+            for (int y = 0; y < 4; y++) {
+                const int e = 4 * g + y, k = 8 * g + 4 * half + y, j = kb + k;
+                float x = s[e] * (back[y] * q_back);
+                if (REL) x += sh.terms[wave][col * 64 + ((((block - wave) & 1) * 32 + k - col + 4 * col) & 63)];
+                if (EXTRA) x = score_of<false>(a, x, h, slope, j - i);
+                if (!full && !win.has(j)) x = -INFINITY;
+                s[e] = x;
+            }
+        }
+        if (compare) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int mk = sh.marks[8 * (e / 4) + 4 * half + e % 4];
+                if (mk < 0 || mk != doc) s[e] = -INFINITY;
+            }
+        }
+
+        float top = s[0];
+#pragma unroll
+        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
+        top = max_halves(top);
+        const float to_log2 = EXTRA ? LOG2E : mul;
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float fade = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * to_log2);
+            l *= fade;
+#pragma unroll
+            for (int x = 0; x < D / 32; x++) acc[x] *= fade;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            f32x8 p;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                p[e] = __builtin_amdgcn_exp2f((s[g * 8 + e] - base) * to_log2);
+                l += p[e];
+            }
+            bf16x8 ph, pm, pl;
+            split3(p, ph, pm, pl);
+#pragma unroll
+            for (int x = 0; x < D / 32; x++) {
+                const bf16x8 vh = __builtin_bit_cast(bf16x8, v_fragment<CHUNKS>(sh.v[0], g * 16, x, lane));
+                const bf16x8 vm = __builtin_bit_cast(bf16x8, v_fragment<CHUNKS>(sh.v[1], g * 16, x, lane));
+                const bf16x8 vl = __builtin_bit_cast(bf16x8, v_fragment<CHUNKS>(sh.v[2], g * 16, x, lane));
+                acc[x] = mfma(vl, ph, acc[x]);
+                acc[x] = mfma(vh, pl, acc[x]);
+                acc[x] = mfma(vm, pm, acc[x]);
+                acc[x] = mfma(vm, ph, acc[x]);
+                acc[x] = mfma(vh, pm, acc[x]);
+                acc[x] = mfma(vh, ph, acc[x]);
+            }
+        }
+    }
+
+    l = sum_halves(l);
+    if (parts.parts > 1) {
+        if (!live) return;
+        const size_t to = (size_t)part * parts.pairs + row * a.heads + h;
+        if (half == 0) {
+            parts.top[to] = EXTRA ? m : m * a.scale;
+            parts.sum[to] = l;
+        }
+        float *o = parts.out + to * a.d;
+#pragma unroll
+        for (int x = 0; x < D / 32; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int oc = x * 32 + 8 * e + 4 * half;
+                if (oc < a.d)
+                    *reinterpret_cast<f32x4 *>(o + oc) =
+                        f32x4{acc[x][4 * e], acc[x][4 * e + 1], acc[x][4 * e + 2], acc[x][4 * e + 3]};
+            }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float *out = static_cast<float *>(a.out) + row * a.ldo + h * a.hso;
+    bool sound = true;
+#pragma unroll
+    for (int x = 0; x < D / 32; x++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const int oc = x * 32 + 8 * e + 4 * half;
+            f32x4 o;
+            for (int y = 0; y < 4; y++) {
+                o[y] = acc[x][4 * e + y] * inv;
+                sound = sound && o[y] - o[y] == 0.0f;
+            }
+            if (live && oc < a.d) *reinterpret_cast<f32x4 *>(out + oc) = o;
+        }
+    // An infinity or NaN among the operands, be it hidden, makes the split products NaN.
+    unsigned long long again = __ballot(live && !sound);
+    again = (again | again >> 32) & 0xffffffffull;
+    while (again) {
+        const int64_t p = wave0 + __builtin_ctzll(again);
+        again &= again - 1;
+        attend_row<float>(a, b, at.head * group + (int)(p % group), (int)(p / group), lane);
+    }
+}
+
+template <int D, bool PAGED, bool EXTRA, bool REL>
+hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
+    const int heads = REL ? a.heads : a.kv_heads;
+    const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / heads), TILE_Q);
+    const size_t groups = (size_t)a.seqs.batch * heads * splits, blocks = div_ceil(groups, 8) * 8 * q_tiles;
+    if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((attn_tile32_kernel<D, PAGED, EXTRA, REL>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a,
+                       parts_of(a, splits), (int)q_tiles, (int)groups);
+    return hipGetLastError();
+}
+
+template <int D, bool REL>
+hipError_t launch_kind(const AttnArgs &a, int splits, hipStream_t s) {
+    const bool extra = a.cap > 0.0f || a.slopes || a.table || a.q_docs;
+    if (a.seqs.tables)
+        return extra ? launch_tile<D, true, true, REL>(a, splits, s) : launch_tile<D, true, false, REL>(a, splits, s);
+    return extra ? launch_tile<D, false, true, REL>(a, splits, s) : launch_tile<D, false, false, REL>(a, splits, s);
+}
+
+}  // namespace
+
+hipError_t launch_attention32(const AttnArgs &a, int splits, hipStream_t s) {
+    if (a.rel) return a.d <= 64 ? launch_kind<64, true>(a, splits, s) : launch_kind<128, true>(a, splits, s);
+    if (a.d <= 64) return launch_kind<64, false>(a, splits, s);
+    if (a.d <= 128) return launch_kind<128, false>(a, splits, s);
+    return launch_kind<256, false>(a, splits, s);
+}
+
+}  // namespace tg
