@@ -11,7 +11,8 @@ LIB = os.path.join(HERE, "lib", "libtelmo_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["api.hip", "kernels_rows.hip", "kernels_gemm.hip", "kernels_gemv.hip", "kernels_tdt.hip", "kernels_exact.hip",
-           "kernels_attn.hip", "kernels_attn16.hip", "kernels_attn32.hip", "kernels_rotary.hip",
+           "kernels_attn.hip", "kernels_attn16.hip", "kernels_attn32.hip", "kernels_attn_few.hip",
+           "kernels_rotary.hip",
            "layout.cpp", "pack.cpp"]
 
 # -ffp-contract=off: no implicit fused multiply-adds, so the f32 epilogue and the exact kernel

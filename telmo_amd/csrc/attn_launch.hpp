@@ -15,4 +15,10 @@ hipError_t launch_attention16(const AttnArgs &a, int splits, hipStream_t s);
 inline bool attention32_fits(const AttnArgs &a) { return !a.rel || a.d <= 128; }
 hipError_t launch_attention32(const AttnArgs &a, int splits, hipStream_t s);
 
+// Few query rows of any type, without position rows and documents.
+inline bool attention_few_fits(const AttnArgs &a) {
+    return !a.rel && !a.q_docs && (size_t)a.seqs.longest * (a.heads / a.kv_heads) <= 16;
+}
+hipError_t launch_attention_few(const AttnArgs &a, int splits, hipStream_t s);
+
 }  // namespace tg

@@ -68,14 +68,17 @@ hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
     return hipGetLastError();
 }
 
-constexpr size_t TARGET = 512;      // workgroups that fill the GPU: two on each of 256 CUs
-constexpr size_t LEAST_KEYS = 256;  // a part works on at least as many
+// How a call is spread: workgroups of `tile` query rows and heads, and how many parts the keys are cut into so that
+// about `target` workgroups run, each with `least` keys or more.
+struct Spread {
+    size_t tile, target, least;
+};
+constexpr Spread TILES{128, 512, 256}, FEW{16, 2048, 512};
 constexpr size_t MOST_PARTS = 64;
 
-// Parts for workgroups of `wgs` without splitting, over up to `keys` keys.
-size_t parts_for(size_t wgs, size_t keys) {
-    size_t n = TARGET / (wgs ? wgs : 1);
-    if (n > keys / LEAST_KEYS) n = keys / LEAST_KEYS;
+size_t parts_for(const Spread &sp, size_t wgs, size_t keys) {
+    size_t n = sp.target / (wgs ? wgs : 1);
+    if (n > keys / sp.least) n = keys / sp.least;
     return n < 1 ? 1 : n > MOST_PARTS ? MOST_PARTS : n;
 }
 
@@ -83,26 +86,34 @@ size_t parts_for(size_t wgs, size_t keys) {
 
 size_t attention_work_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys) {
     // The fewest workgroups that calls of these sizes have give the most parts.
-    const size_t tiles = div_ceil(rows * (heads / kv_heads), 128);
-    const size_t n = parts_for(kv_heads * (tiles > batch ? tiles : batch), keys);
+    const auto parts = [&](const Spread &sp) {
+        const size_t tiles = div_ceil(rows * (heads / kv_heads), sp.tile);
+        return parts_for(sp, kv_heads * (tiles > batch ? tiles : batch), keys);
+    };
+    const size_t x = parts(TILES), y = rows * (heads / kv_heads) <= FEW.tile * batch ? parts(FEW) : 1;
+    const size_t n = x > y ? x : y;
     return n > 1 ? n * part_bytes(rows * heads, d) : 0;
 }
 
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
+    const bool few = attention_few_fits(a);
     // LDS holds the blocks of position rows of heads of up to 128; longer ones take a wavefront per row.
     if (a.type == F32 && !attention32_fits(a)) return launch_rows(a, s);
-    const size_t group = a.rel ? 1 : a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, 128);
+    const Spread &sp = few ? FEW : TILES;
+    const size_t group = a.rel ? 1 : a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, sp.tile);
     size_t keys = a.seqs.tables ? (size_t)a.seqs.width * a.seqs.page
                                 : (size_t)(a.seqs.k_starts ? a.seqs.k_rows : a.seqs.k_rows / a.seqs.batch);
-    if (a.left >= 0 && a.right >= 0 && !a.prefix) {  // no row tile reaches further than its window
-        const size_t reach = (size_t)a.left + a.right + 1 + 128;
+    if (a.left >= 0 && a.right >= 0 && !a.prefix) {  // no tile reaches further than its rows' windows
+        const size_t reach = (size_t)a.left + a.right + 1 + sp.tile;
         keys = keys < reach ? keys : reach;
     }
-    size_t n = parts_for(tiles * (a.heads / group) * a.seqs.batch, keys);
+    size_t n = parts_for(sp, tiles * (a.heads / group) * a.seqs.batch, keys);
     const size_t bytes = part_bytes((size_t)a.seqs.q_rows * a.heads, a.d);
     if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
     if (n < 1) n = 1;
-    const hipError_t e = a.type == F32 ? launch_attention32(a, (int)n, s) : launch_attention16(a, (int)n, s);
+    const hipError_t e = few                ? launch_attention_few(a, (int)n, s)
+                         : a.type == F32 ? launch_attention32(a, (int)n, s)
+                                         : launch_attention16(a, (int)n, s);
     if (e != hipSuccess || n == 1) return e;
     switch (a.type) {
         case F16: return launch_join<_Float16>(a, (int)n, s);

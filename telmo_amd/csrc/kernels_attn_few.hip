@@ -1,0 +1,348 @@
+// Attention of few query rows over many keys (single tokens over a cache): bound by reading the keys and values
+// once.
+//
+// The rows of a sequence that share a key head (its new rows by the group's heads) are the 16 columns of
+// 16 x 16 products. Nothing of the keys is used twice, so LDS does not hold them: each of a workgroup's
+// wavefronts takes key tiles of its own, loads the operands of S' = K Q' from memory into registers as the
+// matrix instructions want them (16 rows by 64 bytes a load) and V by whole rows (a load gives 16 lanes the
+// 16 x 16 bytes of a row), the next tile's loads in flight while it computes. V' wants keys side by side in a
+// register: of 16-bit values, the eight rows that a lane holds are interleaved in registers; of f32 there is
+// nothing to do. The output's columns are numbered so that a lane's loads are contiguous: product x of a chunk
+// holds its value x. The wavefronts' results are joined in LDS, and those of the parts by a second kernel.
+//
+// The products have time to spare, so the 16-bit weights are held as two numbers, f32's as they are on the f32
+// matrix instructions.
+#include "attn_launch.hpp"
+#include "attn_tile.hpp"
+
+namespace tg {
+
+namespace {
+
+constexpr int COLS = 16;
+
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+
+// The greatest (the sum) of the values of the four lanes 16 apart.
+__device__ __forceinline__ float max_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+template <typename T, int D>
+struct Few {
+    static constexpr bool WIDE = sizeof(T) == 4;
+    static constexpr int WAVES = D == 256 ? 4 : 8;          // two on a SIMD, one where a tile fills its registers
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int TILE = WIDE ? 16 : 32;             // keys of a tile
+    static constexpr int CH = WIDE ? 4 : D == 64 ? 4 : 8;   // values of a lane's piece of a V row
+    static constexpr int W = D / (16 * CH);                 // pieces of a V row
+    static constexpr int VROWS = WIDE ? 4 : 8;              // V rows of a lane
+    static constexpr int KS = WIDE ? D / 16 : D / 32;       // 16-byte pieces of a lane's part of a K row
+    static constexpr int KT = TILE / 16;                    // K rows of a lane
+    static constexpr int VW = CH * sizeof(T) / 4;           // words of a V piece
+};
+
+// D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped or biased.
+template <typename T, int D, bool PAGED, bool EXTRA>
+__global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const AttnArgs a, const AttnParts parts, const int q_tiles) {
+    typedef Few<T, D> F;
+    constexpr int TILE = F::TILE, PITCH = D + 4, WAVES = F::WAVES, THREADS = F::THREADS;
+    __shared__ __align__(16) float outs[WAVES][COLS][PITCH];
+    __shared__ float tops[WAVES][COLS], sums[WAVES][COLS];
+    __shared__ int again[COLS];
+
+    int id = blockIdx.x;
+    const int part = id % parts.parts;
+    id /= parts.parts;
+    const int tile = id % q_tiles;
+    id /= q_tiles;
+    const int kvh = id % a.kv_heads, b = id / a.kv_heads;
+    const AttnSpan sp = span_of(a.seqs, b);
+    const int group = a.heads / a.kv_heads;
+    const int pairs = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest) * group, pair0 = tile * COLS;
+    if (pair0 >= pairs) return;
+
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, quarter = lane >> 4, col = lane & 15;
+    const int prefix = a.prefix ? a.prefix[b] : 0;
+    const bool live = pair0 + col < pairs;
+    const int r = live ? (pair0 + col) / group : 0, h = kvh * group + (live ? (pair0 + col) % group : 0);
+    const int i = sp.shift() + r;
+    const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
+    const int last = pair0 + COLS - 1 < pairs - 1 ? pair0 + COLS - 1 : pairs - 1;
+    const AttnWindow w_first = window_of(sp.shift() + pair0 / group, sp.nk, a.left, a.right, prefix);
+    const AttnWindow w_last = window_of(sp.shift() + last / group, sp.nk, a.left, a.right, prefix);
+    const Tiles<TILE> tiles(w_first, w_last);
+    const int n0 = (int)((int64_t)tiles.count * part / parts.parts) + wave;
+    const int n1 = (int)((int64_t)tiles.count * (part + 1) / parts.parts);
+    const int64_t row = (int64_t)sp.q0 + r;
+    const float slope = EXTRA && a.slopes ? a.slopes[h] : 0.0f;
+
+    u32x4 qf[F::KS];
+    {
+        const T *q = static_cast<const T *>(a.q) + row * a.ldq + h * a.hsq;
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int s = 0; s < F::KS; s++) {
+            const int c = s * 4 * E + quarter * E;
+            qf[s] = live && c < a.d ? *reinterpret_cast<const u32x4 *>(q + c) : u32x4{};
+        }
+    }
+
+    const T *kbase = static_cast<const T *>(a.k) + kvh * a.hsk, *vbase = static_cast<const T *>(a.v) + kvh * a.hsv;
+    const bool one_page = PAGED && a.seqs.page % TILE == 0;  // a tile lies in one page
+    u32x4 kr[F::KT][F::KS];
+    uint32_t vr[F::VROWS][F::W][F::VW];
+    uint32_t hidden = 0;  // keys of the loaded tile that have no place
+    const auto load = [&](int kb) {
+        // Offsets of the keys' rows: the lane's own ones for K, those of its eight (four) rows for V.
+        int64_t kat = 0, vat = 0;
+        if (PAGED) {
+            const int key = one_page ? kb : kb + lane % TILE;
+            const int j = key < sp.nk ? key : sp.nk - 1;
+            const int p = page_of(a.seqs, b, j), s = j % a.seqs.page;
+            hidden = (uint32_t)__ballot(p < 0);
+            kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
+            vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
+        }
+        const auto offset = [&](int64_t base, int64_t ld, int key) -> int64_t {
+            const int j = kb + key < sp.nk ? key : sp.nk - 1 - kb;  // within the tile
+            if (!PAGED) return (int64_t)(sp.k0 + kb + j) * ld;
+            if (one_page) return base + j * ld;
+            const int lo = __shfl((int)(uint32_t)base, j), hi = __shfl((int)(base >> 32), j);
+            return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+        };
+        constexpr int E = 16 / sizeof(T);
+#pragma unroll
+        for (int x = 0; x < F::KT; x++) {
+            const T *k = kbase + offset(kat, a.ldk, x * 16 + col);
+#pragma unroll
+            for (int s = 0; s < F::KS; s++) {
+                const int c = s * 4 * E + quarter * E;
+                kr[x][s] = *reinterpret_cast<const u32x4 *>(k + (c < a.d ? c : 0));
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < F::VROWS; e++) {
+            const int key = (e / 4) * 16 + quarter * 4 + e % 4;
+            const T *v = vbase + offset(vat, a.ldv, key);
+            const bool in = kb + key < sp.nk;
+#pragma unroll
+            for (int w = 0; w < F::W; w++) {
+                const int c = w * 16 * F::CH + col * F::CH;
+                const T *at = v + (c < a.d ? c : 0);
+                if constexpr (F::VW == 4) {
+                    const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
+                    for (int y = 0; y < 4; y++) vr[e][w][y] = in && c < a.d ? x[y] : 0u;
+                } else {
+                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
+                    for (int y = 0; y < 2; y++) vr[e][w][y] = in && c < a.d ? x[y] : 0u;
+                }
+            }
+        }
+    };
+
+    f32x4 acc[F::W][F::CH] = {};
+    float m = -INFINITY, l = 0.0f;
+    const float to_log2 = EXTRA ? LOG2E : a.scale * LOG2E;
+    constexpr float SHIFT = __is_same(T, _Float16) ? 8.0f : 0.0f;  // weights below f16's normal numbers
+
+    if (n0 < n1) load(tiles.at(n0));
+    for (int n = n0; n < n1; n += WAVES) {
+        const int kb = tiles.at(n);
+        const uint32_t hide = hidden;
+        f32x4 s[F::KT] = {};
+#pragma unroll
+        for (int x = 0; x < F::KT; x++)
+#pragma unroll
+            for (int e = 0; e < F::KS; e++) {
+                if constexpr (F::WIDE) {
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        s[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][e][y]),
+                                                                    __uint_as_float(qf[e][y]), s[x], 0, 0, 0);
+                } else {
+                    typedef T v8 __attribute__((ext_vector_type(8)));
+                    s[x] = mfma16(__builtin_bit_cast(v8, kr[x][e]), __builtin_bit_cast(v8, qf[e]), s[x]);
+                }
+            }
+        uint32_t vt[F::VROWS][F::W][F::VW];
+#pragma unroll
+        for (int e = 0; e < F::VROWS; e++)
+#pragma unroll
+            for (int w = 0; w < F::W; w++)
+#pragma unroll
+                for (int y = 0; y < F::VW; y++) vt[e][w][y] = vr[e][w][y];
+        if (n + WAVES < n1) load(tiles.at(n + WAVES));
+
+        const bool full = (kb >= w_last.lo && kb + TILE <= w_first.hi) || kb + TILE <= w_first.prefix;
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < F::KT; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int j = kb + x * 16 + quarter * 4 + e;
+                if (EXTRA) s[x][e] = score_of<!F::WIDE>(a, s[x][e], h, slope, j - i);
+                if (!full && !win.has(j)) s[x][e] = -INFINITY;
+                if (PAGED && hide && (one_page || (hide >> (j - kb) & 1))) s[x][e] = -INFINITY;
+                top = fmaxf(top, s[x][e]);
+            }
+        top = max_quarters(top);
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float fade = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * to_log2);
+            l *= fade;
+#pragma unroll
+            for (int w = 0; w < F::W; w++)
+#pragma unroll
+                for (int x = 0; x < F::CH; x++) acc[w][x] *= fade;
+            m = mn;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float p[F::KT][4];
+#pragma unroll
+        for (int x = 0; x < F::KT; x++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                p[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e] - base, to_log2, SHIFT));
+                l += p[x][e];
+            }
+        if constexpr (F::WIDE) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int w = 0; w < F::W; w++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        acc[w][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vt[e][w][x]), p[0][e],
+                                                                         acc[w][x], 0, 0, 0);
+        } else {
+            typedef T v8 __attribute__((ext_vector_type(8)));
+            f32x8 pv;
+#pragma unroll
+            for (int e = 0; e < 8; e++) pv[e] = p[e / 4][e % 4];
+            const v8 ph = __builtin_convertvector(pv, v8);
+            const v8 pl = __builtin_convertvector(pv - __builtin_convertvector(ph, f32x8), v8);
+#pragma unroll
+            for (int w = 0; w < F::W; w++)
+#pragma unroll
+                for (int x = 0; x < F::CH; x++) {
+                    u32x4 v;  // value x of the lane's eight rows
+#pragma unroll
+                    for (int y = 0; y < 4; y++)
+                        v[y] = __builtin_amdgcn_perm(vt[2 * y + 1][w][x / 2], vt[2 * y][w][x / 2],
+                                                     x % 2 ? 0x07060302u : 0x05040100u);
+                    acc[w][x] = mfma16(__builtin_bit_cast(v8, v), pl, acc[w][x]);
+                    acc[w][x] = mfma16(__builtin_bit_cast(v8, v), ph, acc[w][x]);
+                }
+        }
+    }
+
+    // The wavefronts' parts: each thread adds up four values of a column.
+    l = sum_quarters(l);
+    if (t < COLS) again[t] = 0;
+    if (quarter == 0) {
+        tops[wave][col] = EXTRA ? m : m * a.scale;
+        sums[wave][col] = l;
+    }
+#pragma unroll
+    for (int w = 0; w < F::W; w++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int x = 0; x < F::CH; x += 4)
+                *reinterpret_cast<f32x4 *>(&outs[wave][col][w * 16 * F::CH + (quarter * 4 + e) * F::CH + x]) =
+                    f32x4{acc[w][x][e], acc[w][x + 1][e], acc[w][x + 2][e], acc[w][x + 3][e]};
+    __syncthreads();
+    for (int y = t; y < COLS * (D / 4); y += THREADS) {
+        const int oc = y / (D / 4), c = y % (D / 4) * 4, pair = pair0 + oc;
+        if (pair >= pairs || c >= a.d) continue;
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < WAVES; w++) top = fmaxf(top, tops[w][oc]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        f32x4 o = {};
+        for (int w = 0; w < WAVES; w++) {
+            const float weight = exp2f((tops[w][oc] - base) * LOG2E), part_sum = sums[w][oc];
+            if (part_sum == 0.0f) continue;
+            sum = __builtin_fmaf(weight, part_sum, sum);
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(&outs[w][oc][c]);
+            for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(weight, x[e], o[e]);
+        }
+        const int64_t to_row = (int64_t)sp.q0 + pair / group;
+        const int to_head = kvh * group + pair % group;
+        if (parts.parts > 1) {
+            const size_t to = (size_t)part * parts.pairs + to_row * a.heads + to_head;
+            if (c == 0) {
+                parts.top[to] = top;
+                parts.sum[to] = sum;
+            }
+            *reinterpret_cast<f32x4 *>(parts.out + to * a.d + c) = o;
+            continue;
+        }
+        T *out = static_cast<T *>(a.out) + to_row * a.ldo + to_head * a.hso + c;
+        bool sound = true;
+        T v[4];
+        for (int e = 0; e < 4; e++) {
+            const float x = sum == 0.0f ? 0.0f : o[e] / sum;
+            sound = sound && x - x == 0.0f;
+            v[e] = (T)x;
+        }
+        if constexpr (F::WIDE) *reinterpret_cast<u32x4 *>(out) = *reinterpret_cast<u32x4 *>(v);
+        else *reinterpret_cast<u32x2 *>(out) = *reinterpret_cast<u32x2 *>(v);
+        if (!sound && sum - sum == 0.0f) again[oc] = 1;
+    }
+    if (parts.parts > 1) return;
+    // A hidden key's NaN or infinity beside a sound sum of weights, as in the tile kernels.
+    __syncthreads();
+    for (int x = wave; x < COLS; x += WAVES)
+        if (again[x]) attend_row<T>(a, b, kvh * group + (pair0 + x) % group, (pair0 + x) / group, lane);
+}
+
+template <typename T, int D, bool PAGED, bool EXTRA>
+hipError_t launch_few(const AttnArgs &a, int splits, hipStream_t s) {
+    const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / a.kv_heads), COLS);
+    const size_t blocks = q_tiles * a.seqs.batch * a.kv_heads * splits;
+    if (blocks > MAX_ATTN_BLOCKS / 2) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((attn_few_kernel<T, D, PAGED, EXTRA>), dim3((unsigned)blocks), dim3(Few<T, D>::THREADS), 0,
+                       s, a, parts_of(a, splits), (int)q_tiles);
+    return hipGetLastError();
+}
+
+template <typename T, int D>
+hipError_t launch_kind(const AttnArgs &a, int splits, hipStream_t s) {
+    const bool extra = a.cap > 0.0f || a.slopes || a.table;
+    if (a.seqs.tables)
+        return extra ? launch_few<T, D, true, true>(a, splits, s) : launch_few<T, D, true, false>(a, splits, s);
+    return extra ? launch_few<T, D, false, true>(a, splits, s) : launch_few<T, D, false, false>(a, splits, s);
+}
+
+template <typename T>
+hipError_t launch_size(const AttnArgs &a, int splits, hipStream_t s) {
+    if (a.d <= 64) return launch_kind<T, 64>(a, splits, s);
+    if (a.d <= 128) return launch_kind<T, 128>(a, splits, s);
+    return launch_kind<T, 256>(a, splits, s);
+}
+
+}  // namespace
+
+hipError_t launch_attention_few(const AttnArgs &a, int splits, hipStream_t s) {
+    switch (a.type) {
+        case F16: return launch_size<_Float16>(a, splits, s);
+        case BF16: return launch_size<__bf16>(a, splits, s);
+        default: return launch_size<float>(a, splits, s);
+    }
+}
+
+}  // namespace tg
