@@ -1610,6 +1610,9 @@ int check_seqs(tg_ctx *ctx, const tg_attention_desc &a, bool paged, tg::AttnSeqs
     s.width = (int)a.width;
     s.page = (int)a.page;
     s.pages = (int)a.pages;
+    s.page_shift = 31;
+    while (((size_t)1 << (s.page_shift - 31)) < a.page) s.page_shift++;
+    s.page_mul = (uint32_t)((((uint64_t)1 << s.page_shift) + a.page - 1) / a.page);
     int rc = check_rows(ctx, "k", a.k, a.type, rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page));
     if (rc) return rc;
     if ((rc = check_rows(ctx, "v", a.v, a.type, rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page)))) return rc;

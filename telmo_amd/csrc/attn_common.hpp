@@ -76,9 +76,12 @@ __host__ __device__ inline AttnSpan span_of(const AttnSeqs &s, int b) {
     return r;
 }
 
-// The page that holds key position j of sequence b, or -1 where the table names none of the cache's.
-__host__ __device__ inline int page_of(const AttnSeqs &s, int b, int j) {
-    const int p = s.tables[(int64_t)b * s.ldt + j / s.page];
+// The page that holds key position j of sequence b, or -1 where the table names none of the cache's, and the
+// key's row in it.
+__host__ __device__ inline int page_of(const AttnSeqs &s, int b, int j, int &row) {
+    const int n = (int)((uint64_t)(uint32_t)j * s.page_mul >> s.page_shift);
+    row = j - n * s.page;
+    const int p = s.tables[(int64_t)b * s.ldt + n];
     return (unsigned)p < (unsigned)s.pages ? p : -1;
 }
 
@@ -110,21 +113,42 @@ __device__ __forceinline__ float tanh_f32(float x) {
     p = __builtin_fmaf(p, q, -1.0f / 3.0f);
     return a < 0.3f ? __builtin_fmaf(x * q, p, x) : big;
 }
-// tanh to 2^-22 absolutely, with the hardware's reciprocal: for 16-bit rows, whose weights keep less.
-__device__ __forceinline__ float tanh_fast(float x) {
-    return 1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(2.0f * LOG2E * x) + 1.0f);
-}
-
 // A product's score of head h at the distance key - query, with what the call does to scores.
-template <bool FAST>
 __device__ __forceinline__ float score_of(const AttnArgs &a, float dot, int h, float slope, int distance) {
     float s = dot * a.scale;
-    if (a.cap > 0.0f) s = a.cap * (FAST ? tanh_fast(s / a.cap) : tanh_f32(s / a.cap));
+    if (a.cap > 0.0f) s = a.cap * tanh_f32(s / a.cap);
     if (a.slopes) s -= slope * fabsf((float)distance);
     if (a.table)
         s += a.table[(int64_t)h * (2 * a.table_span + 1) + clamp_to(distance, -a.table_span, a.table_span) +
                      a.table_span];
     return s;
+}
+
+// The same of a lane's N products, key_at(e) the e-th one's key: one kind of change after the other. FAST: tanh
+// to 2^-22 absolutely, with the hardware's reciprocal, for 16-bit rows, whose weights keep less. TABLE: there may be a
+// table.
+template <bool FAST, int N, bool TABLE, typename S, typename F>
+__device__ __forceinline__ void scores_of(const AttnArgs &a, S s, F key_at, int h, float slope, int i) {
+    if (a.cap > 0.0f) {
+        const float into = 2.0f * LOG2E * a.scale / a.cap;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            s(e) = FAST ? __builtin_fmaf(-2.0f * a.cap,
+                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s(e) * into) + 1.0f), a.cap)
+                        : a.cap * tanh_f32(s(e) * a.scale / a.cap);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) s(e) *= a.scale;
+    }
+    if (a.slopes) {
+#pragma unroll
+        for (int e = 0; e < N; e++) s(e) = __builtin_fmaf(-slope, fabsf((float)(key_at(e) - i)), s(e));
+    }
+    if (TABLE && a.table) {
+        const float *row = a.table + (int64_t)h * (2 * a.table_span + 1) + a.table_span;
+#pragma unroll
+        for (int e = 0; e < N; e++) s(e) += row[clamp_to(key_at(e) - i, -a.table_span, a.table_span)];
+    }
 }
 
 // Row r of sequence b, head h, by one wavefront from the definition: a lane scores one key of 64 at a time,
@@ -147,10 +171,11 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
         int64_t kat = 0, vat = 0;
         if (shown) {
             if (a.seqs.tables) {
-                const int p = page_of(a.seqs, b, j);
+                int at;
+                const int p = page_of(a.seqs, b, j, at);
                 shown = p >= 0;
-                kat = p * a.psk + (j % a.seqs.page) * a.ldk;
-                vat = p * a.psv + (j % a.seqs.page) * a.ldv;
+                kat = p * a.psk + at * a.ldk;
+                vat = p * a.psv + at * a.ldv;
             } else {
                 kat = (int64_t)(sp.k0 + j) * a.ldk;
                 vat = (int64_t)(sp.k0 + j) * a.ldv;
@@ -170,7 +195,7 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
                     term = __builtin_fmaf(to_f32(q[c]) + (a.rel_v ? a.rel_v[h * a.d + c] : 0.0f), rr[c], term);
                 dot += term;
             }
-            s = score_of<false>(a, dot, h, slope, j - i);
+            s = score_of(a, dot, h, slope, j - i);
             shown = s != -INFINITY;
         }
         unsigned long long live = __ballot(shown);

@@ -45,6 +45,20 @@ __device__ __forceinline__ s16x8 v_fragment(const void *tile, int row, int x, in
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
+// The end of a region without branches of N x PRODUCTS matrix products, each group of them fed by READS reads of LDS,
+// of which the program has issued the first AHEAD groups' before the region: fixes the order that the next group's
+// reads follow each group's products. Left to itself the compiler reads an operand just before the product that takes
+// it and waits out LDS's latency every time.
+template <int N, int READS, int AHEAD, int PRODUCTS = 1>
+__device__ __forceinline__ void feed() {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS, 0);
+        if (n + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // The key tiles that a range of query positions needs: those of the prefix, then those of the window.
 template <int TILE_K>
 struct Tiles {
@@ -80,5 +94,74 @@ struct Place {
         return pair0 < pairs;
     }
 };
+
+// Where a thread's pieces of a tile of keys come from: pieces u = 0 .. PER - 1 are its column of rows row0 + u STEP
+// of the tile. Offsets within a tile fit 32 bits (tile_strides_fit); the tile's own, and its pages', are scalars
+// where STEP rows lie in one page. Rows past the last key are read as that one: they are hidden, and their values
+// are some row's. Lane n of each wavefront looks up the tile's key n a tile ahead: its page and row in it, or its
+// document.
+template <typename T, int TILE_K, int PER, int STEP, bool PAGED>
+struct KeyRows {
+    static constexpr int64_t SIZE = sizeof(T);
+    const char *k, *v;      // the head's first row
+    uint32_t k_row, v_row;  // bytes between rows
+    uint32_t column;        // bytes of the thread's column
+    int row0;
+    int page, at;           // the lane's key's
+    __device__ __forceinline__ KeyRows(const AttnArgs &a, const AttnSpan &sp, int kvh, int row0_, int col) {
+        k = static_cast<const char *>(a.k) + ((PAGED ? 0 : sp.k0 * a.ldk) + kvh * a.hsk) * SIZE;
+        v = static_cast<const char *>(a.v) + ((PAGED ? 0 : sp.k0 * a.ldv) + kvh * a.hsv) * SIZE;
+        k_row = (uint32_t)(a.ldk * SIZE), v_row = (uint32_t)(a.ldv * SIZE);
+        column = (uint32_t)(col * SIZE);
+        row0 = row0_;
+        page = at = 0;
+    }
+    // Looks up the keys of the tile at kb.
+    __device__ __forceinline__ void look(const AttnArgs &a, const AttnSpan &sp, int b, int kb, int lane) {
+        if (!PAGED) return;
+        const int j = kb + lane % TILE_K;
+        page = page_of(a.seqs, b, j < sp.nk ? j : sp.nk - 1, at);
+    }
+    // The keys of the tile that was looked up last that have no page.
+    __device__ __forceinline__ uint64_t homeless() const { return PAGED ? __ballot(page < 0) : 0; }
+    // f(u, key address, value address) for the tile at kb, the last one that was looked up.
+    template <typename F>
+    __device__ __forceinline__ void each(const AttnArgs &a, const AttnSpan &sp, int kb, F f) const {
+        if (PAGED && a.seqs.page % STEP) {
+#pragma unroll
+            for (int u = 0; u < PER; u++) {
+                const int p = __shfl(page, row0 + u * STEP), s = __shfl(at, row0 + u * STEP);
+                const int64_t q = p < 0 ? 0 : p;
+                f(u, k + q * (a.psk * SIZE) + ((uint64_t)(uint32_t)s * k_row + column),
+                  v + q * (a.psv * SIZE) + ((uint64_t)(uint32_t)s * v_row + column));
+            }
+            return;
+        }
+        const bool whole = kb + TILE_K <= sp.nk;
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            // The first of these STEP rows (or the last key, where they lie past it), and the lane's from there.
+            const int first = kb + u * STEP, low = whole || first < sp.nk ? first : sp.nk - 1;
+            int64_t kat, vat;
+            if (PAGED) {
+                const int p = __builtin_amdgcn_readlane(page, u * STEP), s = __builtin_amdgcn_readlane(at, u * STEP);
+                const int64_t q = p < 0 ? 0 : p;
+                kat = q * (a.psk * SIZE) + (uint64_t)(uint32_t)s * k_row;
+                vat = q * (a.psv * SIZE) + (uint64_t)(uint32_t)s * v_row;
+            } else {
+                kat = (uint64_t)(uint32_t)low * k_row;
+                vat = (uint64_t)(uint32_t)low * v_row;
+            }
+            int row = row0;
+            if (!whole) row = first + row0 < sp.nk ? row0 : sp.nk - 1 - low;
+            f(u, k + kat + ((uint32_t)row * k_row + column), v + vat + ((uint32_t)row * v_row + column));
+        }
+    }
+};
+// Whether offsets within a tile of keys fit 32 bits.
+inline bool tile_strides_fit(const AttnArgs &a) {
+    const int64_t most = INT32_MAX / 64 / 4;
+    return a.ldk <= most && a.ldv <= most;
+}
 
 }  // namespace tg

@@ -9,8 +9,8 @@
 // Statistics and sums are held in f32: one pass over the keys carries the running maximum m, the sum of
 // exp(s - m) and the unnormalised output, both rescaled where m grows. Long keys of few rows are split over
 // workgroups and the parts joined by a second kernel, in their order.
-#include "attn_common.hpp"
 #include "attn_launch.hpp"
+#include "attn_tile.hpp"
 
 namespace tg {
 
@@ -18,9 +18,10 @@ namespace {
 
 constexpr int ROW_WAVES = 4;
 
+template <typename T>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_rows_kernel(const AttnArgs a) {
     const int b = blockIdx.z, r = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
-    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<float>(a, b, blockIdx.y, r, threadIdx.x & 63);
+    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<T>(a, b, blockIdx.y, r, threadIdx.x & 63);
 }
 
 // The parts of a row and head, joined by one wavefront: with M the largest maximum, the sums and outputs of
@@ -55,9 +56,10 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArg
     if (!__all(sound) && (sizeof(T) == 4 || l - l == 0.0f)) attend_row<T>(a, b, h, r, lane);
 }
 
+template <typename T>
 hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
     const dim3 grid((unsigned)div_ceil((size_t)a.seqs.longest, ROW_WAVES), (unsigned)a.heads, (unsigned)a.seqs.batch);
-    hipLaunchKernelGGL(attn_rows_kernel, grid, dim3(64 * ROW_WAVES), 0, s, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a);
     return hipGetLastError();
 }
 
@@ -97,8 +99,15 @@ size_t attention_work_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d
 
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
     const bool few = attention_few_fits(a);
-    // LDS holds the blocks of position rows of heads of up to 128; longer ones take a wavefront per row.
-    if (a.type == F32 && !attention32_fits(a)) return launch_rows(a, s);
+    // LDS holds the blocks of position rows of heads of up to 128, and a tile's offsets fit 32 bits up to row strides
+    // of 8 million values: what does not fit takes a wavefront per row.
+    if (!few && (!tile_strides_fit(a) || (a.type == F32 && !attention32_fits(a)))) {
+        switch (a.type) {
+            case F16: return launch_rows<_Float16>(a, s);
+            case BF16: return launch_rows<__bf16>(a, s);
+            default: return launch_rows<float>(a, s);
+        }
+    }
     const Spread &sp = few ? FEW : TILES;
     const size_t group = a.rel ? 1 : a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, sp.tile);
     size_t keys = a.seqs.tables ? (size_t)a.seqs.width * a.seqs.page

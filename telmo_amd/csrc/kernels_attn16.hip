@@ -15,7 +15,10 @@ namespace tg {
 
 namespace {
 
-constexpr int THREADS = 256, TILE_Q = 128, TILE_K = 64;
+constexpr int THREADS = 256, TILE_Q = 128;
+
+// What a call does to its scores, in what it costs: a kernel of each kind.
+enum Extra { PLAIN, CAPS, ALL };  // nothing; caps and slopes; tables and documents too
 
 template <typename T>
 struct Half;
@@ -36,14 +39,16 @@ struct Half<__bf16> {
     }
 };
 
-// D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
-template <typename T, int D, bool PAGED, bool EXTRA>
+// D: head size rounded up to 64, 128 or 256.
+template <typename T, int D, bool PAGED, Extra EXTRA>
 __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(const AttnArgs a, const AttnParts parts,
                                                                               const int q_tiles, const int groups) {
     typedef typename Half<T>::v8 v8;
+    constexpr int TILE_K = D == 256 ? 32 : 64;  // keys of a tile: the output of 256 columns leaves room for 32
+    constexpr int HALVES = TILE_K / 32, N = TILE_K / 2;  // score products of a tile, scores of a lane
+    constexpr int AHEAD = 4;  // operands on their way from LDS
     constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
     __shared__ __align__(16) T ks[TILE_K * D], vs[TILE_K * D];
-    __shared__ int marks[TILE_K];
 
     Place at;
     if (!at.find(a, parts.parts, q_tiles, groups, a.kv_heads, TILE_Q)) return;
@@ -51,7 +56,8 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     const AttnSpan sp = at.sp;
     const int64_t pairs = at.pairs, pair0 = at.pair0;
 
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
     // The lane's query, and the first and last of the wavefront's and the workgroup's.
     const int64_t pair = pair0 + wave * 32 + col;
@@ -84,39 +90,35 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     // This thread's part of the tiles: rows row0 + u STEP, chunk c of each.
     const int row0 = t / CHUNKS, c = t % CHUNKS;
     const bool in_d = c * 8 < a.d;
-    const T *kp = static_cast<const T *>(a.k) + kvh * a.hsk + (in_d ? c * 8 : 0);
-    const T *vp = static_cast<const T *>(a.v) + kvh * a.hsv + (in_d ? c * 8 : 0);
+    KeyRows<T, TILE_K, PER, STEP, PAGED> keys(a, sp, kvh, row0, in_d ? c * 8 : 0);
     u32x4 kr[PER], vr[PER];
-    int mark[PER];
+    uint64_t homeless = 0;  // of the loaded tile's keys
+    int doc_k = 0;          // the lane's key's document
+    const auto look = [&](int kb) { keys.look(a, sp, b, kb, lane); };
     const auto load = [&](int kb) {
-#pragma unroll
-        for (int u = 0; u < PER; u++) {
-            int j = kb + row0 + u * STEP;
-            const bool in = j < sp.nk && in_d;
-            j = j < sp.nk ? j : sp.nk - 1;
-            int64_t kat, vat;
-            if (PAGED) {
-                const int p = page_of(a.seqs, b, j), s = j % a.seqs.page;
-                mark[u] = p < 0 ? -1 : 0;
-                kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
-                vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
-            } else {
-                kat = (int64_t)(sp.k0 + j) * a.ldk;
-                vat = (int64_t)(sp.k0 + j) * a.ldv;
-                if (EXTRA && a.q_docs) mark[u] = a.k_docs[sp.k0 + j];
-            }
-            kr[u] = *reinterpret_cast<const u32x4 *>(kp + kat);
-            vr[u] = *reinterpret_cast<const u32x4 *>(vp + vat);
-            if (!in) kr[u] = vr[u] = u32x4{};
+        homeless = keys.homeless();
+        keys.each(a, sp, kb, [&](int u, const char *k, const char *v) {
+            kr[u] = *reinterpret_cast<const u32x4 *>(k);
+            vr[u] = *reinterpret_cast<const u32x4 *>(v);
+        });
+        if (EXTRA == ALL && a.q_docs) {
+            const int j = kb + lane;
+            doc_k = a.k_docs[sp.k0 + (j < sp.nk ? j : sp.nk - 1)];
         }
+        if (a.d < D)  // the columns that fill D up: values of any kind, but none that meets the queries' zeros
+#pragma unroll
+            for (int u = 0; u < PER; u++) kr[u] = in_d ? kr[u] : u32x4{};
     };
 
     f32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.0f;
     const float mul = a.scale * LOG2E;
-    const bool marked = PAGED || (EXTRA && a.q_docs);
 
-    if (n0 < n1) load(tiles.at(n0));
+    if (n0 < n1) {
+        look(tiles.at(n0));
+        load(tiles.at(n0));
+        if (n0 + 1 < n1) look(tiles.at(n0 + 1));
+    }
     for (int n = n0; n < n1; n++) {
         const int kb = tiles.at(n);
         __syncthreads();  // every wavefront has read the last tile
@@ -125,65 +127,64 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
             const int krow = row0 + u * STEP;
             reinterpret_cast<u32x4 *>(ks)[k_place<CHUNKS>(krow, c)] = kr[u];
             reinterpret_cast<u32x4 *>(vs)[v_place<CHUNKS>(krow, c)] = vr[u];
-            if (marked && c == 0) marks[krow] = mark[u];
         }
         __syncthreads();
+        const uint64_t hide = homeless;
+        const int docs = doc_k;
         if (n + 1 < n1) load(tiles.at(n + 1));
+        if (n + 2 < n1) look(tiles.at(n + 2));
 
         const bool none = !wave_live || ((kb + TILE_K <= w_first.lo || kb >= w_last.hi) && kb >= w_first.prefix);
         if (none) continue;
-        f32x16 s[2] = {};
+        constexpr int SCORES = D / 16 * HALVES;  // products of K: of 16 columns and 32 keys each
+        v8 kf[SCORES];
+        f32x16 s[HALVES] = {};
+        const auto k_fragment = [&](int e) {
+            return reinterpret_cast<const v8 *>(ks)[k_place<CHUNKS>(e % HALVES * 32 + col, e / HALVES * 2 + half)];
+        };
 #pragma unroll
-        for (int e = 0; e < D / 16; e++)
+        for (int e = 0; e < AHEAD; e++) kf[e] = k_fragment(e);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const v8 kf = reinterpret_cast<const v8 *>(ks)[k_place<CHUNKS>(x * 32 + col, e * 2 + half)];
-                s[x] = Half<T>::mfma(kf, qf[e], s[x]);
-            }
+        for (int e = 0; e < SCORES; e++) {
+            s[e % HALVES] = Half<T>::mfma(kf[e], qf[e / HALVES], s[e % HALVES]);
+            if (e + AHEAD < SCORES) kf[e + AHEAD] = k_fragment(e + AHEAD);
+        }
+        feed<SCORES, 1, AHEAD>();
 
         // Scores, and -infinity where the key is not shown.
         const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
-        bool compare = false;  // marks decide key by key
-        if (marked) {
-            const int mk = marks[lane];
-            if (EXTRA && a.q_docs) {
-                const int first = __builtin_amdgcn_readfirstlane(mk);
-                compare = !__all(mk == first && doc == first) || first < 0;
-            } else {
-                compare = __any(mk < 0);
-            }
-        }
-        if (EXTRA) {
-#pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int j = kb + x * 32 + 8 * (e / 4) + 4 * half + e % 4;
-                    s[x][e] = score_of<true>(a, s[x][e], h, slope, j - i);
-                }
-        }
+        if (EXTRA)
+            scores_of<true, N, EXTRA == ALL>(
+                a, [&](int e) -> float & { return reinterpret_cast<float *>(&s[e / 16])[e % 16]; },
+                [&](int e) { return kb + e / 16 * 32 + 8 * (e % 16 / 4) + 4 * half + e % 4; }, h, slope, i);
         if (!full) {
 #pragma unroll
-            for (int x = 0; x < 2; x++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int j = kb + x * 32 + 8 * (e / 4) + 4 * half + e % 4;
-                    if (!win.has(j)) s[x][e] = -INFINITY;
-                }
+            for (int e = 0; e < N; e++)
+                if (!win.has(kb + e / 16 * 32 + 8 * (e % 16 / 4) + 4 * half + e % 4)) s[e / 16][e % 16] = -INFINITY;
         }
-        if (compare) {
+        if (PAGED && hide) {
+            const uint64_t mine = hide >> 4 * half;
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+            for (int e = 0; e < N; e++)
+                if (mine >> (e / 16 * 32 + 8 * (e % 16 / 4) + e % 4) & 1) s[e / 16][e % 16] = -INFINITY;
+        }
+        if (EXTRA == ALL && a.q_docs) {
+            const int first = __builtin_amdgcn_readfirstlane(docs);
+            if (first < 0 || !__all(docs == first && doc == first)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int mk = marks[x * 32 + 8 * (e / 4) + 4 * half + e % 4];
-                    if (mk < 0 || mk != doc) s[x][e] = -INFINITY;
+                for (int e = 0; e < N; e++) {
+                    const int k = e / 16 * 32 + 8 * (e % 16 / 4) + e % 4;
+                    const int lo = __builtin_amdgcn_readlane(docs, k), hi = __builtin_amdgcn_readlane(docs, k + 4);
+                    const int mine = half ? hi : lo;
+                    if (mine < 0 || mine != doc) s[e / 16][e % 16] = -INFINITY;
                 }
+            }
         }
 
         float top = s[0][0];
 #pragma unroll
-        for (int e = 1; e < 32; e++) top = fmaxf(top, s[e / 16][e % 16]);
+        for (int e = 1; e < N; e++) top = fmaxf(top, s[e / 16][e % 16]);
         top = max_halves(top);
         if (__any(top > m)) {
             const float mn = fmaxf(m, top);
@@ -196,9 +197,15 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
         }
         const float base = m == -INFINITY ? 0.0f : m;
         const float off = Half<T>::shift - base * mul;
-        v8 pf[4];
+        v8 pf[N / 8];
+        // The first fragments of V are on their way while the weights are worked out.
+        constexpr int PRODUCTS = N / 8 * (D / 32);
+        s16x8 vf[PRODUCTS];
 #pragma unroll
-        for (int g = 0; g < 4; g++) {
+        for (int e = 0; e < AHEAD; e++) vf[e] = v_fragment<CHUNKS>(vs, e / (D / 32) * 16, e % (D / 32), lane);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int g = 0; g < N / 8; g++) {
             f32x8 p;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -210,11 +217,14 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
             }
             pf[g] = __builtin_convertvector(p, v8);
         }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-#pragma unroll
-            for (int x = 0; x < D / 32; x++)
-                acc[x] = Half<T>::mfma(__builtin_bit_cast(v8, v_fragment<CHUNKS>(vs, g * 16, x, lane)), pf[g], acc[x]);
+        for (int e = 0; e < PRODUCTS; e++) {
+            acc[e % (D / 32)] = Half<T>::mfma(__builtin_bit_cast(v8, vf[e]), pf[e / (D / 32)], acc[e % (D / 32)]);
+            const int next = e + AHEAD;
+            if (next < PRODUCTS) vf[next] = v_fragment<CHUNKS>(vs, next / (D / 32) * 16, next % (D / 32), lane);
+        }
+        feed<PRODUCTS, 2, AHEAD>();
     }
 
     l = sum_halves(l);
@@ -264,7 +274,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     }
 }
 
-template <typename T, int D, bool PAGED, bool EXTRA>
+template <typename T, int D, bool PAGED, Extra EXTRA>
 hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
     const int group = a.heads / a.kv_heads;
     const size_t q_tiles = div_ceil((size_t)a.seqs.longest * group, TILE_Q);
@@ -275,12 +285,16 @@ hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <typename T, int D, bool PAGED>
+hipError_t launch_extra(const AttnArgs &a, int splits, hipStream_t s) {
+    if (a.table || a.q_docs) return launch_tile<T, D, PAGED, ALL>(a, splits, s);
+    if (a.cap > 0.0f || a.slopes) return launch_tile<T, D, PAGED, CAPS>(a, splits, s);
+    return launch_tile<T, D, PAGED, PLAIN>(a, splits, s);
+}
+
 template <typename T, int D>
 hipError_t launch_kind(const AttnArgs &a, int splits, hipStream_t s) {
-    const bool extra = a.cap > 0.0f || a.slopes || a.table || a.q_docs;
-    if (a.seqs.tables)
-        return extra ? launch_tile<T, D, true, true>(a, splits, s) : launch_tile<T, D, true, false>(a, splits, s);
-    return extra ? launch_tile<T, D, false, true>(a, splits, s) : launch_tile<T, D, false, false>(a, splits, s);
+    return a.seqs.tables ? launch_extra<T, D, true>(a, splits, s) : launch_extra<T, D, false>(a, splits, s);
 }
 
 template <typename T>

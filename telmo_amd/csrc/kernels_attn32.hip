@@ -170,7 +170,8 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
             j = j < sp.nk ? j : sp.nk - 1;
             int64_t kat, vat;
             if (PAGED) {
-                const int p = page_of(a.seqs, b, j), s = j % a.seqs.page;
+                int s;
+                const int p = page_of(a.seqs, b, j, s);
                 mark[u] = p < 0 ? -1 : 0;
                 kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
                 vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
@@ -329,7 +330,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
                 const int e = 4 * g + y, k = 8 * g + 4 * half + y, j = kb + k;
                 float x = s[e] * (back[y] * q_back);
                 if (REL) x += sh.terms[wave][col * 64 + ((((block - wave) & 1) * 32 + k - col + 4 * col) & 63)];
-                if (EXTRA) x = score_of<false>(a, x, h, slope, j - i);
+                if (EXTRA) x = score_of(a, x, h, slope, j - i);
                 if (!full && !win.has(j)) x = -INFINITY;
                 s[e] = x;
             }

@@ -112,7 +112,8 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
         if (PAGED) {
             const int key = one_page ? kb : kb + lane % TILE;
             const int j = key < sp.nk ? key : sp.nk - 1;
-            const int p = page_of(a.seqs, b, j), s = j % a.seqs.page;
+            int s;
+            const int p = page_of(a.seqs, b, j, s);
             hidden = (uint32_t)__ballot(p < 0);
             kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
             vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
@@ -194,7 +195,7 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 const int j = kb + x * 16 + quarter * 4 + e;
-                if (EXTRA) s[x][e] = score_of<!F::WIDE>(a, s[x][e], h, slope, j - i);
+                if (EXTRA) s[x][e] = score_of(a, s[x][e], h, slope, j - i);
                 if (!full && !win.has(j)) s[x][e] = -INFINITY;
                 if (PAGED && hide && (one_page || (hide >> (j - kb) & 1))) s[x][e] = -INFINITY;
                 top = fmaxf(top, s[x][e]);

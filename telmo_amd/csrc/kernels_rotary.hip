@@ -134,8 +134,9 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const T *k, int64_t ldk
         if ((int)threadIdx.x < n) {
             const int64_t pos = (int64_t)sp.shift() + r0 + threadIdx.x;
             const bool held = pos >= 0 && pos < sp.nk;
-            page[threadIdx.x] = held ? page_of(q, b, (int)pos) : -1;
-            in_page[threadIdx.x] = held ? (int)(pos % q.page) : 0;
+            int at = 0;
+            page[threadIdx.x] = held ? page_of(q, b, (int)pos, at) : -1;
+            in_page[threadIdx.x] = at;
         }
         for (int t = threadIdx.x; t < n * pairs; t += THREADS)
             table[t / pairs][t % pairs] =

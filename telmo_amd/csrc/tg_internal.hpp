@@ -329,6 +329,9 @@ struct AttnSeqs {
     const int32_t *tables, *lengths;
     int64_t ldt;
     int width, page, pages;  // table entries per sequence, rows per page, pages of the cache
+    // j / page = (j * page_mul) >> page_shift for 0 <= j < 2^31: page_shift = 31 + s with 2^s >= page, and page_mul
+    // = 2^page_shift / page rounded up, which exceeds it by less than 2^s / 2^page_shift = 2^-31 of j.
+    uint32_t page_mul, page_shift;
 };
 
 struct AttnArgs {

@@ -199,8 +199,12 @@ def test_row_numbers_lengths_and_pages_are_cut_to_the_buffers(spans):
 
 
 def test_windows_are_cut_to_the_keys(spans):
-    got = [tuple(int(x) for x in line.split()[1:]) for line in spans("")]
+    got = [tuple(int(x) for x in line.split()[1:]) for line in spans("") if line[0] == "w"]
     assert got == [(0, 10, 0), (3, 6, 0), (0, 0, 0), (10, 10, 10), (0, 10, 0), (0, 0, 3)]
+
+
+def test_pages_are_found_by_multiplication(spans):
+    assert [line for line in spans("") if line[0] == "d"] == ["d 0 1"]
 
 
 def test_scalings_of_the_frequencies():
