@@ -20,28 +20,32 @@ __device__ __forceinline__ float sum_halves(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Where the 16-byte chunk c of a tile's row of CHUNKS chunks lies. K rows are read one chunk of 32 rows at a
-// time and V rows 64 bytes of four rows at a time: either way the chunks of one read fall on different banks.
-template <int CHUNKS>
-__device__ __forceinline__ int k_place(int row, int c) {
-    return row * CHUNKS + (c ^ (CHUNKS == 8 ? (row >> 1) & 7 : row & 15));
-}
-template <int CHUNKS>
-__device__ __forceinline__ int v_place(int row, int c) {
-    return row * CHUNKS + (c ^ (CHUNKS == 8 ? (row << 1) & 4 : (row & 3) << 2));
-}
+// Values between the rows of a tile of 16-bit values in LDS. K rows are read 16 bytes of 16 rows at a time and V rows
+// 64 bytes of four rows at a time: with 16 bytes (64 bytes) between the ends of the rows the pieces of one read fall on
+// different banks, and all pieces that a lane reads lie at constants from one address.
+template <int D>
+constexpr int K_PITCH = D + 8;
+template <int D>
+constexpr int V_PITCH = D + 32;
 
-// Columns 32 x + (lane % 32) of eight rows of a 16-bit tile, the operand V' of 16 keys from row on, in the
-// order in which the first product leaves the keys in a lane: rows 4 (lane / 32) + 0 .. 3, then those 8 on.
-// Two reads of four rows each, transposed by the read.
-template <int CHUNKS>
-__device__ __forceinline__ s16x8 v_fragment(const void *tile, int row, int x, int lane) {
-    const int r = row + (lane >> 5) * 4 + (lane & 15) / 4, c = x * 32 + (lane >> 4 & 1) * 16 + lane % 4 * 4;
-    const short *v = static_cast<const short *>(tile);
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) s16x4 *)(v + v_place<CHUNKS>(r, c / 8) * 8 + c % 8));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (__attribute__((address_space(3))) s16x4 *)(v + v_place<CHUNKS>(r + 8, c / 8) * 8 + c % 8));
+// The lane's place in a tile of K: columns 8 (lane / 32) on of row lane % 32, the operand K of the first 32 rows and 16
+// columns; and in a tile of V: where its transposing reads of the first 16 rows and 32 columns begin.
+template <int D>
+__device__ __forceinline__ int k_lane(int lane) {
+    return (lane & 31) * K_PITCH<D> + (lane >> 5) * 8;
+}
+template <int D>
+__device__ __forceinline__ int v_lane(int lane) {
+    return ((lane >> 5) * 4 + (lane & 15) / 4) * V_PITCH<D> + (lane >> 4 & 1) * 16 + lane % 4 * 4;
+}
+// Columns 32 x + (lane % 32) of 16 rows from row 16 g on, the operand V', in the order in which the first product leaves
+// the keys in a lane: rows 4 (lane / 32) + 0 .. 3, then those 8 on. Two reads of four rows each, transposed by the read.
+template <int D>
+__device__ __forceinline__ s16x8 v_fragment(const void *at, int g, int x) {
+    const short *v = static_cast<const short *>(at) + g * 16 * V_PITCH<D> + x * 32;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)v);
+    const s16x4 hi =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(v + 8 * V_PITCH<D>));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 

@@ -48,7 +48,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     constexpr int HALVES = TILE_K / 32, N = TILE_K / 2;  // score products of a tile, scores of a lane
     constexpr int AHEAD = 4;  // operands on their way from LDS
     constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
-    __shared__ __align__(16) T ks[TILE_K * D], vs[TILE_K * D];
+    __shared__ __align__(16) T k_tiles[2][TILE_K * K_PITCH<D>], v_tiles[2][TILE_K * V_PITCH<D>];
 
     Place at;
     if (!at.find(a, parts.parts, q_tiles, groups, a.kv_heads, TILE_Q)) return;
@@ -114,33 +114,36 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     float m = -INFINITY, l = 0.0f;
     const float mul = a.scale * LOG2E;
 
+    // Two tiles in LDS: while one is worked on, the next one, which left memory a tile ago, is written to the
+    // other, and the one after it leaves memory.
+    uint64_t hide = 0;  // of the tile that is worked on
+    int docs = 0;
+    const auto store = [&](int n) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            *reinterpret_cast<u32x4 *>(&k_tiles[n & 1][row0 * K_PITCH<D> + c * 8 + u * STEP * K_PITCH<D>]) = kr[u];
+            *reinterpret_cast<u32x4 *>(&v_tiles[n & 1][row0 * V_PITCH<D> + c * 8 + u * STEP * V_PITCH<D>]) = vr[u];
+        }
+        hide = homeless;
+        docs = doc_k;
+        if (n + 1 < n1) load(tiles.at(n + 1));
+        if (n + 2 < n1) look(tiles.at(n + 2));
+    };
     if (n0 < n1) {
         look(tiles.at(n0));
         load(tiles.at(n0));
         if (n0 + 1 < n1) look(tiles.at(n0 + 1));
+        store(n0);
+        __syncthreads();
     }
     for (int n = n0; n < n1; n++) {
         const int kb = tiles.at(n);
-        __syncthreads();  // every wavefront has read the last tile
-#pragma unroll
-        for (int u = 0; u < PER; u++) {
-            const int krow = row0 + u * STEP;
-            reinterpret_cast<u32x4 *>(ks)[k_place<CHUNKS>(krow, c)] = kr[u];
-            reinterpret_cast<u32x4 *>(vs)[v_place<CHUNKS>(krow, c)] = vr[u];
-        }
-        __syncthreads();
-        const uint64_t hide = homeless;
-        const int docs = doc_k;
-        if (n + 1 < n1) load(tiles.at(n + 1));
-        if (n + 2 < n1) look(tiles.at(n + 2));
-
-        const bool none = !wave_live || ((kb + TILE_K <= w_first.lo || kb >= w_last.hi) && kb >= w_first.prefix);
-        if (none) continue;
+        const T *ks = k_tiles[n & 1] + k_lane<D>(lane), *vs = v_tiles[n & 1] + v_lane<D>(lane);
         constexpr int SCORES = D / 16 * HALVES;  // products of K: of 16 columns and 32 keys each
         v8 kf[SCORES];
         f32x16 s[HALVES] = {};
         const auto k_fragment = [&](int e) {
-            return reinterpret_cast<const v8 *>(ks)[k_place<CHUNKS>(e % HALVES * 32 + col, e / HALVES * 2 + half)];
+            return *reinterpret_cast<const v8 *>(ks + e % HALVES * 32 * K_PITCH<D> + e / HALVES * 16);
         };
 #pragma unroll
         for (int e = 0; e < AHEAD; e++) kf[e] = k_fragment(e);
@@ -202,7 +205,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
         constexpr int PRODUCTS = N / 8 * (D / 32);
         s16x8 vf[PRODUCTS];
 #pragma unroll
-        for (int e = 0; e < AHEAD; e++) vf[e] = v_fragment<CHUNKS>(vs, e / (D / 32) * 16, e % (D / 32), lane);
+        for (int e = 0; e < AHEAD; e++) vf[e] = v_fragment<D>(vs, e / (D / 32), e % (D / 32));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < N / 8; g++) {
@@ -217,14 +220,16 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
             }
             pf[g] = __builtin_convertvector(p, v8);
         }
+        if (n + 1 < n1) store(n + 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < PRODUCTS; e++) {
             acc[e % (D / 32)] = Half<T>::mfma(__builtin_bit_cast(v8, vf[e]), pf[e / (D / 32)], acc[e % (D / 32)]);
             const int next = e + AHEAD;
-            if (next < PRODUCTS) vf[next] = v_fragment<CHUNKS>(vs, next / (D / 32) * 16, next % (D / 32), lane);
+            if (next < PRODUCTS) vf[next] = v_fragment<D>(vs, next / (D / 32), next % (D / 32));
         }
         feed<PRODUCTS, 2, AHEAD>();
+        __syncthreads();
     }
 
     l = sum_halves(l);

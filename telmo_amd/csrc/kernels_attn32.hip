@@ -81,11 +81,11 @@ __device__ __forceinline__ float row_sum(float x) {
 
 template <int D, bool REL>
 struct Shared {
-    f16x8 k[2][TILE_K * D / 8];
-    bf16x8 v[3][TILE_K * D / 8];
+    _Float16 k[2][TILE_K * K_PITCH<D>];
+    __bf16 v[3][TILE_K * V_PITCH<D>];
     float k_back[TILE_K];
     int marks[TILE_K];
-    f16x8 r[REL ? RING : 1][2][REL ? TILE_K * D / 8 : 1];
+    _Float16 r[REL ? RING : 1][2][REL ? TILE_K * K_PITCH<D> : 8];
     float r_back[REL ? RING : 1][TILE_K], r_add[REL ? RING : 1][TILE_K];
     float terms[REL ? 4 : 1][REL ? 32 * 64 : 1];  // per wavefront [query][64 distances], turned by 4 per query
 };
@@ -210,8 +210,8 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
             add = row_sum<CHUNKS>(add);
             float x[8];
             for (int e = 0; e < 8; e++) x[e] = rr[u][e] * sc.by;
-            const int to = k_place<CHUNKS>(brow, c);
-            split2(x, sh.r[slot][0][to], sh.r[slot][1][to]);
+            const int to = brow * K_PITCH<D> + c * 8;
+            split2(x, *reinterpret_cast<f16x8 *>(&sh.r[slot][0][to]), *reinterpret_cast<f16x8 *>(&sh.r[slot][1][to]));
             if (c == 0) {
                 sh.r_back[slot][brow] = sc.back;
                 sh.r_add[slot][brow] = add;
@@ -224,8 +224,9 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         f32x16 acc = {};
 #pragma unroll
         for (int s = 0; s < D / 16; s++) {
-            const int from = k_place<CHUNKS>(col, s * 2 + half);
-            const f16x8 rh = sh.r[slot][0][from], rl = sh.r[slot][1][from];
+            const int from = k_lane<D>(lane) + s * 16;
+            const f16x8 rh = *reinterpret_cast<const f16x8 *>(&sh.r[slot][0][from]);
+            const f16x8 rl = *reinterpret_cast<const f16x8 *>(&sh.r[slot][1][from]);
             acc = mfma(rl, qh[s], acc);
             acc = mfma(rh, ql[s], acc);
             acc = mfma(rh, qh[s], acc);
@@ -276,15 +277,16 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         __syncthreads();  // every wavefront has read the last tile
 #pragma unroll
         for (int u = 0; u < PER; u++) {
-            const int krow = row0 + u * STEP, kto = k_place<CHUNKS>(krow, c), vto = v_place<CHUNKS>(krow, c);
+            const int krow = row0 + u * STEP, kto = krow * K_PITCH<D> + c * 8, vto = krow * V_PITCH<D> + c * 8;
             float top = 0.0f, x[8];
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(kr[u][e]));
             const Scale sc = scale_for(row_max<CHUNKS>(top));
             for (int e = 0; e < 8; e++) x[e] = kr[u][e] * sc.by;
-            split2(x, sh.k[0][kto], sh.k[1][kto]);
+            split2(x, *reinterpret_cast<f16x8 *>(&sh.k[0][kto]), *reinterpret_cast<f16x8 *>(&sh.k[1][kto]));
             f32x8 v;
             for (int e = 0; e < 8; e++) v[e] = vr[u][e];
-            split3(v, sh.v[0][vto], sh.v[1][vto], sh.v[2][vto]);
+            split3(v, *reinterpret_cast<bf16x8 *>(&sh.v[0][vto]), *reinterpret_cast<bf16x8 *>(&sh.v[1][vto]),
+                   *reinterpret_cast<bf16x8 *>(&sh.v[2][vto]));
             if (c == 0) {
                 sh.k_back[krow] = sc.back;
                 if (marked) sh.marks[krow] = mark[u];
@@ -303,8 +305,9 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         f32x16 s = {};
 #pragma unroll
         for (int e = 0; e < D / 16; e++) {
-            const int from = k_place<CHUNKS>(col, e * 2 + half);
-            const f16x8 kh = sh.k[0][from], kl = sh.k[1][from];
+            const int from = k_lane<D>(lane) + e * 16;
+            const f16x8 kh = *reinterpret_cast<const f16x8 *>(&sh.k[0][from]);
+            const f16x8 kl = *reinterpret_cast<const f16x8 *>(&sh.k[1][from]);
             s = mfma(kl, qh[e], s);
             s = mfma(kh, ql[e], s);
             s = mfma(kh, qh[e], s);
@@ -369,9 +372,9 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
             split3(p, ph, pm, pl);
 #pragma unroll
             for (int x = 0; x < D / 32; x++) {
-                const bf16x8 vh = __builtin_bit_cast(bf16x8, v_fragment<CHUNKS>(sh.v[0], g * 16, x, lane));
-                const bf16x8 vm = __builtin_bit_cast(bf16x8, v_fragment<CHUNKS>(sh.v[1], g * 16, x, lane));
-                const bf16x8 vl = __builtin_bit_cast(bf16x8, v_fragment<CHUNKS>(sh.v[2], g * 16, x, lane));
+                const bf16x8 vh = __builtin_bit_cast(bf16x8, v_fragment<D>(sh.v[0] + v_lane<D>(lane), g, x));
+                const bf16x8 vm = __builtin_bit_cast(bf16x8, v_fragment<D>(sh.v[1] + v_lane<D>(lane), g, x));
+                const bf16x8 vl = __builtin_bit_cast(bf16x8, v_fragment<D>(sh.v[2] + v_lane<D>(lane), g, x));
                 acc[x] = mfma(vl, ph, acc[x]);
                 acc[x] = mfma(vh, pl, acc[x]);
                 acc[x] = mfma(vm, pm, acc[x]);
