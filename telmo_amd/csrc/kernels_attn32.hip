@@ -84,10 +84,30 @@ struct Shared {
     _Float16 k[2][TILE_K * K_PITCH<D>];
     __bf16 v[3][TILE_K * V_PITCH<D>];
     float k_back[TILE_K];
-    int marks[TILE_K];
     _Float16 r[REL ? RING : 1][2][REL ? TILE_K * K_PITCH<D> : 8];
     float r_back[REL ? RING : 1][TILE_K], r_add[REL ? RING : 1][TILE_K];
     float terms[REL ? 4 : 1][REL ? 32 * 64 : 1];  // per wavefront [query][64 distances], turned by 4 per query
+};
+
+// Eight values of a row of K or of position rows as they go into LDS.
+struct Split2 {
+    f16x8 hi, lo;
+    float back, add;  // of the whole row: the scale's inverse, the product with wu
+};
+template <int CHUNKS>
+__device__ __forceinline__ Split2 split_row(const float *x) {
+    Split2 r;
+    float top = 0.0f, y[8];
+    for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[e]));
+    const Scale sc = scale_for(row_max<CHUNKS>(top));
+    for (int e = 0; e < 8; e++) y[e] = x[e] * sc.by;
+    split2(y, r.hi, r.lo);
+    r.back = sc.back;
+    r.add = 0.0f;
+    return r;
+}
+struct Split3 {
+    bf16x8 hi, mid, lo;
 };
 
 // D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
@@ -95,6 +115,8 @@ template <int D, bool PAGED, bool EXTRA, bool REL>
 __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_kernel(
     const AttnArgs a, const AttnParts parts, const int q_tiles, const int groups) {
     constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
+    constexpr int STEPS = D / 16;  // products along a row
+    constexpr int AHEAD = 2;       // groups of operands on their way from LDS
     __shared__ __align__(16) Shared<D, REL> sh;
 
     Place at;
@@ -104,7 +126,8 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
     const AttnSpan sp = at.sp;
     const int64_t pairs = at.pairs, pair0 = at.pair0;
 
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5, col = lane & 31;
+    const int t = threadIdx.x, lane = t & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
     const int64_t pair = pair0 + wave * 32 + col;
     const bool live = pair < pairs;
@@ -127,13 +150,13 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
     const float slope = EXTRA && a.slopes ? a.slopes[h] : 0.0f;
 
     // The lane's half of its query (plus u), split.
-    f16x8 qh[D / 16], ql[D / 16];
+    f16x8 qh[STEPS], ql[STEPS];
     float q_back;
     {
         const float *q = static_cast<const float *>(a.q) + row * a.ldq + h * a.hsq;
-        float x[D / 16][8], top = 0.0f;
+        float x[STEPS][8], top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) {
+        for (int s = 0; s < STEPS; s++) {
             const int c = s * 16 + half * 8;
             const bool in = live && c < a.d;
             if (in) {
@@ -148,7 +171,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         const Scale sc = scale_for(max_halves(top));
         q_back = sc.back;
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) {
+        for (int s = 0; s < STEPS; s++) {
             for (int e = 0; e < 8; e++) x[s][e] *= sc.by;
             split2(x[s], qh[s], ql[s]);
         }
@@ -157,95 +180,124 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
     // This thread's part of the tiles: rows row0 + u STEP, chunk c of each.
     const int row0 = t / CHUNKS, c = t % CHUNKS;
     const bool in_d = c * 8 < a.d;
-    const float *kp = static_cast<const float *>(a.k) + kvh * a.hsk + (in_d ? c * 8 : 0);
-    const float *vp = static_cast<const float *>(a.v) + kvh * a.hsv + (in_d ? c * 8 : 0);
+    KeyRows<float, TILE_K, PER, STEP, PAGED> keys(a, sp, kvh, row0, in_d ? c * 8 : 0);
     const float *rp = REL ? a.rel + h * a.hsrel + (in_d ? c * 8 : 0) : nullptr;
     float kr[PER][8], vr[PER][8], rr[PER][8], wu[8];
-    int mark[PER];
+    uint64_t homeless = 0;  // of the loaded tile's keys
+    int doc_k = 0;          // the lane's key's document
+    const auto look = [&](int kb) { keys.look(a, sp, b, kb, lane); };
     const auto load = [&](int kb) {
-#pragma unroll
-        for (int u = 0; u < PER; u++) {
-            int j = kb + row0 + u * STEP;
-            const bool in = j < sp.nk && in_d;
-            j = j < sp.nk ? j : sp.nk - 1;
-            int64_t kat, vat;
-            if (PAGED) {
-                int s;
-                const int p = page_of(a.seqs, b, j, s);
-                mark[u] = p < 0 ? -1 : 0;
-                kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
-                vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
-            } else {
-                kat = (int64_t)(sp.k0 + j) * a.ldk;
-                vat = (int64_t)(sp.k0 + j) * a.ldv;
-                if (EXTRA && a.q_docs) mark[u] = a.k_docs[sp.k0 + j];
-            }
-            load8(kp + kat, kr[u]);
-            load8(vp + vat, vr[u]);
-            for (int e = 0; e < 8; e++) kr[u][e] = in ? kr[u][e] : 0.0f, vr[u][e] = in ? vr[u][e] : 0.0f;
+        homeless = keys.homeless();
+        keys.each(a, sp, kb, [&](int u, const char *k, const char *v) {
+            load8(reinterpret_cast<const float *>(k), kr[u]);
+            load8(reinterpret_cast<const float *>(v), vr[u]);
+        });
+        if (EXTRA && a.q_docs) {
+            const int j = kb + col;
+            doc_k = a.k_docs[sp.k0 + (j < sp.nk ? j : sp.nk - 1)];
         }
     };
     // Block n of position rows: distances 32 n - (the workgroup's first position) and on.
     const int first_i = sp.shift() + (int)pair0;
-    const auto load_block = [&](int n) {
+    const auto load_block = [&](int n, float(&x)[PER][8]) {
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             const int64_t distance = (int64_t)n * 32 - first_i + row0 + u * STEP;
             const int64_t at = distance < -a.rel_span ? 0 : distance > a.rel_span ? 2 * (int64_t)a.rel_span : distance + a.rel_span;
-            load8(rp + at * a.ldrel, rr[u]);
-            for (int e = 0; e < 8; e++) rr[u][e] = in_d ? rr[u][e] : 0.0f;
+            load8(rp + at * a.ldrel, x[u]);
         }
     };
-    const auto store_block = [&](int n) {
+    // The columns that fill D up hold values of any kind: zeros in their place meet the queries' zeros.
+    const auto fill = [&](float(&x)[PER][8]) {
+        if (a.d < D)
+#pragma unroll
+            for (int u = 0; u < PER; u++)
+                for (int e = 0; e < 8; e++) x[u][e] = in_d ? x[u][e] : 0.0f;
+    };
+    const auto split_block = [&](float(&x)[PER][8], Split2(&y)[PER]) {
+        fill(x);
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            float add = 0.0f;
+            for (int e = 0; e < 8; e++) add = __builtin_fmaf(wu[e], x[u][e], add);
+            y[u] = split_row<CHUNKS>(x[u]);
+            y[u].add = row_sum<CHUNKS>(add);
+        }
+    };
+    const auto store_block = [&](int n, const Split2(&y)[PER]) {
         const int slot = n & (RING - 1);
 #pragma unroll
         for (int u = 0; u < PER; u++) {
-            const int brow = row0 + u * STEP;
-            float top = 0.0f, add = 0.0f;
-            for (int e = 0; e < 8; e++) {
-                top = fmaxf(top, fabsf(rr[u][e]));
-                add = __builtin_fmaf(wu[e], rr[u][e], add);
-            }
-            const Scale sc = scale_for(row_max<CHUNKS>(top));
-            add = row_sum<CHUNKS>(add);
-            float x[8];
-            for (int e = 0; e < 8; e++) x[e] = rr[u][e] * sc.by;
-            const int to = brow * K_PITCH<D> + c * 8;
-            split2(x, *reinterpret_cast<f16x8 *>(&sh.r[slot][0][to]), *reinterpret_cast<f16x8 *>(&sh.r[slot][1][to]));
+            const int brow = row0 + u * STEP, to = brow * K_PITCH<D> + c * 8;
+            *reinterpret_cast<f16x8 *>(&sh.r[slot][0][to]) = y[u].hi;
+            *reinterpret_cast<f16x8 *>(&sh.r[slot][1][to]) = y[u].lo;
             if (c == 0) {
-                sh.r_back[slot][brow] = sc.back;
-                sh.r_add[slot][brow] = add;
+                sh.r_back[slot][brow] = y[u].back;
+                sh.r_add[slot][brow] = y[u].add;
             }
         }
+    };
+    // The three products along the rows of a tile (hi and lo) in LDS with the queries.
+    const auto along = [&](const _Float16 *hi, const _Float16 *lo) {
+        f16x8 xh[STEPS], xl[STEPS];
+        f32x16 s = {};
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) {
+            xl[e] = *reinterpret_cast<const f16x8 *>(lo + e * 16);
+            xh[e] = *reinterpret_cast<const f16x8 *>(hi + e * 16);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < STEPS; e++) {
+            s = mfma(xl[e], qh[e], s);
+            s = mfma(xh[e], ql[e], s);
+            s = mfma(xh[e], qh[e], s);
+            if (e + AHEAD < STEPS) {
+                xl[e + AHEAD] = *reinterpret_cast<const f16x8 *>(lo + (e + AHEAD) * 16);
+                xh[e + AHEAD] = *reinterpret_cast<const f16x8 *>(hi + (e + AHEAD) * 16);
+            }
+        }
+        feed<STEPS, 2, AHEAD, 3>();
+        return s;
     };
     // T of block n for the wavefront's queries, into its ring of two blocks.
     const auto terms_of = [&](int n) {
         const int slot = n & (RING - 1);
-        f32x16 acc = {};
+        const f32x16 acc = along(sh.r[slot][0] + k_lane<D>(lane), sh.r[slot][1] + k_lane<D>(lane));
+        f32x4 back[4], add[4];
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) {
-            const int from = k_lane<D>(lane) + s * 16;
-            const f16x8 rh = *reinterpret_cast<const f16x8 *>(&sh.r[slot][0][from]);
-            const f16x8 rl = *reinterpret_cast<const f16x8 *>(&sh.r[slot][1][from]);
-            acc = mfma(rl, qh[s], acc);
-            acc = mfma(rh, ql[s], acc);
-            acc = mfma(rh, qh[s], acc);
+        for (int e = 0; e < 4; e++) {
+            back[e] = *reinterpret_cast<const f32x4 *>(&sh.r_back[slot][8 * e + 4 * half]);
+            add[e] = *reinterpret_cast<const f32x4 *>(&sh.r_add[slot][8 * e + 4 * half]);
         }
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-            const int d0 = 8 * e + 4 * half;  // the lane's four distances of this register group
-            const f32x4 back = *reinterpret_cast<const f32x4 *>(&sh.r_back[slot][d0]);
-            const f32x4 add = *reinterpret_cast<const f32x4 *>(&sh.r_add[slot][d0]);
-            f32x4 x;
-            for (int y = 0; y < 4; y++) x[y] = __builtin_fmaf(acc[4 * e + y], back[y] * q_back, add[y]);
-            *reinterpret_cast<f32x4 *>(&sh.terms[wave][col * 64 + (((n & 1) * 32 + d0 + 4 * col) & 63)]) = x;
+            f32x4 x;  // the lane's four distances of this register group
+            for (int y = 0; y < 4; y++) x[y] = __builtin_fmaf(acc[4 * e + y], back[e][y] * q_back, add[e][y]);
+            *reinterpret_cast<f32x4 *>(
+                &sh.terms[wave][col * 64 + (((n & 1) * 32 + 8 * e + 4 * half + 4 * col) & 63)]) = x;
         }
     };
 
     f32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.0f;
     const float mul = a.scale * LOG2E;
-    const bool marked = PAGED || (EXTRA && a.q_docs);
+
+    // The loaded tile as it goes into LDS. With position rows, where one wavefront has a SIMD to itself, it is split
+    // while the last products of the tile before run; without, just before, in fewer registers.
+    Split2 ks[PER], rs[PER];
+    Split3 vs[PER];
+    const auto split = [&]() {
+        fill(kr);
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            ks[u] = split_row<CHUNKS>(kr[u]);
+            f32x8 v;
+            for (int e = 0; e < 8; e++) v[e] = vr[u][e];
+            split3(v, vs[u].hi, vs[u].mid, vs[u].lo);
+        }
+        if (REL) split_block(rr, rs);
+    };
 
     if (REL) {
         for (int e = 0; e < 8; e++) {
@@ -254,95 +306,97 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         }
     }
     if (n0 < n1) {
+        look(tiles.at(n0));
         load(tiles.at(n0));
-        if (REL) load_block(tiles.at(n0) / TILE_K);
+        if (REL) load_block(tiles.at(n0) / TILE_K, rr);
+        if (n0 + 1 < n1) look(tiles.at(n0 + 1));
+        if (REL) split();
     }
     for (int n = n0; n < n1; n++) {
         const int kb = tiles.at(n), block = kb / TILE_K;
         if (REL && (n == n0 || tiles.at(n - 1) != kb - TILE_K)) {
             // The first tile of a run: the four blocks before its own, and T of each wavefront's first.
-            float keep[PER][8];
-            for (int u = 0; u < PER; u++)
-                for (int e = 0; e < 8; e++) keep[u][e] = rr[u][e];
+            float x[RING][PER][8];
+#pragma unroll
+            for (int y = 0; y < RING; y++) load_block(block - 1 - y, x[y]);
             __syncthreads();
-            for (int x = 1; x <= RING; x++) {
-                load_block(block - x);
-                store_block(block - x);
+#pragma unroll
+            for (int y = 0; y < RING; y++) {
+                Split2 z[PER];
+                split_block(x[y], z);
+                store_block(block - 1 - y, z);
             }
             __syncthreads();
             terms_of(block - 1 - wave);
-            for (int u = 0; u < PER; u++)
-                for (int e = 0; e < 8; e++) rr[u][e] = keep[u][e];
         }
+        if (!REL) split();
         __syncthreads();  // every wavefront has read the last tile
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             const int krow = row0 + u * STEP, kto = krow * K_PITCH<D> + c * 8, vto = krow * V_PITCH<D> + c * 8;
-            float top = 0.0f, x[8];
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(kr[u][e]));
-            const Scale sc = scale_for(row_max<CHUNKS>(top));
-            for (int e = 0; e < 8; e++) x[e] = kr[u][e] * sc.by;
-            split2(x, *reinterpret_cast<f16x8 *>(&sh.k[0][kto]), *reinterpret_cast<f16x8 *>(&sh.k[1][kto]));
-            f32x8 v;
-            for (int e = 0; e < 8; e++) v[e] = vr[u][e];
-            split3(v, *reinterpret_cast<bf16x8 *>(&sh.v[0][vto]), *reinterpret_cast<bf16x8 *>(&sh.v[1][vto]),
-                   *reinterpret_cast<bf16x8 *>(&sh.v[2][vto]));
-            if (c == 0) {
-                sh.k_back[krow] = sc.back;
-                if (marked) sh.marks[krow] = mark[u];
-            }
+            *reinterpret_cast<f16x8 *>(&sh.k[0][kto]) = ks[u].hi;
+            *reinterpret_cast<f16x8 *>(&sh.k[1][kto]) = ks[u].lo;
+            *reinterpret_cast<bf16x8 *>(&sh.v[0][vto]) = vs[u].hi;
+            *reinterpret_cast<bf16x8 *>(&sh.v[1][vto]) = vs[u].mid;
+            *reinterpret_cast<bf16x8 *>(&sh.v[2][vto]) = vs[u].lo;
+            if (c == 0) sh.k_back[krow] = ks[u].back;
         }
-        if (REL) store_block(block);
+        if (REL) store_block(block, rs);
+        const uint64_t hide = homeless;
+        const int docs = doc_k;
         __syncthreads();
         if (n + 1 < n1) {
             load(tiles.at(n + 1));
-            if (REL) load_block(tiles.at(n + 1) / TILE_K);
+            if (REL) load_block(tiles.at(n + 1) / TILE_K, rr);
         }
+        if (n + 2 < n1) look(tiles.at(n + 2));
 
-        if (REL) terms_of(block - wave);
-        const bool none = !wave_live || ((kb + TILE_K <= w_first.lo || kb >= w_last.hi) && kb >= w_first.prefix);
-        if (none) continue;
-        f32x16 s = {};
-#pragma unroll
-        for (int e = 0; e < D / 16; e++) {
-            const int from = k_lane<D>(lane) + e * 16;
-            const f16x8 kh = *reinterpret_cast<const f16x8 *>(&sh.k[0][from]);
-            const f16x8 kl = *reinterpret_cast<const f16x8 *>(&sh.k[1][from]);
-            s = mfma(kl, qh[e], s);
-            s = mfma(kh, ql[e], s);
-            s = mfma(kh, qh[e], s);
-        }
-
-        // Scores, and -infinity where the key is not shown.
-        const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
-        bool compare = false;  // marks decide key by key
-        if (marked) {
-            const int mk = sh.marks[col];
-            if (EXTRA && a.q_docs) {
-                const int first = __builtin_amdgcn_readfirstlane(mk);
-                compare = !__all(mk == first && doc == first) || first < 0;
-            } else {
-                compare = __any(mk < 0);
-            }
-        }
-#pragma unroll
-        for (int g = 0; g < 4; g++) {
-            const f32x4 back = *reinterpret_cast<const f32x4 *>(&sh.k_back[8 * g + 4 * half]);
-#pragma unroll
-            for (int y = 0; y < 4; y++) {
-                const int e = 4 * g + y, k = 8 * g + 4 * half + y, j = kb + k;
-                float x = s[e] * (back[y] * q_back);
-                if (REL) x += sh.terms[wave][col * 64 + ((((block - wave) & 1) * 32 + k - col + 4 * col) & 63)];
-                if (EXTRA) x = score_of(a, x, h, slope, j - i);
-                if (!full && !win.has(j)) x = -INFINITY;
-                s[e] = x;
-            }
-        }
-        if (compare) {
+        float terms[16];
+        if (REL) {
+            terms_of(block - wave);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const int mk = sh.marks[8 * (e / 4) + 4 * half + e % 4];
-                if (mk < 0 || mk != doc) s[e] = -INFINITY;
+                const int k = 8 * (e / 4) + 4 * half + e % 4;
+                terms[e] = sh.terms[wave][col * 64 + ((((block - wave) & 1) * 32 + k - col + 4 * col) & 63)];
+            }
+        }
+        f32x4 back[4];
+#pragma unroll
+        for (int g = 0; g < 4; g++) back[g] = *reinterpret_cast<const f32x4 *>(&sh.k_back[8 * g + 4 * half]);
+        f32x16 s = along(sh.k[0] + k_lane<D>(lane), sh.k[1] + k_lane<D>(lane));
+
+        // Scores, and -infinity where the key is not shown.
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const float scale = back[e / 4][e % 4] * q_back;
+            s[e] = REL ? __builtin_fmaf(s[e], scale, terms[e]) : s[e] * scale;
+        }
+        const auto key_at = [&](int e) { return kb + 8 * (e / 4) + 4 * half + e % 4; };
+        if (EXTRA)
+            scores_of<false, 16, true>(
+                a, [&](int e) -> float & { return reinterpret_cast<float *>(&s)[e]; }, key_at, h, slope, i);
+        const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
+        if (!full) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (!win.has(key_at(e))) s[e] = -INFINITY;
+        }
+        if (PAGED && hide) {
+            const uint32_t mine = (uint32_t)hide >> 4 * half;
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (mine >> (8 * (e / 4) + e % 4) & 1) s[e] = -INFINITY;
+        }
+        if (EXTRA && a.q_docs) {
+            const int first = __builtin_amdgcn_readfirstlane(docs);
+            if (first < 0 || !__all(docs == first && doc == first)) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int k = 8 * (e / 4) + e % 4;
+                    const int lo = __builtin_amdgcn_readlane(docs, k), hi = __builtin_amdgcn_readlane(docs, k + 4);
+                    const int mine = half ? hi : lo;
+                    if (mine < 0 || mine != doc) s[e] = -INFINITY;
+                }
             }
         }
 
@@ -360,6 +414,19 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
             m = mn;
         }
         const float base = m == -INFINITY ? 0.0f : m;
+
+        // The weights, then per 16 keys and 32 columns six products of three operands each.
+        constexpr int PRODUCTS = 2 * (D / 32);
+        bf16x8 vh[PRODUCTS], vm[PRODUCTS], vl[PRODUCTS], ph[2], pm[2], pl[2];
+        const __bf16 *v_at = sh.v[0] + v_lane<D>(lane);
+        const auto read_v = [&](int e) {
+            const __bf16 *from = v_at;
+            vl[e] = __builtin_bit_cast(bf16x8, v_fragment<D>(from + 2 * TILE_K * V_PITCH<D>, e / (D / 32), e % (D / 32)));
+            vh[e] = __builtin_bit_cast(bf16x8, v_fragment<D>(from, e / (D / 32), e % (D / 32)));
+            vm[e] = __builtin_bit_cast(bf16x8, v_fragment<D>(from + TILE_K * V_PITCH<D>, e / (D / 32), e % (D / 32)));
+        };
+        read_v(0);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int g = 0; g < 2; g++) {
             f32x8 p;
@@ -368,21 +435,21 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
                 p[e] = __builtin_amdgcn_exp2f((s[g * 8 + e] - base) * to_log2);
                 l += p[e];
             }
-            bf16x8 ph, pm, pl;
-            split3(p, ph, pm, pl);
-#pragma unroll
-            for (int x = 0; x < D / 32; x++) {
-                const bf16x8 vh = __builtin_bit_cast(bf16x8, v_fragment<D>(sh.v[0] + v_lane<D>(lane), g, x));
-                const bf16x8 vm = __builtin_bit_cast(bf16x8, v_fragment<D>(sh.v[1] + v_lane<D>(lane), g, x));
-                const bf16x8 vl = __builtin_bit_cast(bf16x8, v_fragment<D>(sh.v[2] + v_lane<D>(lane), g, x));
-                acc[x] = mfma(vl, ph, acc[x]);
-                acc[x] = mfma(vh, pl, acc[x]);
-                acc[x] = mfma(vm, pm, acc[x]);
-                acc[x] = mfma(vm, ph, acc[x]);
-                acc[x] = mfma(vh, pm, acc[x]);
-                acc[x] = mfma(vh, ph, acc[x]);
-            }
+            split3(p, ph[g], pm[g], pl[g]);
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < PRODUCTS; e++) {
+            const int g = e / (D / 32), x = e % (D / 32);
+            acc[x] = mfma(vl[e], ph[g], acc[x]);
+            acc[x] = mfma(vh[e], pl[g], acc[x]);
+            acc[x] = mfma(vm[e], pm[g], acc[x]);
+            if (e + 1 < PRODUCTS) read_v(e + 1);
+            acc[x] = mfma(vm[e], ph[g], acc[x]);
+            acc[x] = mfma(vh[e], pm[g], acc[x]);
+            acc[x] = mfma(vh[e], ph[g], acc[x]);
+        }
+        if (REL && n + 1 < n1) split();
     }
 
     l = sum_halves(l);
