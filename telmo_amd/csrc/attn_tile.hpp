@@ -20,6 +20,16 @@ __device__ __forceinline__ float sum_halves(float x) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// The same over the four lanes 16 apart.
+__device__ __forceinline__ float max_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
 // Values between the rows of a tile of 16-bit values in LDS. K rows are read 16 bytes of 16 rows at a time and V rows
 // 64 bytes of four rows at a time: with 16 bytes (64 bytes) between the ends of the rows the pieces of one read fall on
 // different banks, and all pieces that a lane reads lie at constants from one address.

@@ -1,19 +1,22 @@
 // Attention over f32 rows on the matrix cores, tiles of 128 query rows by 32 keys, to f32's accuracy.
 //
-// The f32 matrix instructions run at an eighth of the rate that the 16-bit ones have for the same shape and k,
-// so each f32 operand is held as a sum of 16-bit ones. For the scores a row x of q, k or the position rows is
-// scaled by a power of two to |x| < 2^15 and held as h + l in f16, 22 bits of it; three products h h', h l' and
-// l h' leave out less than 2^-22 of each term. The weights and the values, which may not share a scale (a
-// value is weighted by other rows' weights), are held as three bf16 each, 24 bits, and six products leave out
-// less than 2^-23. The 32 x 32 x 16 products then cost 3 and 6 instructions in the place of 8 f32 ones that
-// take 8 times as long in all; layout and softmax are those of the 16-bit kernel.
+// The f32 matrix instructions run at a sixteenth of the 16-bit ones' rate, so each f32 operand is held as a sum of
+// 16-bit ones. For the scores a row x of q, k or the position rows is scaled by a power of two to |x| < 2^15 and held
+// as h + l in f16, 22 bits of it; three products h h', h l' and l h' leave out less than 2^-22 of each term. The weights
+// and the values, which may not share a scale (a value is weighted by other rows' weights), are held as three bf16 each,
+// 24 bits, and six products leave out less than 2^-23.
 //
-// Position rows: with T[c, i] = (q_i + w) r_c, the score of key j needs T[j - i, i]. In a tile of 32 queries by
-// 32 keys the distances j - i are those of two blocks of 32 position rows, and the second one is the first
-// of the next tile: each tile adds one product of 32 rows, kept in LDS as [query][64 distances], a ring of
-// two blocks, from which a lane reads its own diagonal. The blocks of the workgroup's wavefronts, whose queries
-// are 32 apart, are the same ones tiles apart: LDS holds the last four. (q + w) r = (q + u) r + (w - u) r, the
-// second part a number per position row, so one copy of the queries serves both products.
+// The layout is that of the 16-bit kernel with 16 x 16 x 32 products: eight wavefronts of 16 queries each, a lane
+// holding one query's scores with 8 of the 32 keys. Two wavefronts to a SIMD, so that one's splitting and exponentials
+// run beside the other's products: with four wavefronts of 32 queries, which read half as much LDS, 16 sequences of 750
+// rows with position rows took 385 us.
+//
+// Position rows: with T[c, i] = (q_i + w) r_c, the score of key j needs T[j - i, i]. The distances j - i of a
+// wavefront's 16 queries and a tile's 32 keys lie in two blocks of 32 position rows, and the second one is the first
+// of the next tile: each tile adds one product of 32 rows, kept in LDS as [query][64 distances], a ring of two blocks,
+// from which a lane reads its own diagonal. Wavefronts whose queries are 32 apart use the same blocks tiles apart: LDS
+// holds the last four. (q + w) r = (q + u) r + (w - u) r, the second part a number per position row, so one copy of
+// the queries serves both products.
 #include "attn_launch.hpp"
 #include "attn_tile.hpp"
 
@@ -21,7 +24,7 @@ namespace tg {
 
 namespace {
 
-constexpr int THREADS = 256, TILE_Q = 128, TILE_K = 32, RING = 4;
+constexpr int WAVES = 8, THREADS = 64 * WAVES, TILE_Q = 16 * WAVES, TILE_K = 32, RING = 4;
 
 // The power of two that brings a row whose largest magnitude is `top` below 2^15, and its inverse. Both stay
 // normal numbers: a row of subnormals is scaled less, which loses nothing that f32 sums would keep.
@@ -35,23 +38,40 @@ __device__ __forceinline__ Scale scale_for(float top) {
 
 // Eight values as sums of two f16 (three bf16) ones.
 __device__ __forceinline__ void split2(const float *x, f16x8 &hi, f16x8 &lo) {
-    f32x8 v;
+    f32x8 v, r;
     for (int e = 0; e < 8; e++) v[e] = x[e];
     hi = __builtin_convertvector(v, f16x8);
-    lo = __builtin_convertvector(v - __builtin_convertvector(hi, f32x8), f16x8);
+    for (int e = 0; e < 8; e++) r[e] = __builtin_fmaf((float)hi[e], -1.0f, v[e]);
+    lo = __builtin_convertvector(r, f16x8);
 }
-__device__ __forceinline__ void split3(const f32x8 v, bf16x8 &hi, bf16x8 &mid, bf16x8 &lo) {
-    hi = __builtin_convertvector(v, bf16x8);
-    const f32x8 r = v - __builtin_convertvector(hi, f32x8);
-    mid = __builtin_convertvector(r, bf16x8);
-    lo = __builtin_convertvector(r - __builtin_convertvector(mid, f32x8), bf16x8);
+struct Split3 {
+    bf16x8 hi, mid, lo;
+};
+// Two values rounded to bf16 in one word, and what that leaves of them.
+__device__ __forceinline__ uint32_t bf16_pair(float &a, float &b) {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+__device__ __forceinline__ Split3 split3(const float *x) {
+    u32x4 w[3];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        float a = x[2 * e], b = x[2 * e + 1];
+#pragma unroll
+        for (int y = 0; y < 3; y++) w[y][e] = bf16_pair(a, b);
+    }
+    return Split3{__builtin_bit_cast(bf16x8, w[0]), __builtin_bit_cast(bf16x8, w[1]), __builtin_bit_cast(bf16x8, w[2])};
 }
 
-__device__ __forceinline__ f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
 // Reductions over the CHUNKS neighbouring lanes that hold one row: quads, halves and whole rows of 16 lanes
@@ -79,15 +99,29 @@ __device__ __forceinline__ float row_sum(float x) {
     return x;
 }
 
+// Values between the rows of a plane of V: its transposing reads take 32 bytes of eight rows at a time.
+template <int D>
+constexpr int V_STEP = D + 16;
+
 template <int D, bool REL>
 struct Shared {
     _Float16 k[2][TILE_K * K_PITCH<D>];
-    __bf16 v[3][TILE_K * V_PITCH<D>];
+    __bf16 v[3][TILE_K * V_STEP<D>];
     float k_back[TILE_K];
     _Float16 r[REL ? RING : 1][2][REL ? TILE_K * K_PITCH<D> : 8];
     float r_back[REL ? RING : 1][TILE_K], r_add[REL ? RING : 1][TILE_K];
-    float terms[REL ? 4 : 1][REL ? 32 * 64 : 1];  // per wavefront [query][64 distances], turned by 4 per query
+    float terms[REL ? WAVES : 1][REL ? 16 * 64 : 1];  // per wavefront [query][64 distances], turned by 4 per query
 };
+
+// Columns 16 x + (lane % 16) of a plane's 32 rows, the operand V', in the order in which the score products leave the
+// keys in a lane: rows 4 (lane / 16) + 0 .. 3 of the first 16 and of the last.
+template <int D>
+__device__ __forceinline__ bf16x8 v_columns(const __bf16 *at, int x) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)(at + x * 16));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4 *)(at + 16 * V_STEP<D> + x * 16));
+    return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
 
 // Eight values of a row of K or of position rows as they go into LDS.
 struct Split2 {
@@ -106,16 +140,13 @@ __device__ __forceinline__ Split2 split_row(const float *x) {
     r.add = 0.0f;
     return r;
 }
-struct Split3 {
-    bf16x8 hi, mid, lo;
-};
-
 // D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
 template <int D, bool PAGED, bool EXTRA, bool REL>
-__global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_kernel(
+__global__ __launch_bounds__(THREADS, 2) void attn_tile32_kernel(
     const AttnArgs a, const AttnParts parts, const int q_tiles, const int groups) {
-    constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
-    constexpr int STEPS = D / 16;  // products along a row
+    // Heads of up to 64 have half as many pieces as threads: two threads handle each alike.
+    constexpr int CHUNKS = D / 8, PER = D <= 128 ? 1 : D / 128, STEP = TILE_K / PER;
+    constexpr int STEPS = D / 32;  // products along a row
     constexpr int AHEAD = 2;       // groups of operands on their way from LDS
     __shared__ __align__(16) Shared<D, REL> sh;
 
@@ -126,15 +157,15 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
     const AttnSpan sp = at.sp;
     const int64_t pairs = at.pairs, pair0 = at.pair0;
 
-    const int t = threadIdx.x, lane = t & 63, half = lane >> 5, col = lane & 31;
+    const int t = threadIdx.x, lane = t & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
-    const int64_t pair = pair0 + wave * 32 + col;
+    const int64_t pair = pair0 + wave * 16 + col;
     const bool live = pair < pairs;
     const int r = live ? (int)(pair / group) : 0, h = at.head * group + (live ? (int)(pair % group) : 0);
     const int i = sp.shift() + r;
     const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
-    const int64_t wave0 = pair0 + wave * 32, wave1 = wave0 + 31 < pairs - 1 ? wave0 + 31 : pairs - 1;
+    const int64_t wave0 = pair0 + wave * 16, wave1 = wave0 + 15 < pairs - 1 ? wave0 + 15 : pairs - 1;
     const int64_t pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
     const auto window_at = [&](int64_t p) {
         return window_of(sp.shift() + (int)(p / group), sp.nk, a.left, a.right, prefix);
@@ -149,7 +180,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
     const int doc = a.q_docs ? (live ? a.q_docs[row] : -1) : 0;
     const float slope = EXTRA && a.slopes ? a.slopes[h] : 0.0f;
 
-    // The lane's half of its query (plus u), split.
+    // The lane's quarter of its query (plus u), split.
     f16x8 qh[STEPS], ql[STEPS];
     float q_back;
     {
@@ -157,7 +188,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         float x[STEPS][8], top = 0.0f;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
-            const int c = s * 16 + half * 8;
+            const int c = s * 32 + quarter * 8;
             const bool in = live && c < a.d;
             if (in) {
                 load8(q + c, x[s]);
@@ -168,7 +199,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
                 for (int e = 0; e < 8; e++) x[s][e] += a.rel_u[(int64_t)h * a.d + c + e];
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[s][e]));
         }
-        const Scale sc = scale_for(max_halves(top));
+        const Scale sc = scale_for(max_quarters(top));
         q_back = sc.back;
 #pragma unroll
         for (int s = 0; s < STEPS; s++) {
@@ -178,7 +209,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
     }
 
     // This thread's part of the tiles: rows row0 + u STEP, chunk c of each.
-    const int row0 = t / CHUNKS, c = t % CHUNKS;
+    const int row0 = t / CHUNKS % TILE_K, c = t % CHUNKS;
     const bool in_d = c * 8 < a.d;
     KeyRows<float, TILE_K, PER, STEP, PAGED> keys(a, sp, kvh, row0, in_d ? c * 8 : 0);
     const float *rp = REL ? a.rel + h * a.hsrel + (in_d ? c * 8 : 0) : nullptr;
@@ -193,7 +224,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
             load8(reinterpret_cast<const float *>(v), vr[u]);
         });
         if (EXTRA && a.q_docs) {
-            const int j = kb + col;
+            const int j = kb + lane % TILE_K;
             doc_k = a.k_docs[sp.k0 + (j < sp.nk ? j : sp.nk - 1)];
         }
     };
@@ -237,54 +268,65 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
             }
         }
     };
-    // The three products along the rows of a tile (hi and lo) in LDS with the queries.
-    const auto along = [&](const _Float16 *hi, const _Float16 *lo) {
-        f16x8 xh[STEPS], xl[STEPS];
-        f32x16 s = {};
+    // The three products of 32 rows (hi and lo, in LDS) with the queries: rows 16 x + 4 quarter + e in s[x][e].
+    const int k_at = col * K_PITCH<D> + quarter * 8;
+    const auto along = [&](const _Float16 *hi, const _Float16 *lo, f32x4(&s)[2]) {
+        f16x8 xh[STEPS][2], xl[STEPS][2];
+        const auto read = [&](int e) {
 #pragma unroll
-        for (int e = 0; e < AHEAD; e++) {
-            xl[e] = *reinterpret_cast<const f16x8 *>(lo + e * 16);
-            xh[e] = *reinterpret_cast<const f16x8 *>(hi + e * 16);
-        }
+            for (int x = 0; x < 2; x++) {
+                xl[e][x] = *reinterpret_cast<const f16x8 *>(lo + k_at + x * 16 * K_PITCH<D> + e * 32);
+                xh[e][x] = *reinterpret_cast<const f16x8 *>(hi + k_at + x * 16 * K_PITCH<D> + e * 32);
+            }
+        };
+        s[0] = s[1] = f32x4{};
+#pragma unroll
+        for (int e = 0; e < AHEAD; e++) read(e);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int e = 0; e < STEPS; e++) {
-            s = mfma(xl[e], qh[e], s);
-            s = mfma(xh[e], ql[e], s);
-            s = mfma(xh[e], qh[e], s);
-            if (e + AHEAD < STEPS) {
-                xl[e + AHEAD] = *reinterpret_cast<const f16x8 *>(lo + (e + AHEAD) * 16);
-                xh[e + AHEAD] = *reinterpret_cast<const f16x8 *>(hi + (e + AHEAD) * 16);
-            }
+            s[0] = mfma(xl[e][0], qh[e], s[0]);
+            s[1] = mfma(xl[e][1], qh[e], s[1]);
+            s[0] = mfma(xh[e][0], ql[e], s[0]);
+            s[1] = mfma(xh[e][1], ql[e], s[1]);
+            s[0] = mfma(xh[e][0], qh[e], s[0]);
+            s[1] = mfma(xh[e][1], qh[e], s[1]);
+            if (e + AHEAD < STEPS) read(e + AHEAD);
         }
-        feed<STEPS, 2, AHEAD, 3>();
-        return s;
+        feed<STEPS, 4, AHEAD, 6>();
     };
     // T of block n for the wavefront's queries, into its ring of two blocks.
     const auto terms_of = [&](int n) {
         const int slot = n & (RING - 1);
-        const f32x16 acc = along(sh.r[slot][0] + k_lane<D>(lane), sh.r[slot][1] + k_lane<D>(lane));
-        f32x4 back[4], add[4];
+        f32x4 s[2], back[2], add[2];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            back[e] = *reinterpret_cast<const f32x4 *>(&sh.r_back[slot][8 * e + 4 * half]);
-            add[e] = *reinterpret_cast<const f32x4 *>(&sh.r_add[slot][8 * e + 4 * half]);
+        for (int x = 0; x < 2; x++) {
+            back[x] = *reinterpret_cast<const f32x4 *>(&sh.r_back[slot][x * 16 + quarter * 4]);
+            add[x] = *reinterpret_cast<const f32x4 *>(&sh.r_add[slot][x * 16 + quarter * 4]);
         }
+        along(sh.r[slot][0], sh.r[slot][1], s);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            f32x4 x;  // the lane's four distances of this register group
-            for (int y = 0; y < 4; y++) x[y] = __builtin_fmaf(acc[4 * e + y], back[e][y] * q_back, add[e][y]);
+        for (int x = 0; x < 2; x++) {
+            f32x4 y;
+            for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(s[x][e], back[x][e] * q_back, add[x][e]);
             *reinterpret_cast<f32x4 *>(
-                &sh.terms[wave][col * 64 + (((n & 1) * 32 + 8 * e + 4 * half + 4 * col) & 63)]) = x;
+                &sh.terms[wave][col * 64 + (((n & 1) * 32 + x * 16 + quarter * 4 + 4 * col) & 63)]) = y;
         }
     };
+    // Where the term of the lane's key 16 x + 4 quarter + e lies when its block is an even one; the odd ones' lie 32 on
+    // in the ring of 64, the bit of 32 turned over. Odd wavefronts' queries are 16 on from their block's.
+    int term_at[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        term_at[e] = col * 64 + ((e / 4 * 16 + 4 * quarter + e % 4 - (wave & 1) * 16 + 3 * col) & 63);
 
-    f32x16 acc[D / 32] = {};
+    f32x4 acc[D / 16] = {};
     float m = -INFINITY, l = 0.0f;
     const float mul = a.scale * LOG2E;
 
-    // The loaded tile as it goes into LDS. With position rows, where one wavefront has a SIMD to itself, it is split
-    // while the last products of the tile before run; without, just before, in fewer registers.
+    // The loaded tile as it goes into LDS, split while the last products of the tile before run where the registers
+    // hold both.
+    constexpr bool EARLY = D <= 128;
     Split2 ks[PER], rs[PER];
     Split3 vs[PER];
     const auto split = [&]() {
@@ -292,9 +334,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             ks[u] = split_row<CHUNKS>(kr[u]);
-            f32x8 v;
-            for (int e = 0; e < 8; e++) v[e] = vr[u][e];
-            split3(v, vs[u].hi, vs[u].mid, vs[u].lo);
+            vs[u] = split3(vr[u]);
         }
         if (REL) split_block(rr, rs);
     };
@@ -310,7 +350,7 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         load(tiles.at(n0));
         if (REL) load_block(tiles.at(n0) / TILE_K, rr);
         if (n0 + 1 < n1) look(tiles.at(n0 + 1));
-        if (REL) split();
+        if (EARLY) split();
     }
     for (int n = n0; n < n1; n++) {
         const int kb = tiles.at(n), block = kb / TILE_K;
@@ -327,13 +367,13 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
                 store_block(block - 1 - y, z);
             }
             __syncthreads();
-            terms_of(block - 1 - wave);
+            terms_of(block - 1 - wave / 2);
         }
-        if (!REL) split();
+        if (!EARLY) split();
         __syncthreads();  // every wavefront has read the last tile
 #pragma unroll
         for (int u = 0; u < PER; u++) {
-            const int krow = row0 + u * STEP, kto = krow * K_PITCH<D> + c * 8, vto = krow * V_PITCH<D> + c * 8;
+            const int krow = row0 + u * STEP, kto = krow * K_PITCH<D> + c * 8, vto = krow * V_STEP<D> + c * 8;
             *reinterpret_cast<f16x8 *>(&sh.k[0][kto]) = ks[u].hi;
             *reinterpret_cast<f16x8 *>(&sh.k[1][kto]) = ks[u].lo;
             *reinterpret_cast<bf16x8 *>(&sh.v[0][vto]) = vs[u].hi;
@@ -351,50 +391,44 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
         }
         if (n + 2 < n1) look(tiles.at(n + 2));
 
-        float terms[16];
+        float terms[8];
         if (REL) {
-            terms_of(block - wave);
+            const int n_block = block - wave / 2;
+            terms_of(n_block);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int k = 8 * (e / 4) + 4 * half + e % 4;
-                terms[e] = sh.terms[wave][col * 64 + ((((block - wave) & 1) * 32 + k - col + 4 * col) & 63)];
-            }
+            for (int e = 0; e < 8; e++) terms[e] = sh.terms[wave][term_at[e] ^ (n_block & 1) * 32];
         }
-        f32x4 back[4];
+        f32x4 back[2], dots[2];
 #pragma unroll
-        for (int g = 0; g < 4; g++) back[g] = *reinterpret_cast<const f32x4 *>(&sh.k_back[8 * g + 4 * half]);
-        f32x16 s = along(sh.k[0] + k_lane<D>(lane), sh.k[1] + k_lane<D>(lane));
+        for (int x = 0; x < 2; x++) back[x] = *reinterpret_cast<const f32x4 *>(&sh.k_back[x * 16 + quarter * 4]);
+        along(sh.k[0], sh.k[1], dots);
 
         // Scores, and -infinity where the key is not shown.
+        float s[8];
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
+        for (int e = 0; e < 8; e++) {
             const float scale = back[e / 4][e % 4] * q_back;
-            s[e] = REL ? __builtin_fmaf(s[e], scale, terms[e]) : s[e] * scale;
+            s[e] = REL ? __builtin_fmaf(dots[e / 4][e % 4], scale, terms[e]) : dots[e / 4][e % 4] * scale;
         }
-        const auto key_at = [&](int e) { return kb + 8 * (e / 4) + 4 * half + e % 4; };
-        if (EXTRA)
-            scores_of<false, 16, true>(
-                a, [&](int e) -> float & { return reinterpret_cast<float *>(&s)[e]; }, key_at, h, slope, i);
+        const auto key_at = [&](int e) { return kb + e / 4 * 16 + 4 * quarter + e % 4; };
+        if (EXTRA) scores_of<false, 8, true>(a, [&](int e) -> float & { return s[e]; }, key_at, h, slope, i);
         const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
         if (!full) {
 #pragma unroll
-            for (int e = 0; e < 16; e++)
+            for (int e = 0; e < 8; e++)
                 if (!win.has(key_at(e))) s[e] = -INFINITY;
         }
         if (PAGED && hide) {
-            const uint32_t mine = (uint32_t)hide >> 4 * half;
 #pragma unroll
-            for (int e = 0; e < 16; e++)
-                if (mine >> (8 * (e / 4) + e % 4) & 1) s[e] = -INFINITY;
+            for (int e = 0; e < 8; e++)
+                if ((uint32_t)hide >> (key_at(e) - kb) & 1) s[e] = -INFINITY;
         }
         if (EXTRA && a.q_docs) {
             const int first = __builtin_amdgcn_readfirstlane(docs);
             if (first < 0 || !__all(docs == first && doc == first)) {
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    const int k = 8 * (e / 4) + e % 4;
-                    const int lo = __builtin_amdgcn_readlane(docs, k), hi = __builtin_amdgcn_readlane(docs, k + 4);
-                    const int mine = half ? hi : lo;
+                for (int e = 0; e < 8; e++) {
+                    const int mine = __shfl(docs, key_at(e) - kb);
                     if (mine < 0 || mine != doc) s[e] = -INFINITY;
                 }
             }
@@ -402,94 +436,90 @@ __global__ __launch_bounds__(THREADS, REL || D == 256 ? 1 : 2) void attn_tile32_
 
         float top = s[0];
 #pragma unroll
-        for (int e = 1; e < 16; e++) top = fmaxf(top, s[e]);
-        top = max_halves(top);
+        for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
+        top = max_quarters(top);
         const float to_log2 = EXTRA ? LOG2E : mul;
         if (__any(top > m)) {
             const float mn = fmaxf(m, top);
             const float fade = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mn) * to_log2);
             l *= fade;
 #pragma unroll
-            for (int x = 0; x < D / 32; x++) acc[x] *= fade;
+            for (int x = 0; x < D / 16; x++) acc[x] *= fade;
             m = mn;
         }
         const float base = m == -INFINITY ? 0.0f : m;
 
-        // The weights, then per 16 keys and 32 columns six products of three operands each.
-        constexpr int PRODUCTS = 2 * (D / 32);
-        bf16x8 vh[PRODUCTS], vm[PRODUCTS], vl[PRODUCTS], ph[2], pm[2], pl[2];
-        const __bf16 *v_at = sh.v[0] + v_lane<D>(lane);
-        const auto read_v = [&](int e) {
-            const __bf16 *from = v_at;
-            vl[e] = __builtin_bit_cast(bf16x8, v_fragment<D>(from + 2 * TILE_K * V_PITCH<D>, e / (D / 32), e % (D / 32)));
-            vh[e] = __builtin_bit_cast(bf16x8, v_fragment<D>(from, e / (D / 32), e % (D / 32)));
-            vm[e] = __builtin_bit_cast(bf16x8, v_fragment<D>(from + TILE_K * V_PITCH<D>, e / (D / 32), e % (D / 32)));
+        // The weights, then per 16 columns six products of three operands each.
+        constexpr int COLUMNS = D / 16;
+        bf16x8 vh[COLUMNS], vm[COLUMNS], vl[COLUMNS];
+        const __bf16 *v_at = sh.v[0] + (quarter * 4 + col / 4) * V_STEP<D> + col % 4 * 4;
+        const auto read_v = [&](int x) {
+            vl[x] = v_columns<D>(v_at + 2 * TILE_K * V_STEP<D>, x);
+            vh[x] = v_columns<D>(v_at, x);
+            vm[x] = v_columns<D>(v_at + TILE_K * V_STEP<D>, x);
         };
-        read_v(0);
+#pragma unroll
+        for (int x = 0; x < AHEAD; x++) read_v(x);
+        __builtin_amdgcn_sched_barrier(0);
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            p[e] = __builtin_amdgcn_exp2f((s[e] - base) * to_log2);
+            l += p[e];
+        }
+        const Split3 ps = split3(p);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            f32x8 p;
+        for (int x = 0; x < COLUMNS; x += 2) {
+            // Two columns' products in turn: none waits for the one before it.
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                p[e] = __builtin_amdgcn_exp2f((s[g * 8 + e] - base) * to_log2);
-                l += p[e];
-            }
-            split3(p, ph[g], pm[g], pl[g]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+            for (int y = x; y < x + 2; y++) acc[y] = mfma(vl[y], ps.hi, acc[y]);
 #pragma unroll
-        for (int e = 0; e < PRODUCTS; e++) {
-            const int g = e / (D / 32), x = e % (D / 32);
-            acc[x] = mfma(vl[e], ph[g], acc[x]);
-            acc[x] = mfma(vh[e], pl[g], acc[x]);
-            acc[x] = mfma(vm[e], pm[g], acc[x]);
-            if (e + 1 < PRODUCTS) read_v(e + 1);
-            acc[x] = mfma(vm[e], ph[g], acc[x]);
-            acc[x] = mfma(vh[e], pm[g], acc[x]);
-            acc[x] = mfma(vh[e], ph[g], acc[x]);
+            for (int y = x; y < x + 2; y++) acc[y] = mfma(vh[y], ps.lo, acc[y]);
+#pragma unroll
+            for (int y = x; y < x + 2; y++) acc[y] = mfma(vm[y], ps.mid, acc[y]);
+#pragma unroll
+            for (int y = x; y < x + 2; y++) acc[y] = mfma(vm[y], ps.hi, acc[y]);
+#pragma unroll
+            for (int y = x; y < x + 2; y++) acc[y] = mfma(vh[y], ps.mid, acc[y]);
+#pragma unroll
+            for (int y = x; y < x + 2; y++) acc[y] = mfma(vh[y], ps.hi, acc[y]);
+            if (x + 2 < COLUMNS) read_v(x + 2), read_v(x + 3);
         }
-        if (REL && n + 1 < n1) split();
+        feed<COLUMNS / 2, 12, 1, 12>();
+        if (EARLY && n + 1 < n1) split();
     }
 
-    l = sum_halves(l);
+    l = sum_quarters(l);
     if (parts.parts > 1) {
         if (!live) return;
         const size_t to = (size_t)part * parts.pairs + row * a.heads + h;
-        if (half == 0) {
+        if (quarter == 0) {
             parts.top[to] = EXTRA ? m : m * a.scale;
             parts.sum[to] = l;
         }
         float *o = parts.out + to * a.d;
 #pragma unroll
-        for (int x = 0; x < D / 32; x++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int oc = x * 32 + 8 * e + 4 * half;
-                if (oc < a.d)
-                    *reinterpret_cast<f32x4 *>(o + oc) =
-                        f32x4{acc[x][4 * e], acc[x][4 * e + 1], acc[x][4 * e + 2], acc[x][4 * e + 3]};
-            }
+        for (int x = 0; x < D / 16; x++) {
+            const int oc = x * 16 + 4 * quarter;
+            if (oc < a.d) *reinterpret_cast<f32x4 *>(o + oc) = acc[x];
+        }
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float *out = static_cast<float *>(a.out) + row * a.ldo + h * a.hso;
     bool sound = true;
 #pragma unroll
-    for (int x = 0; x < D / 32; x++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int oc = x * 32 + 8 * e + 4 * half;
-            f32x4 o;
-            for (int y = 0; y < 4; y++) {
-                o[y] = acc[x][4 * e + y] * inv;
-                sound = sound && o[y] - o[y] == 0.0f;
-            }
-            if (live && oc < a.d) *reinterpret_cast<f32x4 *>(out + oc) = o;
-        }
+    for (int x = 0; x < D / 16; x++) {
+        const int oc = x * 16 + 4 * quarter;
+        const f32x4 o = acc[x] * inv;
+        for (int y = 0; y < 4; y++) sound = sound && o[y] - o[y] == 0.0f;
+        if (live && oc < a.d) *reinterpret_cast<f32x4 *>(out + oc) = o;
+    }
     // An infinity or NaN among the operands, be it hidden, makes the split products NaN.
     unsigned long long again = __ballot(live && !sound);
-    again = (again | again >> 32) & 0xffffffffull;
+    again |= again >> 32;
+    again = (again | again >> 16) & 0xffff;
     while (again) {
         const int64_t p = wave0 + __builtin_ctzll(again);
         again &= again - 1;
@@ -502,7 +532,7 @@ hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
     const int heads = REL ? a.heads : a.kv_heads;
     const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / heads), TILE_Q);
     const size_t groups = (size_t)a.seqs.batch * heads * splits, blocks = div_ceil(groups, 8) * 8 * q_tiles;
-    if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
+    if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS / 2) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((attn_tile32_kernel<D, PAGED, EXTRA, REL>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a,
                        parts_of(a, splits), (int)q_tiles, (int)groups);
     return hipGetLastError();

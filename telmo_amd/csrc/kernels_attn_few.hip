@@ -31,16 +31,6 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
-// The greatest (the sum) of the values of the four lanes 16 apart.
-__device__ __forceinline__ float max_quarters(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float sum_quarters(float x) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
 template <typename T, int D>
 struct Few {
     static constexpr bool WIDE = sizeof(T) == 4;
