@@ -13,7 +13,8 @@ hipError_t launch_attention16(const AttnArgs &a, int splits, hipStream_t s);
 
 // f32 rows; with position rows only heads of up to 128 (attention32_fits).
 inline bool attention32_fits(const AttnArgs &a) { return !a.rel || a.d <= 128; }
-hipError_t launch_attention32(const AttnArgs &a, int splits, hipStream_t s);
+// Tiles of 64 or 128 query rows.
+hipError_t launch_attention32(const AttnArgs &a, int rows, int splits, hipStream_t s);
 
 // Few query rows of any type, without position rows and documents.
 inline bool attention_few_fits(const AttnArgs &a) {

@@ -86,6 +86,37 @@ struct Tiles {
     __device__ __forceinline__ int at(int n) const { return (n < front ? n : start + n - front) * TILE_K; }
 };
 
+// The keys kb + bit that a query is shown, as bits: its window and prefix, without those that have no page, and with
+// documents (DOCS) its own: the lane holds key kb + lane's document in `docs` and its query's in `doc`. The
+// documents of a tile are few: each is compared once.
+__device__ __forceinline__ uint64_t bits_below(int n) { return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1; }
+template <bool DOCS, int TILE_K>
+__device__ __forceinline__ uint64_t shown_bits(const AttnWindow &w, int kb, uint64_t homeless, int docs, int doc) {
+    uint64_t bits = (bits_below(w.hi - kb) & ~bits_below(w.lo - kb)) | bits_below(w.prefix - kb);
+    bits &= ~homeless;
+    if (DOCS) {
+        uint64_t mine = 0, left = bits_below(TILE_K);
+        while (left) {
+            const int d = __builtin_amdgcn_readlane(docs, __builtin_ctzll(left));
+            const uint64_t same = __ballot(docs == d);
+            if (doc == d) mine = same;
+            left &= ~same;
+        }
+        bits &= doc < 0 ? 0 : mine;
+    }
+    return bits;
+}
+// Whether all of a tile's keys and the wavefront's queries are of one document.
+__device__ __forceinline__ bool one_document(int docs, int doc) {
+    const int first = __builtin_amdgcn_readfirstlane(docs);
+    return first >= 0 && __all(docs == first && doc == first);
+}
+// s where the bit is set, else -infinity.
+__device__ __forceinline__ float shown_or_not(float s, uint32_t bits, int bit) {
+    const uint32_t all = (uint32_t)((int32_t)(bits << (31 - bit)) >> 31);
+    return __uint_as_float((__float_as_uint(s) & all) | (0xff800000u & ~all));
+}
+
 // A workgroup's place in the call. Heads that share a key head are rows of one matrix: pair g r + x is head x
 // of the group in query row r (g is 1 where each head has position rows of its own). Workgroups go round the
 // 8 XCDs in turn: those of one head and part share an XCD and its L2, the rows with the most keys (the last

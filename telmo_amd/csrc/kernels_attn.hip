@@ -25,33 +25,54 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_rows_kernel(const AttnArg
 }
 
 // The parts of a row and head, joined by one wavefront: with M the largest maximum, the sums and outputs of
-// part p count e^(m_p - M) times.
-template <typename T>
+// part p count e^(m_p - M) times. Lane p weighs part p; then each lane adds V values of all parts, in their order,
+// STEP parts' loads on their way at a time.
+template <typename T, int V, int STEP>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArgs a, const AttnParts parts) {
-    const int lane = threadIdx.x & 63, b = blockIdx.z, h = blockIdx.y, r = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
+    typedef float fv __attribute__((ext_vector_type(V)));
+    const int lane = threadIdx.x & 63, b = blockIdx.y;
     const AttnSpan sp = span_of(a.seqs, b);
+    const uint32_t pair = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
+    const int r = (int)(pair / (uint32_t)a.heads), h = (int)(pair % (uint32_t)a.heads);
     if (r >= sp.nq || r >= a.seqs.longest) return;
     const size_t at = (size_t)(sp.q0 + r) * a.heads + h;
-    float m = -INFINITY;
-    for (int p = 0; p < parts.parts; p++) m = fmaxf(m, parts.top[p * parts.pairs + at]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, acc[4] = {};
-    for (int p = 0; p < parts.parts; p++) {
-        const size_t from = p * parts.pairs + at;
-        const float w = exp2f((parts.top[from] - base) * LOG2E), sum = parts.sum[from];
-        if (sum == 0.0f) continue;  // no key of this part was shown
-        l = __builtin_fmaf(w, sum, l);
-        for (int e = 0; e < 4; e++)
-            if (e * 64 + lane < a.d) acc[e] = __builtin_fmaf(w, parts.out[from * a.d + e * 64 + lane], acc[e]);
-    }
-    T *out = static_cast<T *>(a.out) + (int64_t)(sp.q0 + r) * a.ldo + h * a.hso;
-    bool sound = true;
-    for (int e = 0; e < 4; e++)
-        if (e * 64 + lane < a.d) {
-            const float v = l == 0.0f ? 0.0f : acc[e] / l;
-            sound = sound && v - v == 0.0f;
-            out[e * 64 + lane] = (T)v;
+    const bool in = lane * V < a.d;
+    const float *from = parts.out + at * a.d + (in ? lane * V : 0);
+    const auto load = [&](int p, fv(&x)[STEP]) {
+#pragma unroll
+        for (int y = 0; y < STEP; y++)
+            x[y] = *reinterpret_cast<const fv *>(
+                from + (size_t)(p + y < parts.parts ? p + y : parts.parts - 1) * parts.pairs * a.d);
+    };
+    fv x[STEP];
+    load(0, x);
+    const float top = lane < parts.parts ? parts.top[lane * parts.pairs + at] : -INFINITY;
+    const float sum = lane < parts.parts ? parts.sum[lane * parts.pairs + at] : 0.0f;
+    float most = top;
+    for (int o = 32; o; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    // A part that was shown no key weighs nothing.
+    const float weight = sum == 0.0f ? 0.0f : exp2f((top - (most == -INFINITY ? 0.0f : most)) * LOG2E);
+    float l = weight * sum;
+    for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
+    fv acc = {};
+    for (int p = 0; p < parts.parts; p += STEP) {
+        if (p) load(p, x);
+#pragma unroll
+        for (int y = 0; y < STEP; y++) {
+            const float w = p + y < parts.parts ? __shfl(weight, p + y) : 0.0f;
+            if (w != 0.0f)
+                for (int e = 0; e < V; e++) acc[e] = __builtin_fmaf(w, x[y][e], acc[e]);
         }
+    }
+    bool sound = true;
+    if (in) {
+        T *out = static_cast<T *>(a.out) + (int64_t)(sp.q0 + r) * a.ldo + h * a.hso + lane * V;
+        for (int e = 0; e < V; e++) {
+            const float y = l == 0.0f ? 0.0f : acc[e] / l;
+            sound = sound && y - y == 0.0f;
+            out[e] = (T)y;
+        }
+    }
     // As the tile kernels do for rows that they finish themselves.
     if (!__all(sound) && (sizeof(T) == 4 || l - l == 0.0f)) attend_row<T>(a, b, h, r, lane);
 }
@@ -63,11 +84,18 @@ hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
     return hipGetLastError();
 }
 
+template <typename T, int V, int STEP>
+hipError_t launch_join_of(const AttnArgs &a, int splits, hipStream_t s) {
+    const size_t blocks = div_ceil((size_t)a.seqs.longest * a.heads, ROW_WAVES);
+    if (blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL((attn_join_kernel<T, V, STEP>), dim3((unsigned)blocks, (unsigned)a.seqs.batch),
+                       dim3(64 * ROW_WAVES), 0, s, a, parts_of(a, splits));
+    return hipGetLastError();
+}
 template <typename T>
 hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
-    const dim3 grid((unsigned)div_ceil((size_t)a.seqs.longest, ROW_WAVES), (unsigned)a.heads, (unsigned)a.seqs.batch);
-    hipLaunchKernelGGL((attn_join_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a, parts_of(a, splits));
-    return hipGetLastError();
+    if (a.d > 128) return splits > 4 ? launch_join_of<T, 4, 16>(a, splits, s) : launch_join_of<T, 4, 4>(a, splits, s);
+    return splits > 4 ? launch_join_of<T, 2, 16>(a, splits, s) : launch_join_of<T, 2, 4>(a, splits, s);
 }
 
 // How a call is spread: workgroups of `tile` query rows and heads, and how many parts the keys are cut into so that
@@ -75,8 +103,9 @@ hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
 struct Spread {
     size_t tile, target, least;
 };
-constexpr Spread TILES{128, 512, 256}, FEW{16, 2048, 512};
-constexpr size_t MOST_PARTS = 64;
+constexpr Spread TILES16{128, 512, 256}, FEW{16, 2048, 512};
+constexpr Spread TILES32{128, 256, 128}, SMALL32{64, 256, 128};
+constexpr size_t MOST_PARTS = 64;  // a lane of the joining wavefront each
 
 size_t parts_for(const Spread &sp, size_t wgs, size_t keys) {
     size_t n = sp.target / (wgs ? wgs : 1);
@@ -88,12 +117,13 @@ size_t parts_for(const Spread &sp, size_t wgs, size_t keys) {
 
 size_t attention_work_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys) {
     // The fewest workgroups that calls of these sizes have give the most parts.
-    const auto parts = [&](const Spread &sp) {
-        const size_t tiles = div_ceil(rows * (heads / kv_heads), sp.tile);
-        return parts_for(sp, kv_heads * (tiles > batch ? tiles : batch), keys);
-    };
-    const size_t x = parts(TILES), y = rows * (heads / kv_heads) <= FEW.tile * batch ? parts(FEW) : 1;
-    const size_t n = x > y ? x : y;
+    size_t n = 1;
+    for (const Spread &sp : {TILES16, TILES32, SMALL32, FEW}) {
+        const size_t tiles = div_ceil(rows * (heads / kv_heads), sp.tile), x = kv_heads * (tiles > batch ? tiles : batch);
+        if (sp.tile == FEW.tile && rows * (heads / kv_heads) > FEW.tile * batch) continue;
+        const size_t parts = parts_for(sp, x, keys);
+        n = n > parts ? n : parts;
+    }
     return n > 1 ? n * part_bytes(rows * heads, d) : 0;
 }
 
@@ -108,20 +138,32 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
             default: return launch_rows<float>(a, s);
         }
     }
-    const Spread &sp = few ? FEW : TILES;
-    const size_t group = a.rel ? 1 : a.heads / a.kv_heads, tiles = div_ceil((size_t)a.seqs.longest * group, sp.tile);
+    const size_t group = a.rel ? 1 : a.heads / a.kv_heads, sets = (size_t)(a.heads / group) * a.seqs.batch;
+    const auto tiles_of = [&](const Spread &sp) { return div_ceil((size_t)a.seqs.longest * group, sp.tile); };
     size_t keys = a.seqs.tables ? (size_t)a.seqs.width * a.seqs.page
-                                : (size_t)(a.seqs.k_starts ? a.seqs.k_rows : a.seqs.k_rows / a.seqs.batch);
-    if (a.left >= 0 && a.right >= 0 && !a.prefix) {  // no tile reaches further than its rows' windows
-        const size_t reach = (size_t)a.left + a.right + 1 + sp.tile;
-        keys = keys < reach ? keys : reach;
-    }
-    size_t n = parts_for(sp, tiles * (a.heads / group) * a.seqs.batch, keys);
+                  : !a.seqs.k_starts ? (size_t)(a.seqs.k_rows / a.seqs.batch)
+                  : a.seqs.k_starts == a.seqs.q_starts ? (size_t)a.seqs.longest
+                                                       : (size_t)a.seqs.k_rows;
     const size_t bytes = part_bytes((size_t)a.seqs.q_rows * a.heads, a.d);
-    if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
-    if (n < 1) n = 1;
+    const auto parts = [&](const Spread &sp) {
+        size_t reach = keys;
+        if (a.left >= 0 && a.right >= 0 && !a.prefix) {  // no tile reaches further than its rows' windows
+            const size_t most = (size_t)a.left + a.right + 1 + sp.tile;
+            reach = reach < most ? reach : most;
+        }
+        size_t n = parts_for(sp, tiles_of(sp) * sets, reach);
+        if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
+        return n < 1 ? (size_t)1 : n;
+    };
+    Spread sp = few ? FEW : a.type != F32 ? TILES16 : TILES32;
+    size_t n = parts(sp);
+    // f32 tiles of 64 rows where those of 128 leave half of the GPU's 256 CUs empty.
+    if (!few && a.type == F32 && tiles_of(sp) * sets * n <= 128) {
+        sp = SMALL32;
+        n = parts(sp);
+    }
     const hipError_t e = few                ? launch_attention_few(a, (int)n, s)
-                         : a.type == F32 ? launch_attention32(a, (int)n, s)
+                         : a.type == F32 ? launch_attention32(a, (int)sp.tile, (int)n, s)
                                          : launch_attention16(a, (int)n, s);
     if (e != hipSuccess || n == 1) return e;
     switch (a.type) {

@@ -161,28 +161,14 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
             scores_of<true, N, EXTRA == ALL>(
                 a, [&](int e) -> float & { return reinterpret_cast<float *>(&s[e / 16])[e % 16]; },
                 [&](int e) { return kb + e / 16 * 32 + 8 * (e % 16 / 4) + 4 * half + e % 4; }, h, slope, i);
-        if (!full) {
+        const bool same_doc = EXTRA != ALL || !a.q_docs || one_document(docs, doc);
+        if (!full || (PAGED && hide) || !same_doc) {
+            const uint64_t bits = (EXTRA == ALL && !same_doc ? shown_bits<true, TILE_K>(win, kb, hide, docs, doc)
+                                                             : shown_bits<false, TILE_K>(win, kb, hide, docs, doc)) >>
+                                  4 * half;
 #pragma unroll
             for (int e = 0; e < N; e++)
-                if (!win.has(kb + e / 16 * 32 + 8 * (e % 16 / 4) + 4 * half + e % 4)) s[e / 16][e % 16] = -INFINITY;
-        }
-        if (PAGED && hide) {
-            const uint64_t mine = hide >> 4 * half;
-#pragma unroll
-            for (int e = 0; e < N; e++)
-                if (mine >> (e / 16 * 32 + 8 * (e % 16 / 4) + e % 4) & 1) s[e / 16][e % 16] = -INFINITY;
-        }
-        if (EXTRA == ALL && a.q_docs) {
-            const int first = __builtin_amdgcn_readfirstlane(docs);
-            if (first < 0 || !__all(docs == first && doc == first)) {
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const int k = e / 16 * 32 + 8 * (e % 16 / 4) + e % 4;
-                    const int lo = __builtin_amdgcn_readlane(docs, k), hi = __builtin_amdgcn_readlane(docs, k + 4);
-                    const int mine = half ? hi : lo;
-                    if (mine < 0 || mine != doc) s[e / 16][e % 16] = -INFINITY;
-                }
-            }
+                s[e / 16][e % 16] = shown_or_not(s[e / 16][e % 16], (uint32_t)(bits >> e / 16 * 32), 8 * (e % 16 / 4) + e % 4);
         }
 
         float top = s[0][0];

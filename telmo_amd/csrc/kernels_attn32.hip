@@ -24,7 +24,7 @@ namespace tg {
 
 namespace {
 
-constexpr int WAVES = 8, THREADS = 64 * WAVES, TILE_Q = 16 * WAVES, TILE_K = 32, RING = 4;
+constexpr int TILE_K = 32;
 
 // The power of two that brings a row whose largest magnitude is `top` below 2^15, and its inverse. Both stay
 // normal numbers: a row of subnormals is scaled less, which loses nothing that f32 sums would keep.
@@ -103,8 +103,9 @@ __device__ __forceinline__ float row_sum(float x) {
 template <int D>
 constexpr int V_STEP = D + 16;
 
-template <int D, bool REL>
+template <int D, bool REL, int WAVES>
 struct Shared {
+    static constexpr int RING = WAVES / 2;  // blocks of position rows that the wavefronts use at a time
     _Float16 k[2][TILE_K * K_PITCH<D>];
     __bf16 v[3][TILE_K * V_STEP<D>];
     float k_back[TILE_K];
@@ -141,14 +142,16 @@ __device__ __forceinline__ Split2 split_row(const float *x) {
     return r;
 }
 // D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped, biased or cut by documents.
-template <int D, bool PAGED, bool EXTRA, bool REL>
-__global__ __launch_bounds__(THREADS, 2) void attn_tile32_kernel(
+template <int D, bool PAGED, bool EXTRA, bool REL, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
     const AttnArgs a, const AttnParts parts, const int q_tiles, const int groups) {
-    // Heads of up to 64 have half as many pieces as threads: two threads handle each alike.
-    constexpr int CHUNKS = D / 8, PER = D <= 128 ? 1 : D / 128, STEP = TILE_K / PER;
+    constexpr int THREADS = 64 * WAVES, TILE_Q = 16 * WAVES, RING = Shared<D, REL, WAVES>::RING;
+    // Where there are fewer pieces than threads, several threads handle each alike.
+    constexpr int CHUNKS = D / 8, PIECES = TILE_K * CHUNKS, PER = PIECES > THREADS ? PIECES / THREADS : 1;
+    constexpr int STEP = TILE_K / PER;
     constexpr int STEPS = D / 32;  // products along a row
     constexpr int AHEAD = 2;       // groups of operands on their way from LDS
-    __shared__ __align__(16) Shared<D, REL> sh;
+    __shared__ __align__(16) Shared<D, REL, WAVES> sh;
 
     Place at;
     if (!at.find(a, parts.parts, q_tiles, groups, REL ? a.heads : a.kv_heads, TILE_Q)) return;
@@ -413,25 +416,14 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tile32_kernel(
         const auto key_at = [&](int e) { return kb + e / 4 * 16 + 4 * quarter + e % 4; };
         if (EXTRA) scores_of<false, 8, true>(a, [&](int e) -> float & { return s[e]; }, key_at, h, slope, i);
         const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
-        if (!full) {
+        const bool same_doc = !EXTRA || !a.q_docs || one_document(docs, doc);
+        if (!full || (PAGED && hide) || !same_doc) {
+            const uint32_t bits =
+                (uint32_t)(EXTRA && !same_doc ? shown_bits<true, TILE_K>(win, kb, hide, docs, doc)
+                                              : shown_bits<false, TILE_K>(win, kb, hide, docs, doc)) >>
+                4 * quarter;
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (!win.has(key_at(e))) s[e] = -INFINITY;
-        }
-        if (PAGED && hide) {
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if ((uint32_t)hide >> (key_at(e) - kb) & 1) s[e] = -INFINITY;
-        }
-        if (EXTRA && a.q_docs) {
-            const int first = __builtin_amdgcn_readfirstlane(docs);
-            if (first < 0 || !__all(docs == first && doc == first)) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int mine = __shfl(docs, key_at(e) - kb);
-                    if (mine < 0 || mine != doc) s[e] = -INFINITY;
-                }
-            }
+            for (int e = 0; e < 8; e++) s[e] = shown_or_not(s[e], bits, e / 4 * 16 + e % 4);
         }
 
         float top = s[0];
@@ -527,32 +519,39 @@ __global__ __launch_bounds__(THREADS, 2) void attn_tile32_kernel(
     }
 }
 
-template <int D, bool PAGED, bool EXTRA, bool REL>
+template <int D, bool PAGED, bool EXTRA, bool REL, int WAVES>
 hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
     const int heads = REL ? a.heads : a.kv_heads;
-    const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / heads), TILE_Q);
+    const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / heads), 16 * WAVES);
     const size_t groups = (size_t)a.seqs.batch * heads * splits, blocks = div_ceil(groups, 8) * 8 * q_tiles;
     if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS / 2) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((attn_tile32_kernel<D, PAGED, EXTRA, REL>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a,
-                       parts_of(a, splits), (int)q_tiles, (int)groups);
+    hipLaunchKernelGGL((attn_tile32_kernel<D, PAGED, EXTRA, REL, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0,
+                       s, a, parts_of(a, splits), (int)q_tiles, (int)groups);
     return hipGetLastError();
 }
 
-template <int D, bool REL>
+template <int D, bool REL, int WAVES>
 hipError_t launch_kind(const AttnArgs &a, int splits, hipStream_t s) {
     const bool extra = a.cap > 0.0f || a.slopes || a.table || a.q_docs;
     if (a.seqs.tables)
-        return extra ? launch_tile<D, true, true, REL>(a, splits, s) : launch_tile<D, true, false, REL>(a, splits, s);
-    return extra ? launch_tile<D, false, true, REL>(a, splits, s) : launch_tile<D, false, false, REL>(a, splits, s);
+        return extra ? launch_tile<D, true, true, REL, WAVES>(a, splits, s)
+                     : launch_tile<D, true, false, REL, WAVES>(a, splits, s);
+    return extra ? launch_tile<D, false, true, REL, WAVES>(a, splits, s)
+                 : launch_tile<D, false, false, REL, WAVES>(a, splits, s);
+}
+
+template <int WAVES>
+hipError_t launch_size(const AttnArgs &a, int splits, hipStream_t s) {
+    if (a.rel) return a.d <= 64 ? launch_kind<64, true, WAVES>(a, splits, s) : launch_kind<128, true, WAVES>(a, splits, s);
+    if (a.d <= 64) return launch_kind<64, false, WAVES>(a, splits, s);
+    if (a.d <= 128) return launch_kind<128, false, WAVES>(a, splits, s);
+    return launch_kind<256, false, WAVES>(a, splits, s);
 }
 
 }  // namespace
 
-hipError_t launch_attention32(const AttnArgs &a, int splits, hipStream_t s) {
-    if (a.rel) return a.d <= 64 ? launch_kind<64, true>(a, splits, s) : launch_kind<128, true>(a, splits, s);
-    if (a.d <= 64) return launch_kind<64, false>(a, splits, s);
-    if (a.d <= 128) return launch_kind<128, false>(a, splits, s);
-    return launch_kind<256, false>(a, splits, s);
+hipError_t launch_attention32(const AttnArgs &a, int rows, int splits, hipStream_t s) {
+    return rows == 64 ? launch_size<4>(a, splits, s) : launch_size<8>(a, splits, s);
 }
 
 }  // namespace tg

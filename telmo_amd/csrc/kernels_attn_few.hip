@@ -65,7 +65,8 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
     const int pairs = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest) * group, pair0 = tile * COLS;
     if (pair0 >= pairs) return;
 
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, quarter = lane >> 4, col = lane & 15;
+    const int t = threadIdx.x, lane = t & 63, quarter = lane >> 4, col = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
     const bool live = pair0 + col < pairs;
     const int r = live ? (pair0 + col) / group : 0, h = kvh * group + (live ? (pair0 + col) % group : 0);
@@ -96,17 +97,21 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
     u32x4 kr[F::KT][F::KS];
     uint32_t vr[F::VROWS][F::W][F::VW];
     uint32_t hidden = 0;  // keys of the loaded tile that have no place
+    // Lane n of a wavefront looks up the tile's key n (its first key, where the tile lies in one page) a tile ahead.
+    int page = 0, page_row = 0;
+    const auto look = [&](int kb) {
+        if (!PAGED) return;
+        const int key = one_page ? kb : kb + lane % TILE;
+        page = page_of(a.seqs, b, key < sp.nk ? key : sp.nk - 1, page_row);
+    };
     const auto load = [&](int kb) {
         // Offsets of the keys' rows: the lane's own ones for K, those of its eight (four) rows for V.
         int64_t kat = 0, vat = 0;
         if (PAGED) {
-            const int key = one_page ? kb : kb + lane % TILE;
-            const int j = key < sp.nk ? key : sp.nk - 1;
-            int s;
-            const int p = page_of(a.seqs, b, j, s);
-            hidden = (uint32_t)__ballot(p < 0);
-            kat = (p < 0 ? 0 : p) * a.psk + s * a.ldk;
-            vat = (p < 0 ? 0 : p) * a.psv + s * a.ldv;
+            hidden = (uint32_t)__ballot(page < 0);
+            const int64_t p = page < 0 ? 0 : page;
+            kat = p * a.psk + page_row * a.ldk;
+            vat = p * a.psv + page_row * a.ldv;
         }
         const auto offset = [&](int64_t base, int64_t ld, int key) -> int64_t {
             const int j = kb + key < sp.nk ? key : sp.nk - 1 - kb;  // within the tile
@@ -150,7 +155,11 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
     const float to_log2 = EXTRA ? LOG2E : a.scale * LOG2E;
     constexpr float SHIFT = __is_same(T, _Float16) ? 8.0f : 0.0f;  // weights below f16's normal numbers
 
-    if (n0 < n1) load(tiles.at(n0));
+    if (n0 < n1) {
+        look(tiles.at(n0));
+        load(tiles.at(n0));
+        if (n0 + WAVES < n1) look(tiles.at(n0 + WAVES));
+    }
     for (int n = n0; n < n1; n += WAVES) {
         const int kb = tiles.at(n);
         const uint32_t hide = hidden;
@@ -177,19 +186,23 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
 #pragma unroll
                 for (int y = 0; y < F::VW; y++) vt[e][w][y] = vr[e][w][y];
         if (n + WAVES < n1) load(tiles.at(n + WAVES));
+        if (n + 2 * WAVES < n1) look(tiles.at(n + 2 * WAVES));
 
         const bool full = (kb >= w_last.lo && kb + TILE <= w_first.hi) || kb + TILE <= w_first.prefix;
-        float top = -INFINITY;
+        constexpr int N = 4 * F::KT;
+        if (EXTRA)
+            scores_of<!F::WIDE, N, true>(
+                a, [&](int e) -> float & { return reinterpret_cast<float *>(&s[e / 4])[e % 4]; },
+                [&](int e) { return kb + e / 4 * 16 + quarter * 4 + e % 4; }, h, slope, i);
+        if (!full || (PAGED && hide)) {
+            const uint64_t homeless = one_page && hide ? ~0ull : hide;
+            const uint32_t bits = (uint32_t)shown_bits<false, TILE>(win, kb, homeless, 0, 0) >> 4 * quarter;
 #pragma unroll
-        for (int x = 0; x < F::KT; x++)
+            for (int e = 0; e < N; e++) s[e / 4][e % 4] = shown_or_not(s[e / 4][e % 4], bits, e / 4 * 16 + e % 4);
+        }
+        float top = s[0][0];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = kb + x * 16 + quarter * 4 + e;
-                if (EXTRA) s[x][e] = score_of(a, s[x][e], h, slope, j - i);
-                if (!full && !win.has(j)) s[x][e] = -INFINITY;
-                if (PAGED && hide && (one_page || (hide >> (j - kb) & 1))) s[x][e] = -INFINITY;
-                top = fmaxf(top, s[x][e]);
-            }
+        for (int e = 1; e < N; e++) top = fmaxf(top, s[e / 4][e % 4]);
         top = max_quarters(top);
         if (__any(top > m)) {
             const float mn = fmaxf(m, top);
