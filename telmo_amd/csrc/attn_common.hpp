@@ -63,9 +63,9 @@ __host__ __device__ inline AttnSpan span_of(const AttnSeqs &s, int b) {
         r.q0 = b * r.nq;
     }
     if (s.tables) {
-        const int64_t held = (int64_t)s.width * s.page;
+        const int64_t held = (int64_t)s.width * s.page, most = 1 << 30;  // tiles past the last key count in 32 bits too
         r.k0 = 0;
-        r.nk = s.pages ? clamp_to(s.lengths[b], 0, held < INT32_MAX ? (int)held : INT32_MAX) : 0;
+        r.nk = s.pages ? clamp_to(s.lengths[b], 0, (int)(held < most ? held : most)) : 0;
     } else if (s.k_starts) {
         r.k0 = clamp_to(s.k_starts[b], 0, s.k_rows);
         r.nk = clamp_to(s.k_starts[b + 1], r.k0, s.k_rows) - r.k0;

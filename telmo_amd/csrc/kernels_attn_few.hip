@@ -3,12 +3,12 @@
 //
 // The rows of a sequence that share a key head (its new rows by the group's heads) are the 16 columns of
 // 16 x 16 products. Nothing of the keys is used twice, so LDS does not hold them: each of a workgroup's
-// wavefronts takes key tiles of its own, loads the operands of S' = K Q' from memory into registers as the
-// matrix instructions want them (16 rows by 64 bytes a load) and V by whole rows (a load gives 16 lanes the
-// 16 x 16 bytes of a row), the next tile's loads in flight while it computes. V' wants keys side by side in a
-// register: of 16-bit values, the eight rows that a lane holds are interleaved in registers; of f32 there is
-// nothing to do. The output's columns are numbered so that a lane's loads are contiguous: product x of a chunk
-// holds its value x. The wavefronts' results are joined in LDS, and those of the parts by a second kernel.
+// wavefronts takes key tiles of its own and loads the operands of S' = K Q' from memory into registers as the
+// matrix instructions want them (16 rows by 64 bytes a load), and V by whole rows (a load gives 16 lanes the
+// 16 x 16 bytes of a row), two tiles under way at a time. V' wants keys side by side in a register: of 16-bit
+// values, the eight rows that a lane holds are interleaved in registers; of f32 there is nothing to do. The
+// output's columns are numbered so that a lane's loads are contiguous: product x of a piece holds its value x.
+// The wavefronts' results are joined in LDS, and those of the parts by a second kernel.
 //
 // The products have time to spare, so the 16-bit weights are held as two numbers, f32's as they are on the f32
 // matrix instructions.
@@ -31,10 +31,15 @@ __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
 
+// Memory of the GPU, said where the compiler would take an address for LDS's or memory's and wait for both.
+template <typename T>
+using Global = const __attribute__((address_space(1))) T *;
+
 template <typename T, int D>
 struct Few {
     static constexpr bool WIDE = sizeof(T) == 4;
-    static constexpr int WAVES = D == 256 ? 4 : 8;          // two on a SIMD, one where a tile fills its registers
+    // Tiles whose operands are under way, and wavefronts: one on a SIMD where the operands fill its registers.
+    static constexpr int DEPTH = D == 256 ? 1 : 2, WAVES = D == 64 ? 8 : 4;
     static constexpr int THREADS = 64 * WAVES;
     static constexpr int TILE = WIDE ? 16 : 32;             // keys of a tile
     static constexpr int CH = WIDE ? 4 : D == 64 ? 4 : 8;   // values of a lane's piece of a V row
@@ -94,60 +99,81 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
 
     const T *kbase = static_cast<const T *>(a.k) + kvh * a.hsk, *vbase = static_cast<const T *>(a.v) + kvh * a.hsv;
     const bool one_page = PAGED && a.seqs.page % TILE == 0;  // a tile lies in one page
-    u32x4 kr[F::KT][F::KS];
-    uint32_t vr[F::VROWS][F::W][F::VW];
-    uint32_t hidden = 0;  // keys of the loaded tile that have no place
-    // Lane n of a wavefront looks up the tile's key n (its first key, where the tile lies in one page) a tile ahead.
+    // A tile's operands in registers, two tiles' at a time.
+    struct Operands {
+        u32x4 k[F::KT][F::KS];
+        uint32_t v[F::VROWS][F::W][F::VW];
+        uint32_t hidden;  // keys that have no place
+    } buf[F::DEPTH];
+    // Lane n of a wavefront looks up the tile's key n (its first key, where the tile lies in one page).
     int page = 0, page_row = 0;
     const auto look = [&](int kb) {
         if (!PAGED) return;
         const int key = one_page ? kb : kb + lane % TILE;
         page = page_of(a.seqs, b, key < sp.nk ? key : sp.nk - 1, page_row);
     };
-    const auto load = [&](int kb) {
-        // Offsets of the keys' rows: the lane's own ones for K, those of its eight (four) rows for V.
-        int64_t kat = 0, vat = 0;
+    // The wavefront's last tile. Past it loads read one row of it, and what they bring is hidden: two loads are always
+    // under way, so that the compiler knows how many it need not wait for.
+    const int last_tile = n1 - 1 - (n1 - 1 - n0) % WAVES;
+    const auto tile_at = [&](int n) { return tiles.at(n < last_tile ? n : last_tile); };
+    // The operands of tile n, which was looked up last, leave memory; the tile after it is looked up before they do,
+    // so that waiting for its pages does not wait for them. Addresses first: the loads in one run.
+    const auto load = [&](Operands &x, int n) {
+        const int kb = tile_at(n);
+        const bool real = n <= last_tile;
+        int64_t kp[F::KT], vp[F::VROWS];  // offsets from the head's first value
+        const auto key_of = [&](int key) { return !real ? 0 : kb + key < sp.nk ? key : sp.nk - 1 - kb; };  // within the tile
+        const auto v_key = [&](int e) { return (e / 4) * 16 + quarter * 4 + e % 4; };
+        x.hidden = 0;
         if (PAGED) {
-            hidden = (uint32_t)__ballot(page < 0);
+            x.hidden = (uint32_t)__ballot(page < 0);
             const int64_t p = page < 0 ? 0 : page;
-            kat = p * a.psk + page_row * a.ldk;
-            vat = p * a.psv + page_row * a.ldv;
+            const int64_t kat = p * a.psk + page_row * a.ldk, vat = p * a.psv + page_row * a.ldv;
+            if (one_page) {
+#pragma unroll
+                for (int y = 0; y < F::KT; y++) kp[y] = kat + key_of(y * 16 + col) * a.ldk;
+#pragma unroll
+                for (int e = 0; e < F::VROWS; e++) vp[e] = vat + key_of(v_key(e)) * a.ldv;
+            } else {
+                const auto from = [&](int64_t offset, int lane_of) {
+                    const int lo = __shfl((int)(uint32_t)offset, lane_of), hi = __shfl((int)(offset >> 32), lane_of);
+                    return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+                };
+#pragma unroll
+                for (int y = 0; y < F::KT; y++) kp[y] = from(kat, key_of(y * 16 + col));
+#pragma unroll
+                for (int e = 0; e < F::VROWS; e++) vp[e] = from(vat, key_of(v_key(e)));
+            }
+            look(tile_at(n + WAVES));
+        } else {
+            const int64_t k0 = (int64_t)(sp.k0 + kb) * a.ldk, v0 = (int64_t)(sp.k0 + kb) * a.ldv;
+#pragma unroll
+            for (int y = 0; y < F::KT; y++) kp[y] = k0 + key_of(y * 16 + col) * a.ldk;
+#pragma unroll
+            for (int e = 0; e < F::VROWS; e++) vp[e] = v0 + key_of(v_key(e)) * a.ldv;
         }
-        const auto offset = [&](int64_t base, int64_t ld, int key) -> int64_t {
-            const int j = kb + key < sp.nk ? key : sp.nk - 1 - kb;  // within the tile
-            if (!PAGED) return (int64_t)(sp.k0 + kb + j) * ld;
-            if (one_page) return base + j * ld;
-            const int lo = __shfl((int)(uint32_t)base, j), hi = __shfl((int)(base >> 32), j);
-            return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
-        };
         constexpr int E = 16 / sizeof(T);
 #pragma unroll
-        for (int x = 0; x < F::KT; x++) {
-            const T *k = kbase + offset(kat, a.ldk, x * 16 + col);
+        for (int y = 0; y < F::KT; y++)
 #pragma unroll
             for (int s = 0; s < F::KS; s++) {
                 const int c = s * 4 * E + quarter * E;
-                kr[x][s] = *reinterpret_cast<const u32x4 *>(k + (c < a.d ? c : 0));
+                x.k[y][s] = *(Global<u32x4>)(kbase + kp[y] + (c < a.d ? c : 0));
             }
-        }
 #pragma unroll
-        for (int e = 0; e < F::VROWS; e++) {
-            const int key = (e / 4) * 16 + quarter * 4 + e % 4;
-            const T *v = vbase + offset(vat, a.ldv, key);
-            const bool in = kb + key < sp.nk;
+        for (int e = 0; e < F::VROWS; e++)
 #pragma unroll
             for (int w = 0; w < F::W; w++) {
+                // Rows past the last key and columns past d are read as others: weighted by zero, or not stored.
                 const int c = w * 16 * F::CH + col * F::CH;
-                const T *at = v + (c < a.d ? c : 0);
                 if constexpr (F::VW == 4) {
-                    const u32x4 x = *reinterpret_cast<const u32x4 *>(at);
-                    for (int y = 0; y < 4; y++) vr[e][w][y] = in && c < a.d ? x[y] : 0u;
+                    const u32x4 y = *(Global<u32x4>)(vbase + vp[e] + (c < a.d ? c : 0));
+                    for (int z = 0; z < 4; z++) x.v[e][w][z] = y[z];
                 } else {
-                    const u32x2 x = *reinterpret_cast<const u32x2 *>(at);
-                    for (int y = 0; y < 2; y++) vr[e][w][y] = in && c < a.d ? x[y] : 0u;
+                    const u32x2 y = *(Global<u32x2>)(vbase + vp[e] + (c < a.d ? c : 0));
+                    for (int z = 0; z < 2; z++) x.v[e][w][z] = y[z];
                 }
             }
-        }
     };
 
     f32x4 acc[F::W][F::CH] = {};
@@ -155,47 +181,42 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
     const float to_log2 = EXTRA ? LOG2E : a.scale * LOG2E;
     constexpr float SHIFT = __is_same(T, _Float16) ? 8.0f : 0.0f;  // weights below f16's normal numbers
 
-    if (n0 < n1) {
-        look(tiles.at(n0));
-        load(tiles.at(n0));
-        if (n0 + WAVES < n1) look(tiles.at(n0 + WAVES));
-    }
-    for (int n = n0; n < n1; n += WAVES) {
-        const int kb = tiles.at(n);
-        const uint32_t hide = hidden;
+    const auto work = [&](Operands &o, int n) {
+        const int kb = tile_at(n);
+        const bool real = n <= last_tile;
+        const uint32_t hide = o.hidden;
+        if (a.d < D) {  // zeros where the queries' zeros may meet a value of any kind
+            constexpr int E = 16 / sizeof(T);
+#pragma unroll
+            for (int x = 0; x < F::KT; x++)
+#pragma unroll
+                for (int e = 0; e < F::KS; e++)
+                    if (e * 4 * E + quarter * E >= a.d) o.k[x][e] = u32x4{};
+        }
         f32x4 s[F::KT] = {};
 #pragma unroll
-        for (int x = 0; x < F::KT; x++)
+        for (int e = 0; e < F::KS; e++)
 #pragma unroll
-            for (int e = 0; e < F::KS; e++) {
+            for (int x = 0; x < F::KT; x++) {
                 if constexpr (F::WIDE) {
 #pragma unroll
                     for (int y = 0; y < 4; y++)
-                        s[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[x][e][y]),
+                        s[x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(o.k[x][e][y]),
                                                                     __uint_as_float(qf[e][y]), s[x], 0, 0, 0);
                 } else {
                     typedef T v8 __attribute__((ext_vector_type(8)));
-                    s[x] = mfma16(__builtin_bit_cast(v8, kr[x][e]), __builtin_bit_cast(v8, qf[e]), s[x]);
+                    s[x] = mfma16(__builtin_bit_cast(v8, o.k[x][e]), __builtin_bit_cast(v8, qf[e]), s[x]);
                 }
             }
-        uint32_t vt[F::VROWS][F::W][F::VW];
-#pragma unroll
-        for (int e = 0; e < F::VROWS; e++)
-#pragma unroll
-            for (int w = 0; w < F::W; w++)
-#pragma unroll
-                for (int y = 0; y < F::VW; y++) vt[e][w][y] = vr[e][w][y];
-        if (n + WAVES < n1) load(tiles.at(n + WAVES));
-        if (n + 2 * WAVES < n1) look(tiles.at(n + 2 * WAVES));
 
-        const bool full = (kb >= w_last.lo && kb + TILE <= w_first.hi) || kb + TILE <= w_first.prefix;
+        const bool full = real && ((kb >= w_last.lo && kb + TILE <= w_first.hi) || kb + TILE <= w_first.prefix);
         constexpr int N = 4 * F::KT;
         if (EXTRA)
             scores_of<!F::WIDE, N, true>(
                 a, [&](int e) -> float & { return reinterpret_cast<float *>(&s[e / 4])[e % 4]; },
                 [&](int e) { return kb + e / 4 * 16 + quarter * 4 + e % 4; }, h, slope, i);
         if (!full || (PAGED && hide)) {
-            const uint64_t homeless = one_page && hide ? ~0ull : hide;
+            const uint64_t homeless = !real || (one_page && hide) ? ~0ull : hide;
             const uint32_t bits = (uint32_t)shown_bits<false, TILE>(win, kb, homeless, 0, 0) >> 4 * quarter;
 #pragma unroll
             for (int e = 0; e < N; e++) s[e / 4][e % 4] = shown_or_not(s[e / 4][e % 4], bits, e / 4 * 16 + e % 4);
@@ -215,14 +236,12 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
             m = mn;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        float p[F::KT][4];
+        float p[N];
 #pragma unroll
-        for (int x = 0; x < F::KT; x++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                p[x][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[x][e] - base, to_log2, SHIFT));
-                l += p[x][e];
-            }
+        for (int e = 0; e < N; e++) {
+            p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[e / 4][e % 4] - base, to_log2, SHIFT));
+            l += p[e];
+        }
         if constexpr (F::WIDE) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
@@ -230,13 +249,13 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
                 for (int w = 0; w < F::W; w++)
 #pragma unroll
                     for (int x = 0; x < 4; x++)
-                        acc[w][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vt[e][w][x]), p[0][e],
+                        acc[w][x] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(o.v[e][w][x]), p[e],
                                                                          acc[w][x], 0, 0, 0);
         } else {
             typedef T v8 __attribute__((ext_vector_type(8)));
             f32x8 pv;
 #pragma unroll
-            for (int e = 0; e < 8; e++) pv[e] = p[e / 4][e % 4];
+            for (int e = 0; e < 8; e++) pv[e] = p[e];
             const v8 ph = __builtin_convertvector(pv, v8);
             const v8 pl = __builtin_convertvector(pv - __builtin_convertvector(ph, f32x8), v8);
 #pragma unroll
@@ -246,11 +265,30 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
                     u32x4 v;  // value x of the lane's eight rows
 #pragma unroll
                     for (int y = 0; y < 4; y++)
-                        v[y] = __builtin_amdgcn_perm(vt[2 * y + 1][w][x / 2], vt[2 * y][w][x / 2],
+                        v[y] = __builtin_amdgcn_perm(o.v[2 * y + 1][w][x / 2], o.v[2 * y][w][x / 2],
                                                      x % 2 ? 0x07060302u : 0x05040100u);
                     acc[w][x] = mfma16(__builtin_bit_cast(v8, v), pl, acc[w][x]);
                     acc[w][x] = mfma16(__builtin_bit_cast(v8, v), ph, acc[w][x]);
                 }
+        }
+    };
+
+    if (n0 < n1) {
+        look(tile_at(n0));
+        load(buf[0], n0);
+        if constexpr (F::DEPTH == 2) {
+            load(buf[1], n0 + WAVES);
+            for (int n = n0; n <= last_tile; n += 2 * WAVES) {
+                work(buf[0], n);
+                load(buf[0], n + 2 * WAVES);
+                work(buf[1], n + WAVES);
+                load(buf[1], n + 3 * WAVES);
+            }
+        } else {
+            for (int n = n0; n <= last_tile; n += WAVES) {
+                work(buf[0], n);
+                if (n < last_tile) load(buf[0], n + WAVES);
+            }
         }
     }
 
