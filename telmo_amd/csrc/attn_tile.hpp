@@ -119,16 +119,15 @@ __device__ __forceinline__ float shown_or_not(float s, uint32_t bits, int bit) {
 
 // A workgroup's place in the call. Heads that share a key head are rows of one matrix: pair g r + x is head x
 // of the group in query row r (g is 1 where each head has position rows of its own). Workgroups go round the
-// 8 XCDs in turn: those of one head and part share an XCD and its L2, the rows with the most keys (the last
-// ones of causal calls) first.
+// 8 XCDs in turn, and here round the heads and parts: where those are a multiple of 8 all tiles of one share an XCD
+// and its L2, otherwise they spread over all XCDs. The rows with the most keys (the last ones of causal calls) come
+// first.
 struct Place {
     int b, head, part, group;  // head: of k where the group shares a tile, of q otherwise
     int64_t pair0, pairs;      // the tile's first pair, the sequence's pairs
     AttnSpan sp;
     __device__ __forceinline__ bool find(const AttnArgs &a, int parts, int q_tiles, int groups, int heads, int tile_q) {
-        const int id = blockIdx.x, in_xcd = id / 8;
-        const int at = (in_xcd / q_tiles) * 8 + id % 8, tile = q_tiles - 1 - in_xcd % q_tiles;
-        if (at >= groups) return false;
+        const int at = blockIdx.x % groups, tile = q_tiles - 1 - (int)(blockIdx.x / groups);
         part = at % parts;
         head = at / parts % heads;
         b = at / parts / heads;

@@ -269,7 +269,7 @@ template <typename T, int D, bool PAGED, Extra EXTRA>
 hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
     const int group = a.heads / a.kv_heads;
     const size_t q_tiles = div_ceil((size_t)a.seqs.longest * group, TILE_Q);
-    const size_t groups = (size_t)a.seqs.batch * a.kv_heads * splits, blocks = div_ceil(groups, 8) * 8 * q_tiles;
+    const size_t groups = (size_t)a.seqs.batch * a.kv_heads * splits, blocks = groups * q_tiles;
     if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((attn_tile_kernel<T, D, PAGED, EXTRA>), dim3((unsigned)blocks), dim3(THREADS), 0, s, a,
                        parts_of(a, splits), (int)q_tiles, (int)groups);

@@ -523,7 +523,7 @@ template <int D, bool PAGED, bool EXTRA, bool REL, int WAVES>
 hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
     const int heads = REL ? a.heads : a.kv_heads;
     const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / heads), 16 * WAVES);
-    const size_t groups = (size_t)a.seqs.batch * heads * splits, blocks = div_ceil(groups, 8) * 8 * q_tiles;
+    const size_t groups = (size_t)a.seqs.batch * heads * splits, blocks = groups * q_tiles;
     if (q_tiles > INT32_MAX || blocks > MAX_ATTN_BLOCKS / 2) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((attn_tile32_kernel<D, PAGED, EXTRA, REL, WAVES>), dim3((unsigned)blocks), dim3(64 * WAVES), 0,
                        s, a, parts_of(a, splits), (int)q_tiles, (int)groups);
