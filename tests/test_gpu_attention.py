@@ -79,7 +79,7 @@ def check(got, want, tol):
 
 def run_rows(tk, type="f32", heads=2, kv_heads=None, d=64, lengths=(37,), k_lengths=None, layout="rows", cap=0.0,
              left=None, right=None, prefix=None, docs=None, slopes=False, table=None, rel=None, uw=False, scale=None,
-             starts=True, workspace=True, longest=None, seed=1, fill=None, v_mean=0.0):
+             starts=True, workspace=True, longest=None, seed=1):
     """Attention.forward of random rows, checked against the definition; returns the outputs."""
     import torch
 
@@ -115,8 +115,6 @@ def run_rows(tk, type="f32", heads=2, kv_heads=None, d=64, lengths=(37,), k_leng
     space = None
     if workspace:
         space = torch.empty(att.workspace_bytes(nq, max(k_lengths + (1,)), len(lengths)) + 64, dtype=torch.uint8, device="cuda")
-    if fill:
-        fill(k, v, k64, v64)
     options = dict(longest=longest, prefix=None if prefix is None else ints(prefix), q_docs=None if qd is None else ints(qd),
                    rel=None if rl is None else floats(rl), rel_u=None if u is None else floats(u),
                    rel_v=None if w is None else floats(w), workspace=space)
@@ -250,6 +248,112 @@ def test_longer_rows(tk, type):
     run_rows(tk, type, heads=2, kv_heads=1, d=128, lengths=(700,), right=0, workspace=False)
     run_rows(tk, type, heads=1, d=64, lengths=(3,), k_lengths=(5000,), right=0)
     run_rows(tk, type, heads=1, d=64, lengths=(3,), k_lengths=(5000,), right=0, workspace=False)
+
+
+MANY = (130, 200, 0, 129, 257, 1, 140, 131, 180, 133, 128, 160)
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_many_sequences(tk, type):
+    """Enough rows of enough heads for the f32 tiles of 128 rows, which few tiles do without."""
+    run_rows(tk, type, heads=8, lengths=MANY, right=0)
+    run_rows(tk, type, heads=8, d=128, lengths=MANY, left=50, right=20, docs=DOCS["packed"], prefix=(7,) * len(MANY))
+    run_rows(tk, type, heads=16, kv_heads=8, d=72, lengths=MANY, cap=20.0, slopes=True, table=30)
+    run_rows(tk, type, heads=8, d=256, lengths=MANY[:9], right=0)
+
+
+@pytest.mark.parametrize("d,rel", [(128, (256, False)), (64, (100, True)), (128, (40, True)), (48, (256, False))])
+def test_many_sequences_with_position_rows(tk, d, rel):
+    run_rows(tk, "f32", heads=8, d=d, lengths=MANY, rel=rel, uw=True)
+    run_rows(tk, "f32", heads=8, d=d, lengths=MANY, rel=rel, uw=True, left=60, right=10, prefix=(33,) * len(MANY), docs=DOCS["mixed"])
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_workspaces_of_any_size(tk, type):
+    """Fewer parts than wanted fit a smaller workspace; none fits 16 bytes. Two results may each be off by a weight's
+    and an output's rounding and by the sums over the keys."""
+    import torch
+
+    out, att, (q, k, v), options = run_rows(tk, type, heads=2, d=128, lengths=(900,), right=0)
+    full = options.pop("workspace")
+    need = att.workspace_bytes(900, 900)
+    assert need > 0 and full.numel() >= need
+    for size in (need // 2, need // 3, 16):
+        some = torch.full_like(out, 7.0)
+        att.forward(q, k, v, some, workspace=full[:size // 16 * 16], **options)
+        tk.synchronize()
+        half = {"f32": 2.0**-24, "f16": 2.0**-11, "bf16": 2.0**-8}[type]
+        off = float((some.float() - out.float()).abs().max())
+        assert off <= 2 * float(v.float().abs().max()) * (2 * half + (2 * 900 + 32) * 2.0**-24)
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_row_strides_past_the_tiles(tk, type):
+    """Keys 2^23 values and more apart, which a tile's 32-bit offsets do not reach."""
+    import torch
+
+    import telmo_amd
+
+    n, d, ld = 5, 64, (1 << 23) + 64
+    store = torch.empty(n * ld, dtype=dtype(type), device="cuda")
+    far = torch.as_strided(store, (n, 1, d), (ld, d, 1))
+    near = torch.randn(n, 1, d, device="cuda").to(dtype(type))
+    far.copy_(near)
+    q = torch.randn(40, 1, d, device="cuda").to(dtype(type))
+    outs = [torch.zeros_like(q) for _ in range(2)]
+    att = telmo_amd.Attention(tk, 1, d)
+    for k, out in zip((near, far), outs):
+        att.forward(q, k, k, out)
+    tk.synchronize()
+    off = float((outs[0].float() - outs[1].float()).abs().max())
+    assert off <= 4 * {"f32": 2.0**-20, "f16": 2.0**-11, "bf16": 2.0**-8}[type] * float(near.abs().max())
+
+
+def test_forward_with_position_rows_replayed_from_a_graph(tk, gpu_stream):
+    import torch
+
+    out, att, (q, k, v), options = run_rows(tk, "f32", heads=2, d=128, lengths=(500,), rel=(499, False), uw=True)
+    want = out.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=gpu_stream):
+        att.forward(q, k, v, out, **options)
+    for i in range(4):
+        out.fill_(float(i))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out[:500], want[:500]), i
+        att.forward(q, k, v, out, **options)
+        torch.cuda.synchronize()
+        assert torch.equal(out[:500], want[:500]), i
+
+
+def test_two_contexts_at_once(tk):
+    """Two streams' calls overlap, each stream with a context, an Attention and a workspace of its own."""
+    import torch
+
+    import telmo_amd
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(5)
+    q = torch.randn(700, 4, 128, generator=g, device="cuda").half()
+    k, v = (torch.randn(700, 2, 128, generator=g, device="cuda").half() for _ in "kv")
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    kerns = [telmo_amd.Kernels(0, stream=s.cuda_stream) for s in streams]
+    atts = [telmo_amd.Attention(x, 4, 128, kv_heads=2, right=0) for x in kerns]
+    spaces = [torch.empty(a.workspace_bytes(700, 700) + 16, dtype=torch.uint8, device="cuda") for a in atts]
+    outs = [[torch.zeros_like(q) for _ in range(6)] for _ in atts]
+    torch.cuda.synchronize()
+    for i in range(6):
+        for a, o, w in zip(atts, outs, spaces):
+            a.forward(q, k, v, o[i], workspace=w)
+    for x in kerns:
+        x.synchronize()
+    for o in outs:
+        for y in o:
+            assert torch.equal(y, outs[0][0])
+    for x in kerns:
+        x.close()
 
 
 @pytest.mark.parametrize("type", TYPES)
@@ -411,6 +515,36 @@ def test_pages_that_the_cache_does_not_have_are_not_shown(tk, type):
     run_paged(tk, type, new=(1,), lengths=(16,), bad=[(0, 0, -1)])  # nothing left
 
 
+@pytest.mark.parametrize("type,new", itertools.product(TYPES, (1, 30)))
+def test_cached_keys_behind_the_window_may_hold_anything(tk, type, new):
+    import torch
+
+    import telmo_amd
+
+    heads, d, page, total, left = 2, 64, 16, 200, 40
+    rng = np.random.default_rng(8)
+    k, k64 = rows_of(rng, type, 208, heads, d)
+    v, v64 = rows_of(rng, type, 208, heads, d)
+    q, q64 = rows_of(rng, type, new, heads, d)
+    first = total - new - left  # the first key that any query is shown, in the middle of a page
+    k[:first], v[:first] = float("nan"), float("inf")
+    out = torch.zeros_like(q)
+    cache = telmo_amd.PagedCache(tk, k.view(13, page, heads, d), v.view(13, page, heads, d))
+    telmo_amd.Attention(tk, heads, d, left=left, right=0).paged(q, cache, ints([list(range(13))]), ints([total]), out)
+    tk.synchronize()
+    got, shown = out.double().cpu().numpy(), shown_pairs(new, total, left, 0)
+    for h in range(heads):
+        want, size = attend(q64[:, h], k64[:total, h], v64[:total, h], d**-0.5, shown)
+        check(got[:, h], want, tolerance(type, d, total, size, np.abs(v64).max(), False))
+
+
+@pytest.mark.parametrize("type", TYPES)
+def test_chunks_of_many_sequences(tk, type):
+    run_paged(tk, type, heads=8, kv_heads=8, new=(130,) * 9, lengths=(130, 150, 200, 300, 131, 140, 190, 260, 129), page=16)
+    run_paged(tk, type, heads=8, kv_heads=8, d=128, new=(130,) * 9, lengths=(130, 150, 200, 300, 131, 140, 190, 260, 129), page=25,
+              bad=[(3, 2, -1)], slopes=True)
+
+
 @pytest.mark.parametrize("type", TYPES)
 def test_long_caches_split_and_joined(tk, type):
     run_paged(tk, type, heads=2, kv_heads=1, d=64, new=(1, 2), lengths=(9000, 4097), page=64)
@@ -441,7 +575,8 @@ def test_paged_calls_replayed_from_a_graph(tk, gpu_stream, type):
     assert not torch.equal(out[:6], want[:6])
 
 
-def test_strides_whose_offsets_pass_32_bits(tk):
+@pytest.mark.parametrize("new", (1, 30))
+def test_strides_whose_offsets_pass_32_bits(tk, new):
     """Pages of one head whose stride puts the last one beyond 2^32 elements (8.6 GB of f16 address space)."""
     import torch
 
@@ -452,7 +587,7 @@ def test_strides_whose_offsets_pass_32_bits(tk):
     k = torch.as_strided(store, (3, page, 1, d), (stride, d, d, 1))
     small = torch.randn(3, page, 1, d, device="cuda").half()
     k.copy_(small)
-    q = torch.randn(1, 1, d, device="cuda").half()
+    q = torch.randn(new, 1, d, device="cuda").half()
     att, tables, lens = telmo_amd.Attention(tk, 1, d), ints([[2, 0, 1]]), ints([3 * page - 5])
     far, near = torch.zeros_like(q), torch.ones_like(q)
     att.paged(q, telmo_amd.PagedCache(tk, k, k), tables, lens, far)
