@@ -150,6 +150,7 @@ struct KeyRows {
     const char *k, *v;      // the head's first row
     uint32_t k_row, v_row;  // bytes between rows
     uint32_t column;        // bytes of the thread's column
+    uint32_t k_off, v_off;  // bytes from the first of its rows to its piece
     int row0;
     int page, at;           // the lane's key's
     __device__ __forceinline__ KeyRows(const AttnArgs &a, const AttnSpan &sp, int kvh, int row0_, int col) {
@@ -158,6 +159,7 @@ struct KeyRows {
         k_row = (uint32_t)(a.ldk * SIZE), v_row = (uint32_t)(a.ldv * SIZE);
         column = (uint32_t)(col * SIZE);
         row0 = row0_;
+        k_off = row0 * k_row + column, v_off = row0 * v_row + column;
         page = at = 0;
     }
     // Looks up the keys of the tile at kb.
@@ -181,24 +183,33 @@ struct KeyRows {
             }
             return;
         }
-        const bool whole = kb + TILE_K <= sp.nk;
-#pragma unroll
-        for (int u = 0; u < PER; u++) {
-            // The first of these STEP rows (or the last key, where they lie past it), and the lane's from there.
-            const int first = kb + u * STEP, low = whole || first < sp.nk ? first : sp.nk - 1;
-            int64_t kat, vat;
+        // STEP rows from key `first` (or from the last key, where they lie past it).
+        const auto bases = [&](int u, int first, int64_t &kat, int64_t &vat) {
             if (PAGED) {
                 const int p = __builtin_amdgcn_readlane(page, u * STEP), s = __builtin_amdgcn_readlane(at, u * STEP);
                 const int64_t q = p < 0 ? 0 : p;
                 kat = q * (a.psk * SIZE) + (uint64_t)(uint32_t)s * k_row;
                 vat = q * (a.psv * SIZE) + (uint64_t)(uint32_t)s * v_row;
             } else {
-                kat = (uint64_t)(uint32_t)low * k_row;
-                vat = (uint64_t)(uint32_t)low * v_row;
+                kat = (uint64_t)(uint32_t)first * k_row;
+                vat = (uint64_t)(uint32_t)first * v_row;
             }
-            int row = row0;
-            if (!whole) row = first + row0 < sp.nk ? row0 : sp.nk - 1 - low;
-            f(u, k + kat + ((uint32_t)row * k_row + column), v + vat + ((uint32_t)row * v_row + column));
+        };
+        int64_t kat, vat;
+        if (kb + TILE_K <= sp.nk) {
+#pragma unroll
+            for (int u = 0; u < PER; u++) {
+                bases(u, kb + u * STEP, kat, vat);
+                f(u, k + kat + k_off, v + vat + v_off);
+            }
+            return;
+        }
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int first = kb + u * STEP, low = first < sp.nk ? first : sp.nk - 1;
+            bases(u, low, kat, vat);
+            const uint32_t row = first + row0 < sp.nk ? row0 : sp.nk - 1 - low;
+            f(u, k + kat + (row * k_row + column), v + vat + (row * v_row + column));
         }
     }
 };
