@@ -103,16 +103,13 @@ class PagedCache:
         """The cache's part of a description."""
         a.type, a.kv_heads, a.d = self.type, self.kv_heads, self.d
         a.pages, a.page = self.pages, self.page
-        for t, rows in ((self.k, a.k), (self.v, a.v)):
+        for t, rows, which in ((self.k, a.k, "k_page"), (self.v, a.v, "v_page")):
             at, (pages, page, heads, d), (ps, ld, hs, _) = t.data_ptr(), t.shape, t.stride()
             ld, hs = ld if page > 1 else heads * d, hs if heads > 1 else d
             ps = ps if pages > 1 else page * heads * d
             rows.p, rows.ld, rows.hs = at, ld, hs
             rows.len = (pages - 1) * ps + (page - 1) * ld + (heads - 1) * hs + d if t.numel() else 0
-            if t is self.k:
-                a.k_page = ps
-            else:
-                a.v_page = ps
+            setattr(a, which, ps)
 
     def _name_seqs(self, a, rows: int, tables, lengths, q_starts, longest: Optional[int]) -> None:
         """The sequences of `rows` new rows in a: their tables, lengths and first rows."""
@@ -138,6 +135,8 @@ class PagedCache:
         equal share, at key positions lengths[b] - n to lengths[b] - 1, keys rotated for those positions
         by `rotary`. longest: the most rows of one sequence (default: all)."""
         a, kern = _begun(self._desc), self._kernels
+        if rotary is not None and rotary._kernels.device != kern.device:
+            raise TypeError("the rotary positions live on another GPU")
         kn, vn = _lib.Rows(), _lib.Rows()
         rows = _rows(kern, k, self.kv_heads, self.d, "k", kn)
         if _rows(kern, v, self.kv_heads, self.d, "v", vn) != rows or v.dtype != k.dtype:

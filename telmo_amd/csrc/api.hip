@@ -1780,7 +1780,7 @@ int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t 
     if ((rc = check_rows(ctx, "v_new", v_new, type, nv))) return rc;
     const size_t ks = rows_span(a.k, a.page, a.kv_heads, a.d), vs = rows_span(a.v, a.page, a.kv_heads, a.d);
     if (!rows_distinct(a.k, a.page, a.kv_heads, a.d) || !rows_distinct(a.v, a.page, a.kv_heads, a.d) ||
-        (a.pages > 1 && (a.k_page < ks || a.v_page < vs)))
+        (a.pages > 1 && (a.k_page < ks || a.v_page < vs)) || (ks && a.pages && a.k.p == a.v.p))
         return fail(ctx, TG_ERR_SHAPE, "the cache's strides put two rows in one place");
     const size_t size = type_bytes(a.type), from = type_bytes(type);
     const size_t kc = rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page) * size;

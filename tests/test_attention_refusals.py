@@ -141,6 +141,7 @@ def test_rotary(kw, code):
     ({}, dict(v=rows(0, 20, 2, 64)), NULL), ({}, dict(k=rows(AT * 12 + 2, 20, 2, 64)), ALIGN), ({}, dict(k=rows(AT * 2, 20, 2, 64)), ARG),
     ({}, dict(v=rows(AT * 3 + 64, 20, 2, 64)), ARG), (dict(k_page=15 * 128), {}, SHAPE), (dict(v_page=0), {}, SHAPE),
     (dict(k=rows(AT * 2, 7 * 16, 2, 64, hs=32)), {}, SHAPE), (dict(tables=0), {}, NULL), (dict(pages=8), {}, SHAPE),
+    (dict(v=rows(AT * 2, 7 * 16, 2, 64)), {}, SHAPE),
     ({}, dict(rotary=turned(dim=66)), SHAPE)])
 def test_append(kw, new, code):
     from telmo_amd import _lib
@@ -270,6 +271,12 @@ def test_tensors_are_refused_by_place_shape_and_type():
     k = torch.zeros(4, 16, 2, 64)
     cache = attention.PagedCache(Kern, k, k.clone())
     assert (cache._desc.k_page, cache._desc.k.ld, cache._desc.k.hs, cache._desc.k.len) == (2048, 128, 64, 8192)
+    one = attention.PagedCache(Kern, k, k)._desc  # values that are the keys
+    assert (one.k_page, one.v_page, one.v.ld, one.v.len) == (2048, 2048, 128, 8192)
+    rotary = attention.Rotary.__new__(attention.Rotary)
+    rotary._kernels = Gpu
+    with pytest.raises(TypeError, match="another GPU"):
+        cache.append(k[0], k[1], torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), rotary=rotary)
     with pytest.raises(ValueError, match="one type"):
         attention.PagedCache(Kern, k, k.half())
     att, q = attention.Attention(Kern, 4, 64, kv_heads=2), torch.zeros(3, 4, 64)
