@@ -128,19 +128,20 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const T *k, int64_t ldk
     const AttnSpan sp = span_of(q, b);
     const int pairs = r.dim / 2, k_pieces = pieces_of(d, r.dim), pieces = k_pieces + d / 8;
     const int rows = sp.nq < q.longest ? sp.nq : q.longest;
+    // The length as it stands, also past the table: cut to it, new rows would take older ones' places.
+    const int64_t first = (int64_t)q.lengths[b] - sp.nq;
     for (int r0 = blockIdx.x * ROWS; r0 < rows; r0 += gridDim.x * ROWS) {
         const int n = rows - r0 < ROWS ? rows - r0 : ROWS;
         __syncthreads();
         if ((int)threadIdx.x < n) {
-            const int64_t pos = (int64_t)sp.shift() + r0 + threadIdx.x;
+            const int64_t pos = first + r0 + threadIdx.x;
             const bool held = pos >= 0 && pos < sp.nk;
             int at = 0;
             page[threadIdx.x] = held ? page_of(q, b, (int)pos, at) : -1;
             in_page[threadIdx.x] = at;
         }
         for (int t = threadIdx.x; t < n * pairs; t += THREADS)
-            table[t / pairs][t % pairs] =
-                turn(((double)sp.shift() + r0 + t / pairs) * r.turns[t % pairs], r.amplitude);
+            table[t / pairs][t % pairs] = turn((double)(first + r0 + t / pairs) * r.turns[t % pairs], r.amplitude);
         __syncthreads();
         for (int t = threadIdx.x; t < n * heads * pieces; t += THREADS) {
             const int at = t / (heads * pieces), h = t / pieces % heads, piece = t % pieces;

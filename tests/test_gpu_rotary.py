@@ -94,14 +94,14 @@ def test_in_place(tk, interleaved):
 # ------------------------------------------------------------------------------------------ append
 
 def append(tk, type="f32", to="bf16", kv_heads=2, d=64, new=(1, 1), lengths=(1, 30), page=16, dim=None, interleaved=False,
-           layout="rows", starts=True, longest=None, bad=(), k_layout="rows"):
+           layout="rows", starts=True, longest=None, bad=(), k_layout="rows", width=None):
     import torch
 
     import telmo_amd
 
     say("append", type, to, kv_heads, d, new, lengths, page, dim, layout, bad)
-    rng = np.random.default_rng(sum(lengths) + page)
-    batch, width = len(new), max(max(-(-n // page) for n in lengths), 1)
+    rng = np.random.default_rng(abs(sum(lengths)) + page)
+    batch, width = len(new), width or max(max(-(-n // page) for n in lengths), 1)
     pages = batch * width + 1
     tables = rng.permutation(pages)[:batch * width].reshape(batch, width).astype(np.int64)
     for b, entry, value in bad:
@@ -124,7 +124,7 @@ def append(tk, type="f32", to="bf16", kv_heads=2, d=64, new=(1, 1), lengths=(1, 
     for n, total, table in zip(new, lengths, tables):
         for i in range(n if longest is None else min(n, longest)):
             p = total - n + i
-            if 0 <= p < total and 0 <= table[p // page] < pages:
+            if 0 <= p < width * page and 0 <= table[p // page] < pages:
                 at = (table[p // page], p % page)
                 row = k64[r + i:r + i + 1]
                 if dim is not None:
@@ -155,3 +155,10 @@ def test_append_leaves_what_has_no_place(tk):
     append(tk, new=(5, 2), lengths=(3, 0), dim=64)  # fewer positions than rows
     append(tk, new=(20, 20), lengths=(40, 40), bad=[(0, 2, -1), (1, 1, 99)])
     append(tk, new=(20, 5), lengths=(40, 40), longest=6)
+
+
+def test_append_past_the_table_leaves_older_keys(tk):
+    """Lengths that the table has no pages for: the rows behind it have no place, and those before keep
+    theirs; so do lengths below zero."""
+    append(tk, new=(20, 5, 3), lengths=(40, 90, 2**31 - 1), width=2, dim=64)
+    append(tk, new=(6, 6), lengths=(-3, 2), width=2)
