@@ -198,6 +198,11 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
             s = score_of(a, dot, h, slope, j - i);
             shown = s != -INFINITY;
         }
+        // A shown score of NaN or infinity makes the whole row NaN, whatever the other keys hold.
+        if (__any(shown && !(s < INFINITY))) {
+            l = NAN;
+            break;
+        }
         unsigned long long live = __ballot(shown);
         if (!live) continue;
         float top = s;
