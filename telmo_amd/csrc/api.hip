@@ -1634,11 +1634,11 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
     if (!(a.softcap >= 0.0f) || !std::isfinite(a.softcap))
         return fail(ctx, TG_ERR_ARG, "softcap must be finite and not negative");
     if (a.slopes && a.slopes_len < a.heads) return fail(ctx, TG_ERR_SHAPE, "slopes is too short");
-    if (a.table && (a.table_span > MAX_ATTN_ROWS || a.table_len < a.heads * (2 * a.table_span + 1)))
+    if (a.table && (a.table_span >= MAX_ATTN_ROWS || a.table_len < a.heads * (2 * a.table_span + 1)))
         return fail(ctx, TG_ERR_SHAPE, "table is too short");
     if (a.rel) {
         if (a.type != TG_F32) return fail(ctx, TG_ERR_UNSUPPORTED, "position rows are f32 and go with f32 rows");
-        if (a.rel_span > MAX_ATTN_ROWS) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^31 position rows");
+        if (a.rel_span >= MAX_ATTN_ROWS) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^31 position rows");
         const tg_rows rel{a.rel, a.rel_len, a.ldrel, a.hsrel};
         if ((rc = check_rows(ctx, "rel", rel, TG_F32, rows_span(rel, 2 * a.rel_span + 1, a.heads, a.d)))) return rc;
         if ((a.rel_u && a.rel_u_len < a.heads * a.d) || (a.rel_v && a.rel_v_len < a.heads * a.d))
@@ -1691,6 +1691,12 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
         return fail(ctx, TG_ERR_ARG, "out must not overlap q, k or v");
     if (a.workspace && reinterpret_cast<uintptr_t>(a.workspace) % 16)
         return fail(ctx, TG_ERR_ALIGN, "workspace must be 16-byte aligned");
+    const size_t work = a.workspace ? a.workspace_len : 0;
+    if (ranges_overlap(a.workspace, work, a.out.p, o_span * size) ||
+        ranges_overlap(a.workspace, work, a.q.p, q_span * size) ||
+        ranges_overlap(a.workspace, work, a.k.p, k_span * size) ||
+        ranges_overlap(a.workspace, work, a.v.p, v_span * size))
+        return fail(ctx, TG_ERR_ARG, "workspace must not overlap out, q, k or v");
     if (!ctx) return TG_ERR_NULL;
     if (k.seqs.batch == 0 || k.seqs.longest == 0) return TG_OK;
     const auto clip = [](int64_t w) { return w < 0 ? -1 : w > INT32_MAX ? -1 : (int32_t)w; };
@@ -1709,7 +1715,10 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
     k.work = a.workspace, k.work_bytes = a.workspace ? a.workspace_len : 0;
     std::lock_guard<std::mutex> g(ctx->mu);
     TG_HIP(ctx, hipSetDevice(ctx->device));
-    TG_HIP(ctx, tg::launch_attention(k, ctx->stream));
+    const hipError_t e = tg::launch_attention(k, ctx->stream);
+    if (e == hipErrorInvalidConfiguration)
+        return fail(ctx, TG_ERR_UNSUPPORTED, "more tiles than a launch holds: longest bounds those of ragged sequences");
+    TG_HIP(ctx, e);
     return TG_OK;
 }
 

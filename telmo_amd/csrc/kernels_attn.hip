@@ -79,7 +79,9 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArg
 
 template <typename T>
 hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
-    const dim3 grid((unsigned)div_ceil((size_t)a.seqs.longest, ROW_WAVES), (unsigned)a.heads, (unsigned)a.seqs.batch);
+    const size_t blocks = div_ceil((size_t)a.seqs.longest, ROW_WAVES);
+    if (blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)blocks, (unsigned)a.heads, (unsigned)a.seqs.batch);
     hipLaunchKernelGGL((attn_rows_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a);
     return hipGetLastError();
 }

@@ -75,6 +75,9 @@ def call(a, which="tg_attention_device"):
     (dict(q_docs=AT * 7, q_docs_len=19), SHAPE), (dict(q_docs=AT * 7, q_docs_len=20), OK), (dict(k_docs=AT * 7, k_docs_len=20), ARG),
     (dict(q_docs=AT * 7, q_docs_len=20, k_docs=AT * 8, k_docs_len=19), SHAPE),
     (dict(workspace=AT * 7 + 8, workspace_len=64), ALIGN), (dict(tables=AT * 7), ARG), (dict(lengths=AT * 7), ARG),
+    (dict(workspace=AT * 7, workspace_len=64), OK), (dict(workspace=AT - 48, workspace_len=64), ARG), (dict(workspace=AT * 2, workspace_len=64), ARG),
+    (dict(workspace=AT * 3 + 4096, workspace_len=64), ARG), (dict(workspace=AT * 4 + 10224, workspace_len=64), ARG),
+    (dict(table=AT * 7, table_len=1 << 40, table_span=1 << 30), SHAPE), (dict(table=AT * 7, table_len=1 << 40, table_span=(1 << 30) - 1), OK),
     (dict(q_rows=0, k_rows=0, q=rows(0, 0, 4, 64), out=rows(0, 0, 4, 64)), OK), (dict(k_rows=0, k=rows(0, 0, 2, 64), v=rows(0, 0, 2, 64)), OK)])
 def test_attention(kw, code):
     assert call(desc(**kw)) == code
@@ -83,7 +86,8 @@ def test_attention(kw, code):
 @pytest.mark.parametrize("kw,code", [
     ({}, OK), (dict(rel_len=7 * 256 - 1), SHAPE), (dict(rel=AT * 7 + 4), ALIGN), (dict(ldrel=257, rel_len=1 << 20), ALIGN),
     (dict(rel_span=4), SHAPE), (dict(hsrel=0), OK), (dict(rel_u=AT * 8, rel_u_len=255), SHAPE),
-    (dict(rel_u=AT * 8, rel_u_len=256, rel_v=AT * 9, rel_v_len=256), OK), (dict(rel_span=1 << 40), UNSUPPORTED)])
+    (dict(rel_u=AT * 8, rel_u_len=256, rel_v=AT * 9, rel_v_len=256), OK), (dict(rel_span=1 << 40), UNSUPPORTED),
+    (dict(rel_span=1 << 30, rel_len=1 << 50), UNSUPPORTED), (dict(rel_span=(1 << 30) - 1, rel_len=1 << 50), OK)])
 def test_position_rows(kw, code):
     a = desc(type=0, rel=AT * 7, rel_len=7 * 256, ldrel=256, hsrel=64, rel_span=3)
     for name, value in kw.items():

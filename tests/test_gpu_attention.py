@@ -404,6 +404,55 @@ def test_keys_that_a_query_is_not_shown_may_hold_anything(tk, type, what):
             assert not np.isfinite(got[60:90]).any()
 
 
+@pytest.mark.parametrize("type,d,what", itertools.product(TYPES, (64, 136), (np.nan, np.inf)))
+def test_rows_that_see_a_nan_score_are_nan_and_others_are_not(tk, type, d, what):
+    """Queries of NaN or infinity, whose scores are NaN (an infinity's have both signs among their products):
+    whole rows of NaN, beside rows as they are. Over enough keys for a row to end at the first of them."""
+    import torch
+
+    import telmo_amd
+
+    n, heads = 700, 2
+    rng = np.random.default_rng(5)
+    q, q64 = rows_of(rng, type, n, heads, d)
+    k, k64 = rows_of(rng, type, n, heads, d)
+    v, v64 = rows_of(rng, type, n, heads, d)
+    bad = np.r_[3, 100:140, n - 1]
+    q[bad] = what
+    out = torch.zeros_like(q)
+    telmo_amd.Attention(tk, heads, d).forward(q, k, v, out)
+    tk.synchronize()
+    got, clean = out.double().cpu().numpy(), np.setdiff1d(np.arange(n), bad)
+    assert np.isnan(got[bad]).all()
+    shown = np.ones((len(clean), n), bool)
+    for h in range(heads):
+        want, size = attend(q64[clean, h], k64[:, h], v64[:, h], d**-0.5, shown)
+        check(got[clean, h], want, tolerance(type, d, n, size, np.abs(v64).max(), False))
+
+
+@pytest.mark.parametrize("rel", (False, True))
+def test_more_tiles_than_a_launch_holds_are_refused(tk, rel):
+    """Ragged sequences of which any might hold all rows: refused before any launch; their longest makes it fit."""
+    import torch
+
+    import telmo_amd
+
+    # With position rows heads of 136 take a wavefront per row: 2^26 rows are one workgroup too many for it. All rows but
+    # the output's are one (stride 0).
+    batch, rows, heads, d = (1, 1 << 26, 1, 136) if rel else (65535, 1 << 17, 16, 8)
+    q = torch.ones((1, heads, d), dtype=torch.float32 if rel else torch.float16, device="cuda").expand(rows, heads, d)
+    out = torch.zeros((rows, heads, d), dtype=q.dtype, device="cuda")
+    starts = torch.full((batch + 1,), 5, dtype=torch.int32, device="cuda")
+    starts[0] = 0
+    options = dict(rel=torch.zeros((3, d), device="cuda")) if rel else {}
+    att = telmo_amd.Attention(tk, heads, d, left=1, right=1)
+    with pytest.raises(telmo_amd.TelmoError, match="longest"):
+        att.forward(q, q, q, out, q_starts=starts, **options)
+    att.forward(q, q, q, out, q_starts=starts, longest=5, **options)
+    tk.synchronize()
+    assert bool((out[:5] == 1.0).all()) and not bool(out[5:].any())
+
+
 @pytest.mark.parametrize("type", TYPES)
 def test_outputs_do_not_depend_on_the_run(tk, type):
     import torch
