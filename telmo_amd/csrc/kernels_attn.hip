@@ -94,6 +94,8 @@ hipError_t launch_join_of(const AttnArgs &a, int splits, hipStream_t s) {
                        dim3(64 * ROW_WAVES), 0, s, a, parts_of(a, splits));
     return hipGetLastError();
 }
+// More than four parts: 16 parts' loads at a time (a chunk's join with 4 at a time takes as long within 1 us); up to four
+// in one run (750 rows in two parts with 16 40.5 us, with 4 39.5).
 template <typename T>
 hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
     if (a.d > 128) return splits > 4 ? launch_join_of<T, 4, 16>(a, splits, s) : launch_join_of<T, 4, 4>(a, splits, s);
@@ -101,11 +103,24 @@ hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
 }
 
 // How a call is spread: workgroups of `tile` query rows and heads, and how many parts the keys are cut into so that
-// about `target` workgroups run, each with `least` keys or more.
+// about `target` workgroups run, each with `least` keys or more. Without parts a chunk of 509 rows over 32768 keys takes
+// 946 us (with 326), a minute's 750 f32 rows 84 (40), 2000 bf16 rows 52 (40). The targets, in us on either side:
+//
+//   TILES16    target 256, 512, 1024: the chunk 493, 326, 348; 100 rows over 32768 keys 137, 103, 113
+//   TILES32    target 128, 256, 512: 750 rows with position rows 84, 40, 41; 4 x 750 98, 98, 119; 2000 rows 215, 135, 150
+//   SMALL32    instead of TILES32, where that leaves half of the 256 CUs empty: 250 rows 33 (38), 128 rows 14.4 (16.2);
+//              everywhere it would take 750 rows from 40 to 54 and 4 x 750 from 98 to 173
+//   FEW        A CU holds one workgroup, whose start and end (page numbers, a cold pipeline, the wavefronts' sums)
+//              nothing hides; but sequences differ in length, and more workgroups even that out. Target 256, 512, 1024,
+//              2048: 32 sequences of up to 8192 keys 131, 115, 111, 128, all of them 8192 long 189, 195, 201, 225;
+//              16 of 8192 102, 107, 119, 129. 256 keys or more in a part (512): 2048 keys of one sequence 13.4 (15.2),
+//              eight of 750 in f32 21.6 (28.8)
+//   FEW_ALONE  A single sequence's parts are alike: one round of workgroups, 32768 keys 31.5 (36.8). Heads of up to 64
+//              take fewer registers and gain nothing (100,000 keys of 16 heads 97 against 89)
 struct Spread {
     size_t tile, target, least;
 };
-constexpr Spread TILES16{128, 512, 256}, FEW{16, 2048, 512};
+constexpr Spread TILES16{128, 512, 256}, FEW{16, 512, 256}, FEW_ALONE{16, 256, 256};
 constexpr Spread TILES32{128, 256, 128}, SMALL32{64, 256, 128};
 constexpr size_t MOST_PARTS = 64;  // a lane of the joining wavefront each
 
@@ -157,7 +172,7 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
         if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
         return n < 1 ? (size_t)1 : n;
     };
-    Spread sp = few ? FEW : a.type != F32 ? TILES16 : TILES32;
+    Spread sp = few ? (a.seqs.batch == 1 && a.d > 64 ? FEW_ALONE : FEW) : a.type != F32 ? TILES16 : TILES32;
     size_t n = parts(sp);
     // f32 tiles of 64 rows where those of 128 leave half of the GPU's 256 CUs empty.
     if (!few && a.type == F32 && tiles_of(sp) * sets * n <= 128) {
