@@ -26,7 +26,8 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_rows_kernel(const AttnArg
 
 // The parts of a row and head, joined by one wavefront: with M the largest maximum, the sums and outputs of
 // part p count e^(m_p - M) times. Lane p weighs part p; then each lane adds V values of all parts, in their order,
-// STEP parts' loads on their way at a time.
+// STEP parts' loads on their way at a time. Bound by reading the parts: 509 rows of 32 heads of 128 in
+// four parts, 34 MB, 11.6 us (2.9 TB/s); 32 single rows 4.9 us, mostly the latency of its loads in turn.
 template <typename T, int V, int STEP>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArgs a, const AttnParts parts) {
     typedef float fv __attribute__((ext_vector_type(V)));
@@ -112,9 +113,10 @@ hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
 //              everywhere it would take 750 rows from 40 to 54 and 4 x 750 from 98 to 173
 //   FEW        A CU holds one workgroup, whose start and end (page numbers, a cold pipeline, the wavefronts' sums)
 //              nothing hides; but sequences differ in length, and more workgroups even that out. Target 256, 512, 1024,
-//              2048: 32 sequences of up to 8192 keys 131, 115, 111, 128, all of them 8192 long 189, 195, 201, 225;
-//              16 of 8192 102, 107, 119, 129. 256 keys or more in a part (512): 2048 keys of one sequence 13.4 (15.2),
-//              eight of 750 in f32 21.6 (28.8)
+//              2048: 16 sequences of 8192 keys and 8 key heads 102, 107, 119, 129, of up to 8192 keys (512 and 768)
+//              42 to 78, 47 to 77. From one workgroup per CU on, a part more: 32 sequences of up to 8192 keys
+//              110 to 134 us (114 to 150), 64 of up to 4096 108 to 136 (113 to 140), 32 of 8192 each 202 (195).
+//              256 keys or more in a part (512): 2048 keys of one sequence 13.4 (15.2), eight of 750 in f32 21.6 (28.8)
 //   FEW_ALONE  A single sequence's parts are alike: one round of workgroups, 32768 keys 31.5 (36.8). Heads of up to 64
 //              take fewer registers and gain nothing (100,000 keys of 16 heads 97 against 89)
 struct Spread {
@@ -126,6 +128,7 @@ constexpr size_t MOST_PARTS = 64;  // a lane of the joining wavefront each
 
 size_t parts_for(const Spread &sp, size_t wgs, size_t keys) {
     size_t n = sp.target / (wgs ? wgs : 1);
+    if (sp.tile == FEW.tile && wgs >= 256) n++;
     if (n > keys / sp.least) n = keys / sp.least;
     return n < 1 ? 1 : n > MOST_PARTS ? MOST_PARTS : n;
 }

@@ -5,7 +5,9 @@
 // frequency of one radian keeps 2^-4 radians), so the turns p f / 2 pi are a 64-bit product whose whole
 // turns are dropped in 64 bits; what is left is exact enough in 32. A workgroup takes rows, works out
 // each row's sines and cosines once into LDS and rotates all heads with them: the kernel moves x in and
-// out and the 64-bit work is one pair in each head's place.
+// out and the 64-bit work is one pair in each head's place. Bound by memory: 16384 rows of 32 heads of 128 in
+// bf16, half of each rotated, 268 MB in 64.4 us (4.2 TB/s; a large copy 4.8); eight rows take the time of a call,
+// 7.5 us. Four rows to a workgroup keep 256 lanes busy with the pairs of heads of 128 in one step.
 #include "attn_common.hpp"
 
 namespace tg {
@@ -117,6 +119,8 @@ __global__ __launch_bounds__(THREADS) void rotary_kernel(const T *x, int64_t ldx
     }
 }
 
+// The rows of all sequences, a page lookup per row. 4 x 2047 rows of 8 f32 heads of 128 into bf16 pages: 101 MB of reads
+// and writes in 19.7 us (5.1 TB/s).
 template <typename T, typename U>
 __global__ __launch_bounds__(THREADS) void append_kernel(const T *k, int64_t ldk, int64_t hsk, const T *v,
                                                          int64_t ldv, int64_t hsv, U *ck, int64_t ldck, int64_t hsck,
