@@ -339,7 +339,11 @@ int tg_dwconv1d_quant_device(tg_ctx *ctx, const float *x, size_t x_len, size_t l
  * gets zeros. Keys that no query is shown may hold anything.
  * Scores, softmax statistics and sums are f32; with 16-bit types the weights round to that type (half a
  * step) before they multiply the values, and the outputs once. f32 rows are computed to f32's accuracy.
- * Rows of q and out behind the last sequence are neither read nor written. */
+ * A shown score of NaN or +infinity makes its row NaN. Rows of q and out behind the last sequence are neither
+ * read nor written. Sequences hold up to 2^30 keys. Fast for every sequence and head size but these, which
+ * take a wavefront per row: position rows with heads past 128, and row strides past 8 million values (chunks of
+ * rows; single tokens take any). A row whose shown keys are sound beside hidden ones that hold NaN or infinity
+ * may be computed twice. */
 typedef struct {
     const void *p; /* device, 16-byte aligned */
     size_t len;    /* elements reachable from p */
@@ -361,7 +365,8 @@ typedef struct {
     size_t rel_u_len, rel_v_len;
     size_t batch;                 /* sequences, at most 65535 */
     size_t q_rows, k_rows;        /* rows of q and out, rows of k and v (k_rows unused when paged) */
-    size_t longest;               /* most query rows of a sequence; rows past it stay as they were. 0: any */
+    size_t longest;               /* most query rows of a sequence; rows past it stay as they were. 0: any, and
+                                   * ragged sequences launch tiles for all rows each (TG_ERR_UNSUPPORTED past 2^23) */
     const int32_t *q_starts;      /* device, batch + 1 first rows (the last one: the end), or null: sequences */
     const int32_t *k_starts;      /*   of equal length, stacked along the rows. k_starts null: as q_starts */
     size_t q_starts_len, k_starts_len;
@@ -379,7 +384,8 @@ typedef struct {
     size_t lengths_len;
     size_t pages, page;           /* pages of the cache, rows per page */
     size_t k_page, v_page;        /* elements between pages of k and of v */
-    void *workspace;              /* device, 16-byte aligned, or null: see tg_attention_workspace_bytes */
+    void *workspace;              /* device, 16-byte aligned, apart from q, k, v and out, or null: see
+                                   * tg_attention_workspace_bytes */
     size_t workspace_len;         /* bytes */
 } tg_attention_desc;
 /* Device pointers, queued on the context's stream; nothing is allocated, so the calls can be captured
@@ -413,7 +419,9 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
  * q_starts[b] .. of k_new and v_new, or equal lengths) is written at key position lengths[b] - n + r, its key
  * rotated for that position first where rotary is given. desc names the cache as tg_attention_paged_device
  * reads it (type, kv_heads, d, k, v, k_page, v_page, page, pages, tables, lengths, batch, q_rows, q_starts,
- * longest). Rows whose position has no page are not written; two rows in one place leave either of them. */
+ * longest). Rows whose position is negative or has no page are not written, lengths past the table's included
+ * (unlike attention's, they are not cut to it); two rows in one place leave either of them. k and v are not one
+ * tensor. */
 int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
                            const tg_rotary *rotary);
 

@@ -12,7 +12,7 @@ quantised wherever the product is their only reader:
     att   LayerNorm(norm_att)       -> quantised rows
           qkv                       -> f32 q, k, v (the attention core reads them)
           [pos_proj of the positions, when given]
-          attention(q, k, v) -> att  (the caller's; outside this path: the V third stands in)
+          attention(q, k, v) -> att  (the argument, e.g. Attention.for_layer; the V third without one)
           out, x += .                                          tg_matmul_device (quantises att)
     conv  LayerNorm(norm_conv)      -> quantised rows
           pw1 + GLU                 -> f32                     tg_matmul_quantized_glu_device

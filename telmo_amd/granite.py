@@ -9,7 +9,7 @@ rows resident in GPU memory, every int8 product on the library's fast path:
           ff1.down + bias, x += 0.5 * .                       tg_matmul_quantized_device
     att   LayerNorm(norm_att)      -> quantised rows
           qkv (no bias)            -> f32 q, k, v (the attention core reads them)
-          attention(q, k, v) -> att  (the caller's; outside this path: the V third stands in)
+          attention(q, k, v) -> att  (the argument, e.g. Attention.for_layer; the V third without one)
           out + bias, x += .                                  tg_matmul_device (quantises att)
     conv  LayerNorm(norm_conv)     -> quantised rows of the t input frames
           pw1 + bias, GLU          -> f32 [t, conv_channels]  tg_matmul_quantized_glu_device
