@@ -124,19 +124,24 @@ __device__ __forceinline__ float shown_or_not(float s, uint32_t bits, int bit) {
 // first.
 struct Place {
     int b, head, part, group;  // head: of k where the group shares a tile, of q otherwise
-    int64_t pair0, pairs;      // the tile's first pair, the sequence's pairs
+    int pair0, pairs;          // the tile's first pair, the sequence's pairs: 2^24 tiles of 128 at most
     AttnSpan sp;
     __device__ __forceinline__ bool find(const AttnArgs &a, int parts, int q_tiles, int groups, int heads, int tile_q) {
-        const int at = blockIdx.x % groups, tile = q_tiles - 1 - (int)(blockIdx.x / groups);
-        part = at % parts;
-        head = at / parts % heads;
-        b = at / parts / heads;
-        group = a.heads / heads;
+        const uint32_t tiles = blockIdx.x / (uint32_t)groups, at = blockIdx.x - tiles * (uint32_t)groups;
+        const uint32_t set = at / (uint32_t)parts;
+        const int tile = q_tiles - 1 - (int)tiles;
+        part = (int)(at - set * (uint32_t)parts);
+        b = (int)(set / (uint32_t)heads);
+        head = (int)(set - (uint32_t)b * (uint32_t)heads);
+        group = (int)((uint32_t)a.heads / (uint32_t)heads);
         sp = span_of(a.seqs, b);
-        pairs = (int64_t)(sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest) * group;
-        pair0 = (int64_t)tile * tile_q;
+        pairs = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest) * group;
+        pair0 = tile * tile_q;
         return pair0 < pairs;
     }
+    // The query row of a pair, and its head in the group.
+    __device__ __forceinline__ int row_of(int pair) const { return (int)((uint32_t)pair / (uint32_t)group); }
+    __device__ __forceinline__ int head_of(int pair) const { return pair - row_of(pair) * group; }
 };
 
 // Where a thread's pieces of a tile of keys come from: pieces u = 0 .. PER - 1 are its column of rows row0 + u STEP

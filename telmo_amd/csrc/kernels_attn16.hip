@@ -62,21 +62,21 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     if (!at.find(a, parts.parts, q_tiles, groups, a.kv_heads, TILE_Q)) return;
     const int part = at.part, kvh = at.head, b = at.b, group = at.group;
     const AttnSpan sp = at.sp;
-    const int64_t pairs = at.pairs, pair0 = at.pair0;
+    const int pairs = at.pairs, pair0 = at.pair0;
 
     const int t = threadIdx.x, lane = t & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
     // The lane's query, and the first and last of the wavefront's and the workgroup's.
-    const int64_t pair = pair0 + wave * 32 + col;
+    const int pair = pair0 + wave * 32 + col;
     const bool live = pair < pairs;
-    const int r = live ? (int)(pair / group) : 0, h = kvh * group + (live ? (int)(pair % group) : 0);
+    const int r = live ? at.row_of(pair) : 0, h = kvh * group + (live ? at.head_of(pair) : 0);
     const int i = sp.shift() + r;
     const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
-    const int64_t wave0 = pair0 + wave * 32, wave1 = wave0 + 31 < pairs - 1 ? wave0 + 31 : pairs - 1;
-    const int64_t pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
-    const auto window_at = [&](int64_t p) {
-        return window_of(sp.shift() + (int)(p / group), sp.nk, a.left, a.right, prefix);
+    const int wave0 = pair0 + wave * 32, wave1 = wave0 + 31 < pairs - 1 ? wave0 + 31 : pairs - 1;
+    const int pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
+    const auto window_at = [&](int p) {
+        return window_of(sp.shift() + at.row_of(p), sp.nk, a.left, a.right, prefix);
     };
     const bool wave_live = wave0 < pairs;
     const AttnWindow w_first = window_at(wave_live ? wave0 : 0), w_last = window_at(wave_live ? wave1 : 0);
@@ -267,9 +267,9 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     unsigned long long again = __ballot(live && worst > 0.0f && l - l == 0.0f);
     again = (again | again >> 32) & 0xffffffffull;
     while (again) {
-        const int64_t p = wave0 + __builtin_ctzll(again);
+        const int p = wave0 + __builtin_ctzll(again);
         again &= again - 1;
-        attend_row<T>(a, b, kvh * group + (int)(p % group), (int)(p / group), lane);
+        attend_row<T>(a, b, kvh * group + at.head_of(p), at.row_of(p), lane);
     }
 }
 

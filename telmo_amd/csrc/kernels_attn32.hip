@@ -160,20 +160,20 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
     const int part = at.part, b = at.b, group = at.group;
     const int kvh = REL ? at.head / (a.heads / a.kv_heads) : at.head;
     const AttnSpan sp = at.sp;
-    const int64_t pairs = at.pairs, pair0 = at.pair0;
+    const int pairs = at.pairs, pair0 = at.pair0;
 
     const int t = threadIdx.x, lane = t & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
-    const int64_t pair = pair0 + wave * 16 + col;
+    const int pair = pair0 + wave * 16 + col;
     const bool live = pair < pairs;
-    const int r = live ? (int)(pair / group) : 0, h = at.head * group + (live ? (int)(pair % group) : 0);
+    const int r = live ? at.row_of(pair) : 0, h = at.head * group + (live ? at.head_of(pair) : 0);
     const int i = sp.shift() + r;
     const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
-    const int64_t wave0 = pair0 + wave * 16, wave1 = wave0 + 15 < pairs - 1 ? wave0 + 15 : pairs - 1;
-    const int64_t pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
-    const auto window_at = [&](int64_t p) {
-        return window_of(sp.shift() + (int)(p / group), sp.nk, a.left, a.right, prefix);
+    const int wave0 = pair0 + wave * 16, wave1 = wave0 + 15 < pairs - 1 ? wave0 + 15 : pairs - 1;
+    const int pair1 = pair0 + TILE_Q - 1 < pairs - 1 ? pair0 + TILE_Q - 1 : pairs - 1;
+    const auto window_at = [&](int p) {
+        return window_of(sp.shift() + at.row_of(p), sp.nk, a.left, a.right, prefix);
     };
     const bool wave_live = wave0 < pairs;
     const AttnWindow w_first = window_at(wave_live ? wave0 : 0), w_last = window_at(wave_live ? wave1 : 0);
@@ -515,9 +515,9 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
     again |= again >> 32;
     again = (again | again >> 16) & 0xffff;
     while (again) {
-        const int64_t p = wave0 + __builtin_ctzll(again);
+        const int p = wave0 + __builtin_ctzll(again);
         again &= again - 1;
-        attend_row<float>(a, b, at.head * group + (int)(p % group), (int)(p / group), lane);
+        attend_row<float>(a, b, at.head * group + at.head_of(p), at.row_of(p), lane);
     }
 }
 
