@@ -58,34 +58,31 @@ struct Few {
 
 // D: head size rounded up to 64, 128 or 256. EXTRA: scores are capped or biased.
 template <typename T, int D, bool PAGED, bool EXTRA>
-__global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const AttnArgs a, const AttnParts parts, const int q_tiles) {
+__global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const AttnArgs a, const AttnParts parts) {
     typedef Few<T, D> F;
     constexpr int TILE = F::TILE, PITCH = D + 4, WAVES = F::WAVES, THREADS = F::THREADS;
     __shared__ __align__(16) float outs[WAVES][COLS][PITCH];
     __shared__ float tops[WAVES][COLS], sums[WAVES][COLS];
     __shared__ int again[COLS];
 
-    int id = blockIdx.x;
-    const int part = id % parts.parts;
-    id /= parts.parts;
-    const int tile = id % q_tiles;
-    id /= q_tiles;
-    const int kvh = id % a.kv_heads, b = id / a.kv_heads;
+    const uint32_t set = blockIdx.x / (uint32_t)parts.parts;
+    const int part = (int)(blockIdx.x - set * (uint32_t)parts.parts);
+    const int b = (int)(set / (uint32_t)a.kv_heads), kvh = (int)set - b * a.kv_heads;
     const AttnSpan sp = span_of(a.seqs, b);
-    const int group = a.heads / a.kv_heads;
-    const int pairs = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest) * group, pair0 = tile * COLS;
-    if (pair0 >= pairs) return;
+    const int group = (int)((uint32_t)a.heads / (uint32_t)a.kv_heads);
+    const int pairs = (sp.nq < a.seqs.longest ? sp.nq : a.seqs.longest) * group;  // COLS at most
+    if (pairs == 0) return;
+    const auto row_of = [&](int pair) { return (int)((uint32_t)pair / (uint32_t)group); };
 
     const int t = threadIdx.x, lane = t & 63, quarter = lane >> 4, col = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);  // a scalar, and what follows from it
     const int prefix = a.prefix ? a.prefix[b] : 0;
-    const bool live = pair0 + col < pairs;
-    const int r = live ? (pair0 + col) / group : 0, h = kvh * group + (live ? (pair0 + col) % group : 0);
+    const bool live = col < pairs;
+    const int r = live ? row_of(col) : 0, h = kvh * group + (live ? col - r * group : 0);
     const int i = sp.shift() + r;
     const AttnWindow win = window_of(i, sp.nk, a.left, a.right, prefix);
-    const int last = pair0 + COLS - 1 < pairs - 1 ? pair0 + COLS - 1 : pairs - 1;
-    const AttnWindow w_first = window_of(sp.shift() + pair0 / group, sp.nk, a.left, a.right, prefix);
-    const AttnWindow w_last = window_of(sp.shift() + last / group, sp.nk, a.left, a.right, prefix);
+    const AttnWindow w_first = window_of(sp.shift(), sp.nk, a.left, a.right, prefix);
+    const AttnWindow w_last = window_of(sp.shift() + row_of(pairs - 1), sp.nk, a.left, a.right, prefix);
     const Tiles<TILE> tiles(w_first, w_last);
     const int n0 = (int)((int64_t)tiles.count * part / parts.parts) + wave;
     const int n1 = (int)((int64_t)tiles.count * (part + 1) / parts.parts);
@@ -315,8 +312,8 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
                     f32x4{acc[w][x][e], acc[w][x + 1][e], acc[w][x + 2][e], acc[w][x + 3][e]};
     __syncthreads();
     for (int y = t; y < COLS * (D / 4); y += THREADS) {
-        const int oc = y / (D / 4), c = y % (D / 4) * 4, pair = pair0 + oc;
-        if (pair >= pairs || c >= a.d) continue;
+        const int oc = y / (D / 4), c = y % (D / 4) * 4;
+        if (oc >= pairs || c >= a.d) continue;
         float top = -INFINITY, sum = 0.0f;
         for (int w = 0; w < WAVES; w++) top = fmaxf(top, tops[w][oc]);
         const float base = top == -INFINITY ? 0.0f : top;
@@ -328,8 +325,9 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
             const f32x4 x = *reinterpret_cast<const f32x4 *>(&outs[w][oc][c]);
             for (int e = 0; e < 4; e++) o[e] = __builtin_fmaf(weight, x[e], o[e]);
         }
-        const int64_t to_row = (int64_t)sp.q0 + pair / group;
-        const int to_head = kvh * group + pair % group;
+        const int pair_row = row_of(oc);
+        const int64_t to_row = (int64_t)sp.q0 + pair_row;
+        const int to_head = kvh * group + oc - pair_row * group;
         if (parts.parts > 1) {
             const size_t to = (size_t)part * parts.pairs + to_row * a.heads + to_head;
             if (c == 0) {
@@ -355,16 +353,15 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
     // A hidden key's NaN or infinity beside a sound sum of weights, as in the tile kernels.
     __syncthreads();
     for (int x = wave; x < COLS; x += WAVES)
-        if (again[x]) attend_row<T>(a, b, kvh * group + (pair0 + x) % group, (pair0 + x) / group, lane);
+        if (again[x]) attend_row<T>(a, b, kvh * group + x - row_of(x) * group, row_of(x), lane);
 }
 
 template <typename T, int D, bool PAGED, bool EXTRA>
 hipError_t launch_few(const AttnArgs &a, int splits, hipStream_t s) {
-    const size_t q_tiles = div_ceil((size_t)a.seqs.longest * (a.heads / a.kv_heads), COLS);
-    const size_t blocks = q_tiles * a.seqs.batch * a.kv_heads * splits;
+    const size_t blocks = (size_t)a.seqs.batch * a.kv_heads * splits;
     if (blocks > MAX_ATTN_BLOCKS / 2) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((attn_few_kernel<T, D, PAGED, EXTRA>), dim3((unsigned)blocks), dim3(Few<T, D>::THREADS), 0,
-                       s, a, parts_of(a, splits), (int)q_tiles);
+                       s, a, parts_of(a, splits));
     return hipGetLastError();
 }
 
