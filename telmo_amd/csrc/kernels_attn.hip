@@ -95,12 +95,17 @@ hipError_t launch_join_of(const AttnArgs &a, int splits, hipStream_t s) {
                        dim3(64 * ROW_WAVES), 0, s, a, parts_of(a, splits));
     return hipGetLastError();
 }
-// More than four parts: 16 parts' loads at a time (a chunk's join with 4 at a time takes as long within 1 us); up to four
-// in one run (750 rows in two parts with 16 40.5 us, with 4 39.5).
+// The parts' loads on their way at a time, 4, 8 or 16: past the last part they repeat it, so not many more than there
+// are (750 rows in five parts with 16 41.7 us, with 8 41.1; a chunk's four with 4 as with 16 within 1 us).
+template <typename T, int V>
+hipError_t launch_join_by(const AttnArgs &a, int splits, hipStream_t s) {
+    return splits > 8   ? launch_join_of<T, V, 16>(a, splits, s)
+           : splits > 4 ? launch_join_of<T, V, 8>(a, splits, s)
+                        : launch_join_of<T, V, 4>(a, splits, s);
+}
 template <typename T>
 hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
-    if (a.d > 128) return splits > 4 ? launch_join_of<T, 4, 16>(a, splits, s) : launch_join_of<T, 4, 4>(a, splits, s);
-    return splits > 4 ? launch_join_of<T, 2, 16>(a, splits, s) : launch_join_of<T, 2, 4>(a, splits, s);
+    return a.d > 128 ? launch_join_by<T, 4>(a, splits, s) : launch_join_by<T, 2>(a, splits, s);
 }
 
 // How a call is spread: workgroups of `tile` query rows and heads, and how many parts the keys are cut into so that
