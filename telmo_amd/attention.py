@@ -11,14 +11,22 @@ context's stream and nothing is allocated but by ``Rotary``'s constructor.
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from typing import Optional
 
 import numpy as np
 
 from . import _lib
 from .kernels import Kernels, Precision, _check
+
+# Neighbouring fields of the descriptions, written at once: a call of a few microseconds is queued for every token.
+_ROWS = struct.Struct("@PNNN")  # a tg_rows
+_SEQS = struct.Struct("@NNNNPPNN")  # batch to k_starts_len of a tg_attention_desc
+_PAGES = struct.Struct("@PNNNPNNNNN")  # its tables to v_page
+_CACHE = struct.Struct("@PNNNPNNN")  # its k and v
+_AT_SEQS, _AT_Q, _AT_K, _AT_V, _AT_OUT, _AT_PAGES = (getattr(_lib.AttentionDesc, name).offset for name in
+                                                     ("batch", "q", "k", "v", "out", "tables"))
 
 _TYPES = {}  # torch's types, made on first use
 _INT32, _FLOAT32 = "int32", "float32"
@@ -45,8 +53,8 @@ def _type(t, name: str) -> int:
     return p
 
 
-def _rows(kern: Kernels, t, heads: int, d: int, name: str, into) -> int:
-    """Fills the tg_rows `into` from t, [rows, heads, d] or [rows, heads * d]; returns the rows."""
+def _rows(kern: Kernels, t, heads: int, d: int, name: str, into, at: int = 0) -> int:
+    """Writes t, [rows, heads, d] or [rows, heads * d], as a tg_rows at byte `at` of `into`; returns the rows."""
     _on(kern, t, name)
     shape, stride = t.shape, t.stride()
     if len(shape) == 3 and shape[1] == heads and shape[2] == d:
@@ -59,8 +67,7 @@ def _rows(kern: Kernels, t, heads: int, d: int, name: str, into) -> int:
         raise ValueError(f"{name}: a head's values must be contiguous")
     rows = shape[0]
     ld = stride[0] if rows > 1 else heads * d
-    into.p, into.ld, into.hs = t.data_ptr(), ld, hs
-    into.len = (rows - 1) * ld + (heads - 1) * hs + d if rows else 0
+    _ROWS.pack_into(into, at, t.data_ptr(), (rows - 1) * ld + (heads - 1) * hs + d if rows else 0, ld, hs)
     return rows
 
 
@@ -72,6 +79,15 @@ def _array(kern: Kernels, t, kind: str, name: str, n: int) -> int:
     if not t.is_contiguous() or t.numel() < n:
         raise ValueError(f"{name} must be contiguous and hold {n} values")
     return t.data_ptr()
+
+
+def _count(longest: Optional[int]) -> int:
+    """The most rows of a sequence, 0 where any number."""
+    if longest is None:
+        return 0
+    if longest < 0:
+        raise ValueError("longest must not be negative")
+    return longest
 
 
 def _begun(desc):
@@ -97,19 +113,19 @@ class PagedCache:
         self.pages, self.page, self.kv_heads, self.d = k.shape
         self.type = _type(k, "k")
         a = self._desc = _lib.AttentionDesc()
-        self._name(a)
-
-    def _name(self, a) -> None:
-        """The cache's part of a description."""
         a.type, a.kv_heads, a.d = self.type, self.kv_heads, self.d
-        a.pages, a.page = self.pages, self.page
-        for t, rows, which in ((self.k, a.k, "k_page"), (self.v, a.v, "v_page")):
-            at, (pages, page, heads, d), (ps, ld, hs, _) = t.data_ptr(), t.shape, t.stride()
-            ld, hs = ld if page > 1 else heads * d, hs if heads > 1 else d
-            ps = ps if pages > 1 else page * heads * d
-            rows.p, rows.ld, rows.hs = at, ld, hs
-            rows.len = (pages - 1) * ps + (page - 1) * ld + (heads - 1) * hs + d if t.numel() else 0
-            setattr(a, which, ps)
+        self._k, self._k_page = self._strides(k)
+        self._v, self._v_page = self._strides(v)
+        a.pages, a.page, a.k_page, a.v_page = self.pages, self.page, self._k_page, self._v_page
+        _CACHE.pack_into(a, _AT_K, *self._k, *self._v)
+
+    def _strides(self, t):
+        """t's tg_rows, and the values between its pages."""
+        (pages, page, heads, d), (ps, ld, hs, _) = t.shape, t.stride()
+        ld, hs = ld if page > 1 else heads * d, hs if heads > 1 else d
+        ps = ps if pages > 1 else page * heads * d
+        span = (pages - 1) * ps + (page - 1) * ld + (heads - 1) * hs + d if t.numel() else 0
+        return (t.data_ptr(), span, ld, hs), ps
 
     def _name_seqs(self, a, rows: int, tables, lengths, q_starts, longest: Optional[int]) -> None:
         """The sequences of `rows` new rows in a: their tables, lengths and first rows."""
@@ -121,12 +137,11 @@ class PagedCache:
         if width > 1 and one != 1:
             raise ValueError("a sequence's table must be contiguous")
         ldt = ldt if batch > 1 else width
-        a.batch, a.q_rows, a.longest = batch, rows, longest or 0
-        a.tables, a.ldt, a.width = tables.data_ptr(), ldt, width
-        a.tables_len = (batch - 1) * ldt + width if batch else 0
-        a.lengths, a.lengths_len = _array(kern, lengths, _INT32, "lengths", batch), batch
-        if q_starts is not None:
-            a.q_starts, a.q_starts_len = _array(kern, q_starts, _INT32, "q_starts", batch + 1), batch + 1
+        _PAGES.pack_into(a, _AT_PAGES, tables.data_ptr(), (batch - 1) * ldt + width if batch else 0, ldt, width,
+                         _array(kern, lengths, _INT32, "lengths", batch), batch, self.pages, self.page, self._k_page,
+                         self._v_page)
+        at, n = (0, 0) if q_starts is None else (_array(kern, q_starts, _INT32, "q_starts", batch + 1), batch + 1)
+        _SEQS.pack_into(a, _AT_SEQS, batch, rows, 0, _count(longest), at, 0, n, 0)
 
     def append(self, k, v, tables, lengths, q_starts=None, longest: Optional[int] = None,
                rotary: Optional["Rotary"] = None) -> None:
@@ -188,8 +203,8 @@ class Attention:
 
     def _fill(self, a, q, out, prefix, workspace) -> int:
         kern = self._kernels
-        rows = _rows(kern, q, self.heads, self.head_dim, "q", a.q)
-        if _rows(kern, out, self.heads, self.head_dim, "out", a.out) != rows or out.dtype != q.dtype:
+        rows = _rows(kern, q, self.heads, self.head_dim, "q", a, _AT_Q)
+        if _rows(kern, out, self.heads, self.head_dim, "out", a, _AT_OUT) != rows or out.dtype != q.dtype:
             raise ValueError("out must have q's rows and type")
         if prefix is not None:
             a.prefix, a.prefix_len = _array(kern, prefix, _INT32, "prefix", 1), prefix.numel()
@@ -216,19 +231,20 @@ class Attention:
         a, kern = _begun(self._desc), self._kernels
         a.type = _type(q, "q")
         rows = self._fill(a, q, out, prefix, workspace)
-        keys = _rows(kern, k, self.kv_heads, self.head_dim, "k", a.k)
-        if _rows(kern, v, self.kv_heads, self.head_dim, "v", a.v) != keys:
+        keys = _rows(kern, k, self.kv_heads, self.head_dim, "k", a, _AT_K)
+        if _rows(kern, v, self.kv_heads, self.head_dim, "v", a, _AT_V) != keys:
             raise ValueError("k and v must have the same rows")
         if k.dtype != q.dtype or v.dtype != q.dtype:
             raise TypeError("q, k and v must have one type")
+        q_at = q_n = k_at = k_n = 0
         if q_starts is not None:
-            batch = q_starts.numel() - 1
-            a.q_starts, a.q_starts_len = _array(kern, q_starts, _INT32, "q_starts", 1), batch + 1
+            q_at, q_n = _array(kern, q_starts, _INT32, "q_starts", 1), q_starts.numel()
+            batch = q_n - 1
         if batch < 0:
             raise ValueError("batch must not be negative")
-        a.batch, a.q_rows, a.k_rows, a.longest = batch, rows, keys, longest or 0
         if k_starts is not None:
-            a.k_starts, a.k_starts_len = _array(kern, k_starts, _INT32, "k_starts", batch + 1), batch + 1
+            k_at, k_n = _array(kern, k_starts, _INT32, "k_starts", batch + 1), batch + 1
+        _SEQS.pack_into(a, _AT_SEQS, batch, rows, keys, _count(longest), q_at, k_at, q_n, k_n)
         if q_docs is not None:
             a.q_docs, a.q_docs_len = _array(kern, q_docs, _INT32, "q_docs", rows), rows
         if k_docs is not None:
@@ -284,8 +300,8 @@ class Attention:
         if cache._kernels.device != kern.device:
             raise TypeError("the cache lives on another GPU")
         rows = self._fill(a, q, out, prefix, workspace)
-        c = cache._desc
-        a.type, a.k, a.v, a.k_page, a.v_page, a.pages, a.page = c.type, c.k, c.v, c.k_page, c.v_page, c.pages, c.page
+        a.type = cache.type
+        _CACHE.pack_into(a, _AT_K, *cache._k, *cache._v)
         cache._name_seqs(a, rows, tables, lengths, q_starts, longest)
         rc = _lib.lib().tg_attention_paged_device(kern._ctx, a)
         if rc:

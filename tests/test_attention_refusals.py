@@ -293,3 +293,26 @@ def test_tensors_are_refused_by_place_shape_and_type():
         att.paged(q, cache, tables, lens, torch.zeros(2, 4, 64))
     with pytest.raises(ValueError, match="go with rel"):
         att.forward(q, q[:, :2], q[:, 2:], torch.zeros_like(q), rel_u=torch.zeros(4, 64))
+    for call in (lambda: att.forward(q, q[:, :2], q[:, 2:], torch.zeros_like(q), longest=-1),
+                 lambda: att.paged(q, cache, tables, lens, torch.zeros_like(q), longest=-1)):
+        with pytest.raises(ValueError, match="longest"):
+            call()
+
+
+def test_descriptions_are_written_where_their_fields_lie():
+    """The neighbouring fields that the wrappers write at once, read back by name."""
+    from telmo_amd import _lib, attention
+
+    a = _lib.AttentionDesc()
+    attention._ROWS.pack_into(a, attention._AT_Q, 1, 2, 3, 4)
+    attention._ROWS.pack_into(a, attention._AT_OUT, 5, 6, 7, 8)
+    attention._CACHE.pack_into(a, attention._AT_K, *range(11, 19))
+    attention._SEQS.pack_into(a, attention._AT_SEQS, *range(21, 29))
+    attention._PAGES.pack_into(a, attention._AT_PAGES, *range(31, 41))
+    rows = [(r.p, r.len, r.ld, r.hs) for r in (a.q, a.k, a.v, a.out)]
+    assert rows == [(1, 2, 3, 4), (11, 12, 13, 14), (15, 16, 17, 18), (5, 6, 7, 8)]
+    assert [getattr(a, n) for n in ("batch", "q_rows", "k_rows", "longest", "q_starts", "k_starts", "q_starts_len",
+                                    "k_starts_len")] == list(range(21, 29))
+    assert [getattr(a, n) for n in ("tables", "tables_len", "ldt", "width", "lengths", "lengths_len", "pages", "page",
+                                    "k_page", "v_page")] == list(range(31, 41))
+    assert a.prefix is None and a.workspace is None and a.q_docs is None
