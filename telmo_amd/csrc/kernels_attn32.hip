@@ -8,10 +8,11 @@
 //
 // The layout is that of the 16-bit kernel with 16 x 16 x 32 products: eight wavefronts of 16 queries each, a lane
 // holding one query's scores with 8 of the 32 keys. Two wavefronts to a SIMD, so that one's splitting and exponentials
-// run beside the other's products: 16 sequences of 750 rows of 8 heads of 128 with position rows take 308 us (180 TFLOP/s
+// run beside the other's products: 16 sequences of 750 rows of 8 heads of 128 with position rows take 306 us (181 TFLOP/s
 // of f32, past the 154 that a large library product reaches on the f32 units), with four wavefronts of 32 queries,
 // which read half as much LDS, 385. Bound by the splitting and the softmax on the vector units (43 % busy) in turn with
-// the products (32 %). Tiles of 64 rows run the same with four wavefronts, for calls that leave CUs empty.
+// the products (32 %). Tiles of 64 rows run the same with four wavefronts, for calls that leave CUs empty: there 32 keys
+// take a workgroup 3.2 us and its start 10 (7 without position rows).
 //
 // Position rows: with T[c, i] = (q_i + w) r_c, the score of key j needs T[j - i, i]. The distances j - i of a
 // wavefront's 16 queries and a tile's 32 keys lie in two blocks of 32 position rows, and the second one is the first

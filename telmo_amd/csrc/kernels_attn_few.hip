@@ -14,7 +14,7 @@
 // matrix instructions.
 //
 // 32 sequences of 8192 keys, 8 key heads of 128 in bf16: 1.07 GB in 202 us, 5.3 TB/s (a large copy moves 4.8). The same
-// call by the tiles of 128 rows takes 209, without parts 338; eight sequences of 750 f16 keys 15.2 (19.9), one of
+// call by the tiles of 128 rows takes 209, without parts 338; eight sequences of 750 f16 keys 14.7 (19.9), one of
 // 100,000 keys and heads of 64 94 (114). One tile under way and twice the wavefronts: 140 for 128 us at lengths of
 // up to 8192, two workgroups to a CU in fewer registers 120 to 137 for 113 to 134.
 #include "attn_launch.hpp"
