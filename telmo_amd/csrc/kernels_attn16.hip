@@ -55,6 +55,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     constexpr int TILE_K = D == 256 ? 32 : 64;  // keys of a tile: the output of 256 columns leaves registers for 32
     constexpr int HALVES = TILE_K / 32, N = TILE_K / 2;  // score products of a tile, scores of a lane
     constexpr int AHEAD = 4;  // operands on their way from LDS
+    constexpr float NEAR = 1024.0f;
     constexpr int CHUNKS = D / 8, PER = TILE_K * CHUNKS / THREADS, STEP = THREADS / CHUNKS;
     __shared__ __align__(16) T k_tiles[2][TILE_K * K_PITCH<D>], v_tiles[2][TILE_K * V_PITCH<D>];
 
@@ -121,6 +122,11 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
     f32x16 acc[D / 32] = {};
     float m = -INFINITY, l = 0.0f;
     const float mul = a.scale * LOG2E;
+    // Plain scores are scaled and lowered by the base in one operation, the exponent's: off by half a step of base mul
+    // for all keys of a tile alike, 2^-14 at most below NEAR. Past NEAR each tile comes through the gate and takes the
+    // base off first, in f32 exactly wherever the weight is not nothing: rows of 10^4 have exponents of 10^9, whose
+    // half step is far more than f16's weights can take.
+    float off = Half<T>::shift, gate = -INFINITY;
 
     // Two tiles in LDS: while one is worked on, the next one, which left memory a tile ago, is written to the
     // other, and the one after it leaves memory.
@@ -183,17 +189,26 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
 #pragma unroll
         for (int e = 1; e < N; e++) top = fmaxf(top, s[e / 16][e % 16]);
         top = max_halves(top);
-        if (__any(top > m)) {
+        if (__any(top > (EXTRA ? m : gate))) {
             const float mn = fmaxf(m, top);
             const float fade = m == -INFINITY ? 0.0f
                                               : __builtin_amdgcn_exp2f(EXTRA ? (m - mn) * LOG2E : (m - mn) * mul);
             l *= fade;
 #pragma unroll
             for (int x = 0; x < D / 32; x++) acc[x] *= fade;
-            m = mn;
+            m = gate = mn;
+            if (!EXTRA) {
+                const float base = m == -INFINITY ? 0.0f : m, far = base * mul;
+                off = Half<T>::shift - far;
+                if (__any(!(fabsf(far) < NEAR))) {
+                    off = Half<T>::shift;
+                    gate = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < N; e++) s[e / 16][e % 16] -= base;
+                }
+            }
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        const float off = Half<T>::shift - base * mul;
         v8 pf[N / 8];
         // The first fragments of V are on their way while the weights are worked out.
         constexpr int PRODUCTS = N / 8 * (D / 32);

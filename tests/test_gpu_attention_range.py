@@ -1,0 +1,67 @@
+"""Attention far from rows of N(0, 1), on an MI355X, against the definition in 64 bits."""
+import itertools
+
+import numpy as np
+import pytest
+
+from attention_oracle import attend, tolerance
+from test_gpu_attention import TYPES, check, dtype, say
+
+pytestmark = pytest.mark.gpu
+
+
+def given(type, x):
+    """x as a GPU tensor of the type, and what it holds in float64 on the host."""
+    import torch
+
+    t = torch.from_numpy(np.asarray(x, np.float32)).to(dtype(type))
+    return t.cuda(), t.double().numpy()
+
+
+def run(tk, q, k, v, split=True, rel=None, rel_u=None, rel_v=None, **options):
+    """Attention.forward of one sequence [rows, heads, d], in parts where split; the outputs in float64."""
+    import torch
+
+    import telmo_amd
+
+    att = telmo_amd.Attention(tk, q.shape[1], q.shape[2], kv_heads=k.shape[1], **options)
+    out = torch.full_like(q, 7.0)
+    space = torch.empty(att.workspace_bytes(q.shape[0], k.shape[0]) + 16, dtype=torch.uint8, device="cuda") if split else None
+    starts = [torch.tensor([0, x.shape[0]], dtype=torch.int32, device="cuda") for x in (q, k)]
+    att.forward(q, k, v, out, q_starts=starts[0], k_starts=starts[1], rel=rel, rel_u=rel_u, rel_v=rel_v, workspace=space)
+    tk.synchronize()
+    return out.double().cpu().numpy()
+
+
+# ------------------------------------------------------------------------------------- large scores
+
+@pytest.mark.parametrize("type,n,d", itertools.product(TYPES, (5, 150), (64, 128, 256)))
+def test_large_rows_that_see_one_key_get_its_value(tk, type, n, d):
+    """Scores of up to 10^9: the one shown key weighs 1 and the output is its value."""
+    say("one key", type, n, d)
+    rng = np.random.default_rng(n + d)
+    (q, _), (k, _), (v, v64) = (given(type, x * rng.standard_normal((n, 2, d))) for x in (1e4, 1e4, 1.0))
+    got = run(tk, q, k, v, left=0, right=0)
+    # f32: the weight's and the value's parts are sums of three 8-bit ones, each exact, added in f32.
+    assert np.all(np.abs(got - v64) <= (2.0**-22 * np.abs(v64) if type == "f32" else 0.0))
+
+
+@pytest.mark.parametrize("type,n,d,scale", itertools.product(TYPES, (4, 300), (64, 128, 256), (2.0**-7, 2.0)))
+def test_scores_that_differ_little_far_from_zero(tk, type, n, d, scale):
+    """Every score is a large power of two plus a small multiple of 2^7 scale, exact in f32 (2^30 + 2^7 x in all
+    partial sums), so the weights are those of small differences, at 2^23 and their ties at 2^31."""
+    say("far scores", type, n, d, scale)
+    rng = np.random.default_rng(n + d)
+    q, k = np.zeros((n, 2, d)), np.zeros((500, 2, d))
+    q[..., 0], k[..., 0] = 2.0**15, 2.0**15
+    q[..., 1:5], k[..., 1:5] = 8.0 * rng.integers(-2, 3, (n, 2, 4)), 16.0 * rng.integers(-2, 3, (500, 2, 4))
+    (q, q64), (k, k64), (v, v64) = given(type, q), given(type, k), given(type, rng.standard_normal((500, 2, d)))
+    for split in (True, False):
+        got = run(tk, q, k, v, split, scale=scale)
+        for h in range(2):
+            want, _ = attend(q64[:, h], k64[:, h], v64[:, h], scale, np.ones((n, 500), bool))
+            # The scores are exact; the exponent, at most 32 log2(e) where a weight is more than 2^-46, is off by three
+            # half steps of itself (the factor's, its product's, the base's).
+            tol = tolerance(type, d, 500, 0.0, np.abs(v64).max(), False)
+            check(got[:, h], want, tol + np.abs(v64).max() * 2 * 3 * 47 * 2.0**-24)
+
