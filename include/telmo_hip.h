@@ -338,7 +338,8 @@ int tg_dwconv1d_quant_device(tg_ctx *ctx, const float *x, size_t x_len, size_t l
  * (docs equal and not negative). A query that is shown no key, or only keys whose score is -infinity,
  * gets zeros. Keys that no query is shown may hold anything.
  * Scores, softmax statistics and sums are f32; with 16-bit types the weights round to that type (half a
- * step) before they multiply the values, and the outputs once. f32 rows are computed to f32's accuracy.
+ * step) before they multiply the values, and the outputs once, and a softcap of up to 256 moves the scores by up
+ * to 2^-22 of itself. f32 rows are computed to f32's accuracy.
  * A shown score of NaN or +infinity makes its row NaN. Rows of q and out behind the last sequence are neither
  * read nor written. Sequences hold up to 2^30 keys. Fast for every sequence and head size but these, which
  * take a wavefront per row: position rows with heads past 128, and row strides past 8 million values (chunks of

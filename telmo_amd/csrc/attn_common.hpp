@@ -124,18 +124,29 @@ __device__ __forceinline__ float score_of(const AttnArgs &a, float dot, int h, f
     return s;
 }
 
-// The same of a lane's N products, key_at(e) the e-th one's key: one kind of change after the other. FAST: tanh
-// to 2^-22 absolutely, with the hardware's reciprocal, for 16-bit rows, whose weights keep less. TABLE: there may be a
-// table.
+// Whether 16-bit rows take the hardware's reciprocal for their cap's tanh: it is off by 2^-22 absolutely, so the
+// scores by at most 2^-14, an eighth of what f16's weights round away. The bound grows with the cap; larger ones take
+// the tanh that is relative to the score, and so do caps so small that the factor before the score has no f32.
+__host__ __device__ __forceinline__ float cap_factor(const AttnArgs &a) { return 2.0f * LOG2E * a.scale / a.cap; }
+__host__ __device__ __forceinline__ bool fast_cap(const AttnArgs &a) {
+    return a.cap <= 256.0f && cap_factor(a) < INFINITY;
+}
+
+// The same of a lane's N products, key_at(e) the e-th one's key: one kind of change after the other. FAST: fast_cap's
+// where it holds, which a call without TABLE has seen to. TABLE: there may be a table.
 template <bool FAST, int N, bool TABLE, typename S, typename F>
 __device__ __forceinline__ void scores_of(const AttnArgs &a, S s, F key_at, int h, float slope, int i) {
     if (a.cap > 0.0f) {
-        const float into = 2.0f * LOG2E * a.scale / a.cap;
+        if (FAST && (!TABLE || fast_cap(a))) {
+            const float into = cap_factor(a);
 #pragma unroll
-        for (int e = 0; e < N; e++)
-            s(e) = FAST ? __builtin_fmaf(-2.0f * a.cap,
-                                         __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s(e) * into) + 1.0f), a.cap)
-                        : a.cap * tanh_f32(s(e) * a.scale / a.cap);
+            for (int e = 0; e < N; e++)
+                s(e) = __builtin_fmaf(-2.0f * a.cap,
+                                      __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s(e) * into) + 1.0f), a.cap);
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; e++) s(e) = a.cap * tanh_f32(s(e) * a.scale / a.cap);
+        }
     } else {
 #pragma unroll
         for (int e = 0; e < N; e++) s(e) *= a.scale;

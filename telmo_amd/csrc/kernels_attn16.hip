@@ -26,7 +26,7 @@ constexpr int THREADS = 256, TILE_Q = 128;
 
 // What a call does to its scores, in what it costs: a kernel of each kind, since the plain one folds the scale
 // into the exponent and holds no choices in its loop.
-enum Extra { PLAIN, CAPS, ALL };  // nothing; caps and slopes; tables and documents too
+enum Extra { PLAIN, CAPS, ALL };  // nothing; caps (fast_cap) and slopes; tables, documents and any caps too
 
 template <typename T>
 struct Half;
@@ -301,7 +301,7 @@ hipError_t launch_tile(const AttnArgs &a, int splits, hipStream_t s) {
 
 template <typename T, int D, bool PAGED>
 hipError_t launch_extra(const AttnArgs &a, int splits, hipStream_t s) {
-    if (a.table || a.q_docs) return launch_tile<T, D, PAGED, ALL>(a, splits, s);
+    if (a.table || a.q_docs || (a.cap > 0.0f && !fast_cap(a))) return launch_tile<T, D, PAGED, ALL>(a, splits, s);
     if (a.cap > 0.0f || a.slopes) return launch_tile<T, D, PAGED, CAPS>(a, splits, s);
     return launch_tile<T, D, PAGED, PLAIN>(a, splits, s);
 }

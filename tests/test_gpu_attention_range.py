@@ -4,7 +4,7 @@ import itertools
 import numpy as np
 import pytest
 
-from attention_oracle import attend, tolerance
+from attention_oracle import attend, shown_pairs, tolerance
 from test_gpu_attention import TYPES, check, dtype, say
 
 pytestmark = pytest.mark.gpu
@@ -31,6 +31,11 @@ def run(tk, q, k, v, split=True, rel=None, rel_u=None, rel_v=None, **options):
     att.forward(q, k, v, out, q_starts=starts[0], k_starts=starts[1], rel=rel, rel_u=rel_u, rel_v=rel_v, workspace=space)
     tk.synchronize()
     return out.double().cpu().numpy()
+
+
+def own_size(q, k, scale, shown):
+    """The largest sum of magnitudes behind a shown score, without a cap's."""
+    return float(((np.abs(q) @ np.abs(k).T) * scale)[shown].max())
 
 
 # ------------------------------------------------------------------------------------- large scores
@@ -64,4 +69,26 @@ def test_scores_that_differ_little_far_from_zero(tk, type, n, d, scale):
             # half steps of itself (the factor's, its product's, the base's).
             tol = tolerance(type, d, 500, 0.0, np.abs(v64).max(), False)
             check(got[:, h], want, tol + np.abs(v64).max() * 2 * 3 * 47 * 2.0**-24)
+
+
+# ------------------------------------------------------------------------------------------ caps
+
+@pytest.mark.parametrize("type,n,cap", itertools.product(TYPES, (3, 90), (1e-39, 1e-3, 200.0, 300.0, 1e4, 1e5, 1e7, 1e30)))
+def test_caps_of_any_size(tk, type, n, cap):
+    """A large cap leaves scores as they are, to the score's own size; a small one leaves next to nothing."""
+    say("cap", type, n, cap)
+    rng = np.random.default_rng(n)
+    d, m, scale = 64, 400, 0.5
+    q, k, v = (rng.standard_normal((x, 2, d)) for x in (n, m, m))
+    q[1] = 0.0
+    (q, q64), (k, k64), (v, v64) = (given(type, x) for x in (q, k, v))
+    shown = shown_pairs(n, m, None, 0)
+    got = run(tk, q, k, v, softcap=cap, scale=scale, right=0)
+    for h in range(2):
+        want, _ = attend(q64[:, h], k64[:, h], v64[:, h], scale, shown, float(np.float32(cap)))
+        top = np.abs(v64[:, h]).max()
+        tol = tolerance(type, d, m, own_size(q64[:, h], k64[:, h], scale, shown), top, False)
+        if type != "f32" and cap <= 256:  # such caps of 16-bit rows: scores to 2^-21 of the cap, in weight and sum
+            tol += top * 2 * np.expm1(cap * 2.0**-21)
+        check(got[:, h], want, tol)
 
