@@ -344,7 +344,8 @@ int tg_dwconv1d_quant_device(tg_ctx *ctx, const float *x, size_t x_len, size_t l
  * read nor written. Sequences hold up to 2^30 keys. Fast for every sequence and head size but these, which
  * take a wavefront per row: position rows with heads past 128, and row strides past 8 million values (chunks of
  * rows; single tokens take any). A row whose shown keys are sound beside hidden ones that hold NaN or infinity
- * may be computed twice. */
+ * may be computed twice, and so may an f32 row whose scores are small beside the product of the largest values of
+ * q and of a key (or a position row): outliers that meet zeros. */
 typedef struct {
     const void *p; /* device, 16-byte aligned */
     size_t len;    /* elements reachable from p */

@@ -2,7 +2,10 @@
 //
 // The f32 matrix instructions run at a sixteenth of the 16-bit ones' rate, so each f32 operand is held as a sum of
 // 16-bit ones. For the scores a row x of q, k or the position rows is scaled by a power of two to |x| < 2^15 and held
-// as h + l in f16, 22 bits of it; three products h h', h l' and l h' leave out less than 2^-22 of each term. The weights
+// as h + l in f16, 22 bits of each value within 2^-17 of the row's largest; three products h h', h l' and l h' leave out
+// less than 2^-22 of such terms. Smaller values keep 2^-40 of the row's largest: where that can be more of a score than
+// f32 sums lose (an outlier of q that meets zeros of k, with every other term far below it), the row is computed again
+// by its definition. The weights
 // and the values, which may not share a scale (a value is weighted by other rows' weights), are held as three bf16 each,
 // 24 bits, and six products leave out less than 2^-23.
 //
@@ -301,6 +304,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
         }
         feed<STEPS, 4, AHEAD, 6>();
     };
+    float widest = 0.0f;  // the largest inverse of a scale among the rows that the queries meet
     // T of block n for the wavefront's queries, into its ring of two blocks.
     const auto terms_of = [&](int n) {
         const int slot = n & (RING - 1);
@@ -314,7 +318,10 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
 #pragma unroll
         for (int x = 0; x < 2; x++) {
             f32x4 y;
-            for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(s[x][e], back[x][e] * q_back, add[x][e]);
+            for (int e = 0; e < 4; e++) {
+                y[e] = __builtin_fmaf(s[x][e], back[x][e] * q_back, add[x][e]);
+                widest = fmaxf(widest, back[x][e]);
+            }
             *reinterpret_cast<f32x4 *>(
                 &sh.terms[wave][col * 64 + (((n & 1) * 32 + x * 16 + quarter * 4 + 4 * col) & 63)]) = y;
         }
@@ -415,6 +422,7 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
         for (int e = 0; e < 8; e++) {
             const float scale = back[e / 4][e % 4] * q_back;
             s[e] = REL ? __builtin_fmaf(dots[e / 4][e % 4], scale, terms[e]) : dots[e / 4][e % 4] * scale;
+            widest = fmaxf(widest, back[e / 4][e % 4]);
         }
         const auto key_at = [&](int e) { return kb + e / 4 * 16 + 4 * quarter + e % 4; };
         if (EXTRA) scores_of<false, 8, true>(a, [&](int e) -> float & { return s[e]; }, key_at, h, slope, i);
@@ -486,8 +494,14 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
     }
 
     l = sum_quarters(l);
+    // A pair of f16 is off by up to 2^-25 of its scale's inverse, and each of the other row's d values is at most 2^15 of
+    // its own: both rows' errors move a score by d 2^-9 times the two inverses (twice that with position rows). Up to 2^-20,
+    // or that much of the score where it is more than 1, is what f32 sums of d products lose.
+    const float moved = (REL ? 2.0f : 1.0f) * 0x1p-9f * (float)a.d * q_back * max_quarters(widest) * a.scale;
+    bool sound = !(moved > 0x1p-20f * fmaxf(1.0f, fabsf(EXTRA ? m : m * a.scale)));
     if (parts.parts > 1) {
         if (!live) return;
+        if (!sound) acc[0][0] = NAN;  // for the joining wavefront, unless the part weighs nothing
         const size_t to = (size_t)part * parts.pairs + row * a.heads + h;
         if (quarter == 0) {
             parts.top[to] = EXTRA ? m : m * a.scale;
@@ -503,7 +517,6 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     float *out = static_cast<float *>(a.out) + row * a.ldo + h * a.hso;
-    bool sound = true;
 #pragma unroll
     for (int x = 0; x < D / 16; x++) {
         const int oc = x * 16 + 4 * quarter;

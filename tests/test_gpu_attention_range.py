@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 from attention_oracle import attend, shown_pairs, tolerance
-from test_gpu_attention import TYPES, check, dtype, say
+from test_gpu_attention import TYPES, check, dtype, floats, position_rows, say
 
 pytestmark = pytest.mark.gpu
 
@@ -91,4 +91,44 @@ def test_caps_of_any_size(tk, type, n, cap):
         if type != "f32" and cap <= 256:  # such caps of 16-bit rows: scores to 2^-21 of the cap, in weight and sum
             tol += top * 2 * np.expm1(cap * 2.0**-21)
         check(got[:, h], want, tol)
+
+
+# --------------------------------------------------------------------------- outliers in f32 rows
+
+@pytest.mark.parametrize("n,d,outlier", itertools.product((5, 40, 300), (64, 128, 256), (2.0**18, 2.0**24, 1e9, 1e12, 1e30)))
+def test_rows_with_an_outlier_that_meets_zeros(tk, n, d, outlier):
+    """One column of q (of k) holds values far past the others and zeros in k (in q): the score is what the small
+    values make it."""
+    say("outlier", n, d, outlier)
+    rng = np.random.default_rng(n + d)
+    q, k, v = (rng.standard_normal((x, 2, d)) for x in (n, 700, 700))
+    q[..., 0], k[..., 0] = outlier * rng.choice([-1, 1], (n, 2)), 0.0
+    k[..., 5], q[..., 5] = outlier, 0.0
+    (q, q64), (k, k64), (v, v64) = (given("f32", x) for x in (q, k, v))
+    for split in (True, False):
+        got = run(tk, q, k, v, split)
+        for h in range(2):
+            want, size = attend(q64[:, h], k64[:, h], v64[:, h], d**-0.5, np.ones((n, 700), bool))
+            check(got[:, h], want, tolerance("f32", d, 700, size, np.abs(v64[:, h]).max(), False))
+
+
+@pytest.mark.parametrize("n,d,outlier", itertools.product((40, 300), (64, 128), (2.0**24, 1e12)))
+def test_position_rows_with_an_outlier_that_meets_zeros(tk, n, d, outlier):
+    """A column of the position rows that is zero in the queries, and one of u and w that is zero in the keys and the
+    position rows."""
+    say("position rows, outlier", n, d, outlier)
+    rng = np.random.default_rng(n + d)
+    q, k, v = (rng.standard_normal((n, 2, d)) for _ in "qkv")
+    rel, u, w = rng.standard_normal((2 * n - 1, 2 * d)), rng.standard_normal((2, d)), rng.standard_normal((2, d))
+    rel[:, [3, d + 3]] = outlier
+    q[..., 3], u[:, 3], w[:, 3] = 0.0, 0.0, 0.0
+    u[:, 7], w[:, 7] = outlier, -outlier
+    k[..., 7], rel[:, [7, d + 7]] = 0.0, 0.0
+    (q, q64), (k, k64), (v, v64) = (given("f32", x) for x in (q, k, v))
+    rel, u, w = (x.astype(np.float32) for x in (rel, u, w))
+    got = run(tk, q, k, v, rel=floats(rel), rel_u=floats(u), rel_v=floats(w))
+    for h in range(2):
+        want, size = attend(q64[:, h], k64[:, h], v64[:, h], d**-0.5, np.ones((n, n), bool),
+                            rel=position_rows(n, n, h, rel, d), u=u[h].astype(np.float64), w=w[h].astype(np.float64))
+        check(got[:, h], want, tolerance("f32", d, n, size, np.abs(v64[:, h]).max(), True))
 
