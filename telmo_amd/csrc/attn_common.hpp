@@ -16,6 +16,17 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
+// A weighted mean in the rows' type. Weights that were rounded up take a mean of f16's largest values past 65520, which
+// would round to infinity: a finite mean stays finite.
+template <typename T>
+__device__ __forceinline__ T mean_to(float x) {
+    return (T)x;
+}
+template <>
+__device__ __forceinline__ _Float16 mean_to<_Float16>(float x) {
+    const float y = __builtin_amdgcn_fmed3f(x, -65504.0f, 65504.0f);
+    return (_Float16)(x - x == 0.0f ? y : x);
+}
 
 // Eight values at p (16 bytes of a 16-bit type, 32 of f32; aligned to 16) in 32 bits, and back, rounded
 // to nearest even.

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArg
         for (int e = 0; e < V; e++) {
             const float y = l == 0.0f ? 0.0f : acc[e] / l;
             sound = sound && y - y == 0.0f;
-            out[e] = (T)y;
+            out[e] = mean_to<T>(y);
         }
     }
     // As the tile kernels do for rows that they finish themselves.

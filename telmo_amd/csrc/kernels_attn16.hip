@@ -273,7 +273,7 @@ __global__ __launch_bounds__(THREADS, D == 256 ? 1 : 2) void attn_tile_kernel(co
             for (int y = 0; y < 4; y++) {
                 const float v = acc[x][4 * e + y] * inv;
                 worst = fmaxf(worst, v - v == 0.0f ? 0.0f : 1.0f);
-                o[y] = (T)v;
+                o[y] = mean_to<T>(v);
             }
             if (live && oc < a.d) *reinterpret_cast<u32x2 *>(out + oc) = *reinterpret_cast<u32x2 *>(o);
         }

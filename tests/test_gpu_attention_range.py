@@ -132,3 +132,24 @@ def test_position_rows_with_an_outlier_that_meets_zeros(tk, n, d, outlier):
                             rel=position_rows(n, n, h, rel, d), u=u[h].astype(np.float64), w=w[h].astype(np.float64))
         check(got[:, h], want, tolerance("f32", d, n, size, np.abs(v64[:, h]).max(), True))
 
+
+# ------------------------------------------------------------------- values at the end of their type
+
+@pytest.mark.parametrize("n,split", itertools.product((5, 150), (True, False)))
+def test_f16_values_at_the_end_of_the_type(tk, n, split):
+    """Weights that all round up make the weighted mean of f16's largest value a little more than that, which has no
+    f16: it stays the largest."""
+    say("f16 values", n, split)
+    d, m, high = 64, 900, 65504.0
+    part = np.log(0.5 * (1 + 0.6 * 2.0**-10))  # a weight 0.6 of a step past 1/2 of the largest
+    q, k = np.zeros((n, 1, d)), np.zeros((m, 1, d))
+    q[..., 0], q[..., 1] = 1.0, 2.0**-9
+    k[:, 0, 0] = np.float16(part)
+    k[:, 0, 1] = np.float16((part - k[1, 0, 0]) * 512)
+    k[::100] = 0.0  # the largest weights, some in every part
+    signs = np.where(np.arange(d) % 2, 1.0, -1.0)
+    (q, q64), (k, k64), (v, v64) = given("f16", q), given("f16", k), given("f16", high * signs * np.ones((m, 1, d)))
+    weight = np.exp(k64[1, 0] @ q64[0, 0])
+    assert 2.0**-11 < weight / 0.5 - 1 < 0.7 * 2.0**-10
+    got = run(tk, q, k, v, split, scale=1.0)
+    assert np.all(np.abs(got[:, 0] - high * signs) <= tolerance("f16", d, m, 1.0, high, False))
