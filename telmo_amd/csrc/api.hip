@@ -15,6 +15,7 @@
 #include <cstring>
 #include <mutex>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/telmo_hip.h"
@@ -1567,14 +1568,31 @@ int check_rows(tg_ctx *ctx, const char *name, const tg_rows &r, uint32_t type, s
     return TG_OK;
 }
 
-// Rows that are written: no two heads of any row in one place.
-bool rows_distinct(const tg_rows &r, size_t rows, size_t heads, size_t d) {
-    if (rows <= 1 && heads <= 1) return true;
-    if (heads <= 1) return r.ld >= d;
-    if (rows <= 1) return r.hs >= d;
-    return (r.hs >= d && r.ld >= sat_add(sat_mul(heads - 1, r.hs), d)) ||
-           (r.ld >= d && r.hs >= sat_add(sat_mul(rows - 1, r.ld), d));
-}
+// Runs of d values at the multiples of three steps (rows, heads, pages), the widest step first: n of each, those of one
+// left out. Nested where every step reaches past all that lies at the smaller ones: no two runs in one place.
+struct Runs {
+    size_t n[3], step[3], d;
+    int axes;
+    Runs(const tg_rows &r, size_t rows, size_t heads, size_t d_, size_t pages = 1, size_t page_step = 0) : d(d_), axes(0) {
+        for (const auto &[count, by] : {std::pair{rows, r.ld}, std::pair{heads, r.hs}, std::pair{pages, page_step}}) {
+            if (count <= 1) continue;
+            int at = axes++;
+            for (; at && step[at - 1] < by; at--) n[at] = n[at - 1], step[at] = step[at - 1];
+            n[at] = count, step[at] = by;
+        }
+    }
+    // Values from the first to behind the last of the axes from `axis` on.
+    size_t reach(int axis) const {
+        size_t x = d;
+        for (; axis < axes; axis++) x = sat_add(x, sat_mul(n[axis] - 1, step[axis]));
+        return x;
+    }
+    bool nested() const {
+        for (int i = 0; i < axes; i++)
+            if (step[i] < reach(i + 1)) return false;
+        return true;
+    }
+};
 
 bool ranges_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
@@ -1678,7 +1696,7 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
     const size_t q_span = rows_span(a.q, a.q_rows, a.heads, a.d), o_span = rows_span(a.out, a.q_rows, a.heads, a.d);
     if ((rc = check_rows(ctx, "q", a.q, a.type, q_span))) return rc;
     if ((rc = check_rows(ctx, "out", a.out, a.type, o_span))) return rc;
-    if (!rows_distinct(a.out, a.q_rows, a.heads, a.d))
+    if (!Runs(a.out, a.q_rows, a.heads, a.d).nested())
         return fail(ctx, TG_ERR_SHAPE, "out's strides put two heads in one place");
     const size_t size = type_bytes(a.type);
     const size_t k_span = paged ? rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page)
@@ -1759,7 +1777,7 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
     const size_t x_span = rows_span(x, rows, heads, d), o_span = rows_span(out, rows, heads, d);
     if ((rc = check_rows(ctx, "x", x, type, x_span))) return rc;
     if ((rc = check_rows(ctx, "out", out, out_type, o_span))) return rc;
-    if (!rows_distinct(out, rows, heads, d)) return fail(ctx, TG_ERR_SHAPE, "out's strides put two heads in one place");
+    if (!Runs(out, rows, heads, d).nested()) return fail(ctx, TG_ERR_SHAPE, "out's strides put two heads in one place");
     if (positions && positions_len < rows) return fail(ctx, TG_ERR_SHAPE, "positions is too short");
     const bool same = x.p == out.p && x.ld == out.ld && x.hs == out.hs && type == out_type;
     if (!same && ranges_overlap(x.p, x_span * type_bytes(type), out.p, o_span * type_bytes(out_type)))
@@ -1787,9 +1805,8 @@ int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t 
     const size_t nk = rows_span(k_new, a.q_rows, a.kv_heads, a.d), nv = rows_span(v_new, a.q_rows, a.kv_heads, a.d);
     if ((rc = check_rows(ctx, "k_new", k_new, type, nk))) return rc;
     if ((rc = check_rows(ctx, "v_new", v_new, type, nv))) return rc;
-    const size_t ks = rows_span(a.k, a.page, a.kv_heads, a.d), vs = rows_span(a.v, a.page, a.kv_heads, a.d);
-    if (!rows_distinct(a.k, a.page, a.kv_heads, a.d) || !rows_distinct(a.v, a.page, a.kv_heads, a.d) ||
-        (a.pages > 1 && (a.k_page < ks || a.v_page < vs)) || (ks && a.pages && a.k.p == a.v.p))
+    const Runs kr(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page), vr(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page);
+    if (!kr.nested() || !vr.nested() || (a.pages && a.k.p == a.v.p))
         return fail(ctx, TG_ERR_SHAPE, "the cache's strides put two rows in one place");
     const size_t size = type_bytes(a.type), from = type_bytes(type);
     const size_t kc = rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page) * size;
