@@ -422,8 +422,9 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
  * rotated for that position first where rotary is given. desc names the cache as tg_attention_paged_device
  * reads it (type, kv_heads, d, k, v, k_page, v_page, page, pages, tables, lengths, batch, q_rows, q_starts,
  * longest). Rows whose position is negative or has no page are not written, lengths past the table's included
- * (unlike attention's, they are not cut to it); two rows in one place leave either of them. k and v are not one
- * tensor. */
+ * (unlike attention's, they are not cut to it); two rows in one place leave either of them. The pages, rows and
+ * heads of k (of v) nest in any order; k and v share no value, and where they lie in each other (a page of keys,
+ * then one of values) their strides that reach so far are alike. */
 int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
                            const tg_rotary *rotary);
 

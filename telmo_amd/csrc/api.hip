@@ -1594,6 +1594,19 @@ struct Runs {
     }
 };
 
+// Whether two sets of nested runs, the second one's first value `by` on from the first one's, may share a value: exact
+// where their steps are alike as far as they reach into one another; where they are not, they may.
+bool runs_meet(const Runs &x, const Runs &y, int64_t by, int axis = 0) {
+    if (by >= (int64_t)x.reach(axis) || -by >= (int64_t)y.reach(axis)) return false;
+    if (axis == x.axes && axis == y.axes) return true;
+    if (axis >= x.axes || axis >= y.axes || x.step[axis] != y.step[axis]) return true;
+    // Block i of x and block j of y lie by - (i - j) step apart: nearer than a step, for them to meet.
+    const int64_t step = (int64_t)x.step[axis], low = by / step - (by % step < 0);
+    for (int64_t m = low; m <= low + 1; m++)
+        if (m < (int64_t)x.n[axis] && -m < (int64_t)y.n[axis] && runs_meet(x, y, by - m * step, axis + 1)) return true;
+    return false;
+}
+
 bool ranges_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
@@ -1806,9 +1819,12 @@ int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t 
     if ((rc = check_rows(ctx, "k_new", k_new, type, nk))) return rc;
     if ((rc = check_rows(ctx, "v_new", v_new, type, nv))) return rc;
     const Runs kr(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page), vr(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page);
-    if (!kr.nested() || !vr.nested() || (a.pages && a.k.p == a.v.p))
+    if (!kr.nested() || !vr.nested())
         return fail(ctx, TG_ERR_SHAPE, "the cache's strides put two rows in one place");
     const size_t size = type_bytes(a.type), from = type_bytes(type);
+    const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(a.v.p) - reinterpret_cast<uintptr_t>(a.k.p)) / (int64_t)size;
+    if (a.pages && runs_meet(kr, vr, apart))
+        return fail(ctx, TG_ERR_SHAPE, "k and v share memory, or lie in each other by different strides");
     const size_t kc = rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page) * size;
     const size_t vc = rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page) * size;
     if (ranges_overlap(a.k.p, kc, k_new.p, nk * from) || ranges_overlap(a.k.p, kc, v_new.p, nv * from) ||

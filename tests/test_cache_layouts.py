@@ -2,6 +2,7 @@
 stand answers that the context is null."""
 import itertools
 
+import numpy as np
 import pytest
 
 from test_attention_refusals import AT, OK, SHAPE, paged, rows
@@ -38,3 +39,46 @@ def test_axes_in_any_order(order, gap):
         bad[axis] -= 8 + gap[axis]
         assert append((AT * 2, bad, span), (AT * 3, steps, span)) == SHAPE
         assert append((AT * 2, steps, span), (AT * 3, bad, span)) == SHAPE
+
+
+def places(at, steps, sizes, d):
+    """The values that a cache at `at` takes."""
+    i = np.indices(sizes).reshape(3, -1)
+    return (at + (np.array(steps)[:, None] * i).sum(0)[:, None] + np.arange(d)).ravel()
+
+
+def test_keys_and_values_that_share_memory():
+    """Keys and values at random nested steps in one buffer against their values' places, one by one: none that
+    share a value are written, and all are that do not and step alike."""
+    rng = np.random.default_rng(6)
+    seen = {True: 0, False: 0}
+    for _ in range(4000):
+        sizes, d = tuple(int(x) for x in rng.integers(1, 4, 3)), 8 * int(rng.integers(1, 3))
+        order = rng.permutation(3)
+        steps, span = layout(order, sizes, d, 8 * rng.integers(0, 5, 3))
+        other, other_span = (steps, span) if rng.random() < 0.7 else layout(rng.permutation(3), sizes, d, 8 * rng.integers(0, 5, 3))
+        by = 8 * int(rng.integers(-span // 8 - 2, span // 8 + 3))
+        shared = np.intersect1d(places(0, steps, sizes, d), places(by, other, sizes, d)).size > 0
+        got = append((AT * 2, steps, span), (AT * 2 + 2 * by, other, other_span), sizes, d)
+        if shared:
+            assert got == SHAPE, (sizes, d, steps, other, by)
+        elif steps == other:
+            assert got == OK, (sizes, d, steps, by)
+        seen[shared] += 1
+    assert min(seen.values()) > 500
+
+
+def test_keys_and_values_of_one_buffer():
+    page = PAGE * HEADS * D
+    # A page of keys, then one of values; the values with their heads outermost in the page.
+    keys = [2 * page, HEADS * D, D]
+    span = (PAGES - 1) * 2 * page + page
+    assert append((AT * 2, keys, span), (AT * 2 + 2 * page, keys, span)) == OK
+    assert append((AT * 2, keys, span), (AT * 2 + 2 * page, [2 * page, D, PAGE * D], span)) == OK
+    assert append((AT * 2, keys, span), (AT * 2 + 2 * page - 16, keys, span)) == SHAPE
+    assert append((AT * 2, keys, span), (AT * 2 + 2 * page - 16, [2 * page, D, PAGE * D], span)) == SHAPE
+    # Values one page on from the keys, in the same pages.
+    whole, span = [page, HEADS * D, D], PAGES * page
+    assert append((AT * 2, whole, span), (AT * 2 + 2 * page, whole, span)) == SHAPE
+    assert append((AT * 2, whole, span), (AT * 2, whole, span)) == SHAPE
+    assert append((AT * 2, whole, span), (AT * 2 + 2 * span, whole, span)) == OK
