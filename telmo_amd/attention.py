@@ -7,7 +7,8 @@ with relative positions (src/parakeet.rs:1176-1282), Granite's inside blocks of 
 (src/granite.rs:962-1036), a text encoder's with windows and documents; ``Attention.for_layer`` makes
 that argument. Rows are GPU tensors [rows, heads, d], or [rows, heads * d] with the heads side by
 side, as views at any strides that are whole multiples of 16 bytes; everything is queued on the
-context's stream and nothing is allocated but by ``Rotary``'s constructor.
+context's stream and nothing is allocated but by ``Rotary``'s constructor. Tensors that a call or an object names
+must live until the stream has reached the call, in a captured graph as long as that is replayed.
 """
 from __future__ import annotations
 
@@ -342,7 +343,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", f
 
 class Rotary:
     """Rotary positions over the first dim values of each head: pairs (i, i + dim / 2), or (2 i, 2 i + 1)
-    when interleaved, with the frequencies of rotary_frequencies."""
+    when interleaved, with the frequencies of rotary_frequencies. The object itself may go once its calls are queued."""
 
     def __init__(self, kernels: Kernels, dim: int, base: float = 10000.0, interleaved: bool = False,
                  scaling: str = "none", **options):
@@ -351,9 +352,14 @@ class Rotary:
         self._kernels = kernels
         self.dim, self.interleaved = dim, interleaved
         f, self.amplitude = rotary_frequencies(dim, base, scaling, **options)
-        self.turns = torch.from_numpy(f / (2.0 * math.pi)).to(f"cuda:{kernels.device}")
-        # The upload runs on torch's current stream and the kernels on the context's: wait for it here.
-        torch.cuda.current_stream(kernels.device).synchronize()
+        self.turns = kernels._turns.get(f.tobytes())
+        if self.turns is None:
+            turns = torch.from_numpy(f / (2.0 * math.pi)).to(f"cuda:{kernels.device}")
+            # The upload runs on torch's current stream and the kernels on the context's: wait for it here.
+            torch.cuda.current_stream(kernels.device).synchronize()
+            # Queued kernels and captured graphs read them after this object is gone, and torch's allocator does not know
+            # of them: each set of frequencies, at most 1 KB, stays as long as the context.
+            self.turns = kernels._turns.setdefault(f.tobytes(), turns)
         self._desc = _lib.RotaryDesc(self.turns.data_ptr(), dim // 2, dim, int(bool(interleaved)), self.amplitude)
 
     def apply(self, x, out, positions=None, start: int = 0) -> None:

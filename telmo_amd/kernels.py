@@ -250,6 +250,7 @@ class Kernels:
             raise TelmoError(rc, f"no gfx950 context on device {device}")
         self._ctx = ctx
         self.device = device
+        self._turns = {}  # Rotary's frequencies on the GPU, by their bytes
         self.set_mode(mode)
 
     def set_mode(self, mode: int) -> None:
