@@ -29,6 +29,8 @@ _CACHE = struct.Struct("@PNNNPNNN")  # its k and v
 _AT_SEQS, _AT_Q, _AT_K, _AT_V, _AT_OUT, _AT_PAGES = (getattr(_lib.AttentionDesc, name).offset for name in
                                                      ("batch", "q", "k", "v", "out", "tables"))
 
+_FAR = 1 << 62  # further than any position, and within 64 bits: ctypes cuts what is past them
+
 _TYPES = {}  # torch's types, made on first use
 _INT32, _FLOAT32 = "int32", "float32"
 
@@ -187,7 +189,7 @@ class Attention:
         a.heads, a.kv_heads, a.d = heads, self.kv_heads, head_dim
         a.scale = 1.0 / math.sqrt(head_dim) if scale is None else scale
         a.softcap = softcap
-        a.left, a.right = -1 if left is None else left, -1 if right is None else right
+        a.left, a.right = (-1 if n is None else min(n, _FAR) for n in (left, right))
         if slopes is not None:
             a.slopes, a.slopes_len = _array(kernels, slopes, _FLOAT32, "slopes", heads), slopes.numel()
         if table is not None:
@@ -370,6 +372,8 @@ class Rotary:
         if x.dim() != 3 or out.shape != x.shape:
             raise ValueError("x and out must be [rows, heads, d]")
         rows, heads, d = x.shape
+        if abs(start) > _FAR:
+            raise ValueError("start is past 2^62")
         xr, orr = _lib.Rows(), _lib.Rows()
         _rows(kern, x, heads, d, "x", xr)
         _rows(kern, out, heads, d, "out", orr)
