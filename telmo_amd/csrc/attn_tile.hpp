@@ -111,10 +111,15 @@ __device__ __forceinline__ bool one_document(int docs, int doc) {
     const int first = __builtin_amdgcn_readfirstlane(docs);
     return first >= 0 && __all(docs == first && doc == first);
 }
-// s where the bit is set, else -infinity.
-__device__ __forceinline__ float shown_or_not(float s, uint32_t bits, int bit) {
-    const uint32_t all = (uint32_t)((int32_t)(bits << (31 - bit)) >> 31);
+// All bits where the one is set, else none; and s where all are, else -infinity.
+__device__ __forceinline__ uint32_t shown_mask(uint32_t bits, int bit) {
+    return (uint32_t)((int32_t)(bits << (31 - bit)) >> 31);
+}
+__device__ __forceinline__ float shown_or_not(float s, uint32_t all) {
     return __uint_as_float((__float_as_uint(s) & all) | (0xff800000u & ~all));
+}
+__device__ __forceinline__ float shown_or_not(float s, uint32_t bits, int bit) {
+    return shown_or_not(s, shown_mask(bits, bit));
 }
 
 // A workgroup's place in the call. Heads that share a key head are rows of one matrix: pair g r + x is head x

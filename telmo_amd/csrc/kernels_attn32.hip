@@ -416,25 +416,30 @@ __global__ __launch_bounds__(64 * WAVES, WAVES / 4) void attn_tile32_kernel(
         for (int x = 0; x < 2; x++) back[x] = *reinterpret_cast<const f32x4 *>(&sh.k_back[x * 16 + quarter * 4]);
         along(sh.k[0], sh.k[1], dots);
 
-        // Scores, and -infinity where the key is not shown.
+        // Scores, and -infinity where the key is not shown, unless the whole tile is.
+        const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
+        const bool same_doc = !EXTRA || !a.q_docs || one_document(docs, doc);
+        const bool whole = full && !(PAGED && hide) && same_doc;
         float s[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float scale = back[e / 4][e % 4] * q_back;
             s[e] = REL ? __builtin_fmaf(dots[e / 4][e % 4], scale, terms[e]) : dots[e / 4][e % 4] * scale;
-            widest = fmaxf(widest, back[e / 4][e % 4]);
+            widest = fmaxf(widest, whole ? back[e / 4][e % 4] : 0.0f);
         }
         const auto key_at = [&](int e) { return kb + e / 4 * 16 + 4 * quarter + e % 4; };
         if (EXTRA) scores_of<false, 8, true>(a, [&](int e) -> float & { return s[e]; }, key_at, h, slope, i);
-        const bool full = (kb >= w_last.lo && kb + TILE_K <= w_first.hi) || kb + TILE_K <= w_first.prefix;
-        const bool same_doc = !EXTRA || !a.q_docs || one_document(docs, doc);
-        if (!full || (PAGED && hide) || !same_doc) {
+        if (!whole) {
             const uint32_t bits =
                 (uint32_t)(EXTRA && !same_doc ? shown_bits<true, TILE_K>(win, kb, hide, docs, doc)
                                               : shown_bits<false, TILE_K>(win, kb, hide, docs, doc)) >>
                 4 * quarter;
 #pragma unroll
-            for (int e = 0; e < 8; e++) s[e] = shown_or_not(s[e], bits, e / 4 * 16 + e % 4);
+            for (int e = 0; e < 8; e++) {
+                const uint32_t all = shown_mask(bits, e / 4 * 16 + e % 4);
+                s[e] = shown_or_not(s[e], all);
+                widest = fmaxf(widest, __uint_as_float(__float_as_uint(sh.k_back[e / 4 * 16 + 4 * quarter + e % 4]) & all));
+            }
         }
 
         float top = s[0];

@@ -133,6 +133,22 @@ def test_position_rows_with_an_outlier_that_meets_zeros(tk, n, d, outlier):
         check(got[:, h], want, tolerance("f32", d, n, size, np.abs(v64[:, h]).max(), True))
 
 
+@pytest.mark.parametrize("d,huge", itertools.product((64, 256), (1e18, 1e30)))
+def test_hidden_keys_far_past_the_others(tk, d, huge):
+    """Keys 60 to 69 dwarf the rest: queries that are not shown them get what the others make."""
+    say("hidden", d, huge)
+    n, rng = 200, np.random.default_rng(d)
+    q, k, v = (rng.standard_normal((n, 2, d)) for _ in "qkv")
+    k[60:70] = huge
+    (q, q64), (k, k64), (v, v64) = (given("f32", x) for x in (q, k, v))
+    got, shown = run(tk, q, k, v, left=20, right=0), shown_pairs(n, n, 20, 0)
+    clean = ~shown[:, 60:70].any(1)
+    for h in range(2):
+        want, _ = attend(q64[:, h], k64[:, h], v64[:, h], d**-0.5, shown)
+        size = own_size(q64[clean, h], k64[:, h], d**-0.5, shown[clean])
+        check(got[clean, h], want[clean], tolerance("f32", d, n, size, np.abs(v64[:, h]).max(), False))
+
+
 # ------------------------------------------------------------------- values at the end of their type
 
 @pytest.mark.parametrize("n,split", itertools.product((5, 150), (True, False)))
