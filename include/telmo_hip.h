@@ -399,7 +399,8 @@ int tg_attention_device(tg_ctx *ctx, const tg_attention_desc *desc);
 int tg_attention_paged_device(tg_ctx *ctx, const tg_attention_desc *desc);
 /* A workspace of this many bytes lets a call of `rows` query rows in `batch` sequences of up to `keys` keys
  * split long sequences over the GPU and join the parts; 0 where it would not. With a smaller one, or none,
- * the call does without. Calls that may overlap on the GPU (other streams, captured graphs replayed at
+ * the call does with fewer parts, or without. Paged calls count their parts from the table's width: where that is far past
+ * the lengths, a smaller workspace, or a narrower width, serves them better. Calls that may overlap on the GPU (other streams, captured graphs replayed at
  * once) need workspaces of their own. */
 size_t tg_attention_workspace_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys);
 
@@ -422,7 +423,7 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
  * rotated for that position first where rotary is given. desc names the cache as tg_attention_paged_device
  * reads it (type, kv_heads, d, k, v, k_page, v_page, page, pages, tables, lengths, batch, q_rows, q_starts,
  * longest). Rows whose position is negative or has no page are not written, lengths past the table's included
- * (unlike attention's, they are not cut to it); two rows in one place leave either of them. The pages, rows and
+ * (unlike attention's, they are not cut to it); two rows in one place leave values of either. The pages, rows and
  * heads of k (of v) nest in any order; k and v share no value, and where they lie in each other (a page of keys,
  * then one of values) their strides that reach so far are alike. */
 int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,

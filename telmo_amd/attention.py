@@ -201,7 +201,9 @@ class Attention:
 
     def workspace_bytes(self, rows: int, keys: int, batch: int = 1) -> int:
         """Bytes of workspace with which calls of `rows` query rows in `batch` sequences of up to `keys`
-        keys split long sequences over the GPU (tg_attention_workspace_bytes)."""
+        keys split long sequences over the GPU (tg_attention_workspace_bytes). Over pages `keys` is what the tables
+        hold, and their width decides the parts: for sequences far shorter, name a narrower view of the tables or a
+        smaller workspace."""
         return _lib.lib().tg_attention_workspace_bytes(rows, self.heads, self.kv_heads, self.head_dim, batch, keys)
 
     def _fill(self, a, q, out, prefix, workspace) -> int:

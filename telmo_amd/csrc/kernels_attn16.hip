@@ -11,8 +11,8 @@
 //
 // Bound by the wavefront's own chain: its exponentials, maxima and conversions take as long as its products, and
 // two wavefronts to a SIMD overlap them only in part (matrix units 38 % busy, vector units 42 %, a chunk of 509
-// rows of 32 heads over 32768 paged keys; with capped scores 36 % and 75 %). That chunk runs at 840 TFLOP/s, 8192
-// causal rows with capped scores at 785, where a large library product reaches 1196. LDS carries each tile from
+// rows of 32 heads over 32768 paged keys; with capped scores 36 % and 75 %). That chunk runs at 838 TFLOP/s, 8192
+// causal rows with capped scores at 781, where a large library product reaches 1196. LDS carries each tile from
 // memory to four wavefronts, double buffered; 256 rows and eight wavefronts, sharing each tile by twice as many,
 // made the chunk 5 % faster but short and ragged calls 17 to 19 % slower. Wavefront priorities changed nothing.
 #include "attn_launch.hpp"

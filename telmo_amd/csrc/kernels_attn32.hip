@@ -11,7 +11,7 @@
 //
 // The layout is that of the 16-bit kernel with 16 x 16 x 32 products: eight wavefronts of 16 queries each, a lane
 // holding one query's scores with 8 of the 32 keys. Two wavefronts to a SIMD, so that one's splitting and exponentials
-// run beside the other's products: 16 sequences of 750 rows of 8 heads of 128 with position rows take 306 us (181 TFLOP/s
+// run beside the other's products: 16 sequences of 750 rows of 8 heads of 128 with position rows take 307.5 us (180 TFLOP/s
 // of f32, past the 154 that a large library product reaches on the f32 units), with four wavefronts of 32 queries,
 // which read half as much LDS, 385. Bound by the splitting and the softmax on the vector units (43 % busy) in turn with
 // the products (32 %). Tiles of 64 rows run the same with four wavefronts, for calls that leave CUs empty: there 32 keys
