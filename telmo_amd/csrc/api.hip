@@ -1056,6 +1056,18 @@ int tdt_matrix(tg_ctx *ctx, const tg_weights *w, size_t n, size_t k, const char 
     return TG_OK;
 }
 
+// n tokens of the device's. On the context's stream: a copy on the null stream fails, and ends the capture, while
+// another thread captures a graph, as the step kernels' decode does.
+int read_tokens(tg_ctx *ctx, const int32_t *from, size_t n, tg_token *tokens) {
+    if (!n) return TG_OK;
+    std::vector<int32_t> buf(n * 3);
+    TG_HIP(ctx, hipMemcpyAsync(buf.data(), from, n * 3 * sizeof(int32_t), hipMemcpyDeviceToHost, ctx->stream));
+    TG_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    for (size_t i = 0; i < n; i++)
+        tokens[i] = tg_token{(uint32_t)buf[3 * i], (uint32_t)buf[3 * i + 1], (uint32_t)buf[3 * i + 2]};
+    return TG_OK;
+}
+
 // The decode's outputs from the control block: frame, on_frame, the token count and the tokens.
 int tdt_results(tg_ctx *ctx, tg_tdt *tdt, const tg::TdtCtl *hc, size_t *frame, size_t *on_frame, tg_token *tokens,
                 size_t cap, size_t *count) {
@@ -1063,13 +1075,8 @@ int tdt_results(tg_ctx *ctx, tg_tdt *tdt, const tg::TdtCtl *hc, size_t *frame, s
     *frame = (size_t)hc->t;
     *on_frame = (size_t)hc->on_frame;
     *count = n;
-    const size_t copy = n < cap ? n : cap;
-    if (copy) {
-        std::vector<int32_t> buf(copy * 3);
-        TG_HIP(ctx, hipMemcpy(buf.data(), tdt->tokens, copy * 3 * sizeof(int32_t), hipMemcpyDeviceToHost));
-        for (size_t i = 0; i < copy; i++)
-            tokens[i] = tg_token{(uint32_t)buf[3 * i], (uint32_t)buf[3 * i + 1], (uint32_t)buf[3 * i + 2]};
-    }
+    const int rc = read_tokens(ctx, tdt->tokens, n < cap ? n : cap, tokens);
+    if (rc) return rc;
     if (n > cap) return fail(ctx, TG_ERR_SHAPE, "tokens holds " + std::to_string(cap) + " entries and the decode emitted " + std::to_string(n));
     return TG_OK;
 }
@@ -1478,17 +1485,12 @@ int tg_tdt_decode_streams_device(tg_ctx *ctx, tg_tdt *tdt, tg_tdt_stream *stream
             int rc = TG_OK;
             for (size_t j = 0; j < k; j++) {
                 tg_tdt_stream &st = streams[idx[j]];
-                const size_t n = (size_t)hc[j].ntok, copy = n < st.cap ? n : st.cap;
+                const size_t n = (size_t)hc[j].ntok;
                 st.frame = (size_t)hc[j].t;
                 st.on_frame = (size_t)hc[j].on_frame;
                 st.count = n;
-                if (copy) {
-                    std::vector<int32_t> buf(copy * 3);
-                    TG_HIP(ctx, hipMemcpy(buf.data(), tdt->tokens + toff[j] * 3, copy * 3 * sizeof(int32_t),
-                                          hipMemcpyDeviceToHost));
-                    for (size_t i = 0; i < copy; i++)
-                        st.tokens[i] = tg_token{(uint32_t)buf[3 * i], (uint32_t)buf[3 * i + 1], (uint32_t)buf[3 * i + 2]};
-                }
+                const int read = read_tokens(ctx, tdt->tokens + toff[j] * 3, n < st.cap ? n : st.cap, st.tokens);
+                if (read) return read;
                 if (n > st.cap && rc == TG_OK)
                     rc = fail(ctx, TG_ERR_SHAPE, "tokens holds " + std::to_string(st.cap) +
                                                      " entries and the decode emitted " + std::to_string(n));
