@@ -16,8 +16,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
-// A weighted mean in the rows' type. Weights that were rounded up take a mean of f16's largest values past 65520, which
-// would round to infinity: a finite mean stays finite.
+// A weighted mean in the rows' type. Weights that were rounded up (sums of very many keys) take a mean of f16's largest
+// values past 65520, which would round to infinity: a finite mean stays finite.
 template <typename T>
 __device__ __forceinline__ T mean_to(float x) {
     return (T)x;
@@ -247,7 +247,7 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
     for (int o = 32; o; o >>= 1) l += __shfl_xor(l, o);
     T *out = static_cast<T *>(a.out) + row * a.ldo + h * a.hso;
     for (int e = 0; e < 4; e++)
-        if (e * 64 + lane < a.d) out[e * 64 + lane] = (T)(l == 0.0f ? 0.0f : acc[e] / l);
+        if (e * 64 + lane < a.d) out[e * 64 + lane] = mean_to<T>(l == 0.0f ? 0.0f : acc[e] / l);
 }
 
 // The parts of a call that splits its keys: per part, query row and head the score maximum, the sum of

@@ -343,7 +343,7 @@ __global__ __launch_bounds__((Few<T, D>::THREADS)) void attn_few_kernel(const At
         for (int e = 0; e < 4; e++) {
             const float x = sum == 0.0f ? 0.0f : o[e] / sum;
             sound = sound && x - x == 0.0f;
-            v[e] = (T)x;
+            v[e] = mean_to<T>(x);
         }
         if constexpr (F::WIDE) *reinterpret_cast<u32x4 *>(out) = *reinterpret_cast<u32x4 *>(v);
         else *reinterpret_cast<u32x2 *>(out) = *reinterpret_cast<u32x2 *>(v);

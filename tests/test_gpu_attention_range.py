@@ -169,3 +169,17 @@ def test_f16_values_at_the_end_of_the_type(tk, n, split):
     assert 2.0**-11 < weight / 0.5 - 1 < 0.7 * 2.0**-10
     got = run(tk, q, k, v, split, scale=1.0)
     assert np.all(np.abs(got[:, 0] - high * signs) <= tolerance("f16", d, m, 1.0, high, False))
+
+
+@pytest.mark.parametrize("n", (5, 40))
+def test_f16_values_of_infinity_stay_infinite(tk, n):
+    """A shown value of infinity, or NaN, reaches the output; a finite mean beside it does not change."""
+    d, m = 64, 90
+    q, k, v = (np.random.default_rng(x).standard_normal((x, 1, d)) for x in (n, m, m + 1))
+    v = v[:m]
+    v[3, 0, 0], v[4, 0, 1], v[5, 0, 2] = np.inf, -np.inf, np.nan
+    (q, q64), (k, k64), (v, v64) = (given("f16", x) for x in (q, k, v))
+    got = run(tk, q, k, v)
+    assert np.all(got[:, 0, 0] == np.inf) and np.all(got[:, 0, 1] == -np.inf) and np.all(np.isnan(got[:, 0, 2]))
+    want, size = attend(q64[:, 0], k64[:, 0], v64[:, 0, 3:], d**-0.5, np.ones((n, m), bool))
+    check(got[:, 0, 3:], want, tolerance("f16", d, m, size, np.abs(v64[:, 0, 3:]).max(), False))
