@@ -397,6 +397,19 @@ int tg_attention_device(tg_ctx *ctx, const tg_attention_desc *desc);
 /* A chunk of new rows of each sequence, or a single one, over a paged cache that holds its keys and values
  * (those of the new rows too, tg_cache_append_device). No documents. */
 int tg_attention_paged_device(tg_ctx *ctx, const tg_attention_desc *desc);
+/* A cache in eight bits: k and v of the description hold e4m3 values (a byte each; sign, four bits of exponent, three of
+ * mantissa, up to 448; 0x7f and 0xff are NaN), and each block of `block` rows of a page has an exponent for each head: row
+ * j, head h of page p stands for its values times 2^e with e = exps[p * page stride + j / block * kv_heads + h], from -126 to
+ * 120. d is a multiple of 16; strides of k and v count values, whole multiples of 16. */
+typedef struct {
+    int8_t *k_exps, *v_exps;          /* device, page / block x kv_heads for each page */
+    size_t k_exps_len, v_exps_len;
+    size_t k_page, v_page;            /* exponents between pages */
+    size_t block;                     /* divides the page */
+} tg_cache_e4m3;
+/* tg_attention_paged_device over such a cache: q and out of desc's type. The keys and values count exactly; q is exact in
+ * products of two (f16) or three (f32) parts. Weights round as there, f16's of chunks of rows to bf16 (half a step, 2^-9). */
+int tg_attention_paged_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache);
 /* A workspace of this many bytes lets a call of `rows` query rows in `batch` sequences of up to `keys` keys
  * split long sequences over the GPU and join the parts; 0 where it would not. With a smaller one, or none,
  * the call does with fewer parts, or without. Paged calls count their parts from the table's width: where that is far past
@@ -428,6 +441,14 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
  * then one of values) their strides that reach so far are alike. */
 int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
                            const tg_rotary *rotary);
+
+/* The same into a cache in e4m3. A block's exponent is the least e >= -100 with |x| <= 448 2^e for the finite values of its
+ * new rows (keys rotated), and each value is x 2^-e rounded to nearest, ties to even; NaN and infinities become NaN. A
+ * block that holds older rows of its sequence keeps its exponent where that is large enough; where it grows, its older rows
+ * are rounded again under the new one (powers of two: only values that become subnormal lose bits). Rows of a block behind
+ * the new ones are left as they were. A block takes the new rows of one sequence in a call. */
+int tg_cache_append_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type,
+                                tg_rows k_new, tg_rows v_new, const tg_rotary *rotary);
 
 /* ---- the TDT decoder (src/parakeet.rs:1412-1577) --------------------------------------------
  * Parakeet's prediction network (embedding, LSTM layers, projection) and joint, decoded greedily

@@ -57,6 +57,12 @@ class RotaryDesc(ctypes.Structure):
                 ("amplitude", ctypes.c_float)]
 
 
+class CacheE4m3(ctypes.Structure):
+    """tg_cache_e4m3."""
+    _fields_ = [("k_exps", _p), ("v_exps", _p), ("k_exps_len", _sz), ("v_exps_len", _sz), ("k_page", _sz),
+                ("v_page", _sz), ("block", _sz)]
+
+
 _szp = ctypes.POINTER(_sz)
 
 # name: (restype, argtypes), in the order of include/telmo_hip.h
@@ -103,11 +109,14 @@ SIGNATURES = {
                                                  _sz, _sz, _p, _sz, _p, _sz]),
     "tg_attention_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc)]),
     "tg_attention_paged_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc)]),
+    "tg_attention_paged_e4m3_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc), ctypes.POINTER(CacheE4m3)]),
     "tg_attention_workspace_bytes": (_sz, [_sz, _sz, _sz, _sz, _sz, _sz]),
     "tg_rotary_device": (ctypes.c_int, [_p, _u32, Rows, _u32, Rows, _sz, _sz, _sz, _p, _sz, ctypes.c_int64,
                                         ctypes.POINTER(RotaryDesc)]),
     "tg_cache_append_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc), _u32, Rows, Rows,
                                               ctypes.POINTER(RotaryDesc)]),
+    "tg_cache_append_e4m3_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc), ctypes.POINTER(CacheE4m3), _u32,
+                                                   Rows, Rows, ctypes.POINTER(RotaryDesc)]),
     "tg_tdt_create": (ctypes.c_int, [_p, _p, ctypes.POINTER(_p)]),
     "tg_tdt_destroy": (None, [_p]),
     "tg_tdt_max_rows": (_sz, [_p]),

@@ -102,9 +102,13 @@ def _begun(desc):
 class PagedCache:
     """Keys and values of many sequences in pages: k and v are GPU tensors [pages, page, kv_heads, d] of
     one type (views at any strides that are whole multiples of 16 bytes). Key position j of sequence b is
-    row j % page of page tables[b, j // page]. The tensors are held, not copied."""
+    row j % page of page tables[b, j // page]. The tensors are held, not copied.
 
-    def __init__(self, kernels: Kernels, k, v):
+    In eight bits: k and v are float8_e4m3fn (or uint8, the same bytes), and k_exps and v_exps, int8 GPU tensors
+    [pages, blocks, kv_heads], hold a power of two for each head of each page // blocks rows: a value stands for
+    itself times 2^exponent (tg_cache_e4m3). append chooses the exponents; rows of any type attend over the cache."""
+
+    def __init__(self, kernels: Kernels, k, v, k_exps=None, v_exps=None):
         self._kernels = kernels
         if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype:
             raise ValueError("k and v must be [pages, page, kv_heads, d] of one type")
@@ -114,13 +118,42 @@ class PagedCache:
             _on(kernels, t, name)
         self.k, self.v = k, v
         self.pages, self.page, self.kv_heads, self.d = k.shape
-        self.type = _type(k, "k")
+        self.k_exps, self.v_exps = k_exps, v_exps
+        self._exps = None if k_exps is None and v_exps is None else self._exponents(k_exps, v_exps)
+        self.type = _type(k, "k") if self._exps is None else None  # in eight bits: rows of any type
         a = self._desc = _lib.AttentionDesc()
-        a.type, a.kv_heads, a.d = self.type, self.kv_heads, self.d
+        a.type, a.kv_heads, a.d = self.type or 0, self.kv_heads, self.d
         self._k, self._k_page = self._strides(k)
         self._v, self._v_page = self._strides(v)
         a.pages, a.page, a.k_page, a.v_page = self.pages, self.page, self._k_page, self._v_page
         _CACHE.pack_into(a, _AT_K, *self._k, *self._v)
+
+    def _exponents(self, k_exps, v_exps):
+        """The tg_cache_e4m3 beside the description."""
+        import torch
+
+        if self.k.dtype not in (torch.float8_e4m3fn, torch.uint8):
+            raise TypeError(f"k and v with exponents must be float8_e4m3fn or uint8, not {self.k.dtype}")
+        c, of = _lib.CacheE4m3(), []
+        for t, name in ((k_exps, "k_exps"), (v_exps, "v_exps")):
+            if t is None:
+                raise ValueError("k_exps and v_exps go together")
+            if t.dtype != torch.int8:
+                raise TypeError(f"{name} must be int8, not {t.dtype}")
+            _on(self._kernels, t, name)
+            if t.dim() != 3 or t.shape[0] != self.pages or t.shape[2] != self.kv_heads or t.shape != k_exps.shape:
+                raise ValueError(f"{name} must be [{self.pages}, blocks, {self.kv_heads}], alike for k and v")
+            if t.numel() and not t[0].is_contiguous():
+                raise ValueError(f"{name}: a page's exponents must be contiguous")
+            held = t.shape[1] * t.shape[2]
+            step = t.stride(0) if self.pages > 1 else held
+            of.append((t.data_ptr(), (self.pages - 1) * step + held if t.numel() else 0, step))
+        blocks = k_exps.shape[1]
+        if blocks < 1 or self.page % blocks:
+            raise ValueError("a page must hold whole blocks")
+        (c.k_exps, c.k_exps_len, c.k_page), (c.v_exps, c.v_exps_len, c.v_page) = of
+        c.block = self.page // blocks
+        return c
 
     def _strides(self, t):
         """t's tg_rows, and the values between its pages."""
@@ -151,7 +184,8 @@ class PagedCache:
         """Writes new rows k and v ([rows, kv_heads, d], in their own type) into the pages
         (tg_cache_append_device): the n rows of sequence b, rows q_starts[b] to q_starts[b + 1] or an
         equal share, at key positions lengths[b] - n to lengths[b] - 1, keys rotated for those positions
-        by `rotary`. longest: the most rows of one sequence (default: all)."""
+        by `rotary`. In eight bits (tg_cache_append_e4m3_device) a block's exponent grows where new rows need it, and its
+        older rows are rounded again. longest: the most rows of one sequence (default: all)."""
         a, kern = _begun(self._desc), self._kernels
         if rotary is not None and rotary._kernels.device != kern.device:
             raise TypeError("the rotary positions live on another GPU")
@@ -160,8 +194,11 @@ class PagedCache:
         if _rows(kern, v, self.kv_heads, self.d, "v", vn) != rows or v.dtype != k.dtype:
             raise ValueError("k and v must have the same rows and type")
         self._name_seqs(a, rows, tables, lengths, q_starts, longest)
-        rc = _lib.lib().tg_cache_append_device(kern._ctx, a, _type(k, "k"), kn, vn,
-                                               None if rotary is None else rotary._desc)
+        turned = None if rotary is None else rotary._desc
+        if self._exps is None:
+            rc = _lib.lib().tg_cache_append_device(kern._ctx, a, _type(k, "k"), kn, vn, turned)
+        else:
+            rc = _lib.lib().tg_cache_append_e4m3_device(kern._ctx, a, self._exps, _type(k, "k"), kn, vn, turned)
         if rc:
             _check(rc, kern._ctx)
 
@@ -298,17 +335,22 @@ class Attention:
         """out = attention of new rows over the cache (tg_attention_paged_device), which holds their own
         keys and values too: the n rows of sequence b, rows q_starts[b] to q_starts[b + 1] of q or an equal
         share, stand at the last n of its lengths[b] positions. tables: int32 GPU tensor [batch, entries];
-        lengths: int32 GPU tensor [batch]. q, out and the cache have one type."""
+        lengths: int32 GPU tensor [batch]. q, out and the cache have one type; over a cache in eight bits
+        (tg_attention_paged_e4m3_device) q and out do."""
         a, kern = _begun(self._desc), self._kernels
-        if cache.kv_heads != self.kv_heads or cache.d != self.head_dim or cache.type != _type(q, "q"):
+        rows_type = _type(q, "q")
+        if cache.kv_heads != self.kv_heads or cache.d != self.head_dim or cache.type not in (rows_type, None):
             raise ValueError("the cache's heads, head size and type must be the layer's")
         if cache._kernels.device != kern.device:
             raise TypeError("the cache lives on another GPU")
         rows = self._fill(a, q, out, prefix, workspace)
-        a.type = cache.type
+        a.type = rows_type
         _CACHE.pack_into(a, _AT_K, *cache._k, *cache._v)
         cache._name_seqs(a, rows, tables, lengths, q_starts, longest)
-        rc = _lib.lib().tg_attention_paged_device(kern._ctx, a)
+        if cache._exps is None:
+            rc = _lib.lib().tg_attention_paged_device(kern._ctx, a)
+        else:
+            rc = _lib.lib().tg_attention_paged_e4m3_device(kern._ctx, a, cache._exps)
         if rc:
             _check(rc, kern._ctx)
 

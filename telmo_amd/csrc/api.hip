@@ -1546,7 +1546,8 @@ constexpr size_t MAX_ATTN_ROWS = (size_t)1 << 30;  // rows, keys and strides tha
 constexpr size_t MAX_ATTN_GRID = 65535;            // sequences and heads, each a grid dimension
 
 bool attn_type(uint32_t t) { return t == TG_F32 || t == TG_F16 || t == TG_BF16; }
-size_t type_bytes(uint32_t t) { return t == TG_F32 ? 4 : 2; }
+constexpr uint32_t E4M3 = 8;  // the values of a tg_cache_e4m3, a byte each: no type of rows
+size_t type_bytes(uint32_t t) { return t == TG_F32 ? 4 : t == E4M3 ? 1 : 2; }
 
 // a + b and a * b, SIZE_MAX where they do not fit.
 size_t sat_add(size_t a, size_t b) { return a > SIZE_MAX - b ? SIZE_MAX : a + b; }
@@ -1614,8 +1615,16 @@ bool ranges_overlap(const void *a, size_t a_bytes, const void *b, size_t b_bytes
     return a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
 }
 
-// The heads, sequences and (paged) the cache that attention and append both name, and their lengths.
-int check_seqs(tg_ctx *ctx, const tg_attention_desc &a, bool paged, tg::AttnSeqs &s) {
+// AttnSeqs' multiplier and shift that divide by n.
+void division(size_t n, uint32_t &mul, uint32_t &shift) {
+    shift = 31;
+    while (((size_t)1 << (shift - 31)) < n) shift++;
+    mul = (uint32_t)((((uint64_t)1 << shift) + n - 1) / n);
+}
+
+// The heads, sequences and (paged) the cache that attention and append both name, and their lengths. held: the type of the
+// cache's values.
+int check_seqs(tg_ctx *ctx, const tg_attention_desc &a, bool paged, uint32_t held, tg::AttnSeqs &s) {
     if (!attn_type(a.type)) return fail(ctx, TG_ERR_ARG, "type must be f32, f16 or bf16");
     if (a.d < 8 || a.d > 256 || a.d % 8) return fail(ctx, TG_ERR_UNSUPPORTED, "d must be a multiple of 8 up to 256");
     if (a.kv_heads < 1 || a.kv_heads > MAX_ATTN_GRID || a.batch > MAX_ATTN_GRID)
@@ -1643,24 +1652,37 @@ int check_seqs(tg_ctx *ctx, const tg_attention_desc &a, bool paged, tg::AttnSeqs
     s.width = (int)a.width;
     s.page = (int)a.page;
     s.pages = (int)a.pages;
-    s.page_shift = 31;
-    while (((size_t)1 << (s.page_shift - 31)) < a.page) s.page_shift++;
-    s.page_mul = (uint32_t)((((uint64_t)1 << s.page_shift) + a.page - 1) / a.page);
-    int rc = check_rows(ctx, "k", a.k, a.type, rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page));
+    division(a.page, s.page_mul, s.page_shift);
+    int rc = check_rows(ctx, "k", a.k, held, rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page));
     if (rc) return rc;
-    if ((rc = check_rows(ctx, "v", a.v, a.type, rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page)))) return rc;
-    if (a.k_page * type_bytes(a.type) % 16 || a.v_page * type_bytes(a.type) % 16)
+    if ((rc = check_rows(ctx, "v", a.v, held, rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page)))) return rc;
+    if (a.k_page * type_bytes(held) % 16 || a.v_page * type_bytes(held) % 16)
         return fail(ctx, TG_ERR_ALIGN, "page strides must be multiples of 16 bytes");
     return TG_OK;
 }
 
-int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
+// The exponents of a cache in e4m3 beside its description.
+int check_exps(tg_ctx *ctx, const tg_attention_desc &a, const tg_cache_e4m3 &c) {
+    if (a.d % 16) return fail(ctx, TG_ERR_UNSUPPORTED, "heads of e4m3 values must be multiples of 16");
+    if (!c.block || a.page % c.block) return fail(ctx, TG_ERR_SHAPE, "block must divide the page");
+    const size_t held = sat_mul(a.page / c.block, a.kv_heads);  // of a page
+    if (!a.pages) return TG_OK;
+    if (!c.k_exps || !c.v_exps) return fail(ctx, TG_ERR_NULL, "k_exps or v_exps are null");
+    if (c.k_page > SIZE_MAX / 16 || c.v_page > SIZE_MAX / 16) return fail(ctx, TG_ERR_SHAPE, "exponents do not fit in memory");
+    if (c.k_exps_len < span(a.pages, c.k_page, held) || c.v_exps_len < span(a.pages, c.v_page, held))
+        return fail(ctx, TG_ERR_SHAPE, "k_exps or v_exps is too short");
+    return TG_OK;
+}
+
+int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged, const tg_cache_e4m3 *cache = nullptr) {
     // The arguments need no context: they are judged first, a null context after them.
     if (!desc) return fail(ctx, TG_ERR_NULL, "null description");
     const tg_attention_desc &a = *desc;
     tg::AttnArgs k{};
-    int rc = check_seqs(ctx, a, paged, k.seqs);
+    const uint32_t held = cache ? E4M3 : a.type;
+    int rc = check_seqs(ctx, a, paged, held, k.seqs);
     if (rc) return rc;
+    if (cache && (rc = check_exps(ctx, a, *cache))) return rc;
     if (a.heads < 1 || a.heads > MAX_ATTN_GRID || a.heads % a.kv_heads)
         return fail(ctx, TG_ERR_SHAPE, "kv_heads must divide heads, at most 65535");
     if (!(a.scale > 0.0f) || !std::isfinite(a.scale)) return fail(ctx, TG_ERR_ARG, "scale must be positive and finite");
@@ -1670,6 +1692,7 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
     if (a.table && (a.table_span >= MAX_ATTN_ROWS || a.table_len < a.heads * (2 * a.table_span + 1)))
         return fail(ctx, TG_ERR_SHAPE, "table is too short");
     if (a.rel) {
+        if (cache) return fail(ctx, TG_ERR_UNSUPPORTED, "a cache in e4m3 takes no position rows");
         if (a.type != TG_F32) return fail(ctx, TG_ERR_UNSUPPORTED, "position rows are f32 and go with f32 rows");
         if (a.rel_span >= MAX_ATTN_ROWS) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^31 position rows");
         const tg_rows rel{a.rel, a.rel_len, a.ldrel, a.hsrel};
@@ -1713,23 +1736,30 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
     if ((rc = check_rows(ctx, "out", a.out, a.type, o_span))) return rc;
     if (!Runs(a.out, a.q_rows, a.heads, a.d).nested())
         return fail(ctx, TG_ERR_SHAPE, "out's strides put two heads in one place");
-    const size_t size = type_bytes(a.type);
+    const size_t size = type_bytes(a.type), kv_size = type_bytes(held);
     const size_t k_span = paged ? rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page)
                                 : rows_span(a.k, a.k_rows, a.kv_heads, a.d);
     const size_t v_span = paged ? rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page)
                                 : rows_span(a.v, a.k_rows, a.kv_heads, a.d);
     if (ranges_overlap(a.out.p, o_span * size, a.q.p, q_span * size) ||
-        ranges_overlap(a.out.p, o_span * size, a.k.p, k_span * size) ||
-        ranges_overlap(a.out.p, o_span * size, a.v.p, v_span * size))
+        ranges_overlap(a.out.p, o_span * size, a.k.p, k_span * kv_size) ||
+        ranges_overlap(a.out.p, o_span * size, a.v.p, v_span * kv_size))
         return fail(ctx, TG_ERR_ARG, "out must not overlap q, k or v");
     if (a.workspace && reinterpret_cast<uintptr_t>(a.workspace) % 16)
         return fail(ctx, TG_ERR_ALIGN, "workspace must be 16-byte aligned");
     const size_t work = a.workspace ? a.workspace_len : 0;
     if (ranges_overlap(a.workspace, work, a.out.p, o_span * size) ||
         ranges_overlap(a.workspace, work, a.q.p, q_span * size) ||
-        ranges_overlap(a.workspace, work, a.k.p, k_span * size) ||
-        ranges_overlap(a.workspace, work, a.v.p, v_span * size))
+        ranges_overlap(a.workspace, work, a.k.p, k_span * kv_size) ||
+        ranges_overlap(a.workspace, work, a.v.p, v_span * kv_size))
         return fail(ctx, TG_ERR_ARG, "workspace must not overlap out, q, k or v");
+    if (cache && a.pages) {
+        const size_t exps = a.page / cache->block * a.kv_heads;
+        const size_t ke = span(a.pages, cache->k_page, exps), ve = span(a.pages, cache->v_page, exps);
+        if (ranges_overlap(a.out.p, o_span * size, cache->k_exps, ke) || ranges_overlap(a.out.p, o_span * size, cache->v_exps, ve) ||
+            ranges_overlap(a.workspace, work, cache->k_exps, ke) || ranges_overlap(a.workspace, work, cache->v_exps, ve))
+            return fail(ctx, TG_ERR_ARG, "out and workspace must not overlap the exponents");
+    }
     if (!ctx) return TG_ERR_NULL;
     if (k.seqs.batch == 0 || k.seqs.longest == 0) return TG_OK;
     const auto clip = [](int64_t w) { return w < 0 ? -1 : w > INT32_MAX ? -1 : (int32_t)w; };
@@ -1746,6 +1776,12 @@ int run_attention(tg_ctx *ctx, const tg_attention_desc *desc, bool paged) {
     k.ldrel = (int64_t)a.ldrel, k.hsrel = (int64_t)a.hsrel, k.rel_span = (int)a.rel_span;
     k.prefix = a.prefix;
     k.work = a.workspace, k.work_bytes = a.workspace ? a.workspace_len : 0;
+    if (cache && a.pages) {
+        k.k_exps = cache->k_exps, k.v_exps = cache->v_exps;
+        k.k_epage = (int64_t)cache->k_page, k.v_epage = (int64_t)cache->v_page;
+        k.block = (int)cache->block;
+        division(cache->block, k.block_mul, k.block_shift);
+    }
     std::lock_guard<std::mutex> g(ctx->mu);
     TG_HIP(ctx, hipSetDevice(ctx->device));
     const hipError_t e = tg::launch_attention(k, ctx->stream);
@@ -1766,11 +1802,78 @@ int check_rotary(tg_ctx *ctx, const tg_rotary *r, size_t d, tg::RotaryArgs &out)
     return TG_OK;
 }
 
+int run_append(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type, const tg_rows &k_new,
+               const tg_rows &v_new, const tg_rotary *rotary) {
+    if (!desc) return fail(ctx, TG_ERR_NULL, "null description");
+    const tg_attention_desc &a = *desc;
+    tg::AttnSeqs s;
+    const uint32_t held = cache ? E4M3 : a.type;
+    int rc = check_seqs(ctx, a, true, held, s);
+    if (rc) return rc;
+    if (cache && (rc = check_exps(ctx, a, *cache))) return rc;
+    if (!attn_type(type)) return fail(ctx, TG_ERR_ARG, "type must be f32, f16 or bf16");
+    tg::RotaryArgs r;
+    if ((rc = check_rotary(ctx, rotary, a.d, r))) return rc;
+    const size_t nk = rows_span(k_new, a.q_rows, a.kv_heads, a.d), nv = rows_span(v_new, a.q_rows, a.kv_heads, a.d);
+    if ((rc = check_rows(ctx, "k_new", k_new, type, nk))) return rc;
+    if ((rc = check_rows(ctx, "v_new", v_new, type, nv))) return rc;
+    const Runs kr(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page), vr(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page);
+    if (!kr.nested() || !vr.nested())
+        return fail(ctx, TG_ERR_SHAPE, "the cache's strides put two rows in one place");
+    const size_t size = type_bytes(held), from = type_bytes(type);
+    const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(a.v.p) - reinterpret_cast<uintptr_t>(a.k.p)) / (int64_t)size;
+    if (a.pages && runs_meet(kr, vr, apart))
+        return fail(ctx, TG_ERR_SHAPE, "k and v share memory, or lie in each other by different strides");
+    const size_t kc = rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page) * size;
+    const size_t vc = rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page) * size;
+    if (ranges_overlap(a.k.p, kc, k_new.p, nk * from) || ranges_overlap(a.k.p, kc, v_new.p, nv * from) ||
+        ranges_overlap(a.v.p, vc, k_new.p, nk * from) || ranges_overlap(a.v.p, vc, v_new.p, nv * from))
+        return fail(ctx, TG_ERR_ARG, "the new rows must not overlap the cache");
+    if (cache && a.pages) {
+        const size_t exps = a.page / cache->block * a.kv_heads;
+        if (a.pages > 1 && (cache->k_page < exps || cache->v_page < exps))
+            return fail(ctx, TG_ERR_SHAPE, "the exponents' strides put two blocks in one place");
+        const tg_rows ke{cache->k_exps, 0, exps, exps}, ve{cache->v_exps, 0, exps, exps};
+        const Runs kp(ke, 1, 1, exps, a.pages, cache->k_page), vp(ve, 1, 1, exps, a.pages, cache->v_page);
+        if (runs_meet(kp, vp, (int64_t)(reinterpret_cast<uintptr_t>(cache->v_exps) - reinterpret_cast<uintptr_t>(cache->k_exps))))
+            return fail(ctx, TG_ERR_SHAPE, "k_exps and v_exps share memory, or lie in each other by different strides");
+        for (const auto &[p, n] : {std::pair<const void *, size_t>{cache->k_exps, span(a.pages, cache->k_page, exps)},
+                                   std::pair<const void *, size_t>{cache->v_exps, span(a.pages, cache->v_page, exps)}})
+            if (ranges_overlap(p, n, a.k.p, kc) || ranges_overlap(p, n, a.v.p, vc) || ranges_overlap(p, n, k_new.p, nk * from) ||
+                ranges_overlap(p, n, v_new.p, nv * from))
+                return fail(ctx, TG_ERR_ARG, "the exponents must not overlap the cache's values or the new rows");
+    }
+    if (!ctx) return TG_ERR_NULL;
+    if (s.batch == 0 || s.longest == 0 || s.pages == 0 || s.width == 0) return TG_OK;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    if (cache) {
+        const tg::Cache8 c{static_cast<uint8_t *>(const_cast<void *>(a.k.p)), static_cast<uint8_t *>(const_cast<void *>(a.v.p)),
+                           cache->k_exps, cache->v_exps, (int64_t)a.k.ld, (int64_t)a.k.hs, (int64_t)a.k_page, (int64_t)a.v.ld,
+                           (int64_t)a.v.hs, (int64_t)a.v_page, (int64_t)cache->k_page, (int64_t)cache->v_page,
+                           (int)cache->block};
+        TG_HIP(ctx, tg::launch_append8(k_new.p, (int64_t)k_new.ld, (int64_t)k_new.hs, v_new.p, (int64_t)v_new.ld,
+                                       (int64_t)v_new.hs, type, c, (int)a.kv_heads, (int)a.d, s, r, ctx->stream));
+        return TG_OK;
+    }
+    TG_HIP(ctx, tg::launch_append(k_new.p, (int64_t)k_new.ld, (int64_t)k_new.hs, v_new.p, (int64_t)v_new.ld,
+                                  (int64_t)v_new.hs, type, const_cast<void *>(a.k.p), (int64_t)a.k.ld,
+                                  (int64_t)a.k.hs, (int64_t)a.k_page, const_cast<void *>(a.v.p), (int64_t)a.v.ld,
+                                  (int64_t)a.v.hs, (int64_t)a.v_page, a.type, (int)a.kv_heads, (int)a.d, s, r,
+                                  ctx->stream));
+    return TG_OK;
+}
+
 }  // namespace
 
 int tg_attention_device(tg_ctx *ctx, const tg_attention_desc *desc) { return run_attention(ctx, desc, false); }
 
 int tg_attention_paged_device(tg_ctx *ctx, const tg_attention_desc *desc) { return run_attention(ctx, desc, true); }
+
+int tg_attention_paged_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache) {
+    if (!cache) return fail(ctx, TG_ERR_NULL, "null cache");
+    return run_attention(ctx, desc, true, cache);
+}
 
 size_t tg_attention_workspace_bytes(size_t rows, size_t heads, size_t kv_heads, size_t d, size_t batch, size_t keys) {
     if (!rows || !heads || !kv_heads || heads % kv_heads || heads > MAX_ATTN_GRID || !d || d > 256 || !batch ||
@@ -1809,39 +1912,13 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
 
 int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
                            const tg_rotary *rotary) {
-    if (!desc) return fail(ctx, TG_ERR_NULL, "null description");
-    const tg_attention_desc &a = *desc;
-    tg::AttnSeqs s;
-    int rc = check_seqs(ctx, a, true, s);
-    if (rc) return rc;
-    if (!attn_type(type)) return fail(ctx, TG_ERR_ARG, "type must be f32, f16 or bf16");
-    tg::RotaryArgs r;
-    if ((rc = check_rotary(ctx, rotary, a.d, r))) return rc;
-    const size_t nk = rows_span(k_new, a.q_rows, a.kv_heads, a.d), nv = rows_span(v_new, a.q_rows, a.kv_heads, a.d);
-    if ((rc = check_rows(ctx, "k_new", k_new, type, nk))) return rc;
-    if ((rc = check_rows(ctx, "v_new", v_new, type, nv))) return rc;
-    const Runs kr(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page), vr(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page);
-    if (!kr.nested() || !vr.nested())
-        return fail(ctx, TG_ERR_SHAPE, "the cache's strides put two rows in one place");
-    const size_t size = type_bytes(a.type), from = type_bytes(type);
-    const int64_t apart = (int64_t)(reinterpret_cast<uintptr_t>(a.v.p) - reinterpret_cast<uintptr_t>(a.k.p)) / (int64_t)size;
-    if (a.pages && runs_meet(kr, vr, apart))
-        return fail(ctx, TG_ERR_SHAPE, "k and v share memory, or lie in each other by different strides");
-    const size_t kc = rows_span(a.k, a.page, a.kv_heads, a.d, a.pages, a.k_page) * size;
-    const size_t vc = rows_span(a.v, a.page, a.kv_heads, a.d, a.pages, a.v_page) * size;
-    if (ranges_overlap(a.k.p, kc, k_new.p, nk * from) || ranges_overlap(a.k.p, kc, v_new.p, nv * from) ||
-        ranges_overlap(a.v.p, vc, k_new.p, nk * from) || ranges_overlap(a.v.p, vc, v_new.p, nv * from))
-        return fail(ctx, TG_ERR_ARG, "the new rows must not overlap the cache");
-    if (!ctx) return TG_ERR_NULL;
-    if (s.batch == 0 || s.longest == 0 || s.pages == 0 || s.width == 0) return TG_OK;
-    std::lock_guard<std::mutex> g(ctx->mu);
-    TG_HIP(ctx, hipSetDevice(ctx->device));
-    TG_HIP(ctx, tg::launch_append(k_new.p, (int64_t)k_new.ld, (int64_t)k_new.hs, v_new.p, (int64_t)v_new.ld,
-                                  (int64_t)v_new.hs, type, const_cast<void *>(a.k.p), (int64_t)a.k.ld,
-                                  (int64_t)a.k.hs, (int64_t)a.k_page, const_cast<void *>(a.v.p), (int64_t)a.v.ld,
-                                  (int64_t)a.v.hs, (int64_t)a.v_page, a.type, (int)a.kv_heads, (int)a.d, s, r,
-                                  ctx->stream));
-    return TG_OK;
+    return run_append(ctx, desc, nullptr, type, k_new, v_new, rotary);
+}
+
+int tg_cache_append_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type,
+                                tg_rows k_new, tg_rows v_new, const tg_rotary *rotary) {
+    if (!cache) return fail(ctx, TG_ERR_NULL, "null cache");
+    return run_append(ctx, desc, cache, type, k_new, v_new, rotary);
 }
 
 }  // extern "C"

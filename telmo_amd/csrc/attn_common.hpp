@@ -2,6 +2,7 @@
 // and which keys a query is shown.
 #pragma once
 
+#include "e4m3.hpp"
 #include "tg_internal.hpp"
 
 namespace tg {
@@ -16,6 +17,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(_Float16 x) { return (float)x; }
 __device__ __forceinline__ float to_f32(__bf16 x) { return (float)x; }
+__device__ __forceinline__ float to_f32(e4m3 x) { return e4m3_to_f32(x); }
 // A weighted mean in the rows' type. Weights that were rounded up (sums of very many keys) take a mean of f16's largest
 // values past 65520, which would round to infinity: a finite mean stays finite.
 template <typename T>
@@ -94,6 +96,11 @@ __host__ __device__ inline int page_of(const AttnSeqs &s, int b, int j, int &row
     row = j - n * s.page;
     const int p = s.tables[(int64_t)b * s.ldt + n];
     return (unsigned)p < (unsigned)s.pages ? p : -1;
+}
+
+// Where the exponents of a row of an e4m3 page lie: those of its block, a head each.
+__device__ __forceinline__ int64_t block_at(const AttnArgs &a, int64_t epage, int page, int row) {
+    return page * epage + (int64_t)((uint64_t)(uint32_t)row * a.block_mul >> a.block_shift) * a.kv_heads;
 }
 
 // The keys that a query at position i is shown before documents are compared: lo <= j < hi, or j < prefix.
@@ -176,8 +183,8 @@ __device__ __forceinline__ void scores_of(const AttnArgs &a, S s, F key_at, int 
 // Row r of sequence b, head h, by one wavefront from the definition: a lane scores one key of 64 at a time,
 // then the wavefront adds the weighted value rows of the keys that are shown, and of no others. The tile
 // kernels multiply hidden keys' values by weights of zero, which makes a NaN of a NaN or an infinity: rows that
-// come out of them not finite are computed again by this, slowly.
-template <typename T>
+// come out of them not finite are computed again by this, slowly. C: the keys' type, e4m3 or T.
+template <typename T, typename C = T>
 __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
     const AttnSpan sp = span_of(a.seqs, b);
     const int64_t row = sp.q0 + r;
@@ -191,6 +198,7 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
         const int j = j0 + lane;
         bool shown = j < sp.nk && win.has(j);
         int64_t kat = 0, vat = 0;
+        float k_scale = 1.0f, v_scale = 1.0f;
         if (shown) {
             if (a.seqs.tables) {
                 int at;
@@ -198,6 +206,10 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
                 shown = p >= 0;
                 kat = p * a.psk + at * a.ldk;
                 vat = p * a.psv + at * a.ldv;
+                if (__is_same(C, e4m3) && shown) {
+                    k_scale = two_to(a.k_exps[block_at(a, a.k_epage, p, at) + kvh]);
+                    v_scale = two_to(a.v_exps[block_at(a, a.v_epage, p, at) + kvh]);
+                }
             } else {
                 kat = (int64_t)(sp.k0 + j) * a.ldk;
                 vat = (int64_t)(sp.k0 + j) * a.ldv;
@@ -206,7 +218,7 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
         }
         float s = -INFINITY;
         if (shown) {
-            const T *k = static_cast<const T *>(a.k) + kat + kvh * a.hsk;
+            const C *k = static_cast<const C *>(a.k) + kat + kvh * a.hsk;
             float dot = 0.0f;
             for (int c = 0; c < a.d; c++)
                 dot = __builtin_fmaf(to_f32(q[c]) + (a.rel_u ? a.rel_u[h * a.d + c] : 0.0f), to_f32(k[c]), dot);
@@ -217,6 +229,7 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
                     term = __builtin_fmaf(to_f32(q[c]) + (a.rel_v ? a.rel_v[h * a.d + c] : 0.0f), rr[c], term);
                 dot += term;
             }
+            if (__is_same(C, e4m3)) dot *= k_scale;
             s = score_of(a, dot, h, slope, j - i);
             shown = s != -INFINITY;
         }
@@ -237,8 +250,8 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
         while (live) {
             const int t = __builtin_ctzll(live);
             live &= live - 1;
-            const float w = __shfl(p, t);
-            const T *v = static_cast<const T *>(a.v) + __shfl(vat, t) + kvh * a.hsv;
+            const float w = __is_same(C, e4m3) ? __shfl(p * v_scale, t) : __shfl(p, t);
+            const C *v = static_cast<const C *>(a.v) + __shfl(vat, t) + kvh * a.hsv;
             for (int e = 0; e < 4; e++)
                 if (e * 64 + lane < a.d) acc[e] = __builtin_fmaf(w, to_f32(v[e * 64 + lane]), acc[e]);
         }

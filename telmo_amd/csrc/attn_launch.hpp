@@ -22,4 +22,8 @@ inline bool attention_few_fits(const AttnArgs &a) {
 }
 hipError_t launch_attention_few(const AttnArgs &a, int splits, hipStream_t s);
 
+// The same over a cache in e4m3 (a.k_exps), rows of any type.
+hipError_t launch_attention8(const AttnArgs &a, int splits, hipStream_t s);
+hipError_t launch_attention8_few(const AttnArgs &a, int splits, hipStream_t s);
+
 }  // namespace tg

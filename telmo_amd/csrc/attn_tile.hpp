@@ -10,6 +10,19 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
+// Eight values as N bf16 parts that each cut eight bits off what is left: exact, and an infinity or NaN stays one.
+template <int N>
+__device__ __forceinline__ void cut_parts(const float *x, bf16x8 (&part)[N]) {
+    for (int e = 0; e < 8; e++) {
+        float left = x[e];
+        for (int n = 0; n < N; n++) {
+            const float cut = left - left == 0.0f ? __uint_as_float(__float_as_uint(left) & 0xffff0000u) : left;
+            part[n][e] = (__bf16)cut;
+            left = cut - cut == 0.0f ? left - cut : 0.0f;
+        }
+    }
+}
+
 // The greater (the sum) of a lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_halves(float x) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

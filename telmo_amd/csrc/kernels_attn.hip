@@ -18,17 +18,18 @@ namespace {
 
 constexpr int ROW_WAVES = 4;
 
-template <typename T>
+// C: the keys' type, T or e4m3.
+template <typename T, typename C>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_rows_kernel(const AttnArgs a) {
     const int b = blockIdx.z, r = blockIdx.x * ROW_WAVES + (threadIdx.x >> 6);
-    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<T>(a, b, blockIdx.y, r, threadIdx.x & 63);
+    if (r < span_of(a.seqs, b).nq && r < a.seqs.longest) attend_row<T, C>(a, b, blockIdx.y, r, threadIdx.x & 63);
 }
 
 // The parts of a row and head, joined by one wavefront: with M the largest maximum, the sums and outputs of
 // part p count e^(m_p - M) times. Lane p weighs part p; then each lane adds V values of all parts, in their order,
 // STEP parts' loads on their way at a time. Bound by reading the parts: 509 rows of 32 heads of 128 in
 // four parts, 34 MB, 11.6 us (2.9 TB/s); 32 single rows 4.9 us, mostly the latency of its loads in turn.
-template <typename T, int V, int STEP>
+template <typename T, typename C, int V, int STEP>
 __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArgs a, const AttnParts parts) {
     typedef float fv __attribute__((ext_vector_type(V)));
     const int lane = threadIdx.x & 63, b = blockIdx.y;
@@ -75,37 +76,42 @@ __global__ __launch_bounds__(64 * ROW_WAVES) void attn_join_kernel(const AttnArg
         }
     }
     // As the tile kernels do for rows that they finish themselves.
-    if (!__all(sound) && (sizeof(T) == 4 || l - l == 0.0f)) attend_row<T>(a, b, h, r, lane);
+    if (!__all(sound) && (sizeof(T) == 4 || l - l == 0.0f)) attend_row<T, C>(a, b, h, r, lane);
 }
 
-template <typename T>
-hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
+template <typename T, typename C>
+hipError_t launch_rows_of(const AttnArgs &a, hipStream_t s) {
     const size_t blocks = div_ceil((size_t)a.seqs.longest, ROW_WAVES);
     if (blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
     const dim3 grid((unsigned)blocks, (unsigned)a.heads, (unsigned)a.seqs.batch);
-    hipLaunchKernelGGL((attn_rows_kernel<T>), grid, dim3(64 * ROW_WAVES), 0, s, a);
+    hipLaunchKernelGGL((attn_rows_kernel<T, C>), grid, dim3(64 * ROW_WAVES), 0, s, a);
     return hipGetLastError();
 }
+template <typename T>
+hipError_t launch_rows(const AttnArgs &a, hipStream_t s) {
+    return a.k_exps ? launch_rows_of<T, e4m3>(a, s) : launch_rows_of<T, T>(a, s);
+}
 
-template <typename T, int V, int STEP>
+template <typename T, typename C, int V, int STEP>
 hipError_t launch_join_of(const AttnArgs &a, int splits, hipStream_t s) {
     const size_t blocks = div_ceil((size_t)a.seqs.longest * a.heads, ROW_WAVES);
     if (blocks > MAX_ATTN_BLOCKS) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((attn_join_kernel<T, V, STEP>), dim3((unsigned)blocks, (unsigned)a.seqs.batch),
+    hipLaunchKernelGGL((attn_join_kernel<T, C, V, STEP>), dim3((unsigned)blocks, (unsigned)a.seqs.batch),
                        dim3(64 * ROW_WAVES), 0, s, a, parts_of(a, splits));
     return hipGetLastError();
 }
 // The parts' loads on their way at a time, 4, 8 or 16: past the last part they repeat it, so not many more than there
 // are (750 rows in five parts with 16 41.7 us, with 8 41.1; a chunk's four with 4 as with 16 within 1 us).
-template <typename T, int V>
+template <typename T, typename C, int V>
 hipError_t launch_join_by(const AttnArgs &a, int splits, hipStream_t s) {
-    return splits > 8   ? launch_join_of<T, V, 16>(a, splits, s)
-           : splits > 4 ? launch_join_of<T, V, 8>(a, splits, s)
-                        : launch_join_of<T, V, 4>(a, splits, s);
+    return splits > 8   ? launch_join_of<T, C, V, 16>(a, splits, s)
+           : splits > 4 ? launch_join_of<T, C, V, 8>(a, splits, s)
+                        : launch_join_of<T, C, V, 4>(a, splits, s);
 }
 template <typename T>
 hipError_t launch_join(const AttnArgs &a, int splits, hipStream_t s) {
-    return a.d > 128 ? launch_join_by<T, 4>(a, splits, s) : launch_join_by<T, 2>(a, splits, s);
+    if (a.k_exps) return a.d > 128 ? launch_join_by<T, e4m3, 4>(a, splits, s) : launch_join_by<T, e4m3, 2>(a, splits, s);
+    return a.d > 128 ? launch_join_by<T, T, 4>(a, splits, s) : launch_join_by<T, T, 2>(a, splits, s);
 }
 
 // How a call is spread: workgroups of `tile` query rows and heads, and how many parts the keys are cut into so that
@@ -188,16 +194,18 @@ hipError_t launch_attention(const AttnArgs &a, hipStream_t s) {
         if (n * bytes > a.work_bytes) n = a.work_bytes / bytes;
         return n < 1 ? (size_t)1 : n;
     };
-    Spread sp = few ? (a.seqs.batch == 1 && a.d > 64 ? FEW_ALONE : FEW) : a.type != F32 ? TILES16 : TILES32;
+    const bool tiles32 = !few && a.type == F32 && !a.k_exps;
+    Spread sp = few ? (a.seqs.batch == 1 && a.d > 64 ? FEW_ALONE : FEW) : tiles32 ? TILES32 : TILES16;
     size_t n = parts(sp);
     // f32 tiles of 64 rows where those of 128 leave half of the GPU's 256 CUs empty.
-    if (!few && a.type == F32 && wgs_of(sp) * n <= 128) {
+    if (tiles32 && wgs_of(sp) * n <= 128) {
         sp = SMALL32;
         n = parts(sp);
     }
-    const hipError_t e = few                ? launch_attention_few(a, (int)n, s)
-                         : a.type == F32 ? launch_attention32(a, (int)sp.tile, (int)n, s)
-                                         : launch_attention16(a, (int)n, s);
+    const hipError_t e = a.k_exps  ? (few ? launch_attention8_few(a, (int)n, s) : launch_attention8(a, (int)n, s))
+                         : few     ? launch_attention_few(a, (int)n, s)
+                         : tiles32 ? launch_attention32(a, (int)sp.tile, (int)n, s)
+                                   : launch_attention16(a, (int)n, s);
     if (e != hipSuccess || n == 1) return e;
     switch (a.type) {
         case F16: return launch_join<_Float16>(a, (int)n, s);

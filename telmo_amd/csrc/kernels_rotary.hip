@@ -55,44 +55,58 @@ __device__ __forceinline__ void store_some(U *p, int n, bool aligned, const floa
 __host__ __device__ inline int pair_pieces(int dim) { return (dim / 2 + 7) / 8; }
 __host__ __device__ inline int pieces_of(int d, int dim) { return pair_pieces(dim) + (d - dim + 7) / 8; }
 
-template <typename T, typename U>
-__device__ __forceinline__ void rotate_piece(const T *x, U *out, int piece, int d, int dim, bool interleaved,
-                                             const float2 *table) {
+// A piece's values in 32 bits: n of them from `first` on in v, and as many from `second` on in w (of interleaved pairs the
+// first eight and the rest).
+struct Piece {
+    float v[8], w[8];
+    int first, second, nv, nw;
+    bool v_aligned, w_aligned;  // whether `first` and `second` are multiples of 8
+};
+template <typename T>
+__device__ __forceinline__ Piece piece_of(const T *x, int piece, int d, int dim, bool interleaved, const float2 *table) {
     const int half = dim / 2, turned = pair_pieces(dim);
-    float v[8];
+    Piece p;
     if (piece >= turned) {
-        const int c = dim + (piece - turned) * 8, n = d - c < 8 ? d - c : 8;
-        load_some(x + c, n, dim % 8 == 0, v);
-        store_some(out + c, n, dim % 8 == 0, v);
-        return;
+        const int c = dim + (piece - turned) * 8;
+        p.first = c, p.nv = d - c < 8 ? d - c : 8, p.v_aligned = dim % 8 == 0;
+        p.second = 0, p.nw = 0, p.w_aligned = true;
+        load_some(x + c, p.nv, p.v_aligned, p.v);
+        return p;
     }
     const int i = piece * 8, n = half - i < 8 ? half - i : 8;
-    float w[8];
+    p.v_aligned = true;
     if (interleaved) {
-        const int m = 2 * n < 8 ? 2 * n : 8;
-        load_some(x + 2 * i, m, true, v);
-        load_some(x + 2 * i + 8, 2 * n - m, true, w);
+        p.first = 2 * i, p.nv = 2 * n < 8 ? 2 * n : 8;
+        p.second = 2 * i + 8, p.nw = 2 * n - p.nv, p.w_aligned = true;
+        load_some(x + p.first, p.nv, true, p.v);
+        load_some(x + p.second, p.nw, true, p.w);
         for (int e = 0; e < 8; e += 2) {
             const float2 s = e / 2 < n ? table[i + e / 2] : make_float2(0.0f, 0.0f);
             const float2 t = 4 + e / 2 < n ? table[i + 4 + e / 2] : make_float2(0.0f, 0.0f);
-            const float a = v[e], b = v[e + 1], f = w[e], g = w[e + 1];
-            v[e] = a * s.x - b * s.y, v[e + 1] = b * s.x + a * s.y;
-            w[e] = f * t.x - g * t.y, w[e + 1] = g * t.x + f * t.y;
+            const float a = p.v[e], b = p.v[e + 1], f = p.w[e], g = p.w[e + 1];
+            p.v[e] = a * s.x - b * s.y, p.v[e + 1] = b * s.x + a * s.y;
+            p.w[e] = f * t.x - g * t.y, p.w[e + 1] = g * t.x + f * t.y;
         }
-        store_some(out + 2 * i, m, true, v);
-        store_some(out + 2 * i + 8, 2 * n - m, true, w);
     } else {
-        load_some(x + i, n, true, v);
-        load_some(x + half + i, n, half % 8 == 0, w);
+        p.first = i, p.nv = n;
+        p.second = half + i, p.nw = n, p.w_aligned = half % 8 == 0;
+        load_some(x + p.first, n, true, p.v);
+        load_some(x + p.second, n, p.w_aligned, p.w);
         for (int e = 0; e < 8; e++) {
             const float2 t = e < n ? table[i + e] : make_float2(0.0f, 0.0f);
-            const float a = v[e], b = w[e];
-            v[e] = a * t.x - b * t.y;
-            w[e] = b * t.x + a * t.y;
+            const float a = p.v[e], b = p.w[e];
+            p.v[e] = a * t.x - b * t.y;
+            p.w[e] = b * t.x + a * t.y;
         }
-        store_some(out + i, n, true, v);
-        store_some(out + half + i, n, half % 8 == 0, w);
     }
+    return p;
+}
+template <typename T, typename U>
+__device__ __forceinline__ void rotate_piece(const T *x, U *out, int piece, int d, int dim, bool interleaved,
+                                             const float2 *table) {
+    const Piece p = piece_of(x, piece, d, dim, interleaved, table);
+    store_some(out + p.first, p.nv, p.v_aligned, p.v);
+    store_some(out + p.second, p.nw, p.w_aligned, p.w);
 }
 
 template <typename T, typename U>
@@ -161,6 +175,111 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const T *k, int64_t ldk
     }
 }
 
+// The same into pages of e4m3 values: a block of rows of a page has a power of two for each head, which is known when all of
+// the block's new rows are. A workgroup takes a block of a sequence, a wavefront one head's keys or values in it at a time:
+// first the largest of the new rows, rotated, then the block's exponent, and the rows that were there before in it where
+// that grows, then the new rows again, rounded. What is read twice comes from the CU's cache the second time.
+constexpr int TURNS = 2048;  // sines and cosines held at a time
+
+template <typename T>
+__global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ldk, int64_t hsk, const T *v, int64_t ldv,
+                                                          int64_t hsv, const Cache8 c, int heads, int d, const AttnSeqs q,
+                                                          const RotaryArgs r) {
+    __shared__ float2 table[TURNS];
+    const int b = blockIdx.y;
+    const AttnSpan sp = span_of(q, b);
+    const int rows = sp.nq < q.longest ? sp.nq : q.longest;
+    if (rows <= 0) return;
+    const int64_t first = (int64_t)q.lengths[b] - sp.nq;  // as it stands, also past the table
+    const int64_t at = first < 0 ? 0 : first, end = first + rows < sp.nk ? first + rows : sp.nk;
+    const int64_t step = (int64_t)gridDim.x * c.block;
+    for (int64_t block0 = (at / c.block + blockIdx.x) * c.block; block0 < end; block0 += step) {
+        // The positions of the block, those from lo to hi new.
+        const int64_t lo = block0 > at ? block0 : at, hi = end < block0 + c.block ? end : block0 + c.block;
+        int row0;
+        const int page = page_of(q, b, (int)block0, row0);
+        if (page < 0) continue;
+        const int older = (int)(lo - block0), n = (int)(hi - lo);
+        const int64_t from = (int64_t)sp.q0 + (lo - first);  // the first new row
+        const int pairs = r.dim / 2;
+        const int some = pairs ? min(n, TURNS / pairs) : n;  // rows whose turns fit the table
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const auto fill = [&](int done) {
+            __syncthreads();
+            for (int t = threadIdx.x; t < min(some, n - done) * pairs; t += THREADS)
+                table[t] = turn((double)(lo + done + t / pairs) * r.turns[t % pairs], r.amplitude);
+            __syncthreads();
+        };
+        if (pairs && some == n) fill(0);
+        for (int u0 = blockIdx.z * 4; u0 < 2 * heads; u0 += gridDim.z * 4) {
+            // All wavefronts make the same steps: one past the last unit does the last one's again, and writes nothing.
+            const int unit = min(u0 + wave, 2 * heads - 1);
+            const bool mine = u0 + wave < 2 * heads, key = unit < heads;
+            const int h = key ? unit : unit - heads, dim = key ? r.dim : 0;
+            const T *x = key ? k + from * ldk + h * hsk : v + from * ldv + h * hsv;
+            const int64_t ld = key ? ldk : ldv;
+            const int64_t ldc = key ? c.ldk : c.ldv;
+            uint8_t *rows8 = key ? c.k + page * c.psk + h * c.hsk : c.v + page * c.psv + h * c.hsv;
+            rows8 += row0 * ldc;
+            int8_t *exps = key ? c.k_exps + page * c.k_epage : c.v_exps + page * c.v_epage;
+            exps += (int64_t)(row0 / c.block) * heads + h;
+            const int pieces = pieces_of(d, dim);
+            // f(piece, the block's row) for the wavefront's pieces.
+            const auto each = [&](auto f) {
+                for (int done = 0; done < n; done += some) {
+                    if (pairs && some < n) fill(done);
+                    const int now = min(some, n - done);
+                    for (int t = lane; t < now * pieces; t += 64) {
+                        const int row = t / pieces;
+                        f(piece_of(x + (done + row) * ld, t % pieces, d, dim, r.interleaved, table + row * pairs), done + row);
+                    }
+                }
+            };
+            uint32_t top = 0;
+            each([&](const Piece &p, int) {
+                for (int e = 0; e < 8; e++) {
+                    if (e < p.nv) top = max(top, e4m3_size(p.v[e]));
+                    if (e < p.nw) top = max(top, e4m3_size(p.w[e]));
+                }
+            });
+            for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+            int now = e4m3_exponent(top);
+            if (older) {
+                const int had = *exps;
+                if (had >= now) {
+                    now = had;
+                } else if (mine) {
+                    const float down = two_to(had - now);
+                    for (int t = lane; t < older * (d / 16); t += 64) {
+                        uint32_t *to = reinterpret_cast<uint32_t *>(rows8 + t / (d / 16) * ldc + t % (d / 16) * 16);
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t y = to[e];
+                            to[e] = e4m3_pack(__builtin_amdgcn_cvt_f32_fp8(y, 0), __builtin_amdgcn_cvt_f32_fp8(y, 1),
+                                              __builtin_amdgcn_cvt_f32_fp8(y, 2), __builtin_amdgcn_cvt_f32_fp8(y, 3), down);
+                        }
+                    }
+                }
+            }
+            const float down = two_to(-now);
+            each([&](const Piece &p, int row) {
+                if (!mine) return;
+                uint8_t *to = rows8 + (older + row) * ldc;
+                const auto store = [&](uint8_t *at, const float *y, int count, bool aligned) {
+                    const uint32_t a = e4m3_pack(y[0], y[1], y[2], y[3], down), b = e4m3_pack(y[4], y[5], y[6], y[7], down);
+                    if (count == 8 && aligned) {
+                        *reinterpret_cast<u32x2 *>(at) = u32x2{a, b};
+                    } else {
+                        for (int e = 0; e < count; e++) at[e] = (uint8_t)((e < 4 ? a : b) >> 8 * (e % 4));
+                    }
+                };
+                store(to + p.first, p.v, p.nv, p.v_aligned);
+                if (p.nw) store(to + p.second, p.w, p.nw, p.w_aligned);
+            });
+            if (mine && lane == 0) *exps = (int8_t)now;
+        }
+    }
+}
+
 template <typename T, typename U>
 hipError_t rotary_to(const void *x, int64_t ldx, int64_t hsx, void *out, int64_t ldo, int64_t hso, size_t rows,
                      int heads, int d, const int32_t *positions, int64_t start, const RotaryArgs &r, hipStream_t s) {
@@ -210,6 +329,26 @@ hipError_t launch_append(const void *k, int64_t ldk, int64_t hsk, const void *v,
                            static_cast<U *>(cv), ldcv, hscv, psv, heads, d, q, r);
         return hipGetLastError();
     });
+}
+
+hipError_t launch_append8(const void *k, int64_t ldk, int64_t hsk, const void *v, int64_t ldv, int64_t hsv, uint32_t type,
+                          const Cache8 &c, int heads, int d, const AttnSeqs &q, const RotaryArgs &r, hipStream_t s) {
+    // The blocks that the longest sequence's rows reach into; heads are spread over workgroups as far as those leave the
+    // GPU's 256 CUs without four each.
+    const size_t blocks = div_ceil((size_t)q.longest, (size_t)c.block) + 1, sets = div_ceil((size_t)heads * 2, 4);
+    const size_t spread = div_ceil((size_t)1024, blocks * q.batch);
+    const dim3 grid((unsigned)min_of(blocks, MAX_BLOCKS), (unsigned)q.batch, (unsigned)min_of(spread, sets));
+    const auto launch = [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((append8_kernel<T>), grid, dim3(THREADS), 0, s, static_cast<const T *>(k), ldk, hsk,
+                           static_cast<const T *>(v), ldv, hsv, c, heads, d, q, r);
+        return hipGetLastError();
+    };
+    switch (type) {
+        case F16: return launch(_Float16{});
+        case BF16: return launch(__bf16{});
+        default: return launch(float{});
+    }
 }
 
 }  // namespace tg

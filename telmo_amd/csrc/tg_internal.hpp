@@ -352,6 +352,12 @@ struct AttnArgs {
     AttnSeqs seqs;
     void *work;        // split partials, or null
     size_t work_bytes;
+    // Keys and values in e4m3 (paged): value times 2^exponent, one for each head of each `block` rows of a page, pages
+    // k_epage (v_epage) apart. k_exps null: k and v are of `type`. Row / block as j / page above.
+    const int8_t *k_exps, *v_exps;
+    int64_t k_epage, v_epage;
+    int block;
+    uint32_t block_mul, block_shift;
 };
 hipError_t launch_attention(const AttnArgs &a, hipStream_t s);
 // Bytes with which launch_attention splits the keys of sequences of up to max_keys keys.
@@ -372,6 +378,16 @@ hipError_t launch_append(const void *k, int64_t ldk, int64_t hsk, const void *v,
                          uint32_t type, void *ck, int64_t ldck, int64_t hsck, int64_t psk, void *cv, int64_t ldcv,
                          int64_t hscv, int64_t psv, uint32_t cache_type, int heads, int d, const AttnSeqs &q,
                          const RotaryArgs &r, hipStream_t s);
+
+// The same into pages of e4m3 values with their blocks' exponents (AttnArgs).
+struct Cache8 {
+    uint8_t *k, *v;
+    int8_t *k_exps, *v_exps;
+    int64_t ldk, hsk, psk, ldv, hsv, psv, k_epage, v_epage;
+    int block;
+};
+hipError_t launch_append8(const void *k, int64_t ldk, int64_t hsk, const void *v, int64_t ldv, int64_t hsv, uint32_t type,
+                          const Cache8 &c, int heads, int d, const AttnSeqs &q, const RotaryArgs &r, hipStream_t s);
 
 // The greedy TDT decode (kernels_tdt.hip). The control block lives in device memory; the host
 // writes it before a decode and reads it between batches of steps.
