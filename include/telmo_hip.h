@@ -233,6 +233,38 @@ int tg_matmul_quantized_to_quant_device(tg_ctx *ctx, const void *qa, size_t qa_l
 int tg_linear_glu_device(tg_ctx *ctx, const float *a, size_t a_len, size_t m, const tg_weights *w, float *out,
                          size_t out_len, size_t ldo, const tg_epilogue *epi);
 
+/* ---- weights in eight bits with a scale for each block of 128 x 128 ---------------------------
+ * c = epi(a' w'^T): w' are e4m3 values (a byte each: sign, four bits of exponent, three of mantissa, up to 448; 0x7f and
+ * 0xff are NaN) times an f32 scale for each block of 128 outputs by 128 inputs, and a' is a with each row's groups of 128
+ * inputs rounded to e4m3 times a power of two: the least e >= -100 with |x| <= 448 2^e for the group's finite values, each
+ * x 2^-e rounded to nearest, ties to even (|x| past 240 2^120, which would round past f32, as that). Sums are f32. NaN or infinity in a row make its outputs NaN. No counterpart in
+ * the reference; a context's mode changes nothing here. Row i's outputs depend on m by the order of their f32 sums; 16-bit
+ * outputs of more than 16 rows may be summed by instructions that align the products of 32 inputs before they add them,
+ * off by up to 2^-10 of the largest of each 128. */
+typedef struct tg_weights_e4m3 tg_weights_e4m3;
+/* Row-major values [n][k], rows ldv apart, and scales [ceil(n / 128)][ceil(k / 128)], host pointers (device pointers, read
+ * during the call only). The device copy is the library's own, laid out for the matrix cores. n and k at most 2^24. */
+int tg_weights_e4m3_upload(tg_ctx *ctx, const uint8_t *values, size_t values_len, size_t ldv, const float *scales,
+                           size_t n_scales, size_t n, size_t k, tg_weights_e4m3 **out);
+int tg_weights_e4m3_upload_device(tg_ctx *ctx, const uint8_t *values, size_t values_len, size_t ldv, const float *scales,
+                                  size_t n_scales, size_t n, size_t k, tg_weights_e4m3 **out);
+void tg_weights_e4m3_free(tg_weights_e4m3 *w);
+size_t tg_weights_e4m3_n(const tg_weights_e4m3 *w);
+size_t tg_weights_e4m3_k(const tg_weights_e4m3 *w);
+/* Bytes of the values and scales as they were given. */
+size_t tg_weights_e4m3_bytes(const tg_weights_e4m3 *w);
+/* Row-major f32 weights w[n][k] in that form (host): each block's scale is its largest |w| / 448 (at least 2^-120; blocks
+ * of zeros: 1), values are rounded to nearest, ties to even. Not finite: TG_ERR_ARG. */
+int tg_encode_e4m3(const float *w, size_t n, size_t k, uint8_t *values, size_t values_len, float *scales, size_t n_scales);
+/* The product on device pointers, queued on the context's stream; a of `type` and c of `c_type` (TG_F32, TG_F16 or
+ * TG_BF16), rows at any stride, bias f32. epi as in tg_matmul_device, in f32; c is rounded once. Nothing is allocated: the
+ * rounded rows of more than 16 go to the workspace (device, 16-byte aligned, tg_linear_e4m3_workspace_bytes(m, k)
+ * bytes; 0 up to 16 rows), which calls that may overlap on the GPU must not share. a, c and workspace must not overlap. */
+int tg_linear_e4m3_device(tg_ctx *ctx, uint32_t type, const void *a, size_t a_len, size_t lda, size_t m,
+                          const tg_weights_e4m3 *w, uint32_t c_type, void *c, size_t c_len, size_t ldc, const tg_epilogue *epi,
+                          void *workspace, size_t workspace_len);
+size_t tg_linear_e4m3_workspace_bytes(size_t m, size_t k);
+
 /* ---- row kernels -------------------------------------------------------------------------- */
 
 /* out[r, j] = x[r, j] * sigmoid(x[r, half + j]) for j < half (the GLU of a convolution module),
@@ -443,7 +475,8 @@ int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t 
                            const tg_rotary *rotary);
 
 /* The same into a cache in e4m3. A block's exponent is the least e >= -100 with |x| <= 448 2^e for the finite values of its
- * new rows (keys rotated), and each value is x 2^-e rounded to nearest, ties to even; NaN and infinities become NaN. A
+ * new rows (keys rotated), and each value is x 2^-e rounded to nearest, ties to even (|x| past 240 2^120, which
+ * would round past f32, as that); NaN and infinities become NaN. A
  * block that holds older rows of its sequence keeps its exponent where that is large enough; where it grows, its older rows
  * are rounded again under the new one (powers of two: only values that become subnormal lose bits). Rows of a block behind
  * the new ones are left as they were. A block takes the new rows of one sequence in a call. */

@@ -93,6 +93,15 @@ SIGNATURES = {
     "tg_matmul_quantized_device": (ctypes.c_int, [_p, _p, _sz, _p, _sz, _p, _p, _sz, _sz, _p]),
     "tg_matmul_quantized_glu_device": (ctypes.c_int, [_p, _p, _sz, _p, _sz, _p, _p, _sz, _sz, _p]),
     "tg_matmul_quantized_to_quant_device": (ctypes.c_int, [_p, _p, _sz, _p, _sz, _p, _p, _p, _sz, _p, _sz]),
+    "tg_weights_e4m3_upload": (ctypes.c_int, [_p, _p, _sz, _sz, _p, _sz, _sz, _sz, ctypes.POINTER(_p)]),
+    "tg_weights_e4m3_upload_device": (ctypes.c_int, [_p, _p, _sz, _sz, _p, _sz, _sz, _sz, ctypes.POINTER(_p)]),
+    "tg_weights_e4m3_free": (None, [_p]),
+    "tg_weights_e4m3_n": (_sz, [_p]),
+    "tg_weights_e4m3_k": (_sz, [_p]),
+    "tg_weights_e4m3_bytes": (_sz, [_p]),
+    "tg_encode_e4m3": (ctypes.c_int, [_p, _sz, _sz, _p, _sz, _p, _sz]),
+    "tg_linear_e4m3_device": (ctypes.c_int, [_p, _u32, _p, _sz, _sz, _sz, _p, _u32, _p, _sz, _sz, _p, _p, _sz]),
+    "tg_linear_e4m3_workspace_bytes": (_sz, [_sz, _sz]),
     "tg_glu_device": (ctypes.c_int, [_p, _p, _sz, _sz, _sz, _sz, _p, _sz, _sz]),
     "tg_softmax_device": (ctypes.c_int, [_p, _p, _sz, _sz, _sz, _sz]),
     "tg_average_pairs_device": (ctypes.c_int, [_p, _p, _sz, _sz, _sz, _sz, _sz, _p, _sz, _sz]),

@@ -14,11 +14,13 @@
 #include <cmath>
 #include <cstring>
 #include <mutex>
+#include <new>
 #include <string>
 #include <utility>
 #include <vector>
 
 #include "../../include/telmo_hip.h"
+#include "e4m3_product.hpp"
 #include "tg_internal.hpp"
 
 struct tg_ctx {
@@ -61,6 +63,12 @@ struct tg_ctx {
 
 struct tg_weights {
     tg::DeviceWeights d;
+    int device;
+};
+
+struct tg_weights_e4m3 {
+    tg::E4m3Panels d;
+    size_t n, k;
     int device;
 };
 
@@ -1543,6 +1551,7 @@ int tg_tdt_set_resident_limits(tg_ctx *ctx, tg_tdt *tdt, uint32_t steps_per_laun
 namespace {
 
 constexpr size_t MAX_ATTN_ROWS = (size_t)1 << 30;  // rows, keys and strides that the kernels count in 32 bits
+constexpr size_t MAX_E4M3 = (size_t)1 << 24;       // rows, inputs and outputs of a product in e4m3
 constexpr size_t MAX_ATTN_GRID = 65535;            // sequences and heads, each a grid dimension
 
 bool attn_type(uint32_t t) { return t == TG_F32 || t == TG_F16 || t == TG_BF16; }
@@ -1802,6 +1811,52 @@ int check_rotary(tg_ctx *ctx, const tg_rotary *r, size_t d, tg::RotaryArgs &out)
     return TG_OK;
 }
 
+int upload_e4m3(tg_ctx *ctx, const uint8_t *values, size_t values_len, size_t ldv, const float *scales, size_t n_scales,
+                size_t n, size_t k, tg_weights_e4m3 **out, bool from_device) {
+    if (!out) return fail(ctx, TG_ERR_NULL, "null argument");
+    *out = nullptr;
+    if (n > MAX_E4M3 || k > MAX_E4M3) return fail(ctx, TG_ERR_UNSUPPORTED, "n and k must be at most 2^24");
+    if (ldv < k) return fail(ctx, TG_ERR_SHAPE, "ldv must be >= k");
+    if (values_len < span(n, ldv, k)) return fail(ctx, TG_ERR_SHAPE, "values is too short");
+    if (n_scales < tg::div_ceil(n, 128) * tg::div_ceil(k, 128)) return fail(ctx, TG_ERR_SHAPE, "scales is too short");
+    if (n && k && (!values || !scales)) return fail(ctx, TG_ERR_NULL, "null values or scales");
+    if (reinterpret_cast<uintptr_t>(scales) % 4) return fail(ctx, TG_ERR_ALIGN, "scales must be 4-byte aligned");
+    if (!ctx) return TG_ERR_NULL;
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    tg_weights_e4m3 *w = new (std::nothrow) tg_weights_e4m3();
+    if (!w) return fail(ctx, TG_ERR_NOMEM, "host allocation failed");
+    w->device = ctx->device;
+    w->n = n, w->k = k;
+    w->d.panels = tg::div_ceil(n, 16), w->d.blocks = tg::div_ceil(k, 128);
+    const size_t bytes = tg::e4m3_weight_bytes(n, k), held = tg::div_ceil(n, 128) * w->d.blocks * sizeof(float);
+    uint8_t *laid = nullptr, *raw = nullptr;
+    float *kept = nullptr;
+    hipError_t e = hipSuccess;
+    if (bytes) {
+        e = hipMalloc(&laid, bytes);
+        if (e == hipSuccess) e = hipMalloc(&kept, held);
+        if (e == hipSuccess && !from_device) e = hipMalloc(&raw, n * k);
+        const bool no_memory = e != hipSuccess;
+        if (e == hipSuccess && !from_device) e = hipMemcpy2DAsync(raw, k, values, ldv, k, n, hipMemcpyHostToDevice, ctx->stream);
+        if (e == hipSuccess)
+            e = hipMemcpyAsync(kept, scales, held, from_device ? hipMemcpyDeviceToDevice : hipMemcpyHostToDevice, ctx->stream);
+        if (e == hipSuccess) e = tg::launch_e4m3_weights(from_device ? values : raw, from_device ? ldv : k, n, k, laid, ctx->stream);
+        if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
+        if (raw) (void)hipFree(raw);
+        if (e != hipSuccess) {
+            if (laid) (void)hipFree(laid);
+            if (kept) (void)hipFree(kept);
+            delete w;
+            return no_memory ? fail(ctx, TG_ERR_NOMEM, "device allocation failed") : hip_fail(ctx, e, "weight upload");
+        }
+    }
+    w->d.values = laid;
+    w->d.scales = kept;
+    *out = w;
+    return TG_OK;
+}
+
 int run_append(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type, const tg_rows &k_new,
                const tg_rows &v_new, const tg_rotary *rotary) {
     if (!desc) return fail(ctx, TG_ERR_NULL, "null description");
@@ -1913,6 +1968,72 @@ int tg_rotary_device(tg_ctx *ctx, uint32_t type, tg_rows x, uint32_t out_type, t
 int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t type, tg_rows k_new, tg_rows v_new,
                            const tg_rotary *rotary) {
     return run_append(ctx, desc, nullptr, type, k_new, v_new, rotary);
+}
+
+int tg_weights_e4m3_upload(tg_ctx *ctx, const uint8_t *values, size_t values_len, size_t ldv, const float *scales,
+                           size_t n_scales, size_t n, size_t k, tg_weights_e4m3 **out) {
+    return upload_e4m3(ctx, values, values_len, ldv, scales, n_scales, n, k, out, false);
+}
+
+int tg_weights_e4m3_upload_device(tg_ctx *ctx, const uint8_t *values, size_t values_len, size_t ldv, const float *scales,
+                                  size_t n_scales, size_t n, size_t k, tg_weights_e4m3 **out) {
+    return upload_e4m3(ctx, values, values_len, ldv, scales, n_scales, n, k, out, true);
+}
+
+void tg_weights_e4m3_free(tg_weights_e4m3 *w) {
+    if (!w) return;
+    (void)hipSetDevice(w->device);
+    (void)hipDeviceSynchronize();
+    if (w->d.values) (void)hipFree(const_cast<uint8_t *>(w->d.values));
+    if (w->d.scales) (void)hipFree(const_cast<float *>(w->d.scales));
+    delete w;
+}
+
+size_t tg_weights_e4m3_n(const tg_weights_e4m3 *w) { return w ? w->n : 0; }
+size_t tg_weights_e4m3_k(const tg_weights_e4m3 *w) { return w ? w->k : 0; }
+size_t tg_weights_e4m3_bytes(const tg_weights_e4m3 *w) {
+    return w ? w->n * w->k + tg::div_ceil(w->n, 128) * w->d.blocks * sizeof(float) : 0;
+}
+
+size_t tg_linear_e4m3_workspace_bytes(size_t m, size_t k) {
+    return m > MAX_E4M3 || k > MAX_E4M3 ? 0 : tg::e4m3_work_bytes(m, k);
+}
+
+int tg_linear_e4m3_device(tg_ctx *ctx, uint32_t type, const void *a, size_t a_len, size_t lda, size_t m,
+                          const tg_weights_e4m3 *w, uint32_t c_type, void *c, size_t c_len, size_t ldc, const tg_epilogue *epi,
+                          void *workspace, size_t workspace_len) {
+    if (!w) return fail(ctx, TG_ERR_NULL, "null weights");
+    const size_t n = w->n, k = w->k;
+    if (!attn_type(type) || !attn_type(c_type)) return fail(ctx, TG_ERR_ARG, "types must be f32, f16 or bf16");
+    if (m == 0 || n == 0) return ctx ? TG_OK : TG_ERR_NULL;
+    if (m > MAX_E4M3) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^24 rows");
+    if (lda < k || ldc < n) return fail(ctx, TG_ERR_SHAPE, "lda must be >= k and ldc >= n");
+    if (a_len < span(m, lda, k)) return fail(ctx, TG_ERR_SHAPE, "a is too short");
+    if (c_len < span(m, ldc, n)) return fail(ctx, TG_ERR_SHAPE, "c is too short");
+    if (epi && epi->bias && epi->bias_len < n) return fail(ctx, TG_ERR_SHAPE, "bias is too short");
+    if (epi && epi->act > TG_ACT_SILU) return fail(ctx, TG_ERR_ARG, "unknown activation");
+    if ((!a && k > 0) || !c) return fail(ctx, TG_ERR_NULL, "a or c is null");
+    const size_t from = type_bytes(type), to = type_bytes(c_type), need = tg::e4m3_work_bytes(m, k);
+    if (span(m, lda, k) > SIZE_MAX / 16 || span(m, ldc, n) > SIZE_MAX / 16)
+        return fail(ctx, TG_ERR_SHAPE, "a or c does not fit in memory");
+    if (reinterpret_cast<uintptr_t>(a) % from || reinterpret_cast<uintptr_t>(c) % to)
+        return fail(ctx, TG_ERR_ALIGN, "a and c must be aligned to their values");
+    if (need && (!workspace || workspace_len < need)) return fail(ctx, TG_ERR_SHAPE, "workspace is too small");
+    if (need && reinterpret_cast<uintptr_t>(workspace) % 16) return fail(ctx, TG_ERR_ALIGN, "workspace must be 16-byte aligned");
+    const size_t a_bytes = span(m, lda, k) * from, c_bytes = span(m, ldc, n) * to;
+    if (ranges_overlap(a, a_bytes, c, c_bytes)) return fail(ctx, TG_ERR_ARG, "c must not overlap a");
+    if (need && (ranges_overlap(workspace, need, a, a_bytes) || ranges_overlap(workspace, need, c, c_bytes)))
+        return fail(ctx, TG_ERR_ARG, "workspace must not overlap a or c");
+    if (!ctx) return TG_ERR_NULL;
+    if (w->device != ctx->device) return fail(ctx, TG_ERR_ARG, "the weights live on another device");
+    const tg::E4m3Out o{c, ldc, m, n, c_type, reinterpret_cast<uintptr_t>(c) % (4 * to) == 0 && ldc % 4 == 0,
+                        epi_args(epi, nullptr, false)};
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    const hipError_t e = tg::launch_e4m3_product(type, a, lda, k, w->d, o, workspace, ctx->stream);
+    if (e == hipErrorInvalidConfiguration) return fail(ctx, TG_ERR_UNSUPPORTED, "more tiles than a launch holds");
+    TG_HIP(ctx, e);
+    return TG_OK;
 }
 
 int tg_cache_append_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type,

@@ -34,6 +34,21 @@ float float_of(uint32_t b) {
     return f;
 }
 
+// A value of at most 448 (half a step past it rounds to it) in e4m3, to nearest, ties to even: with 2^E <= |x| < 2^(E + 1)
+// its grid's step is 2^(E - 3), or 2^-9 below 2^-6; m steps are m itself below that, else (E + 6) 8 + m (a carry goes to the
+// next exponent's first value).
+uint8_t to_e4m3(double x) {
+    const uint8_t sign = std::signbit(x) ? 0x80 : 0;
+    const double v = std::fmin(std::fabs(x), 448.0);
+    int E = -6;
+    if (v >= std::ldexp(1.0, -6)) {
+        (void)std::frexp(v, &E);
+        E--;
+    }
+    const int m = (int)std::nearbyint(std::ldexp(v, 3 - E));
+    return sign | (uint8_t)(m < 8 ? m : (E + 6) * 8 + m);
+}
+
 // f32 to IEEE half, rounding to nearest even (src/quant.rs:91-127), worked out on the value
 // rather than its bits: a finite |x| with binary exponent E (x = f 2^E, 0.5 <= f < 1) sits on the
 // half grid of step 2^(E - 11), or 2^-24 below the normal range; rint (nearest, ties to even in the
@@ -143,6 +158,27 @@ void tg_random(float *out, size_t len, uint64_t seed) {
         s ^= s << 17;
         out[i] = (float)(s >> 40) * (1.0f / 16777216.0f) * 2.0f - 1.0f;
     }
+}
+
+int tg_encode_e4m3(const float *w, size_t n, size_t k, uint8_t *values, size_t values_len, float *scales, size_t n_scales) {
+    constexpr size_t BLOCK = 128;
+    const size_t kb = div_ceil(k, BLOCK);
+    if ((n && k > SIZE_MAX / n) || values_len != n * k || n_scales != div_ceil(n, BLOCK) * kb) return TG_ERR_ARG;
+    if (n * k && (!w || !values || !scales)) return TG_ERR_NULL;
+    for (size_t i = 0; i < n * k; i++)
+        if (!std::isfinite(w[i])) return TG_ERR_ARG;
+    for (size_t o0 = 0; o0 < n; o0 += BLOCK)
+        for (size_t b = 0; b < kb; b++) {
+            const size_t o1 = o0 + BLOCK < n ? o0 + BLOCK : n, i0 = b * BLOCK, i1 = i0 + BLOCK < k ? i0 + BLOCK : k;
+            float top = 0.0f;
+            for (size_t o = o0; o < o1; o++)
+                for (size_t i = i0; i < i1; i++) top = std::fmax(top, std::fabs(w[o * k + i]));
+            const float scale = top == 0.0f ? 1.0f : std::fmax(top / 448.0f, std::ldexp(1.0f, -120));
+            scales[o0 / BLOCK * kb + b] = scale;
+            for (size_t o = o0; o < o1; o++)
+                for (size_t i = i0; i < i1; i++) values[o * k + i] = to_e4m3((double)w[o * k + i] / (double)scale);
+        }
+    return TG_OK;
 }
 
 int tg_encode(const float *w, size_t n, size_t k, uint32_t precision, uint8_t *values, size_t values_len,

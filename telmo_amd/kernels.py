@@ -66,6 +66,10 @@ class Precision(enum.IntEnum):
         return bool(_lib.lib().tg_fits(int(self), k))
 
 
+# The types of rows, by their torch names.
+_ROW_TYPES = {"torch.float32": int(Precision.F32), "torch.float16": int(Precision.F16), "torch.bfloat16": int(Precision.BF16)}
+
+
 class Act(enum.IntEnum):
     NONE = 0
     RELU = 1
@@ -196,6 +200,94 @@ class PackedWeights:
             self.close()
         except Exception:
             pass
+
+
+class E4m3Weights:
+    """A matrix of n outputs and k inputs in eight bits (e4m3) with an f32 scale for each block of 128 outputs by 128
+    inputs, uploaded once to the context's device, for Kernels.linear_e4m3_device."""
+
+    def __init__(self, kernels: "Kernels", handle, n: int, k: int):
+        self._kernels = kernels
+        self._handle = handle
+        self._n, self._k = n, k
+
+    @staticmethod
+    def from_parts(kernels: "Kernels", values, scales):
+        """Host numpy arrays: uint8 values [n, k] and float32 scales [ceil(n / 128), ceil(k / 128)]."""
+        values = np.ascontiguousarray(values, np.uint8)
+        n, k = values.shape
+        sc = _f32(np.ascontiguousarray(scales, np.float32))
+        out = ctypes.c_void_p()
+        rc = _lib.lib().tg_weights_e4m3_upload(kernels._ctx, values.ctypes.data_as(ctypes.c_void_p), values.size, k,
+                                               sc.ctypes.data_as(ctypes.c_void_p), sc.size, n, k, ctypes.byref(out))
+        _check(rc, kernels._ctx)
+        return E4m3Weights(kernels, out, n, k)
+
+    @staticmethod
+    def from_device(kernels: "Kernels", values, scales):
+        """from_parts on GPU tensors; values float8_e4m3fn (or uint8, the same bytes), rows at any stride."""
+        import torch
+
+        if values.dim() != 2 or values.dtype not in (torch.float8_e4m3fn, torch.uint8):
+            raise TypeError(f"values must be float8_e4m3fn or uint8 [n, k], not {values.dtype}")
+        n, k = values.shape
+        if values.stride(1) != 1 and k > 1:
+            raise ValueError("a row's values must be contiguous")
+        for t, name in ((values, "values"), (scales, "scales")):
+            if t.get_device() != kernels.device:
+                raise TypeError(f"{name} must be a tensor on the context's GPU {kernels.device}, not on {t.device}")
+        if tuple(scales.shape) != (-(-n // 128), -(-k // 128)):
+            raise ValueError(f"scales must be [{-(-n // 128)}, {-(-k // 128)}]")
+        # The tensors may still be on their way on torch's stream; the upload reads them on the context's.
+        torch.cuda.current_stream(kernels.device).synchronize()
+        ld = values.stride(0) if n > 1 else k
+        out = ctypes.c_void_p()
+        rc = _lib.lib().tg_weights_e4m3_upload_device(kernels._ctx, values.data_ptr(), (n - 1) * ld + k if n else 0, ld,
+                                                      _dev(scales, "float32", "scales"), _len(scales, None, "scales"), n, k,
+                                                      ctypes.byref(out))
+        _check(rc, kernels._ctx)
+        return E4m3Weights(kernels, out, n, k)
+
+    @staticmethod
+    def encode(kernels: "Kernels", rows, n: int, k: int):
+        """Rounds row-major [n, k] f32 rows (host): each block's scale is its largest |w| / 448."""
+        return E4m3Weights.from_parts(kernels, *encode_e4m3(rows, n, k))
+
+    def n(self) -> int:
+        return self._n
+
+    def k(self) -> int:
+        return self._k
+
+    def bytes(self) -> int:
+        return _lib.lib().tg_weights_e4m3_bytes(self._handle)
+
+    def workspace_bytes(self, m: int) -> int:
+        """Bytes of workspace that a product of m rows needs (0 up to 16)."""
+        return _lib.lib().tg_linear_e4m3_workspace_bytes(m, self._k)
+
+    def close(self) -> None:
+        if self._handle:
+            _lib.lib().tg_weights_e4m3_free(self._handle)
+            self._handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+def encode_e4m3(rows, n: int, k: int):
+    """Row-major f32 rows in e4m3: (values uint8 [n, k], scales float32 [ceil(n / 128), ceil(k / 128)])."""
+    rows = _f32(np.ascontiguousarray(rows, np.float32).reshape(-1))
+    if rows.size != n * k:
+        raise ValueError("rows must hold n * k values")
+    values, scales = np.zeros((n, k), np.uint8), np.zeros((-(-n // 128), -(-k // 128)), np.float32)
+    rc = _lib.lib().tg_encode_e4m3(rows.ctypes.data_as(ctypes.c_void_p), n, k, values.ctypes.data_as(ctypes.c_void_p),
+                                   values.size, scales.ctypes.data_as(ctypes.c_void_p), scales.size)
+    _check(rc, None)
+    return values, scales
 
 
 def encode(rows, n: int, k: int, precision: Precision):
@@ -331,6 +423,35 @@ class Kernels:
 
     def linear_device(self, a, m: int, w: PackedWeights, c, epi: Epilogue = Epilogue.PLAIN):
         self.matmul_device(a, w.k(), m, w, c, w.n(), epi)
+
+    def linear_e4m3_device(self, a, w: E4m3Weights, c, epi: Optional[Epilogue] = Epilogue.PLAIN, workspace=None):
+        """c = epi(a w^T) with weights in e4m3 and a's rows rounded to e4m3 in groups of 128 inputs
+        (tg_linear_e4m3_device): GPU tensors a [m, k] and c [m, n] of float32, float16 or bfloat16 each, rows at any stride.
+        workspace: a GPU tensor of w.workspace_bytes(m) bytes, for more than 16 rows."""
+        args = []
+        for t, width, name in ((a, w.k(), "a"), (c, w.n(), "c")):
+            p = _ROW_TYPES.get(str(t.dtype))
+            if p is None:
+                raise TypeError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+            if t.get_device() != self.device:
+                raise TypeError(f"{name} must be a tensor on the context's GPU {self.device}, not on {t.device}")
+            shape, stride = t.shape, t.stride()
+            if len(shape) != 2 or shape[1] != width or shape[0] != a.shape[0]:
+                raise ValueError(f"{name} must be [{a.shape[0]}, {width}], not {list(shape)}")
+            if stride[1] != 1 and width > 1:
+                raise ValueError(f"{name}: a row's values must be contiguous")
+            ld = stride[0] if shape[0] > 1 else width
+            args.append((p, t.data_ptr(), (shape[0] - 1) * ld + width if shape[0] else 0, ld))
+        space, space_len = None, 0
+        if workspace is not None:
+            if workspace.get_device() != self.device or not workspace.is_contiguous():
+                raise ValueError("workspace must be a contiguous tensor on the context's GPU")
+            space, space_len = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        (at, ap, an, lda), (ct, cp, cn, ldc) = args
+        rc = _lib.lib().tg_linear_e4m3_device(self._ctx, at, ap, an, lda, a.shape[0], w._handle, ct, cp, cn, ldc,
+                                              self._epi_dev(epi), space, space_len)
+        if rc:
+            _check(rc, self._ctx)
 
     def linear_glu_device(self, a, m: int, w: PackedWeights, out, ldo: Optional[int] = None,
                           epi: Epilogue = Epilogue.PLAIN, a_len: Optional[int] = None,

@@ -69,3 +69,80 @@ def test_null_caches():
     assert _lib.lib().tg_attention_paged_e4m3_device(None, a, None) == NULL
     assert _lib.lib().tg_attention_paged_e4m3_device(None, None, c) == NULL
     assert _lib.lib().tg_cache_append_e4m3_device(None, a, None, 0, rows(AT * 30, 20, 2, 64), rows(AT * 31, 20, 2, 64), None) == NULL
+
+
+def upload(L, n=200, k=300, values=AT, values_len=None, ldv=300, scales=AT * 2, n_scales=6, out=True, device=True):
+    import ctypes
+
+    handle = ctypes.c_void_p()
+    f = L.tg_weights_e4m3_upload_device if device else L.tg_weights_e4m3_upload
+    return f(None, values, 199 * ldv + k if values_len is None else values_len, ldv, scales, n_scales, n, k,
+             ctypes.byref(handle) if out else None)
+
+
+@pytest.mark.parametrize("device", (True, False))
+@pytest.mark.parametrize("kw,code", [
+    ({}, OK), (dict(out=False), NULL), (dict(n=(1 << 24) + 1), UNSUPPORTED), (dict(k=(1 << 24) + 1), UNSUPPORTED), (dict(ldv=299), SHAPE),
+    (dict(values_len=199 * 300 + 299), SHAPE), (dict(n_scales=5), SHAPE), (dict(values=0), NULL), (dict(scales=0), NULL),
+    (dict(scales=AT + 2), ALIGN), (dict(n=201, ldv=1 << 60), SHAPE),
+])
+def test_uploads_of_e4m3_weights(kw, code, device):
+    from telmo_amd import _lib
+
+    assert upload(_lib.lib(), device=device, **kw) == code
+
+
+def test_products_without_weights():
+    """A product's other refusals need weights, which need a GPU (test_gpu_e4m3_refusals.py)."""
+    from telmo_amd import _lib
+
+    L = _lib.lib()
+    assert L.tg_linear_e4m3_device(None, 0, AT, 100, 10, 10, None, 0, AT * 2, 100, 10, None, None, 0) == NULL
+    L.tg_weights_e4m3_free(None)
+    assert L.tg_weights_e4m3_n(None) == L.tg_weights_e4m3_k(None) == L.tg_weights_e4m3_bytes(None) == 0
+
+
+@pytest.mark.parametrize("m,k,want", ((0, 100, 0), (16, 4096, 0), (17, 128, 2 * 2048 + 2 * 64 + 1024), (33, 640, 3 * 5 * 2048 + 2 * 3 * 64 + 1024),
+                                      ((1 << 24) + 1, 128, 0), (128, (1 << 24) + 1, 0)))
+def test_workspaces_of_products(m, k, want):
+    from telmo_amd import _lib
+
+    assert _lib.lib().tg_linear_e4m3_workspace_bytes(m, k) == want
+
+
+def test_encoding_refuses_what_is_not_finite_and_wrong_lengths():
+    import ctypes
+
+    import numpy as np
+
+    from telmo_amd import TelmoError, _lib, encode_e4m3
+
+    with pytest.raises(TelmoError):
+        encode_e4m3(np.array([1.0, np.nan], np.float32), 1, 2)
+    with pytest.raises(TelmoError):
+        encode_e4m3(np.array([1.0, -np.inf], np.float32), 2, 1)
+    with pytest.raises(ValueError):
+        encode_e4m3(np.zeros(5, np.float32), 2, 3)
+    w, v, s = np.zeros(6, np.float32), np.zeros(6, np.uint8), np.zeros(1, np.float32)
+    at = [x.ctypes.data_as(ctypes.c_void_p) for x in (w, v, s)]
+    assert _lib.lib().tg_encode_e4m3(at[0], 2, 3, at[1], 5, at[2], 1) == ARG
+    assert _lib.lib().tg_encode_e4m3(at[0], 2, 3, at[1], 6, at[2], 2) == ARG
+    assert _lib.lib().tg_encode_e4m3(None, 2, 3, at[1], 6, at[2], 1) == NULL
+
+
+def test_encoding_rounds_to_nearest():
+    """Every value of a block, and points between and beside neighbours, against the definition."""
+    import numpy as np
+
+    from e4m3_oracle import VALUES, encode
+    from telmo_amd import encode_e4m3
+
+    grid = VALUES[:127]
+    x = np.concatenate([grid, (grid[1:] + grid[:-1]) / 2, (grid[1:] + grid[:-1]) / 2 * (1 + 2.0**-20), (grid[1:] + grid[:-1]) / 2 * (1 - 2.0**-20)])
+    x = np.concatenate([x, -x]).astype(np.float32)
+    codes, scales = encode_e4m3(x, 1, x.size)
+    for b in range(scales.shape[1]):
+        part = x[128 * b:128 * b + 128].astype(np.float64)
+        assert np.array_equal(codes[0, 128 * b:128 * b + 128], encode(np.clip(part / float(scales[0, b]), -448, 448)))
+    zeros, one = encode_e4m3(np.zeros(130, np.float32), 130, 1)
+    assert not zeros.any() and np.all(one == 1.0)
