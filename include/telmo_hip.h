@@ -483,6 +483,31 @@ int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t 
 int tg_cache_append_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type,
                                 tg_rows k_new, tg_rows v_new, const tg_rotary *rotary);
 
+/* ---- drawing tokens ---------------------------------------------------------------------------
+ * A token of each row of logits l from a given random number u, where decode_inner takes the largest logit. With w_i =
+ * e^((l_i - max) / temperature) and the tokens in the order of falling logits, equal ones by their numbers: the first top_k
+ * stay, of those the ones before which less than top_p of their weights lie, of those the ones with w >= min_p, the first
+ * one always. The token is the first at which the running sum of those that stay exceeds u times the whole of it, its
+ * probability its weight over that. Weights and sums are held in 64 bits. Temperature 0 (or less, or NaN): the largest
+ * logit, probability 1. NaN and -infinity are never drawn, +infinity shares the row with its like; a row of none gives
+ * token -1, probability 0. */
+typedef struct {
+    float temperature;          /* for all rows: finite, not negative */
+    int32_t top_k;              /* 0: all */
+    float top_p, min_p;         /* 0 to 1; 1 and 0: all */
+    const float *temperatures;  /* device, a value for each row instead, or null */
+    const int32_t *top_ks;
+    const float *top_ps, *min_ps;
+    size_t temperatures_len, top_ks_len, top_ps_len, min_ps_len;
+} tg_sampling;
+/* logits: rows of n (at most 2^22) of `type` (TG_F32, TG_F16 or TG_BF16), ld apart. uniforms: a number from 0 up to 1 for
+ * each row. probs may be null. Device pointers, queued on the context's stream; nothing is allocated. workspace: device,
+ * 16-byte aligned, tg_sample_workspace_bytes(rows, n) bytes (0 for short rows), not shared with calls that may overlap. */
+int tg_sample_device(tg_ctx *ctx, uint32_t type, const void *logits, size_t logits_len, size_t ld, size_t rows, size_t n,
+                     const tg_sampling *options, const float *uniforms, size_t uniforms_len, int32_t *tokens, size_t tokens_len,
+                     float *probs, size_t probs_len, void *workspace, size_t workspace_len);
+size_t tg_sample_workspace_bytes(size_t rows, size_t n);
+
 /* ---- the TDT decoder (src/parakeet.rs:1412-1577) --------------------------------------------
  * Parakeet's prediction network (embedding, LSTM layers, projection) and joint, decoded greedily
  * with every step on the device. The matrices are tg_weights of int8 or Q8_0 values. The network

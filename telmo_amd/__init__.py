@@ -7,6 +7,7 @@ from .attention import Attention, PagedCache, Rotary, rotary_frequencies
 from .kernels import (Act, E4m3Weights, Epilogue, Kernels, PackedWeights, Precision, TdtDecoder, TelmoError, Token, decode,
                       encode, encode_e4m3, random)
 from .pack import Pack
+from .sampling import Sampler
 
-__all__ = ["Act", "Attention", "E4m3Weights", "Epilogue", "Kernels", "Pack", "PackedWeights", "PagedCache", "Precision", "Rotary",
+__all__ = ["Act", "Attention", "E4m3Weights", "Epilogue", "Kernels", "Pack", "PackedWeights", "PagedCache", "Precision", "Rotary", "Sampler",
            "TdtDecoder", "TelmoError", "Token", "decode", "encode", "encode_e4m3", "random", "rotary_frequencies"]

@@ -63,6 +63,13 @@ class CacheE4m3(ctypes.Structure):
                 ("v_page", _sz), ("block", _sz)]
 
 
+class Sampling(ctypes.Structure):
+    """tg_sampling."""
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float), ("temperatures", _p), ("top_ks", _p), ("top_ps", _p), ("min_ps", _p),
+                ("temperatures_len", _sz), ("top_ks_len", _sz), ("top_ps_len", _sz), ("min_ps_len", _sz)]
+
+
 _szp = ctypes.POINTER(_sz)
 
 # name: (restype, argtypes), in the order of include/telmo_hip.h
@@ -126,6 +133,9 @@ SIGNATURES = {
                                               ctypes.POINTER(RotaryDesc)]),
     "tg_cache_append_e4m3_device": (ctypes.c_int, [_p, ctypes.POINTER(AttentionDesc), ctypes.POINTER(CacheE4m3), _u32,
                                                    Rows, Rows, ctypes.POINTER(RotaryDesc)]),
+    "tg_sample_device": (ctypes.c_int, [_p, _u32, _p, _sz, _sz, _sz, _sz, ctypes.POINTER(Sampling), _p, _sz, _p, _sz, _p,
+                                        _sz, _p, _sz]),
+    "tg_sample_workspace_bytes": (_sz, [_sz, _sz]),
     "tg_tdt_create": (ctypes.c_int, [_p, _p, ctypes.POINTER(_p)]),
     "tg_tdt_destroy": (None, [_p]),
     "tg_tdt_max_rows": (_sz, [_p]),

@@ -1552,6 +1552,7 @@ namespace {
 
 constexpr size_t MAX_ATTN_ROWS = (size_t)1 << 30;  // rows, keys and strides that the kernels count in 32 bits
 constexpr size_t MAX_E4M3 = (size_t)1 << 24;       // rows, inputs and outputs of a product in e4m3
+constexpr size_t MAX_SAMPLE_ROWS = (size_t)1 << 20, MAX_SAMPLE_TOKENS = (size_t)1 << 22;
 constexpr size_t MAX_ATTN_GRID = 65535;            // sequences and heads, each a grid dimension
 
 bool attn_type(uint32_t t) { return t == TG_F32 || t == TG_F16 || t == TG_BF16; }
@@ -2033,6 +2034,60 @@ int tg_linear_e4m3_device(tg_ctx *ctx, uint32_t type, const void *a, size_t a_le
     const hipError_t e = tg::launch_e4m3_product(type, a, lda, k, w->d, o, workspace, ctx->stream);
     if (e == hipErrorInvalidConfiguration) return fail(ctx, TG_ERR_UNSUPPORTED, "more tiles than a launch holds");
     TG_HIP(ctx, e);
+    return TG_OK;
+}
+
+size_t tg_sample_workspace_bytes(size_t rows, size_t n) {
+    return rows > MAX_SAMPLE_ROWS || n > MAX_SAMPLE_TOKENS ? 0 : tg::sample_work_bytes(rows, n);
+}
+
+int tg_sample_device(tg_ctx *ctx, uint32_t type, const void *logits, size_t logits_len, size_t ld, size_t rows, size_t n,
+                     const tg_sampling *options, const float *uniforms, size_t uniforms_len, int32_t *tokens, size_t tokens_len,
+                     float *probs, size_t probs_len, void *workspace, size_t workspace_len) {
+    if (!options) return fail(ctx, TG_ERR_NULL, "null options");
+    const tg_sampling &o = *options;
+    if (!attn_type(type)) return fail(ctx, TG_ERR_ARG, "type must be f32, f16 or bf16");
+    if (!(o.temperature >= 0.0f) || !std::isfinite(o.temperature))
+        return fail(ctx, TG_ERR_ARG, "temperature must be finite and not negative");
+    if (o.top_k < 0) return fail(ctx, TG_ERR_ARG, "top_k must not be negative");
+    if (!(o.top_p >= 0.0f && o.top_p <= 1.0f) || !(o.min_p >= 0.0f && o.min_p <= 1.0f))
+        return fail(ctx, TG_ERR_ARG, "top_p and min_p must lie from 0 to 1");
+    if (rows > MAX_SAMPLE_ROWS || n > MAX_SAMPLE_TOKENS)
+        return fail(ctx, TG_ERR_UNSUPPORTED, "at most 2^20 rows and 2^22 tokens");
+    if (rows == 0) return ctx ? TG_OK : TG_ERR_NULL;
+    if (ld < n) return fail(ctx, TG_ERR_SHAPE, "ld must be >= n");
+    if (logits_len < span(rows, ld, n)) return fail(ctx, TG_ERR_SHAPE, "logits is too short");
+    if (uniforms_len < rows || tokens_len < rows || (probs && probs_len < rows))
+        return fail(ctx, TG_ERR_SHAPE, "uniforms, tokens or probs is too short");
+    if ((o.temperatures && o.temperatures_len < rows) || (o.top_ks && o.top_ks_len < rows) || (o.top_ps && o.top_ps_len < rows) ||
+        (o.min_ps && o.min_ps_len < rows))
+        return fail(ctx, TG_ERR_SHAPE, "an option of each row is too short");
+    if ((n && !logits) || !uniforms || !tokens) return fail(ctx, TG_ERR_NULL, "logits, uniforms or tokens are null");
+    if (span(rows, ld, n) > SIZE_MAX / 16) return fail(ctx, TG_ERR_SHAPE, "logits do not fit in memory");
+    if (reinterpret_cast<uintptr_t>(logits) % type_bytes(type) || reinterpret_cast<uintptr_t>(uniforms) % 4 ||
+        reinterpret_cast<uintptr_t>(tokens) % 4 || reinterpret_cast<uintptr_t>(probs) % 4)
+        return fail(ctx, TG_ERR_ALIGN, "buffers must be aligned to their values");
+    const size_t need = tg::sample_work_bytes(rows, n), bytes = span(rows, ld, n) * type_bytes(type);
+    if (need && (!workspace || workspace_len < need)) return fail(ctx, TG_ERR_SHAPE, "workspace is too small");
+    if (need && reinterpret_cast<uintptr_t>(workspace) % 16) return fail(ctx, TG_ERR_ALIGN, "workspace must be 16-byte aligned");
+    const std::pair<const void *, size_t> written[] = {{tokens, rows * 4}, {probs, probs ? rows * 4 : 0}, {workspace, need}};
+    const std::pair<const void *, size_t> read[] = {{logits, bytes}, {uniforms, rows * 4}, {o.temperatures, o.temperatures ? rows * 4 : 0},
+                                                    {o.top_ks, o.top_ks ? rows * 4 : 0}, {o.top_ps, o.top_ps ? rows * 4 : 0},
+                                                    {o.min_ps, o.min_ps ? rows * 4 : 0}};
+    for (size_t i = 0; i < 3; i++) {
+        for (const auto &[p, size] : read)
+            if (ranges_overlap(written[i].first, written[i].second, p, size))
+                return fail(ctx, TG_ERR_ARG, "tokens, probs and workspace must not overlap what is read");
+        for (size_t j = 0; j < i; j++)
+            if (ranges_overlap(written[i].first, written[i].second, written[j].first, written[j].second))
+                return fail(ctx, TG_ERR_ARG, "tokens, probs and workspace must not overlap one another");
+    }
+    if (!ctx) return TG_ERR_NULL;
+    const tg::SampleArgs a{logits, (int64_t)ld, (int)n, o.temperature, o.top_p, o.min_p, o.top_k, o.temperatures, o.top_ps, o.min_ps,
+                           o.top_ks, uniforms, tokens, probs};
+    std::lock_guard<std::mutex> g(ctx->mu);
+    TG_HIP(ctx, hipSetDevice(ctx->device));
+    TG_HIP(ctx, tg::launch_sample(a, type, (int)rows, workspace, ctx->stream));
     return TG_OK;
 }
 

@@ -389,6 +389,23 @@ struct Cache8 {
 hipError_t launch_append8(const void *k, int64_t ldk, int64_t hsk, const void *v, int64_t ldv, int64_t hsv, uint32_t type,
                           const Cache8 &c, int heads, int d, const AttnSeqs &q, const RotaryArgs &r, hipStream_t s);
 
+// Drawing a token of each row of logits (kernels_sample.hip). Options for all rows, or (not null) a value for each.
+struct SampleArgs {
+    const void *logits;
+    int64_t ld;
+    int n;
+    float temperature, top_p, min_p;
+    int top_k;
+    const float *temperatures, *top_ps, *min_ps;
+    const int32_t *top_ks;
+    const float *uniforms;
+    int32_t *tokens;
+    float *probs;  // or null
+};
+constexpr size_t SAMPLE_WHOLE = 16384;  // tokens of a row that one workgroup draws from without a workspace
+size_t sample_work_bytes(size_t rows, size_t n);
+hipError_t launch_sample(const SampleArgs &a, uint32_t type, int rows, void *work, hipStream_t s);
+
 // The greedy TDT decode (kernels_tdt.hip). The control block lives in device memory; the host
 // writes it before a decode and reads it between batches of steps.
 constexpr int TDT_ROWS = 16;            // most frames the joint scores per step; rows of a prediction
