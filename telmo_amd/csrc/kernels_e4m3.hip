@@ -51,21 +51,19 @@ struct Operand<true> {
         }
     }
 };
-// 16 outputs by 16 rows of one block of inputs; rows' powers of two, where they are not in a yet, in byte Q of each lane's
-// word.
-template <int Q>
-__device__ __forceinline__ f32x4 block_product(const Operand<false> &w, const Operand<false> &a, uint32_t powers) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, f32x4{}, 0, 0, 0, 127, Q, (int)powers);
+// Read-only memory that is read by scalar loads.
+typedef const __attribute__((address_space(4))) float *Scalar;
+
+// Product i of 16 outputs by 16 rows of a block of inputs (EXACT: of four), added to `sum`; rows' powers of two, where they
+// are not in a yet, as e + 127 in each lane's row's.
+__device__ __forceinline__ f32x4 block_product(const Operand<false> &w, const Operand<false> &a, uint32_t power, int, f32x4 sum) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, sum, 0, 0, 0, 127, 0, (int)power);
 }
-template <int Q>
-__device__ __forceinline__ f32x4 block_product(const Operand<true> &w, const Operand<true> &a, uint32_t) {
-    f32x4 sum = {};
-#pragma unroll
-    for (int i = 0; i < 4; i++) sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a.v[i], sum, 0, 0, 0);
-    return sum;
+__device__ __forceinline__ f32x4 block_product(const Operand<true> &w, const Operand<true> &a, uint32_t, int i, f32x4 sum) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a.v[i], sum, 0, 0, 0);
 }
-// Byte q of a word of powers, e + 127 each, as 2^e.
-__device__ __forceinline__ float power_of(uint32_t powers, int q) { return __uint_as_float((powers >> 8 * q & 255u) << 23); }
+// e + 127 as 2^e.
+__device__ __forceinline__ float power_of(uint32_t power) { return __uint_as_float(power << 23); }
 __device__ __forceinline__ i32x8 joined(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 __device__ __forceinline__ float max_of_quarters(float x) {
@@ -117,26 +115,18 @@ __device__ __forceinline__ i32x8 round_rows(const T *a, size_t lda, size_t row, 
     return r;
 }
 
-// The rows' fragments and, for each four blocks of inputs, the powers of two of 16 rows' blocks, a byte each.
+// The rows' fragments and powers of two, a wavefront for 16 rows of a block of inputs at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void round_rows_kernel(const T *a, size_t lda, size_t m, size_t k, bool aligned, Rounded to) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const size_t tiles = to.tiles;
-    // A wavefront takes four blocks of 16 rows: one word of powers for each row.
-    for (size_t u = (size_t)blockIdx.x * 4 + wave; u < tiles * to.quads; u += (size_t)gridDim.x * 4) {
-        const size_t tile = u / to.quads, quad = u % to.quads, row = tile * 16 + (lane & 15);
-        uint32_t powers = 0;
-        for (int q = 0; q < 4; q++) {
-            const size_t b = quad * 4 + q;
-            if (b >= to.blocks) break;
-            int e;
-            const i32x8 r = round_rows(a, lda, row, row < m, b, k, aligned, lane >> 4, e);
-            i32x4 *out = reinterpret_cast<i32x4 *>(to.values + (tile * to.blocks + b) * 2048 + lane * 16);
-            out[0] = __builtin_shufflevector(r, r, 0, 1, 2, 3);
-            out[64] = __builtin_shufflevector(r, r, 4, 5, 6, 7);
-            powers |= (uint32_t)(e + 127) << 8 * q;
-        }
-        if (lane < 16) to.powers[(quad * tiles + tile) * 16 + lane] = powers;
+    for (size_t u = (size_t)blockIdx.x * 4 + wave; u < to.tiles * to.blocks; u += (size_t)gridDim.x * 4) {
+        const size_t tile = u / to.blocks, b = u % to.blocks, row = tile * 16 + (lane & 15);
+        int e;
+        const i32x8 r = round_rows(a, lda, row, row < m, b, k, aligned, lane >> 4, e);
+        i32x4 *out = reinterpret_cast<i32x4 *>(to.values + u * 2048 + lane * 16);
+        out[0] = __builtin_shufflevector(r, r, 0, 1, 2, 3);
+        out[64] = __builtin_shufflevector(r, r, 4, 5, 6, 7);
+        if (lane < 16) reinterpret_cast<uint8_t *>(to.powers + (b / 4 * to.tiles + tile) * 16 + lane)[b % 4] = (uint8_t)(e + 127);
     }
 }
 
@@ -155,38 +145,73 @@ __global__ __launch_bounds__(256) void weights_kernel(const uint8_t *src, size_t
 
 // ------------------------------------------------------------------------------------------- outputs
 
-// Four outputs of a row, from column n on, through the epilogue.
-__device__ __forceinline__ void store4(const E4m3Out &o, size_t row, size_t n, f32x4 v) {
-    float old[4] = {};
-    const size_t at = row * o.ld + n;
-    const int count = o.n - n < 4 ? (int)(o.n - n) : 4;
-    const bool whole = count == 4 && o.aligned;
-    const auto type = [&](auto t) {
-        using U = decltype(t);
-        typedef U u4 __attribute__((ext_vector_type(4)));
-        U *c = static_cast<U *>(o.c) + at;
-        if (o.epi.accumulate) {
-            if (whole) {
-                const u4 x = *reinterpret_cast<const u4 *>(c);
-                for (int e = 0; e < 4; e++) old[e] = (float)x[e];
-            } else {
-                for (int e = 0; e < count; e++) old[e] = (float)c[e];
-            }
-        }
-        u4 y;
-        for (int e = 0; e < 4; e++)
-            y[e] = (U)epilogue_vals(v[e], o.epi.bias != nullptr, o.epi.bias && e < count ? o.epi.bias[n + e] : 0.0f, o.epi.act,
-                                    o.epi.scale, o.epi.accumulate, old[e]);
-        if (whole) {
-            *reinterpret_cast<u4 *>(c) = y;
-        } else {
-            for (int e = 0; e < count; e++) c[e] = y[e];
-        }
-    };
-    if (o.type == F32) type(float{});
-    else if (o.type == F16) type(_Float16{});
-    else type(__bf16{});
+// v / (1 + e^-v) to 2^-21 of itself: the exponent's product with log2 e in two parts, the hardware's 2^x and reciprocal.
+// The row kernels' SiLU, with their polynomial and division, takes 40 operations an output, as long as a product of 400
+// inputs. e^-v is cut at 2^126, whose reciprocal is f32's smallest normal number.
+__device__ __forceinline__ float silu(float v) {
+    constexpr float L = 1.44269504088896340736f, REST = 1.92596299112661746887e-8f;  // log2 e = L + REST
+    const float t = -L * v, low = __builtin_fmaf(-L, v, -t) - REST * v;
+    const float e = fminf(__builtin_amdgcn_exp2f(t) * __builtin_fmaf(low, 0.69314718055994530942f, 1.0f), 0x1p126f);
+    return v * __builtin_amdgcn_rcpf(1.0f + e);
 }
+// The epilogue of a lane's rows of four outputs, from column n on. The bias is loaded and waited for once, and what the call
+// says is held in scalar registers: waiting for a load of each row's own would wait for the store of the row before.
+struct Outputs {
+    const E4m3Out &o;
+    size_t n;
+    int count;  // outputs of the four that there are
+    uint32_t type, act, accumulate;
+    float scale;
+    f32x4 bias;
+    bool whole;  // every lane has four outputs or none, which lie aligned, and takes no old ones
+    __device__ __forceinline__ Outputs(const E4m3Out &o_, size_t n_) : o(o_), n(n_) {
+        count = n >= o.n ? 0 : o.n - n < 4 ? (int)(o.n - n) : 4;
+        type = __builtin_amdgcn_readfirstlane(o.type);
+        act = __builtin_amdgcn_readfirstlane(o.epi.act);
+        accumulate = __builtin_amdgcn_readfirstlane(o.epi.accumulate);
+        scale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(o.epi.scale)));
+        whole = o.aligned && o.n % 4 == 0 && !accumulate;
+        bias = f32x4{};
+        if (o.epi.bias)
+            for (int e = 0; e < 4; e++) bias[e] = e < count ? o.epi.bias[n + e] : 0.0f;
+        asm volatile("s_waitcnt vmcnt(0)" : "+v"(bias));
+    }
+    __device__ __forceinline__ f32x4 finished(f32x4 v) const {
+        if (o.epi.bias) v += bias;
+        if (act == ACT_RELU) {
+            for (int e = 0; e < 4; e++) v[e] = v[e] > 0.0f ? v[e] : 0.0f;
+        } else if (act == ACT_SILU) {
+            for (int e = 0; e < 4; e++) v[e] = silu(v[e]);
+        }
+        return v * scale;
+    }
+    // f(row in type U) as the outputs' type wants it.
+    template <typename F>
+    __device__ __forceinline__ void typed(F f) const {
+        if (type == F32) f(float{});
+        else if (type == F16) f(_Float16{});
+        else f(__bf16{});
+    }
+    // A row where `whole` holds.
+    template <typename U>
+    __device__ __forceinline__ void store_whole(size_t row, f32x4 v) const {
+        typedef U u4 __attribute__((ext_vector_type(4)));
+        v = finished(v);
+        u4 y;
+        for (int e = 0; e < 4; e++) y[e] = (U)v[e];
+        if (row < o.m && count) *reinterpret_cast<u4 *>(static_cast<U *>(o.c) + row * o.ld + n) = y;
+    }
+    // Any row.
+    __device__ __forceinline__ void store(size_t row, f32x4 v) const {
+        if (row >= o.m) return;
+        v = finished(v);
+        typed([&](auto u) {
+            using U = decltype(u);
+            U *c = static_cast<U *>(o.c) + row * o.ld + n;
+            for (int e = 0; e < count; e++) c[e] = (U)(accumulate ? (float)c[e] + v[e] : v[e]);
+        });
+    }
+};
 
 // ------------------------------------------------------------------------------------- few rows
 
@@ -208,13 +233,20 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
     const uint8_t *wp[PN];
     for (int p = 0; p < PN; p++) wp[p] = w.values + (size_t)min(panel0 + p, (int)w.panels - 1) * blocks * 2048 + lane * 16;
     const float *scale = w.scales + (size_t)(panel0 / 8) * blocks;
-    for (int b = b0; b < b1; b++) {
-        i32x8 wf[PN];
+    // The next block's weights are on their way while a block is multiplied.
+    i32x8 wf[PN], next[PN];
+    const auto load = [&](int b) {
 #pragma unroll
         for (int p = 0; p < PN; p++) {
             const i32x4 *at = reinterpret_cast<const i32x4 *>(wp[p] + (size_t)b * 2048);
-            wf[p] = joined(at[0], at[64]);
+            next[p] = joined(at[0], at[64]);
         }
+    };
+    if (b0 < b1) load(b0);
+    for (int b = b0; b < b1; b++) {
+#pragma unroll
+        for (int p = 0; p < PN; p++) wf[p] = next[p];
+        load(b + 1 < b1 ? b + 1 : b);
         const auto panel = [&](int p) { return Operand<true>(wf[p], 1.0f); };
         const float s = scale[b];
 #pragma unroll
@@ -230,12 +262,15 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
                 const size_t tile = min(tile0 + t, (int)in.tiles - 1);
                 const i32x4 *at = reinterpret_cast<const i32x4 *>(in.values + (tile * blocks + b) * 2048 + lane * 16);
                 af = joined(at[0], at[64]);
-                up = power_of(in.powers[((size_t)(b / 4) * in.tiles + tile) * 16 + (lane & 15)], b % 4);
+                up = power_of(reinterpret_cast<const uint8_t *>(in.powers + ((size_t)(b / 4) * in.tiles + tile) * 16 + (lane & 15))[b % 4]);
             }
             const Operand<true> rows(af, up);
 #pragma unroll
             for (int p = 0; p < PN; p++) {
-                const f32x4 part = block_product<0>(panel(p), rows, 0);
+                const Operand<true> outs = panel(p);
+                f32x4 part = {};
+#pragma unroll
+                for (int i = 0; i < 4; i++) part = block_product(outs, rows, 0, i, part);
 #pragma unroll
                 for (int e = 0; e < 4; e++) acc[t][p][e] = __builtin_fmaf(part[e], s, acc[t][p][e]);
             }
@@ -263,11 +298,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
     __syncthreads();
     for (int y = threadIdx.x; y < MT * PN * 64; y += 64 * FEW_WAVES) {
         const int l = y % 64, t = y / 64 / PN, p = y / 64 % PN;
-        const size_t row = (size_t)(tile0 + t) * 16 + (l & 15), n = (size_t)(panel0 + p) * 16 + (l >> 4) * 4;
-        if (row >= o.m || n >= o.n) continue;
         f32x4 v = sums[0][t * PN + p][l];
         for (int s = 1; s < SLOTS; s++) v += sums[s][t * PN + p][l];
-        store4(o, row, n, v);
+        Outputs(o, (size_t)(panel0 + p) * 16 + (l >> 4) * 4).store((size_t)(tile0 + t) * 16 + (l & 15), v);
     }
 }
 
@@ -284,19 +317,32 @@ __device__ __forceinline__ void copy_to_lds(const uint8_t *base, uint32_t voff, 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(voff), "s"(base) : "memory", "m0");
 #pragma clang diagnostic pop
 }
-__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+// The same of 64 lanes x 4 bytes.
+__device__ __forceinline__ void copy_words_to_lds(const uint8_t *base, uint32_t voff, uint32_t lds) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds), "v"(voff), "s"(base) : "memory", "m0");
+#pragma clang diagnostic pop
+}
+// Until at most N of the wavefront's copies are on their way.
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    static_assert(N < 64, "vmcnt holds 6 bits");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
 
-// Workgroups of WM x WN wavefronts of TM x TN tiles each. Two stages of a block of inputs in LDS: while one is worked on,
-// the next is copied to the other.
-template <int WM, int WN, int TM, int TN, bool EXACT>
-__global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Rounded in, E4m3Panels w, E4m3Out o, int m_tiles, int n_tiles) {
-    constexpr int WAVES = WM * WN, RT = WM * TM, PT = WN * TN;  // row tiles and panels of the workgroup
-    constexpr int CHUNKS = 2 * (RT + PT), STAGE = CHUNKS * 1024;
-    static_assert(CHUNKS % WAVES == 0 && RT <= 16 && 8 % TN == 0, "");
+// Workgroups of KG groups of WM x WN wavefronts of TM x TN tiles each. The groups share the outputs and take every KG-th
+// block of inputs, and add up their sums in LDS. LDS holds two stages of a block for each group: while one is worked on, the
+// next is copied to the other.
+template <int WM, int WN, int TM, int TN, int KG, bool EXACT>
+__global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, E4m3Panels w, E4m3Out o, int m_tiles, int n_tiles) {
+    constexpr int WAVES = WM * WN, RT = WM * TM, PT = WN * TN;     // wavefronts, row tiles and panels of a group
+    constexpr int CHUNKS = 2 * (RT + PT), STAGE = (CHUNKS + 1) * 1024;  // fragments, and 16 row tiles' powers
+    static_assert(CHUNKS % WAVES == 0 && RT <= 16 && 8 % TN == 0 && WAVES >= 4 && TM % KG == 0, "");
     constexpr int CPW = CHUNKS / WAVES;
-    __shared__ __align__(16) uint8_t smem[2 * STAGE + 2 * 1024];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int wm = wave % WM, wn = wave / WM;
+    __shared__ __align__(16) uint8_t smem[2 * KG * STAGE];
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = all_waves / WAVES, wave = all_waves % WAVES, wm = wave % WM, wn = wave / WM;
     // Neighbours in a grid of tiles, eight tile rows at a time, share an XCD's L2.
     int id = blockIdx.x;
     {
@@ -306,7 +352,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Rounded in, E4m3P
     const int band = id / (8 * n_tiles), in_band = id - band * 8 * n_tiles, high = min(8, m_tiles - band * 8);
     const int mt = band * 8 + in_band % high, nt = in_band / high;
     const int tile0 = mt * RT, panel0 = nt * PT;
-    const int blocks = (int)w.blocks;
+    const int blocks = (int)w.blocks, steps = (blocks + KG - 1) / KG;
 
     const uint8_t *from[CPW];
 #pragma unroll
@@ -315,87 +361,163 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void tile_kernel(Rounded in, E4m3P
         from[c] = x < RT ? in.values + (size_t)min(tile0 + x, (int)in.tiles - 1) * blocks * 2048 + ch % 2 * 1024
                          : w.values + (size_t)min(panel0 + x - RT, (int)w.panels - 1) * blocks * 2048 + ch % 2 * 1024;
     }
-    const uint32_t voff = lane * 16, lds0 = __builtin_amdgcn_readfirstlane(lds_address(smem));
-    const auto issue = [&](int b) __attribute__((always_inline)) {
+    uint8_t *const mine = smem + group * STAGE;
+    const uint32_t voff = lane * 16, lds0 = __builtin_amdgcn_readfirstlane(lds_address(mine));
+    // The group's block of a step (past the last block that one again) to a stage, with the powers of its quad of blocks: of
+    // 16 row tiles, a quarter by each of four wavefronts; what lies behind the last tile's is not used. All wavefronts copy
+    // alike, without a branch, which would leave the compiler to move the products out of their place.
+    const auto issue = [&](int step, int stage) __attribute__((always_inline)) {
+        const int b = min(step * KG + group, blocks - 1);
 #pragma unroll
         for (int c = 0; c < CPW; c++)
-            copy_to_lds(from[c] + (size_t)b * 2048, voff, lds0 + (b & 1) * STAGE + (wave + c * WAVES) * 1024);
-        if (b % 4 == 0 && wave == 0)  // 16 row tiles' powers of four blocks; what lies behind the last tile's is not used
-            copy_to_lds(reinterpret_cast<const uint8_t *>(in.powers + ((size_t)(b / 4) * in.tiles + tile0) * 16), voff,
-                        lds0 + 2 * STAGE + (b / 4 & 1) * 1024);
+            copy_to_lds(from[c] + (size_t)b * 2048, voff, lds0 + stage * KG * STAGE + (wave + c * WAVES) * 1024);
+        copy_words_to_lds(reinterpret_cast<const uint8_t *>(in.powers + ((size_t)(b / 4) * in.tiles + tile0) * 16) + wave % 4 * 256,
+                          lane * 4, lds0 + stage * KG * STAGE + CHUNKS * 1024 + wave % 4 * 256);
     };
-    const float *scale = w.scales + (size_t)((panel0 + wn * TN) / 8) * blocks;
+    // A scalar load: one in a vector register would wait for the copies that left before it.
+    const Scalar scale = (Scalar)(w.scales + (size_t)((panel0 + wn * TN) / 8) * blocks);
 
     f32x4 acc[TM][TN] = {};
-    uint32_t powers[TM];
-    const auto work = [&](auto q, int b) __attribute__((always_inline)) {
-        const uint8_t *st = smem + (b & 1) * STAGE + lane * 16;
+    const auto work = [&](int b, int stage) __attribute__((always_inline)) {
+        const uint8_t *st = mine + stage * KG * STAGE + lane * 16;
         const auto fragment = [&](int x) {
             return joined(*reinterpret_cast<const i32x4 *>(st + x * 2048), *reinterpret_cast<const i32x4 *>(st + x * 2048 + 1024));
         };
-        if constexpr (q.value == 0)
+        uint32_t powers[TM];
 #pragma unroll
-            for (int t = 0; t < TM; t++)
-                powers[t] = *reinterpret_cast<const uint32_t *>(smem + 2 * STAGE + (b / 4 & 1) * 1024 + ((wm * TM + t) * 16 + (lane & 15)) * 4);
+        for (int t = 0; t < TM; t++)
+            powers[t] = mine[stage * KG * STAGE + CHUNKS * 1024 + ((wm * TM + t) * 16 + (lane & 15)) * 4 + (b & 3)];
         const float s = scale[b];
         const auto panel = [&](int p) { return Operand<EXACT>(fragment(RT + wn * TN + p), 1.0f); };
         static_assert(TN == 4, "");
         const Operand<EXACT> wf[TN] = {panel(0), panel(1), panel(2), panel(3)};
+        // While a row tile is multiplied the next one's fragment is read (EXACT: widened, and the one after it read), and the
+        // one before it added up.
+        const auto rows = [&](const i32x8 &bytes, int t) { return Operand<EXACT>(bytes, EXACT ? power_of(powers[t]) : 1.0f); };
+        constexpr int STEPS = EXACT ? 4 : 1;  // products of a block
+        f32x4 part[2][TN];
+        i32x8 bytes = fragment(wm * TM);
+        Operand<EXACT> af = rows(bytes, 0);
+        if (EXACT && TM > 1) bytes = fragment(wm * TM + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t <= TM; t++) {
+            const int now = t < TM ? t : 0;
+            const Operand<EXACT> multiplied = af;
+            if (EXACT ? t + 2 < TM : t + 1 < TM) {
+                const i32x8 next = fragment(wm * TM + t + (EXACT ? 2 : 1));
+                if (EXACT) af = rows(bytes, t + 1);
+                bytes = next;
+                if (!EXACT) af = rows(bytes, t + 1);
+            } else if (EXACT && t + 1 < TM) {
+                af = rows(bytes, t + 1);
+            }
+#pragma unroll
+            for (int i = 0; i < STEPS; i++)
+#pragma unroll
+                for (int p = 0; p < TN; p++) {
+                    if (t < TM) part[t & 1][p] = block_product(wf[p], multiplied, powers[now], i, i ? part[t & 1][p] : f32x4{});
+                    if (t > 0)
+#pragma unroll
+                        for (int e = 4 / STEPS * i; e < 4 / STEPS * (i + 1); e++)
+                            acc[t - 1][p][e] = __builtin_fmaf(part[(t - 1) & 1][p][e], s, acc[t - 1][p][e]);
+                }
+        }
 #pragma unroll
         for (int t = 0; t < TM; t++) {
-            const Operand<EXACT> af(fragment(wm * TM + t), EXACT ? power_of(powers[t], q.value) : 1.0f);
-            f32x4 part[TN];
+            if (t + (EXACT ? 2 : 1) < TM) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 #pragma unroll
-            for (int p = 0; p < TN; p++) part[p] = block_product<q.value>(wf[p], af, powers[t]);
-#pragma unroll
-            for (int p = 0; p < TN; p++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[t][p][e] = __builtin_fmaf(part[p][e], s, acc[t][p][e]);
+            for (int p = 0; p < TN * STEPS; p++) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (EXACT && t + 1 < TM) __builtin_amdgcn_sched_group_barrier(0x002, 1, 0);
+                if (t > 0) __builtin_amdgcn_sched_group_barrier(0x002, 4 / STEPS, 0);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);
     };
-    issue(0);
-    wait_copies();
-    const auto step = [&](auto q, int b) __attribute__((always_inline)) {
-        if (b >= blocks) return;
-        __syncthreads();  // stage b is there, and the one before it has been read
-        if (b + 1 < blocks) issue(b + 1);
-        work(q, b);
-        wait_copies();
+    issue(0, 0);
+    wait_copies<0>();
+    const auto step = [&](int i, int stage) __attribute__((always_inline)) {
+        __syncthreads();  // the step's blocks are there, and the ones before them have been read
+        issue(i + 1, stage ^ 1);
+        work(i * KG + group, stage);
+        wait_copies<0>();
     };
-    for (int b = 0; b < blocks; b += 4) {
-        step(std::integral_constant<int, 0>{}, b);
-        step(std::integral_constant<int, 1>{}, b + 1);
-        step(std::integral_constant<int, 2>{}, b + 2);
-        step(std::integral_constant<int, 3>{}, b + 3);
+    const int whole = blocks / KG;  // steps in which every group has a block
+    int i = 0;
+    for (; i + 2 <= whole; i += 2) {
+        step(i, 0);
+        step(i + 1, 1);
+    }
+    if (i < whole) step(i++, 0);
+    if (i < steps) {
+        __syncthreads();
+        if (i * KG + group < blocks) work(i * KG + group, i & 1);
+    }
+    __syncthreads();
+    // The groups' sums of a tile meet in one of them, a share of the tiles each.
+    constexpr int SHARE = TM / KG;
+    f32x4 sum[SHARE][TN];
+    if constexpr (KG == 2) {
+        f32x4 *const pass = reinterpret_cast<f32x4 *>(smem) + wave * SHARE * TN * 64 + lane;
+        static_assert(2 * WAVES * SHARE * TN * 1024 <= 2 * KG * STAGE, "");
+        constexpr int OTHER = WAVES * SHARE * TN * 64;
+#pragma unroll
+        for (int t = 0; t < SHARE; t++)
+#pragma unroll
+            for (int p = 0; p < TN; p++) {
+                if (group == 0) pass[(t * TN + p) * 64] = acc[SHARE + t][p];
+                else pass[OTHER + (t * TN + p) * 64] = acc[t][p];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < SHARE; t++)
+#pragma unroll
+            for (int p = 0; p < TN; p++) {
+                if (group == 0) sum[t][p] = acc[t][p] + pass[OTHER + (t * TN + p) * 64];
+                else sum[t][p] = pass[(t * TN + p) * 64] + acc[SHARE + t][p];
+            }
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int t = 0; t < TM; t++)
+#pragma unroll
+            for (int p = 0; p < TN; p++) sum[t][p] = acc[t][p];
     }
     // Two tiles' rows at a time go through the wavefront's own part of LDS, so that a row's outputs leave side by side.
-    constexpr int PITCH = TN * 16 + 4;
-    static_assert(WAVES * 32 * PITCH * 4 <= 2 * STAGE && TM % 2 == 0, "");
-    __syncthreads();
-    float *mine = reinterpret_cast<float *>(smem) + wave * 32 * PITCH;
+    constexpr int PITCH = TN * 16 + 4, PAIR = SHARE < 2 ? SHARE : 2;
+    static_assert(KG * WAVES * PAIR * 16 * PITCH * 4 <= 2 * KG * STAGE && SHARE % PAIR == 0, "");
+    const Outputs outputs(o, (size_t)(panel0 + wn * TN) * 16 + lane % 16 * 4);
+    static_assert(TN == 4, "a row's 64 outputs are 16 lanes'");
+    float *const turned = reinterpret_cast<float *>(smem) + all_waves * PAIR * 16 * PITCH;
 #pragma unroll
-    for (int t = 0; t < TM; t += 2) {
+    for (int t = 0; t < SHARE; t += PAIR) {
 #pragma unroll
-        for (int x = 0; x < 2; x++)
+        for (int x = 0; x < PAIR; x++)
 #pragma unroll
             for (int p = 0; p < TN; p++)
-                *reinterpret_cast<f32x4 *>(mine + (x * 16 + (lane & 15)) * PITCH + p * 16 + (lane >> 4) * 4) = acc[t + x][p];
+                *reinterpret_cast<f32x4 *>(turned + (x * 16 + (lane & 15)) * PITCH + p * 16 + (lane >> 4) * 4) = sum[t + x][p];
         __builtin_amdgcn_wave_barrier();
+        const size_t row = (size_t)(tile0 + wm * TM + group * SHARE + t) * 16 + lane / 16;
+        const auto value = [&](int y) { return *reinterpret_cast<const f32x4 *>(turned + (y * 4 + lane / 16) * PITCH + lane % 16 * 4); };
+        if (outputs.whole) {
+            outputs.typed([&](auto u) {
+#pragma unroll
+                for (int y = 0; y < PAIR * 4; y++) outputs.template store_whole<decltype(u)>(row + y * 4, value(y));
+            });
+        } else {
 #pragma unroll 1
-        for (int y = lane; y < 32 * TN * 4; y += 64) {
-            const int r = y / (TN * 4), c = y % (TN * 4) * 4;
-            const size_t row = (size_t)(tile0 + wm * TM + t) * 16 + r, n = (size_t)(panel0 + wn * TN) * 16 + c;
-            if (row < o.m && n < o.n) store4(o, row, n, *reinterpret_cast<const f32x4 *>(mine + r * PITCH + c));
+            for (int y = 0; y < PAIR * 4; y++) outputs.store(row + y * 4, value(y));
         }
         __builtin_amdgcn_wave_barrier();
     }
 }
 
-template <int WM, int WN, int TM, int TN, bool EXACT>
+template <int WM, int WN, int TM, int TN, int KG, bool EXACT>
 hipError_t launch_tiles(const Rounded &in, const E4m3Panels &w, const E4m3Out &o, hipStream_t s) {
     const size_t m_tiles = div_ceil(in.tiles, WM * TM), n_tiles = div_ceil(w.panels, WN * TN);
     if (m_tiles * n_tiles > INT32_MAX / 1024) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL((tile_kernel<WM, WN, TM, TN, EXACT>), dim3((unsigned)(m_tiles * n_tiles)), dim3(64 * WM * WN), 0, s, in, w, o,
+    hipLaunchKernelGGL((tile_kernel<WM, WN, TM, TN, KG, EXACT>), dim3((unsigned)(m_tiles * n_tiles)), dim3(64 * WM * WN * KG), 0, s, in, w, o,
                        (int)m_tiles, (int)n_tiles);
     return hipGetLastError();
 }
@@ -411,21 +533,35 @@ hipError_t launch_few(const T *a, size_t lda, size_t k, bool aligned, const Roun
 template <typename T>
 hipError_t product(const T *a, size_t lda, size_t k, const E4m3Panels &w, const E4m3Out &o, const Rounded &in, hipStream_t s) {
     const bool aligned = reinterpret_cast<uintptr_t>(a) % 16 == 0 && lda * sizeof(T) % 16 == 0;
-    if (!k) return launch_few<float, 4, 4, false>(nullptr, 0, k, aligned, in, w, o, s);  // the epilogue of empty sums
+    if (!k) return launch_few<float, 2, 2, false>(nullptr, 0, k, aligned, in, w, o, s);  // the epilogue of empty sums
     if (o.m <= E4M3_FEW) {
-        if (w.panels >= 1024) return launch_few<T, 1, 4, true>(a, lda, k, aligned, in, w, o, s);
+        // Two panels share the rounding of the rows where that leaves two workgroups to a CU (us, one panel and two): 16 rows
+        // by 4096 x 16384 30.5 20.9, one by 8192 x 8192 29.9 26.4, by 4096 x 4096 11.3 11.8.
+        if (w.panels >= 512) return launch_few<T, 1, 2, true>(a, lda, k, aligned, in, w, o, s);
         return launch_few<T, 1, 1, true>(a, lda, k, aligned, in, w, o, s);
     }
-    const size_t units = in.tiles * in.quads, blocks = div_ceil(units, 4);
+    const size_t units = in.tiles * in.blocks, blocks = div_ceil(units, 4);
     hipLaunchKernelGGL((round_rows_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, a, lda, o.m,
                        k, aligned, in);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const size_t large = div_ceil(in.tiles, 16) * div_ceil(w.panels, 16), middle = div_ceil(in.tiles, 8) * div_ceil(w.panels, 8);
-    if (large >= 256 && o.type != F32) return launch_tiles<2, 4, 8, 4, false>(in, w, o, s);
-    if (middle >= 128 && o.type != F32) return launch_tiles<2, 2, 4, 4, false>(in, w, o, s);
-    if (middle >= 128) return launch_tiles<2, 2, 4, 4, true>(in, w, o, s);
-    return launch_few<float, 4, 4, false>(nullptr, 0, k, aligned, in, w, o, s);
+    // Tiles of 128 x 128 by one group of wavefronts where those fill the 256 CUs twice over, by two groups where they fill
+    // half of them, and blocks spread over eight wavefronts below that (us of a call; one group, two, 64 x 32 outputs and
+    // 32 x 32 by eight wavefronts): 4000 rows by 4096 x 4096 145, 165, 206, 235; 1500 by 1024 x 4096 (384 tiles) 29.6,
+    // 33.2, 39.6, 40.3; 2000 by 2048 x 2048 (256) 32.5, 29.9, 39.3, 42.1; 750 by 1024 x 4096 (192) 21.7, 20.3, 23.3, 24.4;
+    // 256 by 4096 x 4096 (64) 44.0, 38.6, 21.0, 22.7; 750 by 4096 x 1024 (48) 46.2, 41.0, 22.3, 21.1; 64 by 4096 x 4096
+    // 42.7, 37.6, 13.4, 11.2. 16-bit outputs: tiles of 256 x 256 where those fill the CUs.
+    const size_t tiles = div_ceil(in.tiles, 8) * div_ceil(w.panels, 8);  // of 128 x 128
+    if (o.type != F32) {
+        if (div_ceil(in.tiles, 16) * div_ceil(w.panels, 16) >= 256) return launch_tiles<2, 4, 8, 4, 1, false>(in, w, o, s);
+        if (tiles > 256) return launch_tiles<2, 2, 4, 4, 1, false>(in, w, o, s);
+        if (tiles >= 96) return launch_tiles<2, 2, 4, 4, 2, false>(in, w, o, s);
+    } else {
+        if (tiles > 256) return launch_tiles<2, 2, 4, 4, 1, true>(in, w, o, s);
+        if (tiles >= 128) return launch_tiles<2, 2, 4, 4, 2, true>(in, w, o, s);
+    }
+    if (div_ceil(in.tiles, 4) * div_ceil(w.panels, 2) >= 512) return launch_few<float, 4, 2, false>(nullptr, 0, k, aligned, in, w, o, s);
+    return launch_few<float, 2, 2, false>(nullptr, 0, k, aligned, in, w, o, s);
 }
 
 }  // namespace
