@@ -3,14 +3,17 @@
 // predecessors' weights reach top_p of what is left, then before the first one with w < min_p; the first always stays. The
 // token is the first one whose running sum exceeds u times the sum of those kept.
 //
-// Nothing is sorted but what lies next to a border. Weights are whole numbers of 2^-42 (the largest is 1), so that
-// their sums do not depend on their order, and are added into bins of the logits: 32 for each factor of two of the
-// weight, 64 factors, the last one for all that is smaller. Their running counts and sums say in which bin each border
-// lies; that bin's tokens are then gathered, sorted and added up in 64 bits. A bin with more tokens than LDS sorts is first
-// divided by its logits' bits, down to a single value, whose tokens differ in their numbers alone.
+// Nothing is sorted but what lies next to a border. Tokens are counted and their weights added in bins of the logits: 32 for
+// each factor of two of the weight, 64 factors, the last one (of weight 0 in these sums) for all that is smaller. A bin's
+// sum is of 2^(y - floor y) - 1 with y = 32 l log2 e / temperature, in whole numbers of 2^-40, so that it depends neither
+// on the order nor on the row's largest logit; one 64-bit atomic counts a token and adds its weight. The running counts and
+// sums say in which bins each border and the drawn token can lie; the tokens of these bins are gathered in one pass,
+// sorted, and added up in 64 bits. If they are more than LDS sorts, the borders are looked for one after the other, and a
+// bin of too many tokens is first divided by its logits' bits, down to a single value, whose tokens differ in their
+// numbers alone.
 //
-// Rows of up to WHOLE tokens are the work of one workgroup. Longer ones are read in parts by as many workgroups, each of
-// which leaves its bins, counted from its own largest logit, for the row's workgroup to add up.
+// Rows of up to WHOLE tokens are the work of one workgroup, which holds them in registers. Longer ones are read in parts by
+// as many workgroups, each of which leaves its bins, counted from its own largest logit, for the row's workgroup.
 #include "tg_internal.hpp"
 
 namespace tg {
@@ -20,21 +23,23 @@ namespace {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int BINS = 2048, PER_OCTAVE = 32;
 constexpr int LIST = 4096;  // tokens that are sorted at a time
-constexpr int PART_THREADS = 512, PART_VALUES = 64, PART = PART_THREADS * PART_VALUES;
+constexpr int WHOLE = (int)SAMPLE_WHOLE, WHOLE_VALUES = WHOLE / THREADS;
+constexpr int PART_THREADS = 256, PART_VALUES = 64, PART = PART_THREADS * PART_VALUES;
+constexpr int COPIES = 2;     // of the bins that are counted: lanes next to each other add to different ones
+constexpr int SUM_BITS = 49;  // of a counted bin; above them the count of up to 2^14 tokens, whose sum is below 2^48.5
+static_assert(WHOLE <= 1 << 14 && PART <= 1 << 14, "a bin's count and sum share 64 bits");
 constexpr double FIXED = 1024.0;  // added to a weight it leaves steps of 2^-42: 2^22 weights' sum fits 64 bits
 
-// What a part of a row leaves: its bins' counts and sums, relative to its largest logit.
+// What a part of a row leaves: its bins up to the last one that has tokens, relative to its largest logit.
 struct PartBins {
-    uint64_t mass[BINS];
-    uint32_t count[BINS];
+    uint64_t bins[BINS];
     float top;  // -infinity: no token
-    uint32_t pad[3];
+    int used;
+    uint32_t tokens, pad;
 };
 
-template <typename T>
-__device__ __forceinline__ float logit(const T *row, int i) {
-    return (float)row[i];
-}
+// Zeros of either sign are one logit.
+__device__ __forceinline__ float plain(float l) { return l == 0.0f ? 0.0f : l; }
 // A logit as bits that order as it does, larger first: 0 for +infinity.
 __device__ __forceinline__ uint32_t key_of(float l) {
     const uint32_t b = __float_as_uint(l);
@@ -44,8 +49,6 @@ __device__ __forceinline__ float logit_of(uint32_t key) {
     const uint32_t o = ~key;
     return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-// Zeros of either sign are one logit.
-__device__ __forceinline__ float plain(float l) { return l == 0.0f ? 0.0f : l; }
 
 // 2^t for t <= 0 to 2^-47 of itself: Taylor's polynomial of e^x for |x| <= ln 2 / 2.
 __device__ __forceinline__ double exp2_64(double t) {
@@ -66,7 +69,7 @@ __device__ __forceinline__ double exp2_64(double t) {
     return __builtin_ldexp(p, (int)n);
 }
 
-// The row's scale of weights: c = log2 e / temperature.
+// The row's scale of weights: c = log2 e / temperature, y = 32 c l.
 struct Weights {
     double c;
     float top;  // the largest logit
@@ -81,26 +84,73 @@ struct Weights {
         const double b = top_bin - bin_edge(l);
         return b < BINS - 1 ? (int)b : BINS - 1;  // a difference of infinities too
     }
+    // y - floor y, with the product's rounding error: from 0 to 1. (Where y has no fraction left, the logits next to l lie
+    // in other bins far away, and 0 or 1 is the same for all of l's own; 0 for infinity.)
+    __device__ __forceinline__ double fraction(float l) const {
+        const double k = PER_OCTAVE * c, y = (double)l * k, low = __builtin_fma((double)l, k, -y);
+        return fmin(fmax((y - __builtin_floor(y)) + low, 0.0), 1.0);
+    }
+    // 2^(f / 32) - 1 in steps of 2^-40, by Taylor's polynomial up to x^6 (the next one is below 2^-50).
+    static __device__ __forceinline__ uint64_t fixed_share(double f) {
+        const double x = f * (0.69314718055994530942 / PER_OCTAVE);
+        double p = 1.0 / 720.0;
+        p = __builtin_fma(p, x, 1.0 / 120.0);
+        p = __builtin_fma(p, x, 1.0 / 24.0);
+        p = __builtin_fma(p, x, 1.0 / 6.0);
+        p = __builtin_fma(p, x, 0.5);
+        p = __builtin_fma(p, x, 1.0);
+        return (uint64_t)(__builtin_bit_cast(int64_t, __builtin_fma(p, x, 0x1p12)) - __builtin_bit_cast(int64_t, 0x1p12));
+    }
+    __device__ __forceinline__ void count_in(float l, uint64_t *bins) const {
+        const int b = bin(l);
+        const uint64_t share = b == BINS - 1 ? 0 : fixed_share(fraction(l));
+        atomicAdd(reinterpret_cast<unsigned long long *>(&bins[b * COPIES + (threadIdx.x & (COPIES - 1))]),
+                  (unsigned long long)(share + ((uint64_t)1 << SUM_BITS)));
+    }
 };
 
 __device__ __forceinline__ uint64_t fixed(double w) {
     return (uint64_t)(__builtin_bit_cast(int64_t, w + FIXED) - __builtin_bit_cast(int64_t, FIXED));
 }
 __device__ __forceinline__ double unfixed(uint64_t m) { return (double)m * 0x1p-42; }
-// A sum of a part's weights, times the part's largest one.
-__device__ __forceinline__ uint64_t fixed_times(uint64_t m, double share) {
-    return share == 1.0 ? m : (uint64_t)((double)m * share + 0.5);
-}
 
-__device__ __forceinline__ void count_in(const Weights &w, float l, uint32_t *count, uint64_t *mass) {
-    const int b = w.bin(l);
-    atomicAdd(&count[b], 1u);
-    atomicAdd(reinterpret_cast<unsigned long long *>(&mass[b]), (unsigned long long)fixed(w.of(l)));
+// N logits from row[first] on, wherever they lie; -infinity past the n-th of the row.
+template <int N, typename T>
+__device__ __forceinline__ void load(const T *row, int first, int n, float (&l)[N]) {
+    constexpr int PIECE = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Piece {
+        T v[PIECE];
+    };
+    static_assert(N % PIECE == 0, "whole pieces");
+    if (first + N <= n) {
+#pragma unroll
+        for (int i = 0; i < N; i += PIECE) {
+            const Piece x = *reinterpret_cast<const Piece *>(row + first + i);
+#pragma unroll
+            for (int y = 0; y < PIECE; y++) l[i + y] = plain((float)x.v[y]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) l[i] = first + i < n ? plain((float)row[first + i]) : -INFINITY;
+    }
 }
 
 __device__ __forceinline__ float wave_max(float x) {
     for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
     return x;
+}
+
+// The first of n <= 4096 numbers where f holds, n where none does; f holds from there on. By each wavefront for itself.
+template <typename F>
+__device__ __forceinline__ int first_of(int n, F f) {
+    const int lane = threadIdx.x & 63;
+    int low = 0;
+    for (int step = n > 64 ? 64 : 1;; step = 1) {
+        const int at = low + step * (lane + 1) - 1;  // the last number of the lane's step
+        const unsigned long long which = __ballot(at >= n || f(at));
+        low += step * (which ? (int)__builtin_ctzll(which) : 64);
+        if (step == 1 || low >= n) return low < n ? low : n;
+    }
 }
 
 // Running sums of bins.
@@ -113,14 +163,27 @@ struct Bins {
         for (int b = threadIdx.x; b < BINS; b += THREADS) count[b] = 0, fixed_mass()[b] = 0;
         __syncthreads();
     }
+    // The first bin where f(bin, running count, running mass) holds, or the last one that has tokens. (Between bins without
+    // any, sums may grow by a rounding: then the bin before them.)
+    template <typename F>
+    __device__ __forceinline__ int first(uint32_t before, double mass_before, F f) const {
+        const int b = first_of(BINS, [&](int x) { return f(x, before + count[x], mass_before + mass[x]); });
+        if (b < BINS && count[b] > (b ? count[b - 1] : 0u)) return b;
+        const uint32_t c = max(count[min(b, BINS - 1)], 1u);
+        return first_of(BINS, [&](int x) { return count[x] >= c; });
+    }
 };
 
 // What all threads of a row's workgroup share.
 struct Shared {
     Bins row;
     union {
-        Bins part;            // what a bin of too many tokens is divided into, before
-        uint64_t list[LIST];  // its tokens: logit's key and number
+        uint64_t counted[BINS * COPIES];
+        Bins part;  // what a bin of too many tokens is divided into, before
+        struct {
+            uint64_t list[LIST];  // its tokens: logit's key and number
+            double before[LIST];  // the weights of those before in the list
+        };
     };
     double wave_mass[WAVES];
     uint32_t wave_count[WAVES];
@@ -199,22 +262,140 @@ struct Range {
     double mass_before;
 };
 
-template <typename T>
-struct Row {
-    const T *logits;
+// A row's logits: held in registers (HELD), or read again for each pass.
+template <typename T, bool HELD>
+struct Logits {
+    static constexpr int PIECE = 16 / sizeof(T), PIECES = HELD ? WHOLE_VALUES / PIECE : 4;
+    const T *row;
     int n;
-    Weights w;
-    Shared &s;
+    float held[HELD ? PIECES : 1][PIECE];
 
+    __device__ __forceinline__ Logits(const T *row_, int n_) : row(row_), n(n_) {
+        if constexpr (HELD) read(held, 0);
+    }
+    __device__ __forceinline__ static int first(int piece) { return (piece * THREADS + (int)threadIdx.x) * PIECE; }
+    __device__ __forceinline__ void read(float (&l)[PIECES][PIECE], int begin) const {
+#pragma unroll
+        for (int x = 0; x < PIECES; x++) load(row, begin + first(x), n, l[x]);
+    }
     // f(logit, token) for the row's tokens; NaN and -infinity are none.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < n; i += THREADS) {
-            const float l = plain(logit(logits, i));
-            if (l > -INFINITY) f(l, i);
+        if constexpr (HELD) {
+            visit(held, 0, f);
+        } else {
+            for (int begin = 0; begin < n; begin += PIECES * THREADS * PIECE) {
+                float l[PIECES][PIECE];
+                read(l, begin);
+                visit(l, begin, f);
+            }
         }
     }
+    template <typename F>
+    __device__ __forceinline__ void visit(const float (&l)[PIECES][PIECE], int begin, F f) const {
+#pragma unroll
+        for (int x = 0; x < PIECES; x++)
+#pragma unroll
+            for (int y = 0; y < PIECE; y++)
+                if (l[x][y] > -INFINITY) f(l[x][y], begin + first(x) + y);
+    }
+};
+
+// Bins next to each other whose tokens are gathered: their place in the list, and the tokens and weights before them.
+struct Span {
+    int low, high, start = 0, count = 0;
+    uint32_t before = 0;
+    double mass_before = 0.0;
+    __device__ __forceinline__ bool holds(int bin) const { return bin >= low && bin <= high; }
+};
+
+// The row's options.
+struct Chosen {
+    float temperature, top_p, min_p;
+    int top_k;
+    __device__ __forceinline__ Chosen(const SampleArgs &a, int row) {
+        temperature = a.temperatures ? a.temperatures[row] : a.temperature;
+        top_k = a.top_ks ? a.top_ks[row] : a.top_k;
+        top_p = a.top_ps ? a.top_ps[row] : a.top_p;
+        min_p = a.min_ps ? a.min_ps[row] : a.min_p;
+    }
+    // A single token stays.
+    __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f) || top_k == 1 || top_p <= 0.0f; }
+};
+
+struct Drawn {
+    int token;
+    float prob;
+};
+
+// The first tokens of s.list in order.
+__device__ __forceinline__ void sort_list(Shared &s, int count) {
+    __syncthreads();
+    if (count <= THREADS / 4) {  // four lanes count the tokens before one
+        const int i = threadIdx.x / 4;
+        const uint64_t own = i < count ? s.list[i] : 0;
+        int place = 0;
+        if (i < count)
+            for (int y = threadIdx.x & 3; y < count; y += 4) place += s.list[y] < own;
+        place += __shfl_xor(place, 1);
+        place += __shfl_xor(place, 2);
+        __syncthreads();
+        if (i < count && (threadIdx.x & 3) == 0) s.list[place] = own;
+        __syncthreads();
+        return;
+    }
+    int size = 2;
+    while (size < count) size *= 2;
+    for (int i = count + threadIdx.x; i < size; i += THREADS) s.list[i] = ~0ull;
+    for (int block = 2; block <= size; block *= 2)
+        for (int step = block / 2; step; step /= 2) {
+            // Up to 64 apart a wavefront's pairs are its own from the last step on.
+            if (step > 32 || block == 2) __syncthreads();
+            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"), __builtin_amdgcn_wave_barrier();
+            for (int i = threadIdx.x; i < size / 2; i += THREADS) {
+                const int a = 2 * i - (i & (step - 1)), b = a + step;
+                const uint64_t x = s.list[a], y = s.list[b];
+                if ((x > y) == ((a & block) == 0)) s.list[a] = y, s.list[b] = x;
+            }
+        }
+    __syncthreads();
+}
+
+// The tokens of the spans in s.list, in order, and the weights before each.
+template <typename T, bool HELD>
+__device__ __forceinline__ void gather(const Logits<T, HELD> &logits, const Weights &w, Shared &s, const Span &x, const Span &y, const Span &z, int count) {
+    __syncthreads();  // the counted bins lie where the list does
+    if (threadIdx.x == 0) s.listed = 0;
+    __syncthreads();
+    // Logits that may lie in a span, a little more than its own.
+    const auto least_of = [&](const Span &x) {
+        const float l = x.high >= BINS - 1 ? -INFINITY : (float)((w.top_bin - x.high) / (PER_OCTAVE * w.c));
+        return l - (l < INFINITY ? fabsf(l) * 0x1p-20f : 0.0f);
+    };
+    const auto most_of = [&](const Span &x) {
+        const float l = x.low <= 0 ? INFINITY : (float)((w.top_bin - x.low + 1.0) / (PER_OCTAVE * w.c));
+        return l + fabsf(l) * 0x1p-20f;
+    };
+    const float x0 = least_of(x), x1 = most_of(x), y0 = least_of(y), y1 = most_of(y), z0 = least_of(z), z1 = most_of(z);
+    logits.each([&](float l, int i) {
+        if (!((l >= x0 && l <= x1) || (l >= y0 && l <= y1) || (l >= z0 && l <= z1))) return;
+        const int bin = w.bin(l);
+        if (!(x.holds(bin) || y.holds(bin) || z.holds(bin))) return;
+        const uint32_t at = atomicAdd(&s.listed, 1u);
+        if (at < LIST) s.list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
+    });
+    sort_list(s, count);
+    running<LIST / THREADS>(
+        s, [&](int i, uint32_t &c, double &m) { c = 0, m = i < count ? w.of(logit_of((uint32_t)(s.list[i] >> 32))) : 0.0; },
+        [&](int i, uint32_t, double with, double own) { s.before[i] = with - own; });
+    __syncthreads();
+}
+
+template <typename T>
+struct Row {
+    const Logits<T, false> logits;
+    Weights w;
+    Shared &s;
 
     // Counts and fixed weights become running sums.
     __device__ __forceinline__ void sum(Bins &bins) const {
@@ -225,21 +406,11 @@ struct Row {
         __syncthreads();
     }
 
-    // The first bin where f(bin, running count, running mass) holds, or the last one that has tokens; counts and masses
+    // The bin that has tokens where f(bin, running count, running mass) first holds, or the last one; counts and masses
     // after r's.
     template <typename F>
     __device__ __forceinline__ int first_bin(const Bins &bins, F f, Range &r) const {
-        int x = INT32_MAX;
-        for (int i = BINS / THREADS - 1; i >= 0; i--) {
-            const int b = threadIdx.x * (BINS / THREADS) + i;
-            if (f(b, r.before + bins.count[b], r.mass_before + bins.mass[b])) x = b;
-        }
-        int b = least(s, x);
-        if (b == INT32_MAX) {
-            for (int i = BINS / THREADS - 1; i >= 0; i--)
-                if (bins.count[threadIdx.x * (BINS / THREADS) + i] == bins.count[BINS - 1]) x = threadIdx.x * (BINS / THREADS) + i;
-            b = least(s, x);
-        }
+        const int b = bins.first(r.before, r.mass_before, f);
         const uint32_t earlier = b ? bins.count[b - 1] : 0u;
         r.count = bins.count[b] - earlier;
         r.before += earlier;
@@ -271,7 +442,7 @@ struct Row {
             int shift = 0;  // keys of a part: 2^shift
             while ((r.high - r.low) >> shift >= BINS) shift++;
             s.part.clear();
-            each([&](float l, int) {
+            logits.each([&](float l, int) {
                 const uint32_t key = key_of(l);
                 if (key < r.low || key > r.high) return;
                 const uint32_t b = (key - r.low) >> shift;
@@ -295,25 +466,13 @@ struct Row {
         __syncthreads();
         if (threadIdx.x == 0) s.listed = 0;
         __syncthreads();
-        each([&](float l, int i) {
+        logits.each([&](float l, int i) {
             const uint32_t key = key_of(l);
             if (key < r.low || key > r.high) return;
             const uint32_t at = atomicAdd(&s.listed, 1u);
             if (at < LIST) s.list[at] = (uint64_t)key << 32 | (uint32_t)i;
         });
-        int size = 2;
-        while (size < (int)r.count) size *= 2;
-        for (int i = r.count + threadIdx.x; i < size; i += THREADS) s.list[i] = ~0ull;
-        for (int block = 2; block <= size; block *= 2)
-            for (int step = block / 2; step; step /= 2) {
-                __syncthreads();
-                for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-                    const int a = 2 * i - (i & (step - 1)), b = a + step;
-                    const uint64_t x = s.list[a], y = s.list[b];
-                    if ((x > y) == ((a & block) == 0)) s.list[a] = y, s.list[b] = x;
-                }
-            }
-        __syncthreads();
+        sort_list(s, (int)r.count);
     }
 
     // The first token of the range where f(rank, mass before, weight) holds: its place in the range (the range's count where
@@ -363,9 +522,9 @@ struct Row {
         if (r.count <= LIST) return (int)(uint32_t)s.list[place];
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         uint32_t seen = 0;
-        for (int i0 = 0; i0 < n && seen <= (uint32_t)place; i0 += THREADS) {
+        for (int i0 = 0; i0 < logits.n && seen <= (uint32_t)place; i0 += THREADS) {
             const int i = i0 + threadIdx.x;
-            const bool mine = i < n && key_of(plain(logit(logits, i))) == r.low;
+            const bool mine = i < logits.n && key_of(plain((float)logits.row[i])) == r.low;
             const unsigned long long which = __ballot(mine);
             __syncthreads();
             if (lane == 0) s.wave_count[wave] = (uint32_t)__builtin_popcountll(which);
@@ -380,98 +539,24 @@ struct Row {
     }
 };
 
-// The row's options.
-struct Chosen {
-    float temperature, top_p, min_p;
-    int top_k;
-    __device__ __forceinline__ Chosen(const SampleArgs &a, int row) {
-        temperature = a.temperatures ? a.temperatures[row] : a.temperature;
-        top_k = a.top_ks ? a.top_ks[row] : a.top_k;
-        top_p = a.top_ps ? a.top_ps[row] : a.top_p;
-        min_p = a.min_ps ? a.min_ps[row] : a.min_p;
-    }
-    // A single token stays.
-    __device__ __forceinline__ bool greedy() const { return !(temperature > 0.0f) || top_k == 1 || top_p <= 0.0f; }
-};
-
+// The borders one after the other, by their bins' tokens alone or parts of them.
 template <typename T>
-__device__ float row_top(const T *logits, int n, Shared &s) {
-    float top = -INFINITY;
-#pragma unroll 8
-    for (int i = threadIdx.x; i < n; i += THREADS) top = fmaxf(top, logit(logits, i));  // NaN is passed over
-    top = wave_max(top);
-    if ((threadIdx.x & 63) == 0) s.wave_top[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = s.wave_top[0];
-    for (int x = 1; x < WAVES; x++) top = fmaxf(top, s.wave_top[x]);
-    return plain(top);
-}
-
-template <typename T>
-__global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, const PartBins *parts, int part_count) {
-    __shared__ Shared s;
-    const int r = blockIdx.x;
-    const T *logits = static_cast<const T *>(a.logits) + (int64_t)r * a.ld;
-    const Chosen o(a, r);
-    float top = -INFINITY;
-    if (parts) {
-        parts += (size_t)r * part_count;
-        for (int p = 0; p < part_count; p++) top = fmaxf(top, parts[p].top);
-    } else {
-        top = row_top(logits, a.n, s);
-    }
-    const auto answer = [&](int token, float prob) {
-        if (threadIdx.x == 0) {
-            a.tokens[r] = token;
-            if (a.probs) a.probs[r] = prob;
-        }
-    };
-    if (!(top > -INFINITY)) return answer(-1, 0.0f);
-    if (o.greedy()) {
-        int x = INT32_MAX;
-        for (int i = threadIdx.x; i < a.n && x == INT32_MAX; i += THREADS)
-            if (plain(logit(logits, i)) == top) x = i;
-        return answer(least(s, x), 1.0f);
-    }
-    const Row<T> row{logits, a.n, Weights(o.temperature, top), s};
-    const Weights &w = row.w;
-    s.row.clear();
-    if (parts) {
-        // A part's bins, counted from its own largest logit, lie `by` bins further on, the last one taking all past it.
-        for (int p = 0; p < part_count; p++) {
-            const PartBins &x = parts[p];
-            if (!(x.top > -INFINITY)) continue;
-            const double by = x.top == top ? 0.0 : w.top_bin - w.bin_edge(x.top), share = w.of(x.top);
-            const int on = by < BINS - 1 ? (int)by : BINS - 1;
-            for (int y = threadIdx.x; y < BINS; y += THREADS) {
-                const uint32_t count = x.count[y];
-                if (!count) continue;
-                const int b = y + on < BINS - 1 ? y + on : BINS - 1;
-                atomicAdd(&s.row.count[b], count);
-                atomicAdd(reinterpret_cast<unsigned long long *>(&s.row.fixed_mass()[b]), (unsigned long long)fixed_times(x.mass[y], share));
-            }
-        }
-    } else {
-        row.each([&](float l, int) { count_in(w, l, s.row.count, s.row.fixed_mass()); });
-    }
-    row.sum(s.row);
-    const uint32_t all = s.row.count[BINS - 1];
-    uint32_t kept = o.top_k > 0 && (uint32_t)o.top_k < all ? (uint32_t)o.top_k : all;
+__device__ __noinline__ Drawn step_by_step(const T *logits, int n, Weights w, Shared &s, uint32_t k, uint32_t all, double u, double share, double least_weight) {
+    const Row<T> row{Logits<T, false>(logits, n), w, s};
+    uint32_t kept = k;
     double mass = s.row.mass[BINS - 1], weight;
-    if (kept < all) {
-        const uint32_t k = kept;
+    if (k < all) {
         const Range x = row.range_of({}, [&](bool, uint32_t c, double) { return c > k; });
         row.first_token(x, [&](uint32_t rank, double, double) { return rank >= k; }, mass, weight);
     }
-    if (o.top_p < 1.0f || o.min_p > 0.0f) {
-        const double most = o.top_p < 1.0f ? (double)o.top_p * mass : INFINITY, least_weight = o.min_p;
-        const uint32_t k = kept;
+    if (share < INFINITY || least_weight > 0.0) {
+        const double most = share * mass;
         typename Row<T>::Floor floor;
-        if (o.min_p > 0.0f) {
+        if (least_weight > 0.0) {
             __syncthreads();
             if (threadIdx.x < 64) {
                 const uint32_t end = key_of(-INFINITY);
-                const uint32_t key = first_key(key_of(top), end, [&](uint32_t y) { return w.of(plain(logit_of(y))) < least_weight; });
+                const uint32_t key = first_key(key_of(w.top), end, [&](uint32_t y) { return w.of(plain(logit_of(y))) < least_weight; });
                 if (threadIdx.x == 0) s.keys[0] = key, s.first = key == end ? BINS : w.bin(plain(logit_of(key)));
             }
             __syncthreads();
@@ -483,48 +568,240 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
             mass, weight);
         kept = x.before + at;
     }
-    const double target = (double)fminf(a.uniforms[r], 0x1.fffffep-1f) * mass;
+    const double target = u * mass;
     const Range x = row.range_of({}, [&](bool, uint32_t c, double m) { return m > target || c >= kept; });
     const uint32_t last = (kept < x.before + x.count ? kept : x.before + x.count) - 1;
     double before;
     const int at = row.first_token(
         x, [&](uint32_t rank, double sum, double own) { return rank >= last || sum + own > target; }, before, weight);
-    answer(row.token_at(x, at), (float)(weight / mass));
+    return {row.token_at(x, at), (float)(weight / mass)};
+}
+
+// The row's running counts and masses from its own counted bins or its parts'.
+__device__ __forceinline__ void sum_bins(const Weights &w, Shared &s, const PartBins *parts, int part_count) {
+    constexpr int PER = BINS / THREADS;
+    constexpr uint64_t SHARES = ((uint64_t)1 << SUM_BITS) - 1;
+    uint32_t count[PER] = {}, tokens = 0;
+    uint64_t share[PER] = {};
+    const int first = threadIdx.x * PER;
+    if (parts) {
+        // A part's bins lie `on` further on. What then falls past the last bin is known from the tokens' number.
+#pragma unroll 4
+        for (int p = 0; p < part_count; p++) {
+            const PartBins &x = parts[p];
+            if (!(x.top > -INFINITY)) continue;
+            const double by = x.top == w.top ? 0.0 : w.top_bin - w.bin_edge(x.top);
+            const int on = by < BINS - 1 ? (int)by : BINS - 1;
+            tokens += x.tokens;
+#pragma unroll
+            for (int i = 0; i < PER; i++) {
+                const int from = first + i - on;
+                const uint64_t v = from >= 0 && from < x.used && first + i < BINS - 1 ? x.bins[from] : 0;
+                count[i] += (uint32_t)(v >> SUM_BITS);
+                share[i] += v & SHARES;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+            uint64_t v = 0;
+            for (int x = 0; x < COPIES; x++) v += s.counted[(first + i) * COPIES + x];
+            count[i] = (uint32_t)(v >> SUM_BITS);
+            share[i] = v & SHARES;
+        }
+    }
+    // In units of the largest logit's own rounded weight: rows of one logit come out exactly.
+    const uint64_t one = ((uint64_t)1 << 40) + Weights::fixed_share(w.fraction(w.top));
+    const double unit = (double)one * 0x1p-40;
+    running<PER>(
+        s,
+        [&](int i, uint32_t &c, double &m) {
+            c = count[i - first];
+            const uint64_t sum = ((uint64_t)c << 40) + share[i - first];
+            m = i == BINS - 1 || !c ? 0.0 : i == 0 && sum == c * one ? (double)c : (double)sum * 0x1p-40 / unit * exp2_64(i * (-1.0 / PER_OCTAVE));
+        },
+        [&](int i, uint32_t c, double m, double) { s.row.count[i] = parts && i == BINS - 1 ? tokens : c, s.row.mass[i] = m; });
+    __syncthreads();
+}
+
+template <typename T, bool HELD>
+__global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, const PartBins *parts, int part_count) {
+    __shared__ Shared s;
+    const int r = blockIdx.x;
+    const Chosen o(a, r);
+    float top = -INFINITY;
+    if constexpr (!HELD) {
+        parts += (size_t)r * part_count;
+        for (int p = 0; p < part_count; p++) top = fmaxf(top, parts[p].top);
+    }
+    const Logits<T, HELD> logits(static_cast<const T *>(a.logits) + (int64_t)r * a.ld, a.n);
+    if constexpr (HELD) {
+        for (int b = threadIdx.x; b < BINS * COPIES; b += THREADS) s.counted[b] = 0;
+        logits.each([&](float l, int) { top = fmaxf(top, l); });
+        top = wave_max(top);
+        if ((threadIdx.x & 63) == 0) s.wave_top[threadIdx.x >> 6] = top;
+        __syncthreads();
+        top = wave_max(s.wave_top[threadIdx.x & (WAVES - 1)]);
+    }
+    const auto answer = [&](int token, float prob) {
+        if (threadIdx.x == 0) {
+            a.tokens[r] = token;
+            if (a.probs) a.probs[r] = prob;
+        }
+    };
+    if (!(top > -INFINITY)) return answer(-1, 0.0f);
+    if (o.greedy()) {
+        int x = INT32_MAX;
+        if constexpr (HELD) {
+            logits.each([&](float l, int i) { x = min(x, l == top ? i : INT32_MAX); });
+        } else {
+            int p = 0;
+            while (parts[p].top != top) p++;
+            for (int i = threadIdx.x; i < PART && p * PART + i < a.n && x == INT32_MAX; i += THREADS)
+                if (plain((float)logits.row[p * PART + i]) == top) x = p * PART + i;
+        }
+        return answer(least(s, x), 1.0f);
+    }
+    const Weights w(o.temperature, top);
+    if constexpr (HELD) {
+        logits.each([&](float l, int) { w.count_in(l, s.counted); });
+        __syncthreads();
+    }
+    sum_bins(w, s, HELD ? nullptr : parts, part_count);
+
+    const uint32_t all = s.row.count[BINS - 1];
+    const uint32_t k = o.top_k > 0 && (uint32_t)o.top_k < all ? (uint32_t)o.top_k : all;
+    const bool cut_k = k < all, cut = o.top_p < 1.0f || o.min_p > 0.0f;
+    const double u = (double)fminf(a.uniforms[r], 0x1.fffffep-1f), share = o.top_p < 1.0f ? (double)o.top_p : INFINITY;
+    const double least_weight = o.min_p;
+
+    // The bins where the border of top_k lies, those where the next one can lie, given what stays before it, and those
+    // where the token can lie.
+    const auto count_to = [&](int b) { return b < 0 ? 0u : s.row.count[b]; };
+    const auto mass_to = [&](int b) { return b < 0 ? 0.0 : s.row.mass[b]; };
+    const auto first_bin = [&](auto f) { return s.row.first(0, 0.0, f); };
+    Span by_k{}, by_mass{}, drawn{};
+    double low_mass = mass_to(BINS - 1), high_mass = low_mass;
+    uint32_t low_kept = k, high_kept = k;
+    if (cut_k) {
+        by_k.low = by_k.high = first_bin([&](int, uint32_t c, double) { return c > k; });
+        low_mass = mass_to(by_k.low - 1), high_mass = mass_to(by_k.low);
+    }
+    const double low_k = low_mass, high_k = high_mass;
+    if (cut) {
+        int low_floor = BINS, high_floor = BINS;
+        if (o.min_p > 0.0f) {  // the first bin below min_p, or the one before or after it where roundings decide
+            const double past = -__log2f(o.min_p) * PER_OCTAVE;
+            low_floor = past < BINS ? max((int)past - 1, 0) : BINS - 1;
+            high_floor = past < BINS - 4 ? max((int)past + 3, 0) : BINS - 1;
+        }
+        by_mass.low = first_bin([&](int b, uint32_t c, double m) { return c > k || m > share * low_k || b >= low_floor; });
+        by_mass.high = first_bin([&](int b, uint32_t c, double m) { return c > k || m > share * high_k || b >= high_floor; });
+        low_mass = mass_to(by_mass.low - 1), high_mass = mass_to(by_mass.high);
+        low_kept = max(count_to(by_mass.low - 1), 1u), high_kept = min(count_to(by_mass.high), k);
+    }
+    drawn.low = first_bin([&](int, uint32_t c, double m) { return m > u * low_mass || c >= low_kept; });
+    drawn.high = first_bin([&](int, uint32_t c, double m) { return m > u * high_mass || c >= high_kept; });
+    // Spans that overlap are one.
+    const bool one_mass = !cut || by_mass.low <= drawn.high;
+    if (one_mass) {
+        if (cut) drawn.high = max(drawn.high, by_mass.high);
+        by_mass = drawn;
+    }
+    const bool one_k = !cut_k || by_k.low <= by_mass.high;
+    if (one_k) {
+        if (cut_k) by_mass.high = max(by_mass.high, by_k.high);
+        if (one_mass) drawn = by_mass;
+        by_k = by_mass;
+    }
+    const auto place = [&](Span &x, int start) {
+        x.start = start;
+        x.before = count_to(x.low - 1);
+        x.mass_before = mass_to(x.low - 1);
+        x.count = (int)(count_to(x.high) - x.before);
+    };
+    place(drawn, 0);
+    place(by_mass, one_mass ? 0 : drawn.count);
+    place(by_k, one_k ? by_mass.start : by_mass.start + by_mass.count);
+    const int listed = by_k.start + by_k.count;
+    if (listed > LIST) {
+        const Drawn x = step_by_step(logits.row, a.n, w, s, k, all, u, share, least_weight);
+        return answer(x.token, x.prob);
+    }
+    gather(logits, w, s, drawn, by_mass, by_k, listed);
+    const auto weight = [&](int i) { return w.of(logit_of((uint32_t)(s.list[i] >> 32))); };
+    const auto mass_before = [&](const Span &x, int i) { return x.mass_before + (s.before[i] - s.before[x.start]); };
+    const auto rank = [&](const Span &x, int i) { return x.before + (uint32_t)(i - x.start); };
+    double mass = mass_to(BINS - 1);
+    if (cut_k) mass = fmin(fmax(mass_before(by_k, by_k.start + (int)(k - by_k.before)), low_k), high_k);
+    uint32_t kept = k;
+    if (cut) {
+        const double most = share * mass;
+        const int i = by_mass.start + first_of(by_mass.count, [&](int i) {
+            const uint32_t n = rank(by_mass, by_mass.start + i);
+            return n > 0 && (n >= k || mass_before(by_mass, by_mass.start + i) >= most || weight(by_mass.start + i) < least_weight);
+        });
+        kept = rank(by_mass, i);
+        mass = i == by_mass.start ? by_mass.mass_before : mass_before(by_mass, i - 1) + weight(i - 1);
+        mass = fmin(fmax(mass, low_mass), high_mass);
+    }
+    const double target = u * mass;
+    const uint32_t last = min(kept, drawn.before + (uint32_t)drawn.count) - 1;
+    const int i = first_of(drawn.count, [&](int i) { return rank(drawn, i) >= last || mass_before(drawn, i) + weight(i) > target; });
+    answer((int)(uint32_t)s.list[i], (float)(weight(i) / mass));
 }
 
 // The bins of a part of a row: its logits stay in registers from the largest to the weights.
 template <typename T>
 __global__ __launch_bounds__(PART_THREADS) void parts_kernel(const SampleArgs a, PartBins *parts, int part_count) {
-    __shared__ uint64_t mass[BINS];
-    __shared__ uint32_t count[BINS];
-    __shared__ float tops[PART_THREADS / 64];
+    constexpr int PIECE = 16 / sizeof(T), PIECES = PART_VALUES / PIECE, PART_WAVES = PART_THREADS / 64;
+    __shared__ __align__(16) uint64_t bins[BINS * COPIES];
+    __shared__ float tops[PART_WAVES];
+    __shared__ uint32_t tokens;
+    __shared__ int used;
     const int r = blockIdx.x / part_count, p = blockIdx.x % part_count;
     PartBins &out = parts[blockIdx.x];
     const Chosen o(a, r);
     const T *logits = static_cast<const T *>(a.logits) + (int64_t)r * a.ld + (int64_t)p * PART;
     const int n = min(a.n - p * PART, PART);
-    float l[PART_VALUES];
+    float l[PIECES][PIECE];
     float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < PART_VALUES; i++) {
-        const int at = i * PART_THREADS + threadIdx.x;
-        l[i] = at < n ? plain(logit(logits, at)) : -INFINITY;
-    }
+    for (int x = 0; x < PIECES; x++) load(logits, (x * PART_THREADS + (int)threadIdx.x) * PIECE, n, l[x]);
+    for (int b = threadIdx.x; b < BINS * COPIES; b += PART_THREADS) bins[b] = 0;
+    if (threadIdx.x == 0) tokens = 0, used = 0;
 #pragma unroll
-    for (int i = 0; i < PART_VALUES; i++) top = fmaxf(top, l[i]);
-    for (int b = threadIdx.x; b < BINS; b += PART_THREADS) mass[b] = 0, count[b] = 0;
+    for (int x = 0; x < PIECES; x++)
+#pragma unroll
+        for (int y = 0; y < PIECE; y++) top = fmaxf(top, l[x][y]);  // NaN is passed over
     top = wave_max(top);
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    for (int x = 0; x < PART_THREADS / 64; x++) top = fmaxf(top, tops[x]);
-    if (threadIdx.x == 0) out.top = top;
-    if (!(top > -INFINITY) || o.greedy()) return;
+    for (int x = 0; x < PART_WAVES; x++) top = fmaxf(top, tops[x]);
+    if (!(top > -INFINITY) || o.greedy()) {
+        if (threadIdx.x == 0) out.top = top;
+        return;
+    }
     const Weights w(o.temperature, top);
 #pragma unroll
-    for (int i = 0; i < PART_VALUES; i++)
-        if (l[i] > -INFINITY) count_in(w, l[i], count, mass);
+    for (int x = 0; x < PIECES; x++)
+#pragma unroll
+        for (int y = 0; y < PIECE; y++)
+            if (l[x][y] > -INFINITY) w.count_in(l[x][y], bins);
     __syncthreads();
-    for (int b = threadIdx.x; b < BINS; b += PART_THREADS) out.mass[b] = mass[b], out.count[b] = count[b];
+    uint32_t mine = 0;
+    int last = 0;
+    for (int b = threadIdx.x; b < BINS; b += PART_THREADS) {
+        uint64_t v = 0;
+        for (int x = 0; x < COPIES; x++) v += bins[b * COPIES + x];
+        mine += (uint32_t)(v >> SUM_BITS);
+        last = v ? b + 1 : last;
+        out.bins[b] = v;
+    }
+    for (int o2 = 32; o2; o2 >>= 1) mine += __shfl_xor(mine, o2), last = max(last, __shfl_xor(last, o2));
+    if ((threadIdx.x & 63) == 0) atomicAdd(&tokens, mine), atomicMax(&used, last);
+    __syncthreads();
+    if (threadIdx.x == 0) out.top = top, out.used = used, out.tokens = tokens;
 }
 
 int part_count_of(size_t n) { return n <= SAMPLE_WHOLE ? 0 : (int)div_ceil(n, PART); }
@@ -542,8 +819,10 @@ hipError_t launch_sample(const SampleArgs &a, uint32_t type, int rows, void *wor
             hipLaunchKernelGGL((parts_kernel<T>), dim3((unsigned)(rows * count)), dim3(PART_THREADS), 0, s, a, parts, count);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
+            hipLaunchKernelGGL((sample_kernel<T, false>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)parts, count);
+        } else {
+            hipLaunchKernelGGL((sample_kernel<T, true>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)nullptr, 0);
         }
-        hipLaunchKernelGGL((sample_kernel<T>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)parts, count);
         return hipGetLastError();
     };
     switch (type) {
