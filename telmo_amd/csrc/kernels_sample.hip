@@ -4,9 +4,10 @@
 // token is the first one whose running sum exceeds u times the sum of those kept.
 //
 // Nothing is sorted but what lies next to a border. Tokens are counted and their weights added in bins of the logits: 32 for
-// each factor of two of the weight, 64 factors, the last one (of weight 0 in these sums) for all that is smaller. A bin's
-// sum is of 2^(y - floor y) - 1 with y = 32 l log2 e / temperature, in whole numbers of 2^-40, so that it depends neither
-// on the order nor on the row's largest logit; one 64-bit atomic counts a token and adds its weight. The running counts and
+// each factor of two of the weight, 64 factors, the last one (of weight 0 in these sums) for all that is smaller. The bin is
+// floor y with y = 32 l log2 e / temperature, rounded once to steps of 2^-40, and a bin's sum is of 2^(y - floor y) - 1 in
+// whole numbers of 2^-40, so that it depends neither on the order nor on the row's largest logit; one 64-bit atomic counts a
+// token and adds its weight. The running counts and
 // sums say in which bins each border and the drawn token can lie; the tokens of these bins are gathered in one pass,
 // sorted, and added up in 64 bits. If they are more than LDS sorts, the borders are looked for one after the other, and a
 // bin of too many tokens is first divided by its logits' bits, down to a single value, whose tokens differ in their
@@ -30,16 +31,15 @@ constexpr int SUM_BITS = 49;  // of a counted bin; above them the count of up to
 static_assert(WHOLE <= 1 << 14 && PART <= 1 << 14, "a bin's count and sum share 64 bits");
 constexpr double FIXED = 1024.0;  // added to a weight it leaves steps of 2^-42: 2^22 weights' sum fits 64 bits
 
-// What a part of a row leaves: its bins up to the last one that has tokens, relative to its largest logit.
+// What a part of a row leaves: its bins, relative to its largest logit.
 struct PartBins {
     uint64_t bins[BINS];
     float top;  // -infinity: no token
-    int used;
-    uint32_t tokens, pad;
+    uint32_t tokens, pad[2];
 };
 
 // Zeros of either sign are one logit.
-__device__ __forceinline__ float plain(float l) { return l == 0.0f ? 0.0f : l; }
+__device__ __forceinline__ float plain(float l) { return l + 0.0f; }
 // A logit as bits that order as it does, larger first: 0 for +infinity.
 __device__ __forceinline__ uint32_t key_of(float l) {
     const uint32_t b = __float_as_uint(l);
@@ -69,43 +69,59 @@ __device__ __forceinline__ double exp2_64(double t) {
     return __builtin_ldexp(p, (int)n);
 }
 
-// The row's scale of weights: c = log2 e / temperature, y = 32 c l.
+// 2^(f / 32) - 1 in steps of 2^-40 for the fraction f of a place, by Taylor's polynomial up to f^6 (the next term is below
+// 2^-50).
+struct Share {
+    static constexpr double X = 0.69314718055994530942 / PER_OCTAVE;
+    double p[6] = {X * X * X * X * X * X / 720.0, X * X * X * X * X / 120.0, X * X * X * X / 24.0, X * X * X / 6.0, X * X / 2.0, X};
+    // In registers: as constants each would be moved there again for each logit.
+    __device__ __forceinline__ Share() {
+#pragma unroll
+        for (int i = 0; i < 6; i++) asm("" : "+v"(p[i]));
+    }
+    __device__ __forceinline__ uint64_t operator()(double place) const {
+        const double f = __builtin_amdgcn_fract(place);
+        double s = p[0];
+#pragma unroll
+        for (int i = 1; i < 6; i++) s = __builtin_fma(s, f, p[i]);
+        return __builtin_bit_cast(uint64_t, __builtin_fma(s, f, 0x1p12)) - __builtin_bit_cast(uint64_t, 0x1p12);
+    }
+};
+
+// The scale of a row's weights, c = log2 e / temperature, and its bins. y - edge for l, with the edge floor y of the
+// largest logit, lies in (-BINS + 1, 1) and is added to POINT in one rounding: steps of 2^-40, and the bin in the bits above.
+constexpr double POINT = 0x1.8p12;
+constexpr int POINT_BITS = 0x40b800;  // of POINT, the upper 24
 struct Weights {
-    double c;
+    double c, k, shift, edge;
     float top;  // the largest logit
-    double top_bin;
+    bool far;   // logits that differ from it lie in the last bin
     __device__ __forceinline__ Weights(float temperature, float top_) : c(1.44269504088896340736 / temperature), top(top_) {
-        top_bin = bin_edge(top);
+        const double wide = PER_OCTAVE * c, y = (double)top * wide;
+        far = !(__builtin_fabs(y) < 0x1p40);
+        // f32 neighbours are 2^-24 apart at least: 2^14 bins with |y| brought down to 2^38. To infinity everything is far.
+        k = top == INFINITY ? 0x1p-200 : __builtin_ldexp(wide, far ? 39 - __builtin_amdgcn_frexp_exp(y) : 0);
+        edge = __builtin_floor((double)top * k);
+        edge += __builtin_floor(__builtin_fma((double)top, k, POINT - edge) - POINT);
+        edge = top == INFINITY ? INFINITY : edge;
+        shift = top == INFINITY ? POINT - (BINS - 1) : POINT - edge;
     }
-    __device__ __forceinline__ double bin_edge(float l) const { return __builtin_floor((double)l * (PER_OCTAVE * c)); }
     __device__ __forceinline__ double of(float l) const { return l == top ? 1.0 : exp2_64(((double)l - (double)top) * c); }
-    __device__ __forceinline__ int bin(float l) const {
-        if (l == top) return 0;
-        const double b = top_bin - bin_edge(l);
-        return b < BINS - 1 ? (int)b : BINS - 1;  // a difference of infinities too
+    __device__ __forceinline__ double place(float l) const {
+        return fmin(fmax(__builtin_fma((double)l, k, shift), POINT - (BINS - 1)), POINT + 1.0 - 0x1p-40);
     }
-    // y - floor y, with the product's rounding error: from 0 to 1. (Where y has no fraction left, the logits next to l lie
-    // in other bins far away, and 0 or 1 is the same for all of l's own; 0 for infinity.)
-    __device__ __forceinline__ double fraction(float l) const {
-        const double k = PER_OCTAVE * c, y = (double)l * k, low = __builtin_fma((double)l, k, -y);
-        return fmin(fmax((y - __builtin_floor(y)) + low, 0.0), 1.0);
+    static __device__ __forceinline__ uint32_t upper(double place) { return (uint32_t)(__builtin_bit_cast(uint64_t, place) >> 32); }
+    static __device__ __forceinline__ int bin_of(double place) { return POINT_BITS - (int)(upper(place) >> 8); }
+    __device__ __forceinline__ int bin(float l) const { return bin_of(place(l)); }
+    // How much further on the bins lie that are counted from another, lower logit.
+    __device__ __forceinline__ int further(const Weights &w) const {
+        const double by = edge - w.edge;
+        return w.top == top ? 0 : far || w.far || !(by < BINS - 1) ? BINS - 1 : (int)by;
     }
-    // 2^(f / 32) - 1 in steps of 2^-40, by Taylor's polynomial up to x^6 (the next one is below 2^-50).
-    static __device__ __forceinline__ uint64_t fixed_share(double f) {
-        const double x = f * (0.69314718055994530942 / PER_OCTAVE);
-        double p = 1.0 / 720.0;
-        p = __builtin_fma(p, x, 1.0 / 120.0);
-        p = __builtin_fma(p, x, 1.0 / 24.0);
-        p = __builtin_fma(p, x, 1.0 / 6.0);
-        p = __builtin_fma(p, x, 0.5);
-        p = __builtin_fma(p, x, 1.0);
-        return (uint64_t)(__builtin_bit_cast(int64_t, __builtin_fma(p, x, 0x1p12)) - __builtin_bit_cast(int64_t, 0x1p12));
-    }
-    __device__ __forceinline__ void count_in(float l, uint64_t *bins) const {
-        const int b = bin(l);
-        const uint64_t share = b == BINS - 1 ? 0 : fixed_share(fraction(l));
-        atomicAdd(reinterpret_cast<unsigned long long *>(&bins[b * COPIES + (threadIdx.x & (COPIES - 1))]),
-                  (unsigned long long)(share + ((uint64_t)1 << SUM_BITS)));
+    __device__ __forceinline__ void count_in(float l, uint64_t *bins, const Share &share) const {
+        const double at = place(l);
+        atomicAdd(reinterpret_cast<unsigned long long *>(&bins[bin_of(at) * COPIES + (threadIdx.x & (COPIES - 1))]),
+                  (unsigned long long)(share(at) + ((uint64_t)1 << SUM_BITS)));
     }
 };
 
@@ -135,9 +151,29 @@ __device__ __forceinline__ void load(const T *row, int first, int n, float (&l)[
     }
 }
 
+// x of the lane before by a DPP control, `other` where there is none.
+template <int CONTROL, int ROWS = 0xf, typename X>
+__device__ __forceinline__ X from_lane(X x, X other) {
+    if constexpr (sizeof(X) == 4) {
+        return __builtin_bit_cast(X, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, other), __builtin_bit_cast(int, x), CONTROL, ROWS, 0xf, false));
+    } else {
+        const uint64_t a = __builtin_bit_cast(uint64_t, x), b = __builtin_bit_cast(uint64_t, other);
+        return __builtin_bit_cast(X, (uint64_t)from_lane<CONTROL, ROWS>((uint32_t)a, (uint32_t)b) | (uint64_t)from_lane<CONTROL, ROWS>((uint32_t)(a >> 32), (uint32_t)(b >> 32)) << 32);
+    }
+}
+// f over the lanes up to each.
+template <typename X, typename F>
+__device__ __forceinline__ X scan(X x, X none, F f) {
+    x = f(from_lane<0x111>(x, none), x);
+    x = f(from_lane<0x112>(x, none), x);
+    x = f(from_lane<0x114>(x, none), x);
+    x = f(from_lane<0x118>(x, none), x);
+    x = f(from_lane<0x142, 0xa>(x, none), x);
+    return f(from_lane<0x143, 0xc>(x, none), x);
+}
 __device__ __forceinline__ float wave_max(float x) {
-    for (int o = 32; o; o >>= 1) x = fmaxf(x, __shfl_xor(x, o));
-    return x;
+    x = scan(x, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
 // The first of n <= 4096 numbers where f holds, n where none does; f holds from there on. By each wavefront for itself.
@@ -145,12 +181,13 @@ template <typename F>
 __device__ __forceinline__ int first_of(int n, F f) {
     const int lane = threadIdx.x & 63;
     int low = 0;
-    for (int step = n > 64 ? 64 : 1;; step = 1) {
-        const int at = low + step * (lane + 1) - 1;  // the last number of the lane's step
-        const unsigned long long which = __ballot(at >= n || f(at));
-        low += step * (which ? (int)__builtin_ctzll(which) : 64);
-        if (step == 1 || low >= n) return low < n ? low : n;
+    if (n > 64) {
+        const int end = 64 * lane + 63;  // the last number of the lane's 64
+        const unsigned long long which = __ballot(end >= n || f(end));
+        low = 64 * (which ? (int)__builtin_ctzll(which) : 64);
     }
+    const unsigned long long which = __ballot(low + lane >= n || f(low + lane));
+    return min(low + (which ? (int)__builtin_ctzll(which) : 64), n);
 }
 
 // Running sums of bins.
@@ -163,14 +200,36 @@ struct Bins {
         for (int b = threadIdx.x; b < BINS; b += THREADS) count[b] = 0, fixed_mass()[b] = 0;
         __syncthreads();
     }
-    // The first bin where f(bin, running count, running mass) holds, or the last one that has tokens. (Between bins without
-    // any, sums may grow by a rounding: then the bin before them.)
+    // The bin that has tokens where f(bin, running count, running mass) first holds, or the last one.
     template <typename F>
-    __device__ __forceinline__ int first(uint32_t before, double mass_before, F f) const {
-        const int b = first_of(BINS, [&](int x) { return f(x, before + count[x], mass_before + mass[x]); });
+    __device__ __forceinline__ int first(F f) const {
+        return with_tokens(first_of(BINS, [&](int x) { return f(x, count[x], mass[x]); }));
+    }
+    // Between bins without any, sums may grow by a rounding: then the bin before them.
+    __device__ __forceinline__ int with_tokens(int b) const {
         if (b < BINS && count[b] > (b ? count[b - 1] : 0u)) return b;
         const uint32_t c = max(count[min(b, BINS - 1)], 1u);
         return first_of(BINS, [&](int x) { return count[x] >= c; });
+    }
+    // Two of them at a time.
+    struct Border {
+        uint32_t count;
+        double mass;
+        int bin;
+        __device__ __forceinline__ bool past(int b, uint32_t c, double m) const { return c > count || m > mass || b >= bin; }
+    };
+    __device__ __forceinline__ void first(const Border &x, const Border &y, int &at_x, int &at_y) const {
+        static_assert(BINS == 32 * 64, "half a wavefront's lanes look at every 64th bin");
+        const int lane = threadIdx.x & 63, end = 64 * (lane & 31) + 63;
+        const uint32_t c = count[end];
+        const double m = mass[end];
+        const unsigned long long which = __ballot(lane < 32 ? x.past(end, c, m) : y.past(end, c, m));
+        const uint32_t low = (uint32_t)which, high = (uint32_t)(which >> 32);
+        const int at_low = min(low ? __builtin_ctz(low) * 64 : BINS, BINS - 64), at_high = min(high ? __builtin_ctz(high) * 64 : BINS, BINS - 64);
+        const unsigned long long of_x = __ballot(x.past(at_low + lane, count[at_low + lane], mass[at_low + lane]));
+        const unsigned long long of_y = __ballot(y.past(at_high + lane, count[at_high + lane], mass[at_high + lane]));
+        at_x = with_tokens(of_x ? at_low + (int)__builtin_ctzll(of_x) : BINS);
+        at_y = with_tokens(of_y ? at_high + (int)__builtin_ctzll(of_y) : BINS);
     }
 };
 
@@ -204,19 +263,20 @@ __device__ __forceinline__ void running(Shared &s, F f, G g) {
         count += c[i];
         mass += m[i];
     }
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_up(count, o);
-        const double y = __shfl_up(mass, o);
-        if (lane >= o) count += x, mass += y;
-    }
+    count = scan(count, 0u, [](uint32_t a, uint32_t b) { return a + b; });
+    mass = scan(mass, 0.0, [](double a, double b) { return a + b; });
     __syncthreads();
     if (lane == 63) s.wave_count[wave] = count, s.wave_mass[wave] = mass;
     __syncthreads();
-    count = __shfl_up(count, 1), mass = __shfl_up(mass, 1);
-    if (lane == 0) count = 0, mass = 0.0;
+    count = from_lane<0x138>(count, 0u), mass = from_lane<0x138>(mass, 0.0);
     uint32_t before = 0;
     double base = 0.0;
-    for (int x = 0; x < wave; x++) before += s.wave_count[x], base += s.wave_mass[x];
+#pragma unroll
+    for (int x = 0; x < WAVES - 1; x++) {
+        const uint32_t c = s.wave_count[x];
+        const double m = s.wave_mass[x];
+        before += x < wave ? c : 0u, base += x < wave ? m : 0.0;
+    }
     count += before;
     mass += base;
     for (int i = 0; i < PER; i++) {
@@ -265,7 +325,7 @@ struct Range {
 // A row's logits: held in registers (HELD), or read again for each pass.
 template <typename T, bool HELD>
 struct Logits {
-    static constexpr int PIECE = 16 / sizeof(T), PIECES = HELD ? WHOLE_VALUES / PIECE : 4;
+    static constexpr int PIECE = 16 / sizeof(T), PIECES = HELD ? WHOLE_VALUES / PIECE : 32 / PIECE;
     const T *row;
     int n;
     float held[HELD ? PIECES : 1][PIECE];
@@ -306,7 +366,6 @@ struct Span {
     int low, high, start = 0, count = 0;
     uint32_t before = 0;
     double mass_before = 0.0;
-    __device__ __forceinline__ bool holds(int bin) const { return bin >= low && bin <= high; }
 };
 
 // The row's options.
@@ -344,21 +403,46 @@ __device__ __forceinline__ void sort_list(Shared &s, int count) {
         __syncthreads();
         return;
     }
-    int size = 2;
-    while (size < count) size *= 2;
-    for (int i = count + threadIdx.x; i < size; i += THREADS) s.list[i] = ~0ull;
-    for (int block = 2; block <= size; block *= 2)
-        for (int step = block / 2; step; step /= 2) {
-            // Up to 64 apart a wavefront's pairs are its own from the last step on.
-            if (step > 32 || block == 2) __syncthreads();
-            else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"), __builtin_amdgcn_wave_barrier();
-            for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                const uint64_t x = s.list[a], y = s.list[b];
-                if ((x > y) == ((a & block) == 0)) s.list[a] = y, s.list[b] = x;
+    // Runs of 16, then twice as long ones from each two: a token's place is its own in its run and that in the other.
+    constexpr int PER = LIST / THREADS, RUN = 16;
+    static_assert(sizeof(s.before) == sizeof(s.list), "the runs go back and forth");
+    uint64_t *from = s.list, *to = reinterpret_cast<uint64_t *>(s.before);
+    for (int run = 1; run < count; run *= run == 1 ? RUN : 2) {
+#pragma unroll
+        for (int x = 0; x < PER; x++) {
+            const int i = x * THREADS + threadIdx.x;
+            if (i >= count) continue;
+            const uint64_t own = from[i];
+            int place;
+            if (run == 1) {
+                const int start = i & ~(RUN - 1), n = min(RUN, count - start);
+                place = start;
+                if (n == RUN) {
+#pragma unroll
+                    for (int y = 0; y < RUN; y++) place += from[start + y] < own;
+                } else {
+                    for (int y = 0; y < n; y++) place += from[start + y] < own;
+                }
+            } else {
+                const int both = i & ~(2 * run - 1), other = (i & ~(run - 1)) == both ? both + run : both;
+                int low = 0, high = max(min(run, count - other), 0);
+                while (low < high) {
+                    const int mid = (low + high) / 2;
+                    if (from[other + mid] < own) low = mid + 1;
+                    else high = mid;
+                }
+                place = both + (i & (run - 1)) + low;
             }
+            to[place] = own;
         }
-    __syncthreads();
+        __syncthreads();
+        uint64_t *t = from;
+        from = to, to = t;
+    }
+    if (from != s.list) {
+        for (int i = threadIdx.x; i < count; i += THREADS) s.list[i] = from[i];
+        __syncthreads();
+    }
 }
 
 // The tokens of the spans in s.list, in order, and the weights before each.
@@ -367,27 +451,20 @@ __device__ __forceinline__ void gather(const Logits<T, HELD> &logits, const Weig
     __syncthreads();  // the counted bins lie where the list does
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
-    // Logits that may lie in a span, a little more than its own.
-    const auto least_of = [&](const Span &x) {
-        const float l = x.high >= BINS - 1 ? -INFINITY : (float)((w.top_bin - x.high) / (PER_OCTAVE * w.c));
-        return l - (l < INFINITY ? fabsf(l) * 0x1p-20f : 0.0f);
+    const auto within = [](const Span &x, uint32_t upper) {
+        return upper - ((uint32_t)(POINT_BITS - x.high) << 8) < (uint32_t)(x.high - x.low + 1) << 8;
     };
-    const auto most_of = [&](const Span &x) {
-        const float l = x.low <= 0 ? INFINITY : (float)((w.top_bin - x.low + 1.0) / (PER_OCTAVE * w.c));
-        return l + fabsf(l) * 0x1p-20f;
-    };
-    const float x0 = least_of(x), x1 = most_of(x), y0 = least_of(y), y1 = most_of(y), z0 = least_of(z), z1 = most_of(z);
     logits.each([&](float l, int i) {
-        if (!((l >= x0 && l <= x1) || (l >= y0 && l <= y1) || (l >= z0 && l <= z1))) return;
-        const int bin = w.bin(l);
-        if (!(x.holds(bin) || y.holds(bin) || z.holds(bin))) return;
+        const uint32_t upper = Weights::upper(w.place(l));
+        if (!(within(x, upper) | within(y, upper) | within(z, upper))) return;
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < LIST) s.list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
     });
     sort_list(s, count);
-    running<LIST / THREADS>(
-        s, [&](int i, uint32_t &c, double &m) { c = 0, m = i < count ? w.of(logit_of((uint32_t)(s.list[i] >> 32))) : 0.0; },
-        [&](int i, uint32_t, double with, double own) { s.before[i] = with - own; });
+    const auto weight = [&](int i, uint32_t &c, double &m) { c = 0, m = i < count ? w.of(logit_of((uint32_t)(s.list[i] >> 32))) : 0.0; };
+    const auto put = [&](int i, uint32_t, double with, double own) { s.before[i] = with - own; };
+    if (count <= THREADS) running<1>(s, weight, put);
+    else running<LIST / THREADS>(s, weight, put);
     __syncthreads();
 }
 
@@ -410,7 +487,7 @@ struct Row {
     // after r's.
     template <typename F>
     __device__ __forceinline__ int first_bin(const Bins &bins, F f, Range &r) const {
-        const int b = bins.first(r.before, r.mass_before, f);
+        const int b = bins.first([&](int x, uint32_t c, double m) { return f(x, r.before + c, r.mass_before + m); });
         const uint32_t earlier = b ? bins.count[b - 1] : 0u;
         r.count = bins.count[b] - earlier;
         r.before += earlier;
@@ -578,25 +655,25 @@ __device__ __noinline__ Drawn step_by_step(const T *logits, int n, Weights w, Sh
 }
 
 // The row's running counts and masses from its own counted bins or its parts'.
-__device__ __forceinline__ void sum_bins(const Weights &w, Shared &s, const PartBins *parts, int part_count) {
+__device__ __forceinline__ void sum_bins(const Weights &w, float temperature, Shared &s, const PartBins *parts, int part_count) {
     constexpr int PER = BINS / THREADS;
     constexpr uint64_t SHARES = ((uint64_t)1 << SUM_BITS) - 1;
     uint32_t count[PER] = {}, tokens = 0;
     uint64_t share[PER] = {};
     const int first = threadIdx.x * PER;
     if (parts) {
-        // A part's bins lie `on` further on. What then falls past the last bin is known from the tokens' number.
+        // A part's bins lie `on` further on, those of a part of no token past all. What falls past the last bin is known
+        // from the tokens' number.
 #pragma unroll 4
         for (int p = 0; p < part_count; p++) {
             const PartBins &x = parts[p];
-            if (!(x.top > -INFINITY)) continue;
-            const double by = x.top == w.top ? 0.0 : w.top_bin - w.bin_edge(x.top);
-            const int on = by < BINS - 1 ? (int)by : BINS - 1;
+            const int on = w.further(Weights(temperature, x.top));
             tokens += x.tokens;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
                 const int from = first + i - on;
-                const uint64_t v = from >= 0 && from < x.used && first + i < BINS - 1 ? x.bins[from] : 0;
+                uint64_t v = x.bins[max(from, 0)];
+                v = from >= 0 && first + i < BINS - 1 ? v : 0;
                 count[i] += (uint32_t)(v >> SUM_BITS);
                 share[i] += v & SHARES;
             }
@@ -611,14 +688,14 @@ __device__ __forceinline__ void sum_bins(const Weights &w, Shared &s, const Part
         }
     }
     // In units of the largest logit's own rounded weight: rows of one logit come out exactly.
-    const uint64_t one = ((uint64_t)1 << 40) + Weights::fixed_share(w.fraction(w.top));
-    const double unit = (double)one * 0x1p-40;
+    const uint64_t one = ((uint64_t)1 << 40) + Share()(w.place(w.top));
+    const double unit = 0x1p-40 / ((double)one * 0x1p-40);
     running<PER>(
         s,
         [&](int i, uint32_t &c, double &m) {
             c = count[i - first];
             const uint64_t sum = ((uint64_t)c << 40) + share[i - first];
-            m = i == BINS - 1 || !c ? 0.0 : i == 0 && sum == c * one ? (double)c : (double)sum * 0x1p-40 / unit * exp2_64(i * (-1.0 / PER_OCTAVE));
+            m = i == BINS - 1 || !c ? 0.0 : i == 0 && sum == c * one ? (double)c : (double)sum * unit * exp2_64(i * (-1.0 / PER_OCTAVE));
         },
         [&](int i, uint32_t c, double m, double) { s.row.count[i] = parts && i == BINS - 1 ? tokens : c, s.row.mass[i] = m; });
     __syncthreads();
@@ -632,7 +709,8 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
     float top = -INFINITY;
     if constexpr (!HELD) {
         parts += (size_t)r * part_count;
-        for (int p = 0; p < part_count; p++) top = fmaxf(top, parts[p].top);
+        for (int p = threadIdx.x & 63; p < part_count; p += 64) top = fmaxf(top, parts[p].top);
+        top = wave_max(top);
     }
     const Logits<T, HELD> logits(static_cast<const T *>(a.logits) + (int64_t)r * a.ld, a.n);
     if constexpr (HELD) {
@@ -664,10 +742,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
     }
     const Weights w(o.temperature, top);
     if constexpr (HELD) {
-        logits.each([&](float l, int) { w.count_in(l, s.counted); });
+        const Share share;
+        logits.each([&](float l, int) { w.count_in(l, s.counted, share); });
         __syncthreads();
     }
-    sum_bins(w, s, HELD ? nullptr : parts, part_count);
+    sum_bins(w, o.temperature, s, HELD ? nullptr : parts, part_count);
 
     const uint32_t all = s.row.count[BINS - 1];
     const uint32_t k = o.top_k > 0 && (uint32_t)o.top_k < all ? (uint32_t)o.top_k : all;
@@ -679,12 +758,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
     // where the token can lie.
     const auto count_to = [&](int b) { return b < 0 ? 0u : s.row.count[b]; };
     const auto mass_to = [&](int b) { return b < 0 ? 0.0 : s.row.mass[b]; };
-    const auto first_bin = [&](auto f) { return s.row.first(0, 0.0, f); };
     Span by_k{}, by_mass{}, drawn{};
     double low_mass = mass_to(BINS - 1), high_mass = low_mass;
     uint32_t low_kept = k, high_kept = k;
     if (cut_k) {
-        by_k.low = by_k.high = first_bin([&](int, uint32_t c, double) { return c > k; });
+        by_k.low = by_k.high = s.row.first([&](int, uint32_t c, double) { return c > k; });
         low_mass = mass_to(by_k.low - 1), high_mass = mass_to(by_k.low);
     }
     const double low_k = low_mass, high_k = high_mass;
@@ -695,13 +773,11 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
             low_floor = past < BINS ? max((int)past - 1, 0) : BINS - 1;
             high_floor = past < BINS - 4 ? max((int)past + 3, 0) : BINS - 1;
         }
-        by_mass.low = first_bin([&](int b, uint32_t c, double m) { return c > k || m > share * low_k || b >= low_floor; });
-        by_mass.high = first_bin([&](int b, uint32_t c, double m) { return c > k || m > share * high_k || b >= high_floor; });
+        s.row.first({k, share * low_k, low_floor}, {k, share * high_k, high_floor}, by_mass.low, by_mass.high);
         low_mass = mass_to(by_mass.low - 1), high_mass = mass_to(by_mass.high);
         low_kept = max(count_to(by_mass.low - 1), 1u), high_kept = min(count_to(by_mass.high), k);
     }
-    drawn.low = first_bin([&](int, uint32_t c, double m) { return m > u * low_mass || c >= low_kept; });
-    drawn.high = first_bin([&](int, uint32_t c, double m) { return m > u * high_mass || c >= high_kept; });
+    s.row.first({low_kept - 1, u * low_mass, BINS}, {high_kept - 1, u * high_mass, BINS}, drawn.low, drawn.high);
     // Spans that overlap are one.
     const bool one_mass = !cut || by_mass.low <= drawn.high;
     if (one_mass) {
@@ -758,7 +834,6 @@ __global__ __launch_bounds__(PART_THREADS) void parts_kernel(const SampleArgs a,
     __shared__ __align__(16) uint64_t bins[BINS * COPIES];
     __shared__ float tops[PART_WAVES];
     __shared__ uint32_t tokens;
-    __shared__ int used;
     const int r = blockIdx.x / part_count, p = blockIdx.x % part_count;
     PartBins &out = parts[blockIdx.x];
     const Chosen o(a, r);
@@ -769,7 +844,7 @@ __global__ __launch_bounds__(PART_THREADS) void parts_kernel(const SampleArgs a,
 #pragma unroll
     for (int x = 0; x < PIECES; x++) load(logits, (x * PART_THREADS + (int)threadIdx.x) * PIECE, n, l[x]);
     for (int b = threadIdx.x; b < BINS * COPIES; b += PART_THREADS) bins[b] = 0;
-    if (threadIdx.x == 0) tokens = 0, used = 0;
+    if (threadIdx.x == 0) tokens = 0;
 #pragma unroll
     for (int x = 0; x < PIECES; x++)
 #pragma unroll
@@ -779,29 +854,28 @@ __global__ __launch_bounds__(PART_THREADS) void parts_kernel(const SampleArgs a,
     __syncthreads();
     for (int x = 0; x < PART_WAVES; x++) top = fmaxf(top, tops[x]);
     if (!(top > -INFINITY) || o.greedy()) {
-        if (threadIdx.x == 0) out.top = top;
+        if (threadIdx.x == 0) out.top = top, out.tokens = 0;
         return;
     }
     const Weights w(o.temperature, top);
+    const Share share;
 #pragma unroll
     for (int x = 0; x < PIECES; x++)
 #pragma unroll
         for (int y = 0; y < PIECE; y++)
-            if (l[x][y] > -INFINITY) w.count_in(l[x][y], bins);
+            if (l[x][y] > -INFINITY) w.count_in(l[x][y], bins, share);
     __syncthreads();
     uint32_t mine = 0;
-    int last = 0;
     for (int b = threadIdx.x; b < BINS; b += PART_THREADS) {
         uint64_t v = 0;
         for (int x = 0; x < COPIES; x++) v += bins[b * COPIES + x];
         mine += (uint32_t)(v >> SUM_BITS);
-        last = v ? b + 1 : last;
         out.bins[b] = v;
     }
-    for (int o2 = 32; o2; o2 >>= 1) mine += __shfl_xor(mine, o2), last = max(last, __shfl_xor(last, o2));
-    if ((threadIdx.x & 63) == 0) atomicAdd(&tokens, mine), atomicMax(&used, last);
+    for (int x = 32; x; x >>= 1) mine += __shfl_xor(mine, x);
+    if ((threadIdx.x & 63) == 0) atomicAdd(&tokens, mine);
     __syncthreads();
-    if (threadIdx.x == 0) out.top = top, out.used = used, out.tokens = tokens;
+    if (threadIdx.x == 0) out.top = top, out.tokens = tokens;
 }
 
 int part_count_of(size_t n) { return n <= SAMPLE_WHOLE ? 0 : (int)div_ceil(n, PART); }
