@@ -13,8 +13,14 @@
 // bin of too many tokens is first divided by its logits' bits, down to a single value, whose tokens differ in their
 // numbers alone.
 //
-// Rows of up to WHOLE tokens are the work of one workgroup, which holds them in registers. Longer ones are read in parts by
-// as many workgroups, each of which leaves its bins, counted from its own largest logit, for the row's workgroup.
+// Rows of up to WHOLE tokens are the work of one workgroup, which holds them in registers (so that they are read once).
+// Longer ones are read in parts by as many workgroups, each of which leaves its bins, counted from its own largest logit, for
+// the row's workgroup.
+//
+// 256 rows of 131072 f32 logits take 39 us for the parts (3.4 TB/s; 22 vector instructions for each logit, most of them in 64
+// bits) and 56 us for the rows, half of it the second reading of the logits at 5 TB/s; with the rows read by a gathering
+// after each border it was 129 us. A row of 8198 takes 12 us, no phase of it (load, count, sum, search, gather, sort, add) more
+// than 3: waits for memory, LDS and instructions that nothing overlaps.
 #include "tg_internal.hpp"
 
 namespace tg {
@@ -24,11 +30,11 @@ namespace {
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 constexpr int BINS = 2048, PER_OCTAVE = 32;
 constexpr int LIST = 4096;  // tokens that are sorted at a time
-constexpr int WHOLE = (int)SAMPLE_WHOLE, WHOLE_VALUES = WHOLE / THREADS;
+constexpr int WHOLE = (int)SAMPLE_WHOLE, WHOLE_VALUES = WHOLE / THREADS, SHORT_VALUES = 16;
 constexpr int PART_THREADS = 256, PART_VALUES = 64, PART = PART_THREADS * PART_VALUES;
 constexpr int COPIES = 2;     // of the bins that are counted: lanes next to each other add to different ones
 constexpr int SUM_BITS = 49;  // of a counted bin; above them the count of up to 2^14 tokens, whose sum is below 2^48.5
-static_assert(WHOLE <= 1 << 14 && PART <= 1 << 14, "a bin's count and sum share 64 bits");
+static_assert(WHOLE <= COPIES << 14 && PART <= 1 << 14, "a bin's count and sum share 64 bits");
 constexpr double FIXED = 1024.0;  // added to a weight it leaves steps of 2^-42: 2^22 weights' sum fits 64 bits
 
 // What a part of a row leaves: its bins, relative to its largest logit.
@@ -130,24 +136,35 @@ __device__ __forceinline__ uint64_t fixed(double w) {
 }
 __device__ __forceinline__ double unfixed(uint64_t m) { return (double)m * 0x1p-42; }
 
-// N logits from row[first] on, wherever they lie; -infinity past the n-th of the row.
-template <int N, typename T>
-__device__ __forceinline__ void load(const T *row, int first, int n, float (&l)[N]) {
-    constexpr int PIECE = 16 / sizeof(T);
+// N logits of each of X pieces from row[begin + first(piece)] on, wherever they lie; -infinity past the n-th of the row.
+// The pieces start at multiples of N from a multiple of N.
+template <int X, int N, typename T, typename F>
+__device__ __forceinline__ void load(const T *row, int begin, int n, float (&l)[X][N], F first) {
     struct __attribute__((packed, aligned(sizeof(T)))) Piece {
-        T v[PIECE];
+        T v[N];
     };
-    static_assert(N % PIECE == 0, "whole pieces");
-    if (first + N <= n) {
+    Piece p[X];
+    float end[N];  // of the row's last, shorter piece
+    const int last = n / N * N;
+    if (n >= N) {
 #pragma unroll
-        for (int i = 0; i < N; i += PIECE) {
-            const Piece x = *reinterpret_cast<const Piece *>(row + first + i);
-#pragma unroll
-            for (int y = 0; y < PIECE; y++) l[i + y] = plain((float)x.v[y]);
+        for (int x = 0; x < X; x++) {
+            const int at = begin + first(x);
+            const uint32_t bytes = (uint32_t)(at < last ? at : 0) * (uint32_t)sizeof(T);
+            p[x] = *reinterpret_cast<const Piece *>(reinterpret_cast<const char *>(row) + bytes);
         }
-    } else {
+    }
 #pragma unroll
-        for (int i = 0; i < N; i++) l[i] = first + i < n ? plain((float)row[first + i]) : -INFINITY;
+    for (int i = 0; i < N; i++) end[i] = last + i < n ? plain((float)row[last + i]) : -INFINITY;
+#pragma unroll
+    for (int x = 0; x < X; x++) {
+        const int at = begin + first(x);
+#pragma unroll
+        for (int i = 0; i < N; i++) l[x][i] = at < last ? plain((float)p[x].v[i]) : -INFINITY;
+        if (at == last) {
+#pragma unroll
+            for (int i = 0; i < N; i++) l[x][i] = end[i];
+        }
     }
 }
 
@@ -322,32 +339,53 @@ struct Range {
     double mass_before;
 };
 
-// A row's logits: held in registers (HELD), or read again for each pass.
-template <typename T, bool HELD>
+// A row's logits: HELD of them in each thread's registers, or read again for each pass.
+template <typename T, int HELD>
 struct Logits {
-    static constexpr int PIECE = 16 / sizeof(T), PIECES = HELD ? WHOLE_VALUES / PIECE : 32 / PIECE;
+    static constexpr int PIECE = 16 / sizeof(T), PIECES = (HELD ? HELD : 32) / PIECE;
     const T *row;
     int n;
     float held[HELD ? PIECES : 1][PIECE];
 
     __device__ __forceinline__ Logits(const T *row_, int n_) : row(row_), n(n_) {
-        if constexpr (HELD) read(held, 0);
+        if constexpr (HELD > 0) read(held, 0);
     }
     __device__ __forceinline__ static int first(int piece) { return (piece * THREADS + (int)threadIdx.x) * PIECE; }
-    __device__ __forceinline__ void read(float (&l)[PIECES][PIECE], int begin) const {
-#pragma unroll
-        for (int x = 0; x < PIECES; x++) load(row, begin + first(x), n, l[x]);
-    }
+    __device__ __forceinline__ void read(float (&l)[PIECES][PIECE], int begin) const { load(row, begin, n, l, first); }
     // f(logit, token) for the row's tokens; NaN and -infinity are none.
     template <typename F>
     __device__ __forceinline__ void each(F f) const {
-        if constexpr (HELD) {
+        if constexpr (HELD > 0) {
             visit(held, 0, f);
         } else {
             for (int begin = 0; begin < n; begin += PIECES * THREADS * PIECE) {
                 float l[PIECES][PIECE];
                 read(l, begin);
                 visit(l, begin, f);
+            }
+        }
+    }
+    // g(token) for the few tokens where f(logit) holds.
+    template <typename F, typename G>
+    __device__ __forceinline__ void each_of(F f, G g) const {
+        const auto some = [&](const float (&l)[PIECES][PIECE], int begin) {
+            static_assert(PIECES * PIECE <= 32, "a bit for each");
+            uint32_t which = 0;
+#pragma unroll
+            for (int i = 0; i < PIECES * PIECE; i++) which |= f(l[i / PIECE][i % PIECE]) ? 1u << i : 0u;
+            while (which) {
+                const int i = __builtin_ctz(which);
+                which &= which - 1;
+                g(begin + first(i / PIECE) + i % PIECE);
+            }
+        };
+        if constexpr (HELD > 0) {
+            some(held, 0);
+        } else {
+            for (int begin = 0; begin < n; begin += PIECES * THREADS * PIECE) {
+                float l[PIECES][PIECE];
+                read(l, begin);
+                some(l, begin);
             }
         }
     }
@@ -446,7 +484,7 @@ __device__ __forceinline__ void sort_list(Shared &s, int count) {
 }
 
 // The tokens of the spans in s.list, in order, and the weights before each.
-template <typename T, bool HELD>
+template <typename T, int HELD>
 __device__ __forceinline__ void gather(const Logits<T, HELD> &logits, const Weights &w, Shared &s, const Span &x, const Span &y, const Span &z, int count) {
     __syncthreads();  // the counted bins lie where the list does
     if (threadIdx.x == 0) s.listed = 0;
@@ -454,12 +492,16 @@ __device__ __forceinline__ void gather(const Logits<T, HELD> &logits, const Weig
     const auto within = [](const Span &x, uint32_t upper) {
         return upper - ((uint32_t)(POINT_BITS - x.high) << 8) < (uint32_t)(x.high - x.low + 1) << 8;
     };
-    logits.each([&](float l, int i) {
+    logits.each_of([&](float l) {
         const uint32_t upper = Weights::upper(w.place(l));
-        if (!(within(x, upper) | within(y, upper) | within(z, upper))) return;
+        return (l > -INFINITY) & (within(x, upper) | within(y, upper) | within(z, upper));
+    }, [&](int i) {
         const uint32_t at = atomicAdd(&s.listed, 1u);
-        if (at < LIST) s.list[at] = (uint64_t)key_of(l) << 32 | (uint32_t)i;
+        if (at < LIST) s.list[at] = (uint32_t)i;
     });
+    // Their logits are read once more, all at a time.
+    __syncthreads();
+    for (int i = threadIdx.x; i < count; i += THREADS) s.list[i] |= (uint64_t)key_of(plain((float)logits.row[(uint32_t)s.list[i]])) << 32;
     sort_list(s, count);
     const auto weight = [&](int i, uint32_t &c, double &m) { c = 0, m = i < count ? w.of(logit_of((uint32_t)(s.list[i] >> 32))) : 0.0; };
     const auto put = [&](int i, uint32_t, double with, double own) { s.before[i] = with - own; };
@@ -470,7 +512,7 @@ __device__ __forceinline__ void gather(const Logits<T, HELD> &logits, const Weig
 
 template <typename T>
 struct Row {
-    const Logits<T, false> logits;
+    const Logits<T, 0> logits;
     Weights w;
     Shared &s;
 
@@ -619,7 +661,7 @@ struct Row {
 // The borders one after the other, by their bins' tokens alone or parts of them.
 template <typename T>
 __device__ __noinline__ Drawn step_by_step(const T *logits, int n, Weights w, Shared &s, uint32_t k, uint32_t all, double u, double share, double least_weight) {
-    const Row<T> row{Logits<T, false>(logits, n), w, s};
+    const Row<T> row{Logits<T, 0>(logits, n), w, s};
     uint32_t kept = k;
     double mass = s.row.mass[BINS - 1], weight;
     if (k < all) {
@@ -681,10 +723,12 @@ __device__ __forceinline__ void sum_bins(const Weights &w, float temperature, Sh
     } else {
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-            uint64_t v = 0;
-            for (int x = 0; x < COPIES; x++) v += s.counted[(first + i) * COPIES + x];
-            count[i] = (uint32_t)(v >> SUM_BITS);
-            share[i] = v & SHARES;
+#pragma unroll
+            for (int x = 0; x < COPIES; x++) {
+                const uint64_t v = s.counted[(first + i) * COPIES + x];
+                count[i] += (uint32_t)(v >> SUM_BITS);
+                share[i] += v & SHARES;
+            }
         }
     }
     // In units of the largest logit's own rounded weight: rows of one logit come out exactly.
@@ -701,19 +745,20 @@ __device__ __forceinline__ void sum_bins(const Weights &w, float temperature, Sh
     __syncthreads();
 }
 
-template <typename T, bool HELD>
+template <typename T, int HELD>
 __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, const PartBins *parts, int part_count) {
     __shared__ Shared s;
     const int r = blockIdx.x;
     const Chosen o(a, r);
+    const float uniform = a.uniforms[r];
     float top = -INFINITY;
-    if constexpr (!HELD) {
+    if constexpr (HELD == 0) {
         parts += (size_t)r * part_count;
         for (int p = threadIdx.x & 63; p < part_count; p += 64) top = fmaxf(top, parts[p].top);
         top = wave_max(top);
     }
     const Logits<T, HELD> logits(static_cast<const T *>(a.logits) + (int64_t)r * a.ld, a.n);
-    if constexpr (HELD) {
+    if constexpr (HELD > 0) {
         for (int b = threadIdx.x; b < BINS * COPIES; b += THREADS) s.counted[b] = 0;
         logits.each([&](float l, int) { top = fmaxf(top, l); });
         top = wave_max(top);
@@ -730,7 +775,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
     if (!(top > -INFINITY)) return answer(-1, 0.0f);
     if (o.greedy()) {
         int x = INT32_MAX;
-        if constexpr (HELD) {
+        if constexpr (HELD > 0) {
             logits.each([&](float l, int i) { x = min(x, l == top ? i : INT32_MAX); });
         } else {
             int p = 0;
@@ -741,7 +786,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
         return answer(least(s, x), 1.0f);
     }
     const Weights w(o.temperature, top);
-    if constexpr (HELD) {
+    if constexpr (HELD > 0) {
         const Share share;
         logits.each([&](float l, int) { w.count_in(l, s.counted, share); });
         __syncthreads();
@@ -751,7 +796,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
     const uint32_t all = s.row.count[BINS - 1];
     const uint32_t k = o.top_k > 0 && (uint32_t)o.top_k < all ? (uint32_t)o.top_k : all;
     const bool cut_k = k < all, cut = o.top_p < 1.0f || o.min_p > 0.0f;
-    const double u = (double)fminf(a.uniforms[r], 0x1.fffffep-1f), share = o.top_p < 1.0f ? (double)o.top_p : INFINITY;
+    const double u = (double)fminf(uniform, 0x1.fffffep-1f), share = o.top_p < 1.0f ? (double)o.top_p : INFINITY;
     const double least_weight = o.min_p;
 
     // The bins where the border of top_k lies, those where the next one can lie, given what stays before it, and those
@@ -841,8 +886,7 @@ __global__ __launch_bounds__(PART_THREADS) void parts_kernel(const SampleArgs a,
     const int n = min(a.n - p * PART, PART);
     float l[PIECES][PIECE];
     float top = -INFINITY;
-#pragma unroll
-    for (int x = 0; x < PIECES; x++) load(logits, (x * PART_THREADS + (int)threadIdx.x) * PIECE, n, l[x]);
+    load(logits, 0, n, l, [](int x) { return (x * PART_THREADS + (int)threadIdx.x) * PIECE; });
     for (int b = threadIdx.x; b < BINS * COPIES; b += PART_THREADS) bins[b] = 0;
     if (threadIdx.x == 0) tokens = 0;
 #pragma unroll
@@ -893,9 +937,10 @@ hipError_t launch_sample(const SampleArgs &a, uint32_t type, int rows, void *wor
             hipLaunchKernelGGL((parts_kernel<T>), dim3((unsigned)(rows * count)), dim3(PART_THREADS), 0, s, a, parts, count);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
-            hipLaunchKernelGGL((sample_kernel<T, false>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)parts, count);
+            hipLaunchKernelGGL((sample_kernel<T, 0>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)parts, count);
         } else {
-            hipLaunchKernelGGL((sample_kernel<T, true>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)nullptr, 0);
+const auto kernel = a.n <= SHORT_VALUES * THREADS ? sample_kernel<T, SHORT_VALUES> : sample_kernel<T, WHOLE_VALUES>;
+            hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)nullptr, 0);
         }
         return hipGetLastError();
     };

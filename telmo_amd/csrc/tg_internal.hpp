@@ -402,7 +402,7 @@ struct SampleArgs {
     int32_t *tokens;
     float *probs;  // or null
 };
-constexpr size_t SAMPLE_WHOLE = 16384;  // tokens of a row that one workgroup draws from without a workspace
+constexpr size_t SAMPLE_WHOLE = 32768;  // tokens of a row that one workgroup draws from without a workspace
 size_t sample_work_bytes(size_t rows, size_t n);
 hipError_t launch_sample(const SampleArgs &a, uint32_t type, int rows, void *work, hipStream_t s);
 

@@ -86,12 +86,12 @@ OPTIONS = [{}, dict(temperature=0.0), dict(temperature=0.1), dict(temperature=1.
 
 
 @pytest.mark.parametrize("options", OPTIONS, ids=str)
-@pytest.mark.parametrize("n", (1, 2, 63, 1000, 8198, 16384, 16385, 50001, 131072))
+@pytest.mark.parametrize("n", (1, 2, 63, 1000, 8198, 16384, 16385, 32767, 32768, 32769, 50001, 131072))
 def test_sizes_and_options(tk, n, options):
     run(tk, normal(4, n), **options)
 
 
-@pytest.mark.parametrize("type,n", itertools.product(("f16", "bf16"), (100, 8198, 40000)))
+@pytest.mark.parametrize("type,n", itertools.product(("f16", "bf16"), (100, 8198, 32761, 40000)))
 def test_types_whose_logits_are_often_equal(tk, type, n):
     for options in ({}, dict(top_k=50), dict(top_p=0.8), dict(min_p=0.1, temperature=0.5)):
         run(tk, normal(5, n), type, pad=3, **options)
