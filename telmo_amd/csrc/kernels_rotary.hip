@@ -55,58 +55,49 @@ __device__ __forceinline__ void store_some(U *p, int n, bool aligned, const floa
 __host__ __device__ inline int pair_pieces(int dim) { return (dim / 2 + 7) / 8; }
 __host__ __device__ inline int pieces_of(int d, int dim) { return pair_pieces(dim) + (d - dim + 7) / 8; }
 
-// A piece's values in 32 bits: n of them from `first` on in v, and as many from `second` on in w (of interleaved pairs the
-// first eight and the rest).
-struct Piece {
-    float v[8], w[8];
-    int first, second, nv, nw;
-    bool v_aligned, w_aligned;  // whether `first` and `second` are multiples of 8
-};
-template <typename T>
-__device__ __forceinline__ Piece piece_of(const T *x, int piece, int d, int dim, bool interleaved, const float2 *table) {
+// put(first, n, whether `first` is a multiple of 8, n values in 32 bits) for the eights of a piece.
+template <typename T, typename F>
+__device__ __forceinline__ void with_piece(const T *x, int piece, int d, int dim, bool interleaved, const float2 *table, F put) {
     const int half = dim / 2, turned = pair_pieces(dim);
-    Piece p;
+    float v[8];
     if (piece >= turned) {
-        const int c = dim + (piece - turned) * 8;
-        p.first = c, p.nv = d - c < 8 ? d - c : 8, p.v_aligned = dim % 8 == 0;
-        p.second = 0, p.nw = 0, p.w_aligned = true;
-        load_some(x + c, p.nv, p.v_aligned, p.v);
-        return p;
+        const int c = dim + (piece - turned) * 8, n = d - c < 8 ? d - c : 8;
+        load_some(x + c, n, dim % 8 == 0, v);
+        put(c, n, dim % 8 == 0, v);
+        return;
     }
     const int i = piece * 8, n = half - i < 8 ? half - i : 8;
-    p.v_aligned = true;
+    float w[8];
     if (interleaved) {
-        p.first = 2 * i, p.nv = 2 * n < 8 ? 2 * n : 8;
-        p.second = 2 * i + 8, p.nw = 2 * n - p.nv, p.w_aligned = true;
-        load_some(x + p.first, p.nv, true, p.v);
-        load_some(x + p.second, p.nw, true, p.w);
+        const int m = 2 * n < 8 ? 2 * n : 8;
+        load_some(x + 2 * i, m, true, v);
+        load_some(x + 2 * i + 8, 2 * n - m, true, w);
         for (int e = 0; e < 8; e += 2) {
             const float2 s = e / 2 < n ? table[i + e / 2] : make_float2(0.0f, 0.0f);
             const float2 t = 4 + e / 2 < n ? table[i + 4 + e / 2] : make_float2(0.0f, 0.0f);
-            const float a = p.v[e], b = p.v[e + 1], f = p.w[e], g = p.w[e + 1];
-            p.v[e] = a * s.x - b * s.y, p.v[e + 1] = b * s.x + a * s.y;
-            p.w[e] = f * t.x - g * t.y, p.w[e + 1] = g * t.x + f * t.y;
+            const float a = v[e], b = v[e + 1], f = w[e], g = w[e + 1];
+            v[e] = a * s.x - b * s.y, v[e + 1] = b * s.x + a * s.y;
+            w[e] = f * t.x - g * t.y, w[e + 1] = g * t.x + f * t.y;
         }
+        put(2 * i, m, true, v);
+        put(2 * i + 8, 2 * n - m, true, w);
     } else {
-        p.first = i, p.nv = n;
-        p.second = half + i, p.nw = n, p.w_aligned = half % 8 == 0;
-        load_some(x + p.first, n, true, p.v);
-        load_some(x + p.second, n, p.w_aligned, p.w);
+        load_some(x + i, n, true, v);
+        load_some(x + half + i, n, half % 8 == 0, w);
         for (int e = 0; e < 8; e++) {
             const float2 t = e < n ? table[i + e] : make_float2(0.0f, 0.0f);
-            const float a = p.v[e], b = p.w[e];
-            p.v[e] = a * t.x - b * t.y;
-            p.w[e] = b * t.x + a * t.y;
+            const float a = v[e], b = w[e];
+            v[e] = a * t.x - b * t.y;
+            w[e] = b * t.x + a * t.y;
         }
+        put(i, n, true, v);
+        put(half + i, n, half % 8 == 0, w);
     }
-    return p;
 }
 template <typename T, typename U>
 __device__ __forceinline__ void rotate_piece(const T *x, U *out, int piece, int d, int dim, bool interleaved,
                                              const float2 *table) {
-    const Piece p = piece_of(x, piece, d, dim, interleaved, table);
-    store_some(out + p.first, p.nv, p.v_aligned, p.v);
-    store_some(out + p.second, p.nw, p.w_aligned, p.w);
+    with_piece(x, piece, d, dim, interleaved, table, [&](int at, int n, bool aligned, const float *v) { store_some(out + at, n, aligned, v); });
 }
 
 template <typename T, typename U>
@@ -337,23 +328,22 @@ __global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ld
             int8_t *exps = key ? c.k_exps + page * c.k_epage : c.v_exps + page * c.v_epage;
             exps += (int64_t)(row0 / c.block) * heads + h;
             const int pieces = pieces_of(d, dim);
-            // f(piece, the block's row) for the wavefront's pieces.
+            // f(the block's row, first, n, aligned, values) for the eights of the wavefront's pieces.
             const auto each = [&](auto f) {
                 for (int done = 0; done < n; done += some) {
                     if (pairs && some < n) fill(done);
                     const int now = min(some, n - done);
                     for (int t = lane; t < now * pieces; t += 64) {
                         const int row = t / pieces;
-                        f(piece_of(x + (done + row) * ld, t % pieces, d, dim, r.interleaved, table + row * pairs), done + row);
+                        with_piece(x + (done + row) * ld, t % pieces, d, dim, r.interleaved, table + row * pairs,
+                                   [&](int at, int count, bool aligned, const float *y) { f(done + row, at, count, aligned, y); });
                     }
                 }
             };
             uint32_t top = 0;
-            each([&](const Piece &p, int) {
-                for (int e = 0; e < 8; e++) {
-                    if (e < p.nv) top = max(top, e4m3_size(p.v[e]));
-                    if (e < p.nw) top = max(top, e4m3_size(p.w[e]));
-                }
+            each([&](int, int, int count, bool, const float *y) {
+                for (int e = 0; e < 8; e++)
+                    if (e < count) top = max(top, e4m3_size(y[e]));
             });
             for (int o = 32; o; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
             int now = e4m3_exponent(top);
@@ -366,19 +356,15 @@ __global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ld
                 }
             }
             const float down = two_to(-now);
-            each([&](const Piece &p, int row) {
+            each([&](int row, int at, int count, bool aligned, const float *y) {
                 if (!mine) return;
-                uint8_t *to = rows8 + (older + row) * ldc;
-                const auto store = [&](uint8_t *at, const float *y, int count, bool aligned) {
-                    const uint32_t a = e4m3_pack(y[0], y[1], y[2], y[3], down), b = e4m3_pack(y[4], y[5], y[6], y[7], down);
-                    if (count == 8 && aligned) {
-                        *reinterpret_cast<u32x2 *>(at) = u32x2{a, b};
-                    } else {
-                        for (int e = 0; e < count; e++) at[e] = (uint8_t)((e < 4 ? a : b) >> 8 * (e % 4));
-                    }
-                };
-                store(to + p.first, p.v, p.nv, p.v_aligned);
-                if (p.nw) store(to + p.second, p.w, p.nw, p.w_aligned);
+                uint8_t *to = rows8 + (older + row) * ldc + at;
+                const uint32_t a = e4m3_pack(y[0], y[1], y[2], y[3], down), b = e4m3_pack(y[4], y[5], y[6], y[7], down);
+                if (count == 8 && aligned) {
+                    *reinterpret_cast<u32x2 *>(to) = u32x2{a, b};
+                } else {
+                    for (int e = 0; e < count; e++) to[e] = (uint8_t)((e < 4 ? a : b) >> 8 * (e % 4));
+                }
             });
             if (mine && lane == 0) *exps = (int8_t)now;
         }
