@@ -440,7 +440,7 @@ typedef struct {
     size_t block;                     /* divides the page */
 } tg_cache_e4m3;
 /* tg_attention_paged_device over such a cache: q and out of desc's type. The keys and values count exactly; q is exact in
- * products of two (f16) or three (f32) parts. Weights round as there, f16's of chunks of rows to bf16 (half a step, 2^-9). */
+ * products of two (f16) or three (f32) parts. Weights round as there, f16's and f32's in as many parts. */
 int tg_attention_paged_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache);
 /* A workspace of this many bytes lets a call of `rows` query rows in `batch` sequences of up to `keys` keys
  * split long sequences over the GPU and join the parts; 0 where it would not. With a smaller one, or none,

@@ -52,11 +52,10 @@ struct Half<__bf16> {
 
 // What is multiplied, for rows of type T over keys of type C. Over e4m3 keys, which bf16 holds exactly with their power
 // of two, rows and weights are sums of bf16 parts of eight bits each: all of f16's bits in two, of f32's in three.
-// f16's weights, too, are rounded once.
 template <typename T, typename C>
 struct Parts16 {
     static constexpr bool BYTES = __is_same(C, e4m3), WIDE = __is_same(T, float);
-    static constexpr int ROW = !BYTES || __is_same(T, __bf16) ? 1 : WIDE ? 3 : 2, WEIGHT = WIDE ? 3 : 1;
+    static constexpr int ROW = !BYTES || __is_same(T, __bf16) ? 1 : WIDE ? 3 : 2, WEIGHT = WIDE ? 3 : ROW;
 };
 template <typename T, typename C>
 struct Multiplied {

@@ -8,6 +8,10 @@
 // eight rows, exchanged in registers before they are widened. K is widened with its row's power of two, which
 // multiplies V's weights instead, exactly. The output's columns are numbered so that a lane's loads are contiguous.
 // The wavefronts' results are joined in LDS, and those of the parts by a second kernel.
+//
+// 32 sequences of up to 8192 keys, 8 key heads of 128 and 32 heads in bf16: 279 MB in 70 us, 4.0 TB/s (a large copy 4.85, reads
+// and writes), and 5 for the join. Eight sequences of 750 keys take 17 us a call, as over keys of 16 bits (15):
+// page numbers, loads and sums wait for one another, not for bytes.
 #include "attn_launch.hpp"
 #include "attn_tile.hpp"
 

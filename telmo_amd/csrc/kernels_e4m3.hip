@@ -92,14 +92,9 @@ __device__ __forceinline__ void load16(const T *row, size_t k0, size_t k, bool a
     }
 }
 
-// The lane's part of a fragment of the rows: row `row` (zeros where there is none) from input 128 b on, rounded under
-// the exponent of the row's group, which the four lanes of a row find together.
-template <typename T>
-__device__ __forceinline__ i32x8 round_rows(const T *a, size_t lda, size_t row, bool real, size_t b, size_t k, bool aligned,
-                                            int quarter, int &e) {
-    float x[2][16] = {};
-    if (real)
-        for (int h = 0; h < 2; h++) load16(a + row * lda, b * 128 + h * 64 + quarter * 16, k, aligned, x[h]);
+// The lane's part of a fragment of the rows: 32 inputs of a row, rounded under the exponent of the row's group, which the
+// four lanes of a row find together.
+__device__ __forceinline__ i32x8 rounded(const float (&x)[2][16], int &e) {
     uint32_t top = 0;
     for (int h = 0; h < 2; h++)
         for (int i = 0; i < 16; i++) {
@@ -114,6 +109,40 @@ __device__ __forceinline__ i32x8 round_rows(const T *a, size_t lda, size_t row, 
             r[4 * h + i] = (int)e4m3_pack(x[h][4 * i], x[h][4 * i + 1], x[h][4 * i + 2], x[h][4 * i + 3], down);
     return r;
 }
+// Of row `row` (zeros where there is none) from input 128 b on.
+template <typename T>
+__device__ __forceinline__ i32x8 round_rows(const T *a, size_t lda, size_t row, bool real, size_t b, size_t k, bool aligned,
+                                            int quarter, int &e) {
+    float x[2][16] = {};
+    if (real)
+        for (int h = 0; h < 2; h++) load16(a + row * lda, b * 128 + h * 64 + quarter * 16, k, aligned, x[h]);
+    return rounded(x, e);
+}
+// The lane's inputs as they lie in memory: a block's can be on their way while the one before is worked on.
+template <typename T>
+struct Inputs {
+    static constexpr int PIECE = 16 / sizeof(T);
+    u32x4 v[2][16 / PIECE];
+    __device__ __forceinline__ void load(const T *at) {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 16 / PIECE; i++) v[h][i] = *reinterpret_cast<const u32x4 *>(at + h * 64 + i * PIECE);
+    }
+    __device__ __forceinline__ i32x8 round(int &e) const {
+        float x[2][16];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                struct Piece {
+                    T v[PIECE];
+                };
+                x[h][i] = (float)__builtin_bit_cast(Piece, v[h][i / PIECE]).v[i % PIECE];
+            }
+        return rounded(x, e);
+    }
+};
 
 // The rows' fragments and powers of two, a wavefront for 16 rows of a block of inputs at a time.
 template <typename T>
@@ -216,9 +245,13 @@ struct Outputs {
 // ------------------------------------------------------------------------------------- few rows
 
 // MT x 16 rows by PN x 16 outputs of a workgroup, the blocks of inputs spread over its wavefronts, whose sums LDS joins in
-// their order. FUSED: 16 rows at most, rounded as they are read; otherwise from their fragments.
+// their order. 16 rows at most are rounded as they are read, more come from their fragments.
+//
+// Bound by the weights' bytes: 16 rows by 4096 x 16384 (68 MB) 20.8 us, 3.3 TB/s (a large copy 4.85), the
+// launch, the rows and their rounding before the first product among them; one row by 2560 x 640 takes the time of a call.
 constexpr int FEW_WAVES = 8;
-template <typename T, int MT, int PN, bool FUSED>
+enum Source { FRAGMENTS, WHOLE, ANY };  // rows rounded before; rounded here, in whole aligned blocks of inputs, or not
+template <typename T, int MT, int PN, Source FROM>
 __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t lda, size_t k, bool aligned, Rounded in,
                                                              E4m3Panels w, E4m3Out o) {
     constexpr int SLOTS = MT * PN >= 8 ? 4 : 8;  // wavefronts' sums in LDS at a time
@@ -232,42 +265,53 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
     const int b0 = wave * per, b1 = b0 + per < blocks ? b0 + per : blocks;
     const uint8_t *wp[PN];
     for (int p = 0; p < PN; p++) wp[p] = w.values + (size_t)min(panel0 + p, (int)w.panels - 1) * blocks * 2048 + lane * 16;
-    const float *scale = w.scales + (size_t)(panel0 / 8) * blocks;
-    // The next block's weights are on their way while a block is multiplied.
-    i32x8 wf[PN], next[PN];
-    const auto load = [&](int b) {
+    const Scalar scale = (Scalar)(w.scales + (size_t)(panel0 / 8) * blocks);
+    // The next block's weights and rows are on their way while a block is multiplied (rows past the last are read as it).
+    struct Block {
+        i32x8 w[PN], rows[MT];
+        uint32_t power[MT];
+        Inputs<T> inputs;
+    } now, next;
+    const size_t row = lane & 15;
+    const T *own = FROM == WHOLE ? a + (row < o.m ? row : o.m - 1) * lda + quarter * 16 : nullptr;
+    const auto load = [&](int b) __attribute__((always_inline)) {
+        if constexpr (FROM == WHOLE) next.inputs.load(own + (size_t)b * 128);
+        if constexpr (FROM == FRAGMENTS)
+#pragma unroll
+            for (int t = 0; t < MT; t++) {
+                const size_t tile = min(tile0 + t, (int)in.tiles - 1);
+                const i32x4 *at = reinterpret_cast<const i32x4 *>(in.values + (tile * blocks + b) * 2048 + lane * 16);
+                next.rows[t] = joined(at[0], at[64]);
+                next.power[t] = reinterpret_cast<const uint8_t *>(in.powers + ((size_t)(b / 4) * in.tiles + tile) * 16 + row)[b % 4];
+            }
 #pragma unroll
         for (int p = 0; p < PN; p++) {
             const i32x4 *at = reinterpret_cast<const i32x4 *>(wp[p] + (size_t)b * 2048);
-            next[p] = joined(at[0], at[64]);
+            next.w[p] = joined(at[0], at[64]);
         }
     };
     if (b0 < b1) load(b0);
     for (int b = b0; b < b1; b++) {
-#pragma unroll
-        for (int p = 0; p < PN; p++) wf[p] = next[p];
+        now = next;
         load(b + 1 < b1 ? b + 1 : b);
-        const auto panel = [&](int p) { return Operand<true>(wf[p], 1.0f); };
         const float s = scale[b];
 #pragma unroll
         for (int t = 0; t < MT; t++) {
             i32x8 af;
             float up;
-            if constexpr (FUSED) {
-                const size_t row = lane & 15;
-                int e;
-                af = round_rows(a, lda, row, row < o.m, b, k, aligned, quarter, e);
-                up = two_to(e);
+            if constexpr (FROM == FRAGMENTS) {
+                af = now.rows[t];
+                up = power_of(now.power[t]);
             } else {
-                const size_t tile = min(tile0 + t, (int)in.tiles - 1);
-                const i32x4 *at = reinterpret_cast<const i32x4 *>(in.values + (tile * blocks + b) * 2048 + lane * 16);
-                af = joined(at[0], at[64]);
-                up = power_of(reinterpret_cast<const uint8_t *>(in.powers + ((size_t)(b / 4) * in.tiles + tile) * 16 + (lane & 15))[b % 4]);
+                int e;
+                if constexpr (FROM == WHOLE) af = now.inputs.round(e);
+                else af = round_rows(a, lda, row, row < o.m, b, k, aligned, quarter, e);
+                up = two_to(e);
             }
             const Operand<true> rows(af, up);
 #pragma unroll
             for (int p = 0; p < PN; p++) {
-                const Operand<true> outs = panel(p);
+                const Operand<true> outs(now.w[p], 1.0f);
                 f32x4 part = {};
 #pragma unroll
                 for (int i = 0; i < 4; i++) part = block_product(outs, rows, 0, i, part);
@@ -334,6 +378,11 @@ __device__ __forceinline__ void wait_copies() {
 // Workgroups of KG groups of WM x WN wavefronts of TM x TN tiles each. The groups share the outputs and take every KG-th
 // block of inputs, and add up their sums in LDS. LDS holds two stages of a block for each group: while one is worked on, the
 // next is copied to the other.
+//
+// 8192 x 8192 x 8192 into bf16 takes 43 us to round the rows (at the rate of a copy) and 470 by tiles of 256 x 256, 2340 TFLOP/s:
+// a block of inputs is 2112 cycles of a CU's matrix instructions, and 192 KB that its wavefronts read from LDS and 64 KB that
+// are copied there are 2048 of LDS, which the two share badly. 750 rows by 1024 x 4096 into f32, EXACT, take 20 us: 192 tiles
+// for 256 CUs, eight blocks of inputs each, between a start and an end that nothing overlaps.
 template <int WM, int WN, int TM, int TN, int KG, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, E4m3Panels w, E4m3Out o, int m_tiles, int n_tiles) {
     constexpr int WAVES = WM * WN, RT = WM * TM, PT = WN * TN;     // wavefronts, row tiles and panels of a group
@@ -522,23 +571,25 @@ hipError_t launch_tiles(const Rounded &in, const E4m3Panels &w, const E4m3Out &o
     return hipGetLastError();
 }
 
-template <typename T, int MT, int PN, bool FUSED>
+template <typename T, int MT, int PN, Source FROM>
 hipError_t launch_few(const T *a, size_t lda, size_t k, bool aligned, const Rounded &in, const E4m3Panels &w, const E4m3Out &o,
                       hipStream_t s) {
     const dim3 grid((unsigned)div_ceil(w.panels, PN), (unsigned)div_ceil(div_ceil(o.m, 16), MT));
-    hipLaunchKernelGGL((few_kernel<T, MT, PN, FUSED>), grid, dim3(64 * FEW_WAVES), 0, s, a, lda, k, aligned, in, w, o);
+    hipLaunchKernelGGL((few_kernel<T, MT, PN, FROM>), grid, dim3(64 * FEW_WAVES), 0, s, a, lda, k, aligned, in, w, o);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t product(const T *a, size_t lda, size_t k, const E4m3Panels &w, const E4m3Out &o, const Rounded &in, hipStream_t s) {
     const bool aligned = reinterpret_cast<uintptr_t>(a) % 16 == 0 && lda * sizeof(T) % 16 == 0;
-    if (!k) return launch_few<float, 2, 2, false>(nullptr, 0, k, aligned, in, w, o, s);  // the epilogue of empty sums
+    if (!k) return launch_few<float, 2, 2, FRAGMENTS>(nullptr, 0, k, aligned, in, w, o, s);  // the epilogue of empty sums
     if (o.m <= E4M3_FEW) {
         // Two panels share the rounding of the rows where that leaves two workgroups to a CU (us, one panel and two): 16 rows
         // by 4096 x 16384 30.5 20.9, one by 8192 x 8192 29.9 26.4, by 4096 x 4096 11.3 11.8.
-        if (w.panels >= 512) return launch_few<T, 1, 2, true>(a, lda, k, aligned, in, w, o, s);
-        return launch_few<T, 1, 1, true>(a, lda, k, aligned, in, w, o, s);
+        const bool two = w.panels >= 512;
+        if (aligned && k % 128 == 0)
+            return two ? launch_few<T, 1, 2, WHOLE>(a, lda, k, aligned, in, w, o, s) : launch_few<T, 1, 1, WHOLE>(a, lda, k, aligned, in, w, o, s);
+        return two ? launch_few<T, 1, 2, ANY>(a, lda, k, aligned, in, w, o, s) : launch_few<T, 1, 1, ANY>(a, lda, k, aligned, in, w, o, s);
     }
     const size_t units = in.tiles * in.blocks, blocks = div_ceil(units, 4);
     hipLaunchKernelGGL((round_rows_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, a, lda, o.m,
@@ -560,8 +611,8 @@ hipError_t product(const T *a, size_t lda, size_t k, const E4m3Panels &w, const 
         if (tiles > 256) return launch_tiles<2, 2, 4, 4, 1, true>(in, w, o, s);
         if (tiles >= 128) return launch_tiles<2, 2, 4, 4, 2, true>(in, w, o, s);
     }
-    if (div_ceil(in.tiles, 4) * div_ceil(w.panels, 2) >= 512) return launch_few<float, 4, 2, false>(nullptr, 0, k, aligned, in, w, o, s);
-    return launch_few<float, 2, 2, false>(nullptr, 0, k, aligned, in, w, o, s);
+    if (div_ceil(in.tiles, 4) * div_ceil(w.panels, 2) >= 512) return launch_few<float, 4, 2, FRAGMENTS>(nullptr, 0, k, aligned, in, w, o, s);
+    return launch_few<float, 2, 2, FRAGMENTS>(nullptr, 0, k, aligned, in, w, o, s);
 }
 
 }  // namespace

@@ -814,7 +814,7 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(const SampleArgs a, con
     if (cut) {
         int low_floor = BINS, high_floor = BINS;
         if (o.min_p > 0.0f) {  // the first bin below min_p, or the one before or after it where roundings decide
-            const double past = -__log2f(o.min_p) * PER_OCTAVE;
+            const double past = fmaxf(-__log2f(o.min_p) * PER_OCTAVE, -4.0f);
             low_floor = past < BINS ? max((int)past - 1, 0) : BINS - 1;
             high_floor = past < BINS - 4 ? max((int)past + 3, 0) : BINS - 1;
         }

@@ -5,7 +5,7 @@ import itertools
 import numpy as np
 import pytest
 
-from attention_oracle import HALF_STEP, attend, rotate, shown_pairs, tolerance
+from attention_oracle import attend, rotate, shown_pairs, tolerance
 from e4m3_oracle import VALUES, encode, exponent, half_step
 from test_gpu_attention import check, distance_bias, dtype, floats, ints, rows_of, say
 
@@ -16,8 +16,8 @@ TYPES = ("f32", "f16", "bf16")
 
 def allowed(type, d, keys, size, top):
     """The attention's tolerance with what eight-bit keys change: f16 and f32 rows are multiplied in two or three parts,
-    up to three times the sums (counted as four by the form for position rows), and f16's weights are rounded to bf16."""
-    return tolerance(type, d, keys, size, top, type != "bf16") + (top * HALF_STEP["bf16"] if type == "f16" else 0.0)
+    up to three times the sums (counted as four by the form for position rows)."""
+    return tolerance(type, d, keys, size, top, type != "bf16")
 
 
 def pages_of(rng, pages, page, blocks, kv_heads, d, low=-6, high=3):

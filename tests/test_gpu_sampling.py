@@ -148,6 +148,25 @@ def test_options_of_each_row(tk):
             top_p=rng.choice([0.2, 0.9, 1.0, 1.5], rows), min_p=rng.choice([0.0, 0.1, 2.0, -1.0], rows))
 
 
+@pytest.mark.parametrize("n", (50, 9000, 40000))
+def test_options_of_rows_past_their_ranges(tk, n):
+    """A smallest share past 1 leaves the first token (and its equals), whatever it is; NaN stands for none."""
+    x = np.round(normal(8, n))
+    run(tk, x, min_p=np.array([np.inf, 3e38, 1.0001, 1.0, 1e-45, 1e-30, 0.0, -np.inf]))
+    import torch
+
+    import telmo_amd
+
+    logits, u = torch.from_numpy(x.astype(np.float32)).cuda(), torch.linspace(0, 0.99, 8, device="cuda")
+    drawn = []
+    for options in ({}, dict(top_p=torch.full((8,), np.nan, device="cuda"), min_p=torch.full((8,), np.nan, device="cuda"))):
+        sampler = telmo_amd.Sampler(tk, **options)
+        drawn.append(torch.zeros(8, dtype=torch.int32, device="cuda"))
+        sampler.sample(logits, u, drawn[-1], workspace=torch.zeros(sampler.workspace_bytes(8, n), dtype=torch.uint8, device="cuda"))
+    tk.synchronize()
+    assert torch.equal(*drawn)
+
+
 def test_many_rows_and_empty_calls(tk):
     run(tk, normal(1500, 300), top_p=0.9)
     run(tk, normal(0, 300))
