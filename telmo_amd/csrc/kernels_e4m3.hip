@@ -18,6 +18,8 @@
 // Operands lie in memory as the instruction takes them ("fragments"): for 16 rows (outputs) and a block of 128 inputs 2 KB
 // in two halves of 64 lanes by 16 bytes, lane 16 g + r of half h holding the inputs 64 h + 16 g + [0, 16) of row r. Both
 // sides number the inputs alike, so any such order gives the sum. Reads of LDS and copies to it are linear.
+#include <type_traits>
+
 #include "e4m3.hpp"
 #include "e4m3_product.hpp"
 
@@ -97,16 +99,27 @@ __device__ __forceinline__ void load16(const T *row, size_t k0, size_t k, bool a
 __device__ __forceinline__ i32x8 rounded(const float (&x)[2][16], int &e) {
     uint32_t top = 0;
     for (int h = 0; h < 2; h++)
-        for (int i = 0; i < 16; i++) {
-            const uint32_t size = e4m3_size(x[h][i]);
-            top = top > size ? top : size;
-        }
+        for (int i = 0; i < 16; i++) top = max(top, __float_as_uint(x[h][i]) & 0x7fffffffu);
+    // Below 2^127 no value needs a bound, or a look at whether it is finite: three operations for each instead of nine.
+    const bool plain = !__any(top >= 0x7f000000u);
+    if (!plain) {
+        top = 0;
+        for (int h = 0; h < 2; h++)
+            for (int i = 0; i < 16; i++) top = max(top, e4m3_size(x[h][i]));
+    }
     e = e4m3_exponent(__float_as_uint(max_of_quarters(__uint_as_float(top))));
     const float down = two_to(-e);
     i32x8 r;
     for (int h = 0; h < 2; h++)
-        for (int i = 0; i < 4; i++)
-            r[4 * h + i] = (int)e4m3_pack(x[h][4 * i], x[h][4 * i + 1], x[h][4 * i + 2], x[h][4 * i + 3], down);
+        for (int i = 0; i < 4; i++) {
+            const float *y = x[h] + 4 * i;
+            if (plain) {
+                const int two = __builtin_amdgcn_cvt_pk_fp8_f32(y[0] * down, y[1] * down, 0, false);
+                r[4 * h + i] = __builtin_amdgcn_cvt_pk_fp8_f32(y[2] * down, y[3] * down, two, true);
+            } else {
+                r[4 * h + i] = (int)e4m3_pack(y[0], y[1], y[2], y[3], down);
+            }
+        }
     return r;
 }
 // Of row `row` (zeros where there is none) from input 128 b on.
@@ -247,8 +260,9 @@ struct Outputs {
 // MT x 16 rows by PN x 16 outputs of a workgroup, the blocks of inputs spread over its wavefronts, whose sums LDS joins in
 // their order. 16 rows at most are rounded as they are read, more come from their fragments.
 //
-// Bound by the weights' bytes: 16 rows by 4096 x 16384 (68 MB) 20.8 us, 3.3 TB/s (a large copy 4.85), the
-// launch, the rows and their rounding before the first product among them; one row by 2560 x 640 takes the time of a call.
+// Bound by the weights' bytes: 16 rows of bf16 by 4096 x 16384 (68 MB) 16.8 us, 4.1 TB/s (a large copy 4.85). The rows' rounding
+// is what a wavefront works longest on: with nine operations a value instead of three it took 19.5, and where each block
+// waited for its rows 20.8. One row by 640 x 2560 takes the time of a call.
 constexpr int FEW_WAVES = 8;
 enum Source { FRAGMENTS, WHOLE, ANY };  // rows rounded before; rounded here, in whole aligned blocks of inputs, or not
 template <typename T, int MT, int PN, Source FROM>
@@ -584,12 +598,19 @@ hipError_t product(const T *a, size_t lda, size_t k, const E4m3Panels &w, const 
     const bool aligned = reinterpret_cast<uintptr_t>(a) % 16 == 0 && lda * sizeof(T) % 16 == 0;
     if (!k) return launch_few<float, 2, 2, FRAGMENTS>(nullptr, 0, k, aligned, in, w, o, s);  // the epilogue of empty sums
     if (o.m <= E4M3_FEW) {
-        // Two panels share the rounding of the rows where that leaves two workgroups to a CU (us, one panel and two): 16 rows
-        // by 4096 x 16384 30.5 20.9, one by 8192 x 8192 29.9 26.4, by 4096 x 4096 11.3 11.8.
-        const bool two = w.panels >= 512;
-        if (aligned && k % 128 == 0)
-            return two ? launch_few<T, 1, 2, WHOLE>(a, lda, k, aligned, in, w, o, s) : launch_few<T, 1, 1, WHOLE>(a, lda, k, aligned, in, w, o, s);
-        return two ? launch_few<T, 1, 2, ANY>(a, lda, k, aligned, in, w, o, s) : launch_few<T, 1, 1, ANY>(a, lda, k, aligned, in, w, o, s);
+        // Each workgroup reads the rows again, and rounds them: two panels share that where they leave a workgroup to a CU, and
+        // four where twice as many bytes of rows would be read (us, one panel, two and four): 16 rows of bf16 by 4096 x 4096 8.5
+        // 9.6 12.4, by 4096 x 8192 14.3 10.6 14.1, by 4096 x 16384 24.8 16.6 20.5, by 1024 x 32768 22.6 13.1 11.7; of f32 by
+        // 4096 x 4096 12.5 13.3 16.2, by 4096 x 8192 21.9 14.4 17.4, by 4096 x 16384 40.7 24.9 23.1; one row of bf16 by 8192 x
+        // 8192 20.9 18.2 20.3.
+        const auto launch = [&](auto pn) {
+            constexpr int PN = decltype(pn)::value;
+            if (aligned && k % 128 == 0) return launch_few<T, 1, PN, WHOLE>(a, lda, k, aligned, in, w, o, s);
+            return launch_few<T, 1, PN, ANY>(a, lda, k, aligned, in, w, o, s);
+        };
+        if (w.panels * sizeof(T) >= 4096) return launch(std::integral_constant<int, 4>{});
+        if (w.panels >= 512) return launch(std::integral_constant<int, 2>{});
+        return launch(std::integral_constant<int, 1>{});
     }
     const size_t units = in.tiles * in.blocks, blocks = div_ceil(units, 4);
     hipLaunchKernelGGL((round_rows_kernel<T>), dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, s, a, lda, o.m,
