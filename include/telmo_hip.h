@@ -488,9 +488,9 @@ int tg_cache_append_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, cons
  * e^((l_i - max) / temperature) and the tokens in the order of falling logits, equal ones by their numbers: the first top_k
  * stay, of those the ones before which less than top_p of their weights lie, of those the ones with w >= min_p, the first
  * one always. The token is the first at which the running sum of those that stay exceeds u times the whole of it, its
- * probability its weight over that. Weights and sums are held in 64 bits. Temperature 0 (or less, or NaN): the largest
- * logit, probability 1. NaN and -infinity are never drawn, +infinity shares the row with its like; a row of none gives
- * token -1, probability 0. */
+ * probability its weight over that. Weights and sums are held in 64 bits (sums to 2^-41 of them). Temperature 0 (or less, or
+ * NaN): the largest logit, probability 1. NaN and -infinity are never drawn, +infinity shares the row with its like; a row of
+ * none gives token -1, probability 0. */
 typedef struct {
     float temperature;          /* for all rows: finite, not negative */
     int32_t top_k;              /* 0: all */

@@ -42,8 +42,9 @@ def draw(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 
 
 def run(tk, x, type="f32", seed=1, uniforms=None, pad=0, **options):
-    """Draws from x [rows, n] and checks each row. Running sums are off by 2^-43 of the largest weight for each token, so a
-    draw nearer than n 2^-42 to a border may fall on its other side."""
+    """Draws from x [rows, n] and checks each row. Running sums are off by 2^-41 of themselves (half a step of 2^-40 of
+    its bin's lower edge for each weight; where a crowded bin is divided, 2^-43 of the largest weight for each token), so a
+    draw nearer than n 2^-42 to a border (there is none for n = 1) may fall on its other side."""
     import torch
 
     import telmo_amd
