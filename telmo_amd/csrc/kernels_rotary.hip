@@ -188,7 +188,7 @@ __device__ __forceinline__ void lower_rows(uint8_t *rows8, int64_t ldc, int olde
 // of a rotated half each, or 16 in a row) of every 64 / pieces-th row, STEPS of them at a time, and keeps a block of as many
 // in registers from the largest to the rounding; a longer block's rows are read again. No piece is cut, so that a step is
 // loads and products without branches. Bound by memory: 8188 rows of 8 heads of 128 in f32, keys rotated, blocks of 16, 84 MB
-// in 18 us (4.6 TB/s); with four steps, and so half the wavefronts, 23, by cut pieces 25. Eight single rows take 7.
+// in 18 us (4.6 TB/s); with four steps, and so half the wavefronts, 23, by cut pieces 25. Eight single rows take 6.
 template <typename T, bool HALVES>
 __global__ __launch_bounds__(THREADS) void append8_whole_kernel(const T *k, int64_t ldk, int64_t hsk, const T *v, int64_t ldv,
                                                                 int64_t hsv, const Cache8 c, int heads, int d, const AttnSeqs q,

@@ -19,7 +19,7 @@
 //
 // 256 rows of 131072 f32 logits take 39 us for the parts (3.4 TB/s; 22 vector instructions for each logit, most of them in 64
 // bits) and 56 us for the rows, half of it the second reading of the logits at 5 TB/s; with the rows read by a gathering
-// after each border it was 129 us. A row of 8198 takes 12 us, no phase of it (load, count, sum, search, gather, sort, add) more
+// after each border it was 129 us. A row of 8198 takes 14 us, no phase of it (load, count, sum, search, gather, sort, add) more
 // than 3: waits for memory, LDS and instructions that nothing overlaps.
 #include "tg_internal.hpp"
 
