@@ -550,6 +550,7 @@ struct Row {
         Range r{0, 0, 0, 0, 0.0};
         const int bin = first_bin(s.row, [&](int b, uint32_t c, double m) { return f(b >= floor.bin, c, m); }, r);
         const uint32_t all = key_of(-INFINITY), start = key_of(w.top);
+        __syncthreads();  // all have the floor's key, and the ends of the range before
         if (threadIdx.x < 128) {  // a wavefront for either end
             const int b = bin + (threadIdx.x >> 6);
             const uint32_t key = b == 0 ? start : b == BINS ? all : first_key(start, all, [&](uint32_t k) { return w.bin(plain(logit_of(k))) >= b; });
