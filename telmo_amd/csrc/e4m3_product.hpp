@@ -14,6 +14,9 @@ struct E4m3Panels {
     const float *scales;
     size_t panels, blocks;
 };
+// The row of scales of a panel's outputs, eight panels each. Workgroups reach past the last panel, whose row stands for
+// those that there are not.
+__host__ __device__ inline size_t e4m3_scale_row(size_t panel, size_t panels) { return (panel < panels ? panel : panels - 1) / 8; }
 inline size_t e4m3_weight_bytes(size_t n, size_t k) { return div_ceil(n, 16) * div_ceil(k, 128) * 2048; }
 
 // Outputs: m rows of n, ld apart, of a type of rows. aligned: four of a row from a multiple of four on lie aligned.

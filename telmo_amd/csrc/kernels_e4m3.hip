@@ -279,7 +279,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
     const int b0 = wave * per, b1 = b0 + per < blocks ? b0 + per : blocks;
     const uint8_t *wp[PN];
     for (int p = 0; p < PN; p++) wp[p] = w.values + (size_t)min(panel0 + p, (int)w.panels - 1) * blocks * 2048 + lane * 16;
-    const Scalar scale = (Scalar)(w.scales + (size_t)(panel0 / 8) * blocks);
+    const Scalar scale = (Scalar)(w.scales + e4m3_scale_row(panel0, w.panels) * blocks);
     // The next block's weights and rows are on their way while a block is multiplied (rows past the last are read as it).
     struct Block {
         i32x8 w[PN], rows[MT];
@@ -438,7 +438,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
                           lane * 4, lds0 + stage * KG * STAGE + CHUNKS * 1024 + wave % 4 * 256);
     };
     // A scalar load: one in a vector register would wait for the copies that left before it.
-    const Scalar scale = (Scalar)(w.scales + (size_t)((panel0 + wn * TN) / 8) * blocks);
+    const Scalar scale = (Scalar)(w.scales + e4m3_scale_row(panel0 + wn * TN, w.panels) * blocks);
 
     f32x4 acc[TM][TN] = {};
     const auto work = [&](int b, int stage) __attribute__((always_inline)) {
