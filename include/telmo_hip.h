@@ -259,7 +259,8 @@ int tg_encode_e4m3(const float *w, size_t n, size_t k, uint8_t *values, size_t v
 /* The product on device pointers, queued on the context's stream; a of `type` and c of `c_type` (TG_F32, TG_F16 or
  * TG_BF16), rows at any stride, bias f32. epi as in tg_matmul_device, in f32; c is rounded once. Nothing is allocated: the
  * rounded rows of more than 16 go to the workspace (device, 16-byte aligned, tg_linear_e4m3_workspace_bytes(m, k)
- * bytes; 0 up to 16 rows), which calls that may overlap on the GPU must not share. a, c and workspace must not overlap. */
+ * bytes; 0 up to 16 rows), which calls that may overlap on the GPU must not share. a, c and workspace must not overlap. At most
+ * 2^24 rows, and 2^23 tiles of 128 x 128 outputs. */
 int tg_linear_e4m3_device(tg_ctx *ctx, uint32_t type, const void *a, size_t a_len, size_t lda, size_t m,
                           const tg_weights_e4m3 *w, uint32_t c_type, void *c, size_t c_len, size_t ldc, const tg_epilogue *epi,
                           void *workspace, size_t workspace_len);

@@ -2008,6 +2008,7 @@ int tg_linear_e4m3_device(tg_ctx *ctx, uint32_t type, const void *a, size_t a_le
     if (!attn_type(type) || !attn_type(c_type)) return fail(ctx, TG_ERR_ARG, "types must be f32, f16 or bf16");
     if (m == 0 || n == 0) return ctx ? TG_OK : TG_ERR_NULL;
     if (m > MAX_E4M3) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^24 rows");
+    if (!tg::e4m3_fits(m, n)) return fail(ctx, TG_ERR_UNSUPPORTED, "more than 2^23 tiles of 128 x 128 outputs");
     if (lda < k || ldc < n) return fail(ctx, TG_ERR_SHAPE, "lda must be >= k and ldc >= n");
     if (a_len < span(m, lda, k)) return fail(ctx, TG_ERR_SHAPE, "a is too short");
     if (c_len < span(m, ldc, n)) return fail(ctx, TG_ERR_SHAPE, "c is too short");
@@ -2031,9 +2032,7 @@ int tg_linear_e4m3_device(tg_ctx *ctx, uint32_t type, const void *a, size_t a_le
                         epi_args(epi, nullptr, false)};
     std::lock_guard<std::mutex> g(ctx->mu);
     TG_HIP(ctx, hipSetDevice(ctx->device));
-    const hipError_t e = tg::launch_e4m3_product(type, a, lda, k, w->d, o, workspace, ctx->stream);
-    if (e == hipErrorInvalidConfiguration) return fail(ctx, TG_ERR_UNSUPPORTED, "more tiles than a launch holds");
-    TG_HIP(ctx, e);
+    TG_HIP(ctx, tg::launch_e4m3_product(type, a, lda, k, w->d, o, workspace, ctx->stream));
     return TG_OK;
 }
 

@@ -35,6 +35,10 @@ struct Rounded {
     uint32_t *powers;
     size_t tiles, blocks, quads;
 };
+// Tiles of 128 x 128 outputs that a call may have: as workgroups of 256 threads, or a quarter as many of 512, a launch's
+// threads stay below 2^32. Their outputs in 16 bits fill a GPU's memory.
+constexpr size_t E4M3_TILES = (size_t)1 << 23;
+inline bool e4m3_fits(size_t m, size_t n) { return div_ceil(m, 128) * div_ceil(n, 128) <= E4M3_TILES; }
 // Rows that are rounded as they are read, without a workspace.
 constexpr size_t E4M3_FEW = 16;
 inline size_t e4m3_work_bytes(size_t m, size_t k) {

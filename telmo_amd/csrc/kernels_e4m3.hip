@@ -579,7 +579,6 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
 template <int WM, int WN, int TM, int TN, int KG, bool EXACT>
 hipError_t launch_tiles(const Rounded &in, const E4m3Panels &w, const E4m3Out &o, hipStream_t s) {
     const size_t m_tiles = div_ceil(in.tiles, WM * TM), n_tiles = div_ceil(w.panels, WN * TN);
-    if (m_tiles * n_tiles > INT32_MAX / 1024) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL((tile_kernel<WM, WN, TM, TN, KG, EXACT>), dim3((unsigned)(m_tiles * n_tiles)), dim3(64 * WM * WN * KG), 0, s, in, w, o,
                        (int)m_tiles, (int)n_tiles);
     return hipGetLastError();
