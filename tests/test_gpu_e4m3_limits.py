@@ -21,8 +21,41 @@ def test_too_many_tiles_leave_the_workspace_alone(tk):
     rc = _lib.lib().tg_linear_e4m3_device(tk._ctx, 0, a.data_ptr(), a.numel(), k, m, w._handle, 0, 1 << 50, m * n, n, None,
                                           space.data_ptr(), space.numel())
     tk.synchronize()
-    assert rc == UNSUPPORTED
-    assert bool((space == 0xA5).all())
-    # An allocator's leftovers are not for the tests after this one.
+    left_alone = bool((space == 0xA5).all())  # not in the assertion, whose report would take the tensor apart
     del a, space
     torch.cuda.empty_cache()
+    assert rc == UNSUPPORTED and left_alone
+
+
+def test_many_rows_without_inputs(tk):
+    """The epilogue of empty sums, for more rows than a launch's second dimension has workgroups."""
+    import torch
+
+    import telmo_amd
+
+    m, n = (1 << 22) + 5, 3
+    w = telmo_amd.E4m3Weights.from_device(tk, torch.zeros((n, 0), dtype=torch.uint8, device="cuda"), torch.zeros((1, 0), device="cuda"))
+    a, c = torch.zeros((m, 0), device="cuda"), torch.full((m + 1, n), 2.0, device="cuda")
+    bias = torch.tensor([1.0, -2.0, 3.0], device="cuda")
+    space = torch.zeros(w.workspace_bytes(m), dtype=torch.uint8, device="cuda")
+    tk.linear_e4m3_device(a, w, c[:m], telmo_amd.Epilogue(bias=bias, scale=0.5), workspace=space)
+    tk.synchronize()
+    assert torch.equal(c[:m], (0.5 * bias).expand(m, n)) and bool((c[m] == 2.0).all())
+
+
+def test_many_rows_of_few_inputs(tk):
+    """More rows than the rounding has workgroups for at a time: whole numbers, which e4m3 and the sums hold exactly."""
+    import torch
+
+    import telmo_amd
+
+    m, k, n = (1 << 22) + 5, 2, 3
+    values = torch.tensor([[0x38, 0x40], [0x40, 0x38], [0x38, 0xB8]], dtype=torch.uint8, device="cuda")  # 1 2, 2 1, 1 -1
+    w = telmo_amd.E4m3Weights.from_device(tk, values, torch.ones((1, 1), device="cuda"))
+    a = (torch.arange(m * k, device="cuda") % 17 - 8).float().reshape(m, k)
+    c = torch.full((m + 1, n), 2.0, device="cuda")
+    space = torch.zeros(w.workspace_bytes(m), dtype=torch.uint8, device="cuda")
+    tk.linear_e4m3_device(a, w, c[:m], workspace=space)
+    tk.synchronize()
+    x, y = a[:, 0], a[:, 1]
+    assert torch.equal(c[:m], torch.stack([x + 2 * y, 2 * x + y, x - y], 1)) and bool((c[m] == 2.0).all())
