@@ -3,8 +3,9 @@
 //
 //   c_ij = sum over blocks b of S[j / 128][b] sum over k in b of 2^e_ib a8_ik w8_jk
 //
-// S is one number for all of a wavefront's outputs, and one multiply-add per output adds a block to its f32 sum. The inner
-// sum is made in one of two ways:
+// S is one number for all of a wavefront's outputs. Its power of two is multiplied into the weights, which costs nothing and
+// rounds nothing, so that no sum overflows that would not with the weights as they stand; what is left of it, from 1 to 2,
+// goes into the multiply-add per output that adds a block to its f32 sum. The inner sum is made in one of two ways:
 //
 //   EXACT    the values are widened to bf16, which holds them exactly (the rows' with their power of two), and multiplied
 //            16 x 16 x 32 at a time: products are exact and sums f32. Few rows, which are bound by the weights' bytes, and
@@ -56,16 +57,27 @@ struct Operand<true> {
 // Read-only memory that is read by scalar loads.
 typedef const __attribute__((address_space(4))) float *Scalar;
 
-// Product i of 16 outputs by 16 rows of a block of inputs (EXACT: of four), added to `sum`; rows' powers of two, where they
-// are not in a yet, as e + 127 in each lane's row's.
-__device__ __forceinline__ f32x4 block_product(const Operand<false> &w, const Operand<false> &a, uint32_t power, int, f32x4 sum) {
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, sum, 0, 0, 0, 127, 0, (int)power);
+// Product i of 16 outputs by 16 rows of a block of inputs (EXACT: of four), added to `sum`; powers of two, where they are not
+// in w and a yet, as e + 127, the rows' each in its lanes.
+__device__ __forceinline__ f32x4 block_product(const Operand<false> &w, const Operand<false> &a, uint32_t w_power, uint32_t power, int,
+                                               f32x4 sum) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w.v, a.v, sum, 0, 0, 0, (int)w_power, 0, (int)power);
 }
-__device__ __forceinline__ f32x4 block_product(const Operand<true> &w, const Operand<true> &a, uint32_t, int i, f32x4 sum) {
+__device__ __forceinline__ f32x4 block_product(const Operand<true> &w, const Operand<true> &a, uint32_t, uint32_t, int i, f32x4 sum) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(w.v[i], a.v[i], sum, 0, 0, 0);
 }
 // e + 127 as 2^e.
 __device__ __forceinline__ float power_of(uint32_t power) { return __uint_as_float(power << 23); }
+// A block's scale as 2^g, which the weights take (g + 127), and the rest. g stays where bf16 holds 448 2^g and 2^-9 2^g as
+// normal numbers: a scale past that leaves more than 1 to 2, in products that are then far from f32's ends.
+struct BlockScale {
+    uint32_t power;
+    float rest;
+    __device__ __forceinline__ explicit BlockScale(float s) {
+        power = min(max(__float_as_uint(s) >> 23 & 255u, 27u), 227u);
+        rest = s * power_of(254u - power);
+    }
+};
 __device__ __forceinline__ i32x8 joined(i32x4 a, i32x4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 
 __device__ __forceinline__ float max_of_quarters(float x) {
@@ -284,6 +296,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
     struct Block {
         i32x8 w[PN], rows[MT];
         uint32_t power[MT];
+        float scale;
         Inputs<T> inputs;
     } now, next;
     const size_t row = lane & 15;
@@ -303,12 +316,14 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
             const i32x4 *at = reinterpret_cast<const i32x4 *>(wp[p] + (size_t)b * 2048);
             next.w[p] = joined(at[0], at[64]);
         }
+        next.scale = scale[b];
     };
     if (b0 < b1) load(b0);
     for (int b = b0; b < b1; b++) {
         now = next;
         load(b + 1 < b1 ? b + 1 : b);
-        const float s = scale[b];
+        const BlockScale s(now.scale);
+        const float w_up = power_of(s.power);
 #pragma unroll
         for (int t = 0; t < MT; t++) {
             i32x8 af;
@@ -325,12 +340,12 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few_kernel(const T *a, size_t 
             const Operand<true> rows(af, up);
 #pragma unroll
             for (int p = 0; p < PN; p++) {
-                const Operand<true> outs(now.w[p], 1.0f);
+                const Operand<true> outs(now.w[p], w_up);
                 f32x4 part = {};
 #pragma unroll
-                for (int i = 0; i < 4; i++) part = block_product(outs, rows, 0, i, part);
+                for (int i = 0; i < 4; i++) part = block_product(outs, rows, 0, 0, i, part);
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[t][p][e] = __builtin_fmaf(part[e], s, acc[t][p][e]);
+                for (int e = 0; e < 4; e++) acc[t][p][e] = __builtin_fmaf(part[e], s.rest, acc[t][p][e]);
             }
         }
     }
@@ -437,11 +452,12 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
         copy_words_to_lds(reinterpret_cast<const uint8_t *>(in.powers + ((size_t)(b / 4) * in.tiles + tile0) * 16) + wave % 4 * 256,
                           lane * 4, lds0 + stage * KG * STAGE + CHUNKS * 1024 + wave % 4 * 256);
     };
-    // A scalar load: one in a vector register would wait for the copies that left before it.
+    // A scalar load: one in a vector register would wait for the copies that left before it. A step's is loaded in the one before.
     const Scalar scale = (Scalar)(w.scales + e4m3_scale_row(panel0 + wn * TN, w.panels) * blocks);
 
     f32x4 acc[TM][TN] = {};
-    const auto work = [&](int b, int stage) __attribute__((always_inline)) {
+    const auto scale_of = [&](int step) { return scale[min(step * KG + group, blocks - 1)]; };
+    const auto work = [&](int b, int stage, float scale_now) __attribute__((always_inline)) {
         const uint8_t *st = mine + stage * KG * STAGE + lane * 16;
         const auto fragment = [&](int x) {
             return joined(*reinterpret_cast<const i32x4 *>(st + x * 2048), *reinterpret_cast<const i32x4 *>(st + x * 2048 + 1024));
@@ -450,8 +466,9 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
 #pragma unroll
         for (int t = 0; t < TM; t++)
             powers[t] = mine[stage * KG * STAGE + CHUNKS * 1024 + ((wm * TM + t) * 16 + (lane & 15)) * 4 + (b & 3)];
-        const float s = scale[b];
-        const auto panel = [&](int p) { return Operand<EXACT>(fragment(RT + wn * TN + p), 1.0f); };
+        const BlockScale s(scale_now);
+        const float w_up = power_of(s.power);
+        const auto panel = [&](int p) { return Operand<EXACT>(fragment(RT + wn * TN + p), w_up); };
         static_assert(TN == 4, "");
         const Operand<EXACT> wf[TN] = {panel(0), panel(1), panel(2), panel(3)};
         // While a row tile is multiplied the next one's fragment is read (EXACT: widened, and the one after it read), and the
@@ -479,11 +496,11 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
             for (int i = 0; i < STEPS; i++)
 #pragma unroll
                 for (int p = 0; p < TN; p++) {
-                    if (t < TM) part[t & 1][p] = block_product(wf[p], multiplied, powers[now], i, i ? part[t & 1][p] : f32x4{});
+                    if (t < TM) part[t & 1][p] = block_product(wf[p], multiplied, s.power, powers[now], i, i ? part[t & 1][p] : f32x4{});
                     if (t > 0)
 #pragma unroll
                         for (int e = 4 / STEPS * i; e < 4 / STEPS * (i + 1); e++)
-                            acc[t - 1][p][e] = __builtin_fmaf(part[(t - 1) & 1][p][e], s, acc[t - 1][p][e]);
+                            acc[t - 1][p][e] = __builtin_fmaf(part[(t - 1) & 1][p][e], s.rest, acc[t - 1][p][e]);
                 }
         }
 #pragma unroll
@@ -499,11 +516,14 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
         __builtin_amdgcn_sched_barrier(0);
     };
     issue(0, 0);
+    float scale_next = scale_of(0);
     wait_copies<0>();
     const auto step = [&](int i, int stage) __attribute__((always_inline)) {
         __syncthreads();  // the step's blocks are there, and the ones before them have been read
         issue(i + 1, stage ^ 1);
-        work(i * KG + group, stage);
+        const float scale_now = scale_next;
+        scale_next = scale_of(i + 1);
+        work(i * KG + group, stage, scale_now);
         wait_copies<0>();
     };
     const int whole = blocks / KG;  // steps in which every group has a block
@@ -515,7 +535,7 @@ __global__ __launch_bounds__(64 * WM * WN * KG, 2) void tile_kernel(Rounded in, 
     if (i < whole) step(i++, 0);
     if (i < steps) {
         __syncthreads();
-        if (i * KG + group < blocks) work(i * KG + group, i & 1);
+        if (i * KG + group < blocks) work(i * KG + group, i & 1, scale_next);
     }
     __syncthreads();
     // The groups' sums of a tile meet in one of them, a share of the tiles each.

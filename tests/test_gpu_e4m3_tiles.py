@@ -1,12 +1,79 @@
-"""The product in eight bits where its tiles take it, on an MI355X, against the definition in 64 bits: many rows, outputs of
-16 bits."""
+"""The product in eight bits by each of its kernels on an MI355X, against the definition in 64 bits: many rows, outputs of 16
+bits, values at f32's ends."""
+import numpy as np
 import pytest
 
-from test_gpu_e4m3_product import run
+from attention_oracle import HALF_STEP
+from test_gpu_attention import dtype, say
+from test_gpu_e4m3_product import rounded_rows, run, stood_for
 
 pytestmark = pytest.mark.gpu
+
+# Rows by which 1100 outputs take each kernel. Into f32: a few rows (as they lie, or not aligned), rounded rows by wavefronts
+# that spread the inputs, tiles of two groups of wavefronts and of one. Into 16 bits: the tiles' e4m3 products, and 256 x 256.
+N = 1100
+KERNELS = [(6, "f32"), (40, "f32"), (2100, "f32"), (4200, "f32"), (6, "bf16"), (40, "bf16"), (2100, "bf16"), (4200, "bf16"), (13100, "bf16")]
 
 
 def test_wide_tiles_past_the_last_scales(tk):
     """Tiles of 256 x 256 whose second half has no outputs and no scales: 1100 outputs are nine blocks of 128."""
-    run(tk, 13100, 272, 1100, "bf16", "bf16")
+    run(tk, 13100, 272, N, "bf16", "bf16")
+
+
+def multiplied(tk, a, codes, scales, to, bias=None, act=0):
+    """c for f32 rows; where no call of it is finite in 64 bits it is not looked at."""
+    import torch
+
+    import telmo_amd
+
+    say("product e4m3", a.shape, codes.shape, to, act)
+    m, n = len(a), len(codes)
+    w = telmo_amd.E4m3Weights.from_parts(tk, codes, scales)
+    c = torch.full((m, n), 3.0, dtype=dtype(to), device="cuda")
+    space = torch.zeros(w.workspace_bytes(m), dtype=torch.uint8, device="cuda")
+    epi = telmo_amd.Epilogue(bias=None if bias is None else torch.from_numpy(bias).cuda(), act=telmo_amd.Act(act))
+    tk.linear_e4m3_device(torch.from_numpy(a).cuda(), w, c, epi, workspace=space)
+    tk.synchronize()
+    return c.double().cpu().numpy()
+
+
+def off_by(ar, wr, to):
+    """How far sums may be off: test_gpu_e4m3_product.run's bound."""
+    m, k = ar.shape
+    tol = (2 * k + 64) * HALF_STEP["f32"] * (np.abs(ar) @ np.abs(wr).T)
+    if to != "f32" and m > 16:
+        for x in range(0, k, 128):
+            tol += 2.0**-10 * np.abs(ar[:, x:x + 128]).max(1)[:, None] * np.abs(wr[:, x:x + 128]).max(1)
+    return tol
+
+
+@pytest.mark.parametrize("k", (256, 300))
+@pytest.mark.parametrize("m,to", KERNELS)
+def test_sums_are_finite_where_the_outputs_are(tk, m, to, k):
+    """Rows next to f32's largest values by weights of code 448 and small scales, and rows next to the least exponent by scales
+    that are as large: what is multiplied is far from f32's ends only with the scale."""
+    rng = np.random.default_rng(m + k)
+    codes = rng.integers(0, 256, (N, k)).astype(np.uint8)
+    codes[codes & 0x7F == 0x7F] = 0x7E
+    blocks = (-(-N // 128), -(-k // 128))
+    for low, high, lowest, highest in ((2.0**110, 3e38, -14, -11), (2.0**100, 3e38, -126, -100), (2.0**-98, 2.0**-90, 90, 118),
+                                       (2.0**-20, 2.0**20, -120, 100)):
+        a = (rng.choice([-1, 1], (m, k)) * 2.0 ** rng.uniform(np.log2(low), np.log2(high), (m, k))).astype(np.float32)
+        a[rng.random((m, k)) < 0.98] = 0.0
+        scales = (2.0 ** rng.uniform(lowest, highest, blocks)).astype(np.float32)
+        ar, wr = rounded_rows(a.astype(np.float64)), stood_for(codes, scales)
+        want, most = ar @ wr.T, np.abs(ar) @ np.abs(wr).T
+        got = multiplied(tk, a, codes, scales, to)
+        good = most < 2.0**126  # past that f32's own sums may be infinite
+        assert good.mean() > 0.9
+        tol = off_by(ar, wr, to) + 2.0**-120
+        tol = tol + (0 if to == "f32" else HALF_STEP[to]) * (np.abs(want) + tol)
+        off = np.abs(got - want)[good]
+        assert np.all(np.isfinite(got[good])) and np.all(off <= tol[good]), (low, lowest, (off - tol[good]).max())
+
+
+@pytest.mark.parametrize("m,to", KERNELS)
+def test_zeros_by_the_largest_scales_are_zeros(tk, m, to):
+    scales = np.full((9, 1), 2.0**119, np.float32)
+    got = multiplied(tk, np.full((m, 128), 3e38, np.float32), np.zeros((N, 128), np.uint8), scales, to)
+    assert np.all(got == 0.0)
