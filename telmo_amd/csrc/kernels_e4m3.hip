@@ -199,14 +199,17 @@ __global__ __launch_bounds__(256) void weights_kernel(const uint8_t *src, size_t
 
 // ------------------------------------------------------------------------------------------- outputs
 
-// v / (1 + e^-v) to 2^-21 of itself: the exponent's product with log2 e in two parts, the hardware's 2^x and reciprocal.
-// The row kernels' SiLU, with their polynomial and division, takes 40 operations an output, as long as a product of 400
-// inputs. e^-v is cut at 2^126, whose reciprocal is f32's smallest normal number.
+// v / (1 + e^-v) to 2^-21 of itself from -87 on, where e^-v has a reciprocal that f32 holds as a normal number; 0 below, where
+// it is less than 2^-119. The exponent's product with log2 e in two parts, of v cut where e^-v is nothing beside 1, the
+// hardware's 2^x and reciprocal: the row kernels' SiLU, with their polynomial and division, takes 40 operations an output, as
+// long as a product of 400 inputs.
 __device__ __forceinline__ float silu(float v) {
     constexpr float L = 1.44269504088896340736f, REST = 1.92596299112661746887e-8f;  // log2 e = L + REST
-    const float t = -L * v, low = __builtin_fmaf(-L, v, -t) - REST * v;
-    const float e = fminf(__builtin_amdgcn_exp2f(t) * __builtin_fmaf(low, 0.69314718055994530942f, 1.0f), 0x1p126f);
-    return v * __builtin_amdgcn_rcpf(1.0f + e);
+    constexpr float LEAST = -87.0f;
+    const float x = __builtin_amdgcn_fmed3f(v, LEAST, 128.0f);
+    const float t = -L * x, low = __builtin_fmaf(-L, x, -t) - REST * x;
+    const float e = __builtin_amdgcn_exp2f(t) * __builtin_fmaf(low, 0.69314718055994530942f, 1.0f);
+    return v < LEAST ? -0.0f : v * __builtin_amdgcn_rcpf(1.0f + e);
 }
 // The epilogue of a lane's rows of four outputs, from column n on. The bias is loaded and waited for once, and what the call
 // says is held in scalar registers: waiting for a load of each row's own would wait for the store of the row before.

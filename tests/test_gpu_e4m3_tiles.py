@@ -77,3 +77,26 @@ def test_zeros_by_the_largest_scales_are_zeros(tk, m, to):
     scales = np.full((9, 1), 2.0**119, np.float32)
     got = multiplied(tk, np.full((m, 128), 3e38, np.float32), np.zeros((N, 128), np.uint8), scales, to)
     assert np.all(got == 0.0)
+
+
+@pytest.mark.parametrize("m,to", KERNELS + [(6, "f16"), (2100, "f16"), (13100, "f16")])
+def test_silu_of_any_sum(tk, m, to):
+    """SiLU of sums of zeros and a bias, over all of f32. It is off by a step of the exponential and of the reciprocal and
+    five roundings, 2^-21 in all, or as much as it is below -87, 87 e^-87."""
+    rng = np.random.default_rng(9)
+    ends = [0.0, -0.0, 2.0**-140, 87.0, 87.5, 88.5, 100.0, 104.0, 127.9, 128.1, 1e10, 1e30, 1e37, 1e38, 2.3586e38, 2.36e38, 3e38, 3.4e38, np.inf]
+    v = np.concatenate([ends, np.negative(ends), [np.nan], rng.uniform(-110, 110, 500), rng.standard_normal(300) * 3,
+                        rng.choice([-1, 1], N) * 2.0 ** rng.uniform(-126, 127.9, N)])[:N].astype(np.float32)
+    got = multiplied(tk, np.zeros((m, 130), np.float32), np.full((N, 130), 0x38, np.uint8), np.ones((9, 2), np.float32), to, bias=v, act=2)
+    v = v.astype(np.float64)
+    with np.errstate(over="ignore", invalid="ignore"):
+        want = np.where(v == -np.inf, 0.0, v / (1 + np.exp(-v)))
+    tol = np.abs(want) * 2.0**-21 + 2.0**-119
+    tol += np.abs(want) * (1 + 2.0**-21) * HALF_STEP[to] + (2.0**-25 if to == "f16" else 0.0)
+    largest = 65504.0 if to == "f16" else float(np.finfo(np.float32).max) if to == "f32" else 2.0**128 * (1 - 2.0**-8)
+    for r in (0, m // 2, m - 1):
+        assert np.array_equal(np.isnan(got[r]), np.isnan(v))
+        assert np.all(got[r][v > largest * 1.01] == np.inf)
+        near = np.abs(want) <= largest
+        off = np.abs(got[r][near] - want[near])
+        assert np.all(off <= tol[near]), v[near][off > tol[near]]
