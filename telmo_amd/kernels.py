@@ -214,9 +214,13 @@ class E4m3Weights:
     @staticmethod
     def from_parts(kernels: "Kernels", values, scales):
         """Host numpy arrays: uint8 values [n, k] and float32 scales [ceil(n / 128), ceil(k / 128)]."""
-        values = np.ascontiguousarray(values, np.uint8)
+        values, scales = np.asarray(values), np.asarray(scales)
+        if values.ndim != 2 or values.dtype != np.uint8:
+            raise TypeError(f"values must be uint8 [n, k], the bytes of e4m3 values, not {values.dtype} {list(values.shape)}")
         n, k = values.shape
-        sc = _f32(np.ascontiguousarray(scales, np.float32))
+        if scales.shape != (-(-n // 128), -(-k // 128)):
+            raise ValueError(f"scales must be [{-(-n // 128)}, {-(-k // 128)}], not {list(scales.shape)}")
+        values, sc = np.ascontiguousarray(values), _f32(np.ascontiguousarray(scales, np.float32))
         out = ctypes.c_void_p()
         rc = _lib.lib().tg_weights_e4m3_upload(kernels._ctx, values.ctypes.data_as(ctypes.c_void_p), values.size, k,
                                                sc.ctypes.data_as(ctypes.c_void_p), sc.size, n, k, ctypes.byref(out))
