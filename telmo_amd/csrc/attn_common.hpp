@@ -220,8 +220,10 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
         if (shown) {
             const C *k = static_cast<const C *>(a.k) + kat + kvh * a.hsk;
             float dot = 0.0f;
-            for (int c = 0; c < a.d; c++)
-                dot = __builtin_fmaf(to_f32(q[c]) + (a.rel_u ? a.rel_u[h * a.d + c] : 0.0f), to_f32(k[c]), dot);
+            for (int c = 0; c < a.d; c++) {
+                const float y = __is_same(C, e4m3) ? to_f32(k[c]) * k_scale : to_f32(k[c]);
+                dot = __builtin_fmaf(to_f32(q[c]) + (a.rel_u ? a.rel_u[h * a.d + c] : 0.0f), y, dot);
+            }
             if (a.rel) {
                 const float *rr = a.rel + (clamp_to(j - i, -a.rel_span, a.rel_span) + a.rel_span) * a.ldrel + h * a.hsrel;
                 float term = 0.0f;
@@ -229,7 +231,6 @@ __device__ void attend_row(const AttnArgs &a, int b, int h, int r, int lane) {
                     term = __builtin_fmaf(to_f32(q[c]) + (a.rel_v ? a.rel_v[h * a.d + c] : 0.0f), rr[c], term);
                 dot += term;
             }
-            if (__is_same(C, e4m3)) dot *= k_scale;
             s = score_of(a, dot, h, slope, j - i);
             shown = s != -INFINITY;
         }
