@@ -432,8 +432,9 @@ int tg_attention_device(tg_ctx *ctx, const tg_attention_desc *desc);
 int tg_attention_paged_device(tg_ctx *ctx, const tg_attention_desc *desc);
 /* A cache in eight bits: k and v of the description hold e4m3 values (a byte each; sign, four bits of exponent, three of
  * mantissa, up to 448; 0x7f and 0xff are NaN), and each block of `block` rows of a page has an exponent for each head: row
- * j, head h of page p stands for its values times 2^e with e = exps[p * page stride + j / block * kv_heads + h], from -126 to
- * 120. d is a multiple of 16; strides of k and v count values, whole multiples of 16. */
+ * j, head h of page p stands for its values times 2^e with e = exps[p * page stride + j / block * kv_heads + h], from -100
+ * to 120 (appends choose none below; under lower ones single tokens of f32 lose bits of their weights). d is a multiple of
+ * 16; strides of k and v count values, whole multiples of 16. */
 typedef struct {
     int8_t *k_exps, *v_exps;          /* device, page / block x kv_heads for each page */
     size_t k_exps_len, v_exps_len;

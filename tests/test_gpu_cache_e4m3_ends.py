@@ -46,3 +46,11 @@ def attended(tk, type, new, total, low, high, hidden_nan, q_size=1.0, v_low=-6, 
 def test_large_rows_by_small_keys(tk, type, new, hidden_nan):
     """q of 2^118 by keys under 2^-100: their products are moderate, q's by the keys' codes are not."""
     attended(tk, type, new, 200, -100, -98, hidden_nan, q_size=2.0**118)
+
+
+@pytest.mark.parametrize("type,new", [(t, n) for t in ("f32", "bf16") for n in (1, 30)])
+@pytest.mark.parametrize("low,high", ((-100, -100), (-100, -92), (-100, 100), (100, 112)))
+def test_values_of_the_least_and_largest_exponents(tk, type, new, low, high):
+    """The least exponent leaves an f32 weight's three parts normal numbers of bf16; under the largest ones 40
+    values of 448 stay below f32's end together."""
+    attended(tk, type, new, 200, -6, 3, False, v_low=low, v_high=high)
