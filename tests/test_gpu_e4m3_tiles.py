@@ -100,3 +100,79 @@ def test_silu_of_any_sum(tk, m, to):
         near = np.abs(want) <= largest
         off = np.abs(got[r][near] - want[near])
         assert np.all(off <= tol[near]), v[near][off > tol[near]]
+
+
+@pytest.mark.parametrize("type,n", [("f32", 8200), ("f16", 8201), ("bf16", 8200), ("f32", 16400), ("bf16", 32800), ("f16", 32783)])
+@pytest.mark.parametrize("m,k", ((1, 256), (16, 300), (5, 1000), (16, 1024)))
+def test_few_rows_by_very_many_outputs(tk, m, k, type, n):
+    """Two panels of outputs to a workgroup, and four; rows in whole blocks, and not."""
+    run(tk, m, k, n, type, "f32" if m == 5 else type, bias=False)
+
+
+# Tiles of two groups of wavefronts, of one, and of 256 x 256, for about 1100 outputs in 16 bits.
+TILES = (1300, 4200, 13100)
+
+
+@pytest.mark.parametrize("type,to", [("f32", "f16"), ("f16", "f16"), ("bf16", "bf16"), ("f32", "bf16"), ("f16", "bf16")])
+@pytest.mark.parametrize("m", TILES)
+def test_tiles_into_16_bits(tk, m, type, to):
+    run(tk, m, 384, 1100, type, to, act=2, scale=-1.5)
+    run(tk, m - 19, 200, 1099, type, to, bias=False)  # outputs that end inside a lane's four
+    run(tk, m, 130, 1100, type, to, act=1, accumulate=True, scale=0.5, pad=4, offset=0)
+    run(tk, m + 1, 128, 1101, type, to, accumulate=True, pad=3, offset=1)
+
+
+@pytest.mark.parametrize("m", TILES)
+def test_special_rows_into_16_bits(tk, m):
+    """Outliers, subnormals, zeros, f32's largest values; NaN and infinities make their rows' outputs NaN alone, NaN weights their
+    outputs."""
+    rng = np.random.default_rng(5)
+    a = rng.standard_normal((m, 300)).astype(np.float32)
+    a[0, 7], a[1], a[2, 130:260], a[3] = 1e30, 0.0, 1e-38, 2.0**-140
+    a[4, ::2] *= 1e-3
+    run(tk, m, 300, N, to="bf16", rows=a, bias=False)
+    a[0, 5], a[2, 290], a[5, 0], a[m - 1, 299] = np.nan, np.inf, -np.inf, np.nan
+    run(tk, m, 300, N, to="bf16", rows=a, bias=False)
+    b = np.full((m, 128), 448.0, np.float32)  # at the border of an exponent, and one step past it
+    b[1::2, 3] = np.nextafter(np.float32(448.0), np.float32(500.0))
+    b[2, :] = 3.3e38
+    run(tk, m, 128, N, to="bf16", rows=b, bias=False, codes=np.full((N, 128), 1, np.uint8))
+    codes = rng.integers(0, 127, (N, 200)).astype(np.uint8)
+    codes[37, 150], codes[N - 1, 0] = 0x7F, 0xFF
+    for to in ("f16", "bf16"):
+        run(tk, m, 200, N, to=to, codes=codes, bias=False)
+
+
+@pytest.mark.parametrize("to", ("f16", "bf16"))
+@pytest.mark.parametrize("m", TILES)
+def test_products_that_cancel(tk, m, to):
+    """Pairs of inputs whose products cancel exactly, and small ones beside them: off by 2^-10 of the largest products at most."""
+    rng = np.random.default_rng(m)
+    k = 272
+    a = rng.standard_normal((m, k)).astype(np.float32)
+    a[:, 1::2] = -a[:, ::2]
+    codes = rng.integers(0, 0x7F, (N, k)).astype(np.uint8)
+    codes[:, 1::2] = codes[:, ::2]
+    a[:, 100:104] = rng.standard_normal((m, 4)) * 2.0**-6
+    codes[:, 103] = rng.integers(0, 0x40, N)
+    run(tk, m, k, N, to=to, rows=a, codes=codes, bias=False)
+
+
+@pytest.mark.parametrize("m", TILES)
+def test_tiles_replayed_from_a_graph(tk, gpu_stream, m):
+    import torch
+
+    args, space, c = run(tk, m, 300, N, "bf16", "bf16", act=2)
+    want = c.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=gpu_stream):
+        tk.linear_e4m3_device(*args, workspace=space)
+    for i in range(3):
+        args[2].fill_(float(i))
+        space.fill_(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        same = torch.equal(c, want)
+        tk.linear_e4m3_device(*args, workspace=space)
+        torch.cuda.synchronize()
+        assert same and torch.equal(c, want), i
