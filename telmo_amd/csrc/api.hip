@@ -160,6 +160,8 @@ hipError_t scratch_address(int device, void **out) {
 namespace {
 
 int fail(tg_ctx *ctx, int code, const std::string &msg) {
+    // What is reported here is not the next launch's to report.
+    if (code == TG_ERR_NOMEM || code == TG_ERR_HIP) (void)hipGetLastError();
     if (ctx) {
         std::lock_guard<std::mutex> g(ctx->err_mu);
         ctx->err = msg;

@@ -3,7 +3,7 @@ import pytest
 
 pytestmark = pytest.mark.gpu
 
-UNSUPPORTED = -5
+UNSUPPORTED, NOMEM = -5, -6
 
 
 def test_too_many_tiles_leave_the_workspace_alone(tk):
@@ -59,3 +59,44 @@ def test_many_rows_of_few_inputs(tk):
     tk.synchronize()
     x, y = a[:, 0], a[:, 1]
     assert torch.equal(c[:m], torch.stack([x + 2 * y, 2 * x + y, x - y], 1)) and bool((c[m] == 2.0).all())
+
+
+def test_weights_that_do_not_fit_leave_no_error_behind(tk):
+    """2^48 bytes of weights: the allocation fails before anything is read, and the next call is none the worse."""
+    import ctypes
+
+    import torch
+
+    import telmo_amd
+    from telmo_amd import _lib
+
+    n = 1 << 24
+    w = telmo_amd.E4m3Weights.from_device(tk, torch.zeros((16, 16), dtype=torch.uint8, device="cuda"), torch.ones((1, 1), device="cuda"))
+    a, c = torch.ones((1, 16), device="cuda"), torch.full((1, 16), 2.0, device="cuda")
+    small, out = (ctypes.c_uint8 * 16)(), ctypes.c_void_p()
+    for upload, at in ((_lib.lib().tg_weights_e4m3_upload, ctypes.addressof(small)), (_lib.lib().tg_weights_e4m3_upload_device, a.data_ptr())):
+        assert upload(tk._ctx, at, n * n, n, at, (n // 128)**2, n, n, ctypes.byref(out)) == NOMEM and not out.value
+        tk.linear_e4m3_device(a, w, c)
+        tk.synchronize()
+        assert bool((c == 0).all())
+
+
+def test_other_weights_that_do_not_fit_leave_no_error_behind(tk):
+    """The same of int8 weights, 2^48 bytes of them too."""
+    import ctypes
+
+    import torch
+
+    import telmo_amd
+    from telmo_amd import _lib
+
+    w = telmo_amd.E4m3Weights.from_device(tk, torch.zeros((16, 16), dtype=torch.uint8, device="cuda"), torch.ones((1, 1), device="cuda"))
+    a, c = torch.ones((1, 16), device="cuda"), torch.full((1, 16), 2.0, device="cuda")
+    small, out = (ctypes.c_uint8 * 16)(), ctypes.c_void_p()
+    n = 1 << 24
+    at = ctypes.addressof(small)
+    rc = _lib.lib().tg_weights_upload(tk._ctx, at, n * n, at, n, int(telmo_amd.Precision.INT8), n, n, ctypes.byref(out))
+    assert rc == NOMEM and not out.value
+    tk.linear_e4m3_device(a, w, c)
+    tk.synchronize()
+    assert bool((c == 0).all())
