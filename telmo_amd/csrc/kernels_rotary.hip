@@ -32,6 +32,39 @@ __device__ __forceinline__ float2 turn(double turns, float amplitude) {
     return make_float2(amplitude * (n == 1 || n == 2 ? -cs : cs), amplitude * (n >= 2 ? -sn : sn));
 }
 
+// The same in 64 bits: Taylor's polynomials of sin and cos within an eighth of a turn, to 2^-45. Their coefficients are held
+// in scalar registers: in vector ones they would cost a kernel one wavefront in four.
+__device__ __forceinline__ double scalar(double x) {
+    asm("" : "+s"(x));
+    return x;
+}
+__device__ __forceinline__ double2 turn64(double turns, float amplitude) {
+    const double whole = __builtin_rint(turns), rest = (turns - whole) * 4.0;  // quarter turns, |rest| <= 2
+    const double quarter = __builtin_rint(rest), x = (rest - quarter) * 1.57079632679489661923, y = x * x;
+    double s = scalar(1.0 / 6227020800.0), c = scalar(-1.0 / 87178291200.0);
+    c = __builtin_fma(c, y, scalar(1.0 / 479001600.0));
+    s = __builtin_fma(s, y, scalar(-1.0 / 39916800.0)), c = __builtin_fma(c, y, scalar(-1.0 / 3628800.0));
+    s = __builtin_fma(s, y, scalar(1.0 / 362880.0)), c = __builtin_fma(c, y, scalar(1.0 / 40320.0));
+    s = __builtin_fma(s, y, scalar(-1.0 / 5040.0)), c = __builtin_fma(c, y, scalar(-1.0 / 720.0));
+    s = __builtin_fma(s, y, scalar(1.0 / 120.0)), c = __builtin_fma(c, y, scalar(1.0 / 24.0));
+    s = __builtin_fma(s, y, scalar(-1.0 / 6.0)), c = __builtin_fma(c, y, -0.5);
+    s = __builtin_fma(s * y, x, x), c = __builtin_fma(c, y, 1.0);
+    const int n = (int)quarter & 3;
+    const double cs = n & 1 ? s : c, sn = n & 1 ? c : s;
+    return make_double2(amplitude * (n == 1 || n == 2 ? -cs : cs), amplitude * (n >= 2 ? -sn : sn));
+}
+// (x, y) turned, in the table's bits, and rounded once.
+__device__ __forceinline__ void rotate(float &x, float &y, const float2 &t) {
+    const float a = x, b = y;
+    x = a * t.x - b * t.y;
+    y = b * t.x + a * t.y;
+}
+__device__ __forceinline__ void rotate(float &x, float &y, const double2 &t) {
+    const double a = x, b = y;
+    x = (float)__builtin_fma(a, t.x, -(b * t.y));
+    y = (float)__builtin_fma(b, t.x, a * t.y);
+}
+
 // n <= 8 values at p in 32 bits, in one piece where all eight are wanted and p is aligned.
 template <typename T>
 __device__ __forceinline__ void load_some(const T *p, int n, bool aligned, float *v) {
@@ -56,8 +89,8 @@ __host__ __device__ inline int pair_pieces(int dim) { return (dim / 2 + 7) / 8; 
 __host__ __device__ inline int pieces_of(int d, int dim) { return pair_pieces(dim) + (d - dim + 7) / 8; }
 
 // put(first, n, whether `first` is a multiple of 8, n values in 32 bits) for the eights of a piece.
-template <typename T, typename F>
-__device__ __forceinline__ void with_piece(const T *x, int piece, int d, int dim, bool interleaved, const float2 *table, F put) {
+template <typename T, typename Turn, typename F>
+__device__ __forceinline__ void with_piece(const T *x, int piece, int d, int dim, bool interleaved, const Turn *table, F put) {
     const int half = dim / 2, turned = pair_pieces(dim);
     float v[8];
     if (piece >= turned) {
@@ -73,11 +106,9 @@ __device__ __forceinline__ void with_piece(const T *x, int piece, int d, int dim
         load_some(x + 2 * i, m, true, v);
         load_some(x + 2 * i + 8, 2 * n - m, true, w);
         for (int e = 0; e < 8; e += 2) {
-            const float2 s = e / 2 < n ? table[i + e / 2] : make_float2(0.0f, 0.0f);
-            const float2 t = 4 + e / 2 < n ? table[i + 4 + e / 2] : make_float2(0.0f, 0.0f);
-            const float a = v[e], b = v[e + 1], f = w[e], g = w[e + 1];
-            v[e] = a * s.x - b * s.y, v[e + 1] = b * s.x + a * s.y;
-            w[e] = f * t.x - g * t.y, w[e + 1] = g * t.x + f * t.y;
+            const Turn s = e / 2 < n ? table[i + e / 2] : Turn{}, t = 4 + e / 2 < n ? table[i + 4 + e / 2] : Turn{};
+            rotate(v[e], v[e + 1], s);
+            rotate(w[e], w[e + 1], t);
         }
         put(2 * i, m, true, v);
         put(2 * i + 8, 2 * n - m, true, w);
@@ -85,10 +116,8 @@ __device__ __forceinline__ void with_piece(const T *x, int piece, int d, int dim
         load_some(x + i, n, true, v);
         load_some(x + half + i, n, half % 8 == 0, w);
         for (int e = 0; e < 8; e++) {
-            const float2 t = e < n ? table[i + e] : make_float2(0.0f, 0.0f);
-            const float a = v[e], b = w[e];
-            v[e] = a * t.x - b * t.y;
-            w[e] = b * t.x + a * t.y;
+            const Turn t = e < n ? table[i + e] : Turn{};
+            rotate(v[e], w[e], t);
         }
         put(i, n, true, v);
         put(half + i, n, half % 8 == 0, w);
@@ -170,6 +199,8 @@ __global__ __launch_bounds__(THREADS) void append_kernel(const T *k, int64_t ldk
 // the block's new rows are. A workgroup takes a block of a sequence, a wavefront one head's keys or values in it at a time:
 // first the largest of the new rows, rotated, then the block's exponent, and the rows that were there before in it where
 // that grows, then the new rows again, rounded.
+// The rotation is worked out in 64 bits: next to a border of e4m3 an f32 one rounds three times as many values to the other
+// side as one of exact products and sums in f32 would (6 to 18 of 6.6 million instead of 1 to 7).
 constexpr int TURNS = 2048;  // sines and cosines held at a time
 
 // The older rows of a block, by one wavefront, times `down`.
@@ -194,7 +225,7 @@ __global__ __launch_bounds__(THREADS) void append8_whole_kernel(const T *k, int6
                                                                 int64_t hsv, const Cache8 c, int heads, int d, const AttnSeqs q,
                                                                 const RotaryArgs r) {
     constexpr int STEPS = 2;
-    __shared__ float2 table[TURNS];
+    extern __shared__ double2 table[];  // of a block's rows
     const int b = blockIdx.y;
     const AttnSpan sp = span_of(q, b);
     const int rows = sp.nq < q.longest ? sp.nq : q.longest;
@@ -213,7 +244,7 @@ __global__ __launch_bounds__(THREADS) void append8_whole_kernel(const T *k, int6
         const int64_t from = (int64_t)sp.q0 + (lo - first);  // the first new row
         if (pairs && (int)blockIdx.z * 4 < heads) {  // a workgroup of values alone needs no turns
             __syncthreads();
-            for (int t = threadIdx.x; t < n * pairs; t += THREADS) table[t] = turn((double)(lo + t / pairs) * r.turns[t % pairs], r.amplitude);
+            for (int t = threadIdx.x; t < n * pairs; t += THREADS) table[t] = turn64((double)(lo + t / pairs) * r.turns[t % pairs], r.amplitude);
             __syncthreads();
         }
         for (int unit = blockIdx.z * 4 + wave; unit < 2 * heads; unit += gridDim.z * 4) {
@@ -239,15 +270,9 @@ __global__ __launch_bounds__(THREADS) void append8_whole_kernel(const T *k, int6
                 if (!turned) return;
 #pragma unroll
                 for (int i = 0; i < STEPS; i++) {
-                    const float2 *w = table + min(done + i * apart + own, n - 1) * pairs + piece * 8;
+                    const double2 *w = table + min(done + i * apart + own, n - 1) * pairs + piece * 8;
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float2 t = w[e];
-                        float &f = y[i][HALVES ? e : 2 * e], &g = y[i][HALVES ? e + 8 : 2 * e + 1];
-                        const float f0 = f, g0 = g;
-                        f = f0 * t.x - g0 * t.y;
-                        g = g0 * t.x + f0 * t.y;
-                    }
+                    for (int e = 0; e < 8; e++) rotate(y[i][HALVES ? e : 2 * e], y[i][HALVES ? e + 8 : 2 * e + 1], w[e]);
                 }
             };
             const int chunk = STEPS * apart;
@@ -289,7 +314,7 @@ template <typename T>
 __global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ldk, int64_t hsk, const T *v, int64_t ldv,
                                                           int64_t hsv, const Cache8 c, int heads, int d, const AttnSeqs q,
                                                           const RotaryArgs r) {
-    __shared__ float2 table[TURNS];
+    extern __shared__ double2 table[];  // of a block's rows, or TURNS
     const int b = blockIdx.y;
     const AttnSpan sp = span_of(q, b);
     const int rows = sp.nq < q.longest ? sp.nq : q.longest;
@@ -311,10 +336,10 @@ __global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ld
         const auto fill = [&](int done) {
             __syncthreads();
             for (int t = threadIdx.x; t < min(some, n - done) * pairs; t += THREADS)
-                table[t] = turn((double)(lo + done + t / pairs) * r.turns[t % pairs], r.amplitude);
+                table[t] = turn64((double)(lo + done + t / pairs) * r.turns[t % pairs], r.amplitude);
             __syncthreads();
         };
-        if (pairs && some == n) fill(0);
+        if (pairs && some == n && (int)blockIdx.z * 4 < heads) fill(0);  // a workgroup of values alone needs no turns
         for (int u0 = blockIdx.z * 4; u0 < 2 * heads; u0 += gridDim.z * 4) {
             // All wavefronts make the same steps: one past the last unit does the last one's again, and writes nothing.
             const int unit = min(u0 + wave, 2 * heads - 1);
@@ -327,17 +352,22 @@ __global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ld
             rows8 += row0 * ldc;
             int8_t *exps = key ? c.k_exps + page * c.k_epage : c.v_exps + page * c.v_epage;
             exps += (int64_t)(row0 / c.block) * heads + h;
-            const int pieces = pieces_of(d, dim);
+            const int pieces = pieces_of(d, dim), turned = pair_pieces(dim);
             // f(the block's row, first, n, aligned, values) for the eights of the wavefront's pieces.
             const auto each = [&](auto f) {
                 for (int done = 0; done < n; done += some) {
-                    if (pairs && some < n) fill(done);
+                    if (pairs && some < n && u0 < heads) fill(done);
                     const int now = min(some, n - done);
-                    for (int t = lane; t < now * pieces; t += 64) {
-                        const int row = t / pieces;
-                        with_piece(x + (done + row) * ld, t % pieces, d, dim, r.interleaved, table + row * pairs,
-                                   [&](int at, int count, bool aligned, const float *y) { f(done + row, at, count, aligned, y); });
-                    }
+                    const auto some_pieces = [&](int piece0, int count) {
+                        for (int t = lane; t < now * count; t += 64) {
+                            const int row = t / count;
+                            with_piece(x + (done + row) * ld, piece0 + t % count, d, dim, r.interleaved, table + row * pairs,
+                                       [&](int at, int n, bool aligned, const float *y) { f(done + row, at, n, aligned, y); });
+                        }
+                    };
+                    // Pieces that are rotated, then the others: a wavefront does either at a time.
+                    some_pieces(0, turned);
+                    some_pieces(turned, pieces - turned);
                 }
             };
             uint32_t top = 0;
@@ -433,7 +463,8 @@ hipError_t launch_append8(const void *k, int64_t ldk, int64_t hsk, const void *v
         using T = decltype(t);
         const bool whole = r.dim % 16 == 0 && (size_t)c.block * (r.dim / 2) <= TURNS;
         const auto kernel = !whole ? append8_kernel<T> : r.interleaved ? append8_whole_kernel<T, false> : append8_whole_kernel<T, true>;
-        hipLaunchKernelGGL(kernel, grid, dim3(THREADS), 0, s, static_cast<const T *>(k), ldk, hsk, static_cast<const T *>(v), ldv, hsv, c,
+        const size_t turns = min_of((size_t)c.block * (r.dim / 2), TURNS) * sizeof(double2);
+        hipLaunchKernelGGL(kernel, grid, dim3(THREADS), turns, s, static_cast<const T *>(k), ldk, hsk, static_cast<const T *>(v), ldv, hsv, c,
                            heads, d, q, r);
         return hipGetLastError();
     };
