@@ -237,10 +237,11 @@ int tg_linear_glu_device(tg_ctx *ctx, const float *a, size_t a_len, size_t m, co
  * c = epi(a' w'^T): w' are e4m3 values (a byte each: sign, four bits of exponent, three of mantissa, up to 448; 0x7f and
  * 0xff are NaN) times an f32 scale for each block of 128 outputs by 128 inputs, and a' is a with each row's groups of 128
  * inputs rounded to e4m3 times a power of two: the least e >= -100 with |x| <= 448 2^e for the group's finite values, each
- * x 2^-e rounded to nearest, ties to even (|x| past 240 2^120, which would round past f32, as that). Sums are f32. NaN or infinity in a row make its outputs NaN. No counterpart in
- * the reference; a context's mode changes nothing here. Row i's outputs depend on m by the order of their f32 sums; 16-bit
- * outputs of more than 16 rows may be summed by instructions that align the products of 32 inputs before they add them,
- * off by up to 2^-10 of the largest of each 128. */
+ * x 2^-e rounded to nearest, ties to even (|x| past 240 2^120, which would round past f32, as that). Sums are f32, of a' w'
+ * with its scales: one overflows where the products as they stand do. NaN or infinity in a row make its sums NaN (which
+ * TG_ACT_RELU, as everywhere, makes 0). No counterpart in the reference; a context's mode changes nothing here. Row i's
+ * outputs depend on m by the order of their f32 sums; 16-bit outputs of more than 16 rows may be summed by instructions that
+ * align the products of 32 inputs before they add them, off by up to 2^-10 of the largest of each 128. */
 typedef struct tg_weights_e4m3 tg_weights_e4m3;
 /* Row-major values [n][k], rows ldv apart, and scales [ceil(n / 128)][ceil(k / 128)], host pointers (device pointers, read
  * during the call only). The device copy is the library's own, laid out for the matrix cores. n and k at most 2^24. */
@@ -477,11 +478,11 @@ int tg_cache_append_device(tg_ctx *ctx, const tg_attention_desc *desc, uint32_t 
                            const tg_rotary *rotary);
 
 /* The same into a cache in e4m3. A block's exponent is the least e >= -100 with |x| <= 448 2^e for the finite values of its
- * new rows (keys rotated), and each value is x 2^-e rounded to nearest, ties to even (|x| past 240 2^120, which
- * would round past f32, as that); NaN and infinities become NaN. A
- * block that holds older rows of its sequence keeps its exponent where that is large enough; where it grows, its older rows
- * are rounded again under the new one (powers of two: only values that become subnormal lose bits). Rows of a block behind
- * the new ones are left as they were. A block takes the new rows of one sequence in a call. */
+ * new rows (keys rotated in 64 bits and rounded to f32), and each value is x 2^-e rounded to nearest, ties to even (|x| past
+ * 240 2^120, which would round past f32, as that); NaN and infinities become NaN. A block that holds older rows of its
+ * sequence keeps its exponent where that is large enough; where it grows, its older rows are rounded again under the new one
+ * (powers of two: only values that become subnormal lose bits). Rows of a block behind the new ones are left as they were. A
+ * block takes the new rows of one sequence in a call. */
 int tg_cache_append_e4m3_device(tg_ctx *ctx, const tg_attention_desc *desc, const tg_cache_e4m3 *cache, uint32_t type,
                                 tg_rows k_new, tg_rows v_new, const tg_rotary *rotary);
 

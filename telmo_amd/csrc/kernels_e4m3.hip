@@ -276,7 +276,7 @@ struct Outputs {
 // MT x 16 rows by PN x 16 outputs of a workgroup, the blocks of inputs spread over its wavefronts, whose sums LDS joins in
 // their order. 16 rows at most are rounded as they are read, more come from their fragments.
 //
-// Bound by the weights' bytes: 16 rows of bf16 by 4096 x 16384 (68 MB) 16.8 us, 4.1 TB/s (a large copy 4.85). The rows' rounding
+// Bound by the weights' bytes: 16 rows of bf16 by 4096 x 16384 (68 MB) 16.8 us, 4.0 TB/s (a large copy 4.85). The rows' rounding
 // is what a wavefront works longest on: with nine operations a value instead of three it took 19.5, and where each block
 // waited for its rows 20.8. One row by 640 x 2560 takes the time of a call.
 constexpr int FEW_WAVES = 8;
@@ -412,7 +412,7 @@ __device__ __forceinline__ void wait_copies() {
 // block of inputs, and add up their sums in LDS. LDS holds two stages of a block for each group: while one is worked on, the
 // next is copied to the other.
 //
-// 8192 x 8192 x 8192 into bf16 takes 40 us to round the rows (at the rate of a copy) and 470 by tiles of 256 x 256, 2340 TFLOP/s:
+// 8192 x 8192 x 8192 into bf16 takes 40 us to round the rows (at the rate of a copy) and 480 by tiles of 256 x 256, 2290 TFLOP/s:
 // a block of inputs is 2112 cycles of a CU's matrix instructions, and 192 KB that its wavefronts read from LDS and 64 KB that
 // are copied there are 2048 of LDS, which the two share badly. 750 rows by 1024 x 4096 into f32, EXACT, take 20 us: 192 tiles
 // for 256 CUs, eight blocks of inputs each, between a start and an end that nothing overlaps.

@@ -218,8 +218,9 @@ __device__ __forceinline__ void lower_rows(uint8_t *rows8, int64_t ldc, int olde
 // Heads whose rotated part is whole pieces of 16 values, in blocks whose turns fit LDS. A lane takes a piece (two eights,
 // of a rotated half each, or 16 in a row) of every 64 / pieces-th row, STEPS of them at a time, and keeps a block of as many
 // in registers from the largest to the rounding; a longer block's rows are read again. No piece is cut, so that a step is
-// loads and products without branches. Bound by memory: 8188 rows of 8 heads of 128 in f32, keys rotated, blocks of 16, 84 MB
-// in 18 us (4.6 TB/s); with four steps, and so half the wavefronts, 23, by cut pieces 25. Eight single rows take 6.
+// loads and products without branches. Bound by memory: four sequences' 6449 rows (2047, 1812, 1365, 1225) of 8 heads of 128 in
+// f32, keys rotated, blocks of 16, 66 MB in 18.3 us (3.6 TB/s); with four steps, and so half the wavefronts, 23, by cut pieces
+// 25. Eight single rows take 6.
 template <typename T, bool HALVES>
 __global__ __launch_bounds__(THREADS) void append8_whole_kernel(const T *k, int64_t ldk, int64_t hsk, const T *v, int64_t ldv,
                                                                 int64_t hsv, const Cache8 c, int heads, int d, const AttnSeqs q,
@@ -309,7 +310,8 @@ __global__ __launch_bounds__(THREADS) void append8_whole_kernel(const T *k, int6
 }
 
 // Any rotated part and block: a table of as many rows' turns as fit, pieces that may be cut. What is read twice comes from
-// the CU's cache the second time.
+// the CU's cache the second time. The 6449 rows above in blocks of 64, whose turns are worked out twice for each set of four
+// heads, take 37 us, and in blocks of 16 with 40 of the 128 values rotated 34.
 template <typename T>
 __global__ __launch_bounds__(THREADS) void append8_kernel(const T *k, int64_t ldk, int64_t hsk, const T *v, int64_t ldv,
                                                           int64_t hsv, const Cache8 c, int heads, int d, const AttnSeqs q,

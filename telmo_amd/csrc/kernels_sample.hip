@@ -35,7 +35,9 @@ constexpr int PART_THREADS = 256, PART_VALUES = 64, PART = PART_THREADS * PART_V
 constexpr int COPIES = 2;     // of the bins that are counted: lanes next to each other add to different ones
 constexpr int SUM_BITS = 49;  // of a counted bin; above them the count of up to 2^14 tokens, whose sum is below 2^48.5
 static_assert(WHOLE <= COPIES << 14 && PART <= 1 << 14, "a bin's count and sum share 64 bits");
-constexpr double FIXED = 1024.0;  // added to a weight it leaves steps of 2^-42: 2^22 weights' sum fits 64 bits
+// Added to a weight it leaves steps of 2^-42. 2^22 weights' sum fits 64 bits, but for 2^22 ones, which come to 0: they are the
+// whole row, in one bin, which is taken whatever its sum.
+constexpr double FIXED = 1024.0;
 
 // What a part of a row leaves: its bins, relative to its largest logit.
 struct PartBins {
@@ -940,7 +942,7 @@ hipError_t launch_sample(const SampleArgs &a, uint32_t type, int rows, void *wor
             if (e != hipSuccess) return e;
             hipLaunchKernelGGL((sample_kernel<T, 0>), dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)parts, count);
         } else {
-const auto kernel = a.n <= SHORT_VALUES * THREADS ? sample_kernel<T, SHORT_VALUES> : sample_kernel<T, WHOLE_VALUES>;
+            const auto kernel = a.n <= SHORT_VALUES * THREADS ? sample_kernel<T, SHORT_VALUES> : sample_kernel<T, WHOLE_VALUES>;
             hipLaunchKernelGGL(kernel, dim3((unsigned)rows), dim3(THREADS), 0, s, a, (const PartBins *)nullptr, 0);
         }
         return hipGetLastError();
