@@ -3,9 +3,10 @@
 //
 //   c_ij = sum over blocks b of S[j / 128][b] sum over k in b of 2^e_ib a8_ik w8_jk
 //
-// S is one number for all of a wavefront's outputs. Its power of two is multiplied into the weights, which costs nothing and
-// rounds nothing, so that no sum overflows that would not with the weights as they stand; what is left of it, from 1 to 2,
-// goes into the multiply-add per output that adds a block to its f32 sum. The inner sum is made in one of two ways:
+// S is one number for all of a wavefront's outputs. Its power of two is multiplied into the weights, which rounds nothing, so
+// that no sum overflows that would not with the weights as they stand (8192^3 523 us; 515 with all of S applied afterwards);
+// what is left of it, from 1 to 2, goes into the multiply-add per output that adds a block to its f32 sum. The inner sum is
+// made in one of two ways:
 //
 //   EXACT    the values are widened to bf16, which holds them exactly (the rows' with their power of two), and multiplied
 //            16 x 16 x 32 at a time: products are exact and sums f32. Few rows, which are bound by the weights' bytes, and
